@@ -288,7 +288,8 @@ def _plain_encode(x, fmt):
     if fmt not in CODE_MAX:
         return x.to(TYPES[fmt]), None
     x = x.float()
-    scale = x.abs().amax(-1).clamp(min=FLOOR) / CODE_MAX[fmt]
+    top = x.abs().amax(-1).clamp(min=FLOOR)
+    scale = top / torch.full_like(top, CODE_MAX[fmt])      # by a tensor: by a number it is a product with 1 / number
     y = x / scale.unsqueeze(-1)
     return (torch.round(y) if fmt == "int8" else y).to(TYPES[fmt]), scale
 
