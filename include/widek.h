@@ -48,6 +48,10 @@ extern "C" {
 #define WIDEK_F32 0
 #define WIDEK_BF16 1
 #define WIDEK_F16 2
+/* Storage formats of a key-value cache besides the three dtypes: 8-bit codes
+ * with one fp32 scale per (token, head). */
+#define WIDEK_I8 3
+#define WIDEK_E4M3 4
 
 #define WIDEK_ACT_NONE 0
 #define WIDEK_ACT_RELU 1
@@ -633,6 +637,93 @@ WIDEK_API int widek_groupnorm_bwd(const void* x, const void* dy, const void* wei
                                   void* dw, void* db, int64_t n, int64_t batch, int64_t c,
                                   int64_t l, int64_t groups, double eps, int dtype,
                                   void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- Decoder attention: norm + rotation, paged cache, single tokens ------
+ *
+ * No counterpart in the reference (its attention is
+ * wide_compiler/core/primitives/wide_attention.py, over whole sequences).
+ *
+ * Common arguments:
+ *   q [n, b, t, hq, d], k and v [n, b, t, hk, d]: strided, channels dense.
+ *   geom, 23 int64 on the host: n, b, t, hq, hk, d, rot, table_rows, then the
+ *     element strides (model, sequence, token, head) of q, of k and of v, and
+ *     (model, sequence, token) of the positions.
+ *   positions: int32, or int64 with pos64 = 1; a negative one marks a padding
+ *     row (zeros out, nothing written, zero gradient). One past the table or
+ *     the cache records WIDEK_DEV_ERR_INDEX and is treated the same way.
+ *   cos, sin: [table_rows, rot / 2] fp32.
+ *   Cache: kc, vc [n, pages, hk, page, d] dense in `fmt` (the tensors' dtype,
+ *     WIDEK_I8 or WIDEK_E4M3), ks, vs [n, pages, hk, page] fp32 for the 8-bit
+ *     formats (else NULL), table int32 page numbers; cgeom, 5 int64: pages,
+ *     page, table columns, table strides over models and sequences. Token p
+ *     of a sequence is in page table[p / page] at offset p % page.
+ *   d <= 256; rot even, rot <= d. */
+
+/* RMS norm of every query and key head and the rotation of its first rot
+ * channels, in one pass: u = x * rsqrt(mean(x^2) + eps) * w[model], then each
+ * pair (i, i + rot/2), or (2i, 2i+1) when interleaved, turned by the angle
+ * whose cos / sin the table holds at the row's position.
+ *   qw, kw: [n, d]; yq [n, b, t, hq, d], yk [n, b, t, hk, d] dense. */
+WIDEK_API int widek_qk_norm_rope_fwd(const void* q, const void* k, const void* qw, const void* kw,
+                                     const float* cos, const float* sin, const void* positions,
+                                     void* yq, void* yk, const int64_t* geom, double eps,
+                                     int interleaved, int pos64, int dtype, void* stream);
+
+/* The same with the keys and the values written to the cache at their
+ * positions (keys after the rotation, quantised from fp32) and the queries
+ * to yq: one launch for a decoder step. */
+WIDEK_API int widek_qk_norm_rope_write_fwd(const void* q, const void* k, const void* v,
+                                           const void* qw, const void* kw, const float* cos,
+                                           const float* sin, const void* positions, void* yq,
+                                           void* kc, void* vc, float* ks, float* vs,
+                                           const void* table, const int64_t* geom,
+                                           const int64_t* cgeom, double eps, int interleaved,
+                                           int pos64, int fmt, int dtype, void* stream);
+
+/* Workspace bytes widek_qk_norm_rope_bwd needs (-1 for bad arguments). */
+WIDEK_API int64_t widek_qk_norm_rope_bwd_workspace(const int64_t* geom);
+
+/* Gradients of widek_qk_norm_rope_fwd: dyq, dyk, dq, dk dense; dqw, dkw
+ * [n, d], nullable. The weight gradients are summed in a fixed order. */
+WIDEK_API int widek_qk_norm_rope_bwd(const void* q, const void* k, const void* qw, const void* kw,
+                                     const float* cos, const float* sin, const void* positions,
+                                     const void* dyq, const void* dyk, void* dq, void* dk,
+                                     void* dqw, void* dkw, const int64_t* geom, double eps,
+                                     int interleaved, int pos64, int dtype, void* workspace,
+                                     int64_t workspace_bytes, void* stream);
+
+/* Writes the keys and values of the tokens at `positions` to the cache. 8-bit
+ * rows: scale = max(max|x|, 2^-40) / Q in fp32 (Q = 127, or 448 for e4m3),
+ * code = x / scale rounded half to even. (hq, rot and table_rows unused.) */
+WIDEK_API int widek_cache_write_fwd(const void* k, const void* v, const void* positions, void* kc,
+                                    void* vc, float* ks, float* vs, const void* table,
+                                    const int64_t* geom, const int64_t* cgeom, int pos64, int fmt,
+                                    int dtype, void* stream);
+
+/* Reads the tokens at `positions` back: k, v [n, b, t, hk, d] dense of
+ * `dtype`, code * scale rounded once; zeros at padding. */
+WIDEK_API int widek_cache_read_fwd(const void* kc, const void* vc, const float* ks,
+                                   const float* vs, const void* table, const void* positions,
+                                   void* k, void* v, const int64_t* geom, const int64_t* cgeom,
+                                   int pos64, int fmt, int dtype, void* stream);
+
+/* Workspace bytes widek_decode_attention_fwd needs (-1 for bad arguments). */
+WIDEK_API int64_t widek_decode_attention_workspace(const int64_t* geom, const int64_t* cgeom,
+                                                   int64_t window);
+
+/* Attention of one new token of every sequence over its cache: query head h
+ * reads key head h / (hq / hk), softmax(scale * q k^T) v over the tokens p
+ * with max(0, len - window) <= p < len (window 0: all); zeros where none is.
+ *   q [n, b, hq, d] strided, out [n, b, hq, d] dense, lengths int32 (int64
+ *   with len64 = 1).
+ *   geom, 10 int64: n, b, hq, hk, d, strides of q (model, sequence, head),
+ *   strides of lengths (model, sequence). */
+WIDEK_API int widek_decode_attention_fwd(const void* q, const void* kc, const void* vc,
+                                         const float* ks, const float* vs, const void* table,
+                                         const void* lengths, void* out, const int64_t* geom,
+                                         const int64_t* cgeom, double scale, int64_t window,
+                                         int len64, int fmt, int dtype, void* workspace,
+                                         int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,816 @@
+// Row kernels of decoder attention: RMS norm of every query and key head with
+// the position rotation, the paged cache's write and read, and the gradients
+// of the norm + rotation.
+//
+// A row is one head of one token: D channels, D <= 256.
+//   norm      u = x r w, r = 1 / sqrt(mean(x^2) + eps), w per (model, channel)
+//   rotation  each pair (a, b) of the first R channels, turned by the angle of
+//             its position: y_a = u_a cos - u_b sin, y_b = u_b cos + u_a sin.
+//             Pairs are (i, i + R/2), or (2i, 2i + 1) when interleaved.
+//   gradient  du = dy turned back, dw = sum over rows of du x r, g = du w,
+//             dx = r (g - x r^2 mean(g x))
+// A row whose position is negative is padding: zeros out, nothing written,
+// zero gradient. A position outside the table or the cache records an index
+// error and does the same.
+//
+// Mapping: a power of two of lanes share a row and each lane holds both
+// members of its pairs (vector A at u VEC and vector B at u VEC + R/2; one
+// after the other for the interleaved order, the channels past R and rows
+// without a rotation), so that the rotation needs no exchange between lanes
+// and the norm one reduction. Every channel is read once and written once,
+// in 16-byte vectors where sizes and strides allow it. All of it is bound by
+// memory: 2 D bytes in and out per row of a 16-bit type against ~10 flops a
+// channel.
+#include "paged_cache.cuh"
+
+#include <initializer_list>
+
+namespace widek {
+
+int cache_args(PagedCache& c, const char* what, void* k, void* v, float* ks, float* vs, const void* table,
+               const int64_t* cgeom, int64_t calls, int64_t hk, int64_t d, int fmt, int dtype) {
+    if (!cgeom) return set_error(WIDEK_ERR_INVALID, "%s: null cache geometry", what);
+    const int64_t pages = cgeom[0], page = cgeom[1], cols = cgeom[2];
+    if (pages < 0 || page < 1 || cols < 0)
+        return set_error(WIDEK_ERR_INVALID, "%s: bad cache sizes pages=%lld page=%lld columns=%lld", what,
+                         (long long)pages, (long long)page, (long long)cols);
+    if (!cache_fmt_8bit(fmt) && fmt != dtype)
+        return set_error(WIDEK_ERR_INVALID, "%s: the cache's type %d is neither 8-bit nor the tensors' type %d", what,
+                         fmt, dtype);
+    if (page > 0x7fffffff || cols > 0x7fffffff || (hk > 0 && pages > 0x7fffffff / hk / page))
+        return set_error(WIDEK_ERR_INVALID, "%s: one model's pool holds over 2^31 rows (pages=%lld, heads=%lld, "
+                         "page=%lld)", what, (long long)pages, (long long)hk, (long long)page);
+    if (cols * page > 0x7fffffff)
+        return set_error(WIDEK_ERR_INVALID, "%s: a sequence spans over 2^31 tokens", what);
+    if (calls > 0 && hk > 0 && d > 0 && pages > 0 && cols > 0 && (!k || !v || !table || (cache_fmt_8bit(fmt) && (!ks || !vs))))
+        return set_error(WIDEK_ERR_INVALID, "%s: null cache pointer", what);
+    c = PagedCache{k, v, ks, vs, static_cast<const int*>(table), cgeom[3], cgeom[4], (int)pages, (int)page, (int)cols,
+                   FastDiv::make((uint32_t)page)};
+    return WIDEK_OK;
+}
+
+namespace {
+
+constexpr int kThreads = 256;
+
+struct Strides {
+    int64_t n, b, t, h;
+};
+
+struct RowArgs {
+    const void *q, *k, *v, *qw, *kw;
+    const float *cs, *sn;
+    const void* pos;
+    void *yq, *yk, *yv;
+    Strides sq, sk, sv;
+    int64_t pos_n, pos_b, pos_t;
+    int pos64, n, b, t, hq, hk, d, rot, table_rows, inter, lanes_log2;
+    uint32_t rows;
+    float eps;
+    FastDiv heads, tdiv, bdiv;
+    PagedCache c;
+    int* err;
+};
+
+// VEC consecutive elements of T as one load / store.
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+    T v[VEC];
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T* p, float* out) {
+    const Pack<T, VEC> r = *reinterpret_cast<const Pack<T, VEC>*>(p);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) out[i] = to_f<T>(r.v[i]);
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T* p, const float* in) {
+    Pack<T, VEC> r;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) r.v[i] = from_f<T>(in[i]);
+    *reinterpret_cast<Pack<T, VEC>*>(p) = r;
+}
+
+// VEC floats of a cos / sin row (16-byte loads at most).
+template <int VEC>
+__device__ __forceinline__ void load_table(const float* p, float* out) {
+    constexpr int W = VEC < 4 ? VEC : 4;
+#pragma unroll
+    for (int i = 0; i < VEC; i += W) load_vec<float, W>(p + i, out + i);
+}
+
+// The lanes of this thread's row. A warp's rows may be of different kinds, so
+// each row reduces among its own lanes, which always arrive together.
+__device__ __forceinline__ unsigned group_mask(int lanes) {
+    return lanes == 32 ? 0xffffffffu : ((1u << lanes) - 1u) << (threadIdx.x & 31 & ~(lanes - 1));
+}
+
+__device__ __forceinline__ float group_sum(float v, int lanes, unsigned mask) {
+    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
+    return v;
+}
+
+// The larger of two magnitudes, NaN if either is (fmaxf would drop it).
+__device__ __forceinline__ float amax2(float x, float y) { return (x != x || y != y) ? x + y : fmaxf(x, y); }
+
+// Channels of unit u (first elements of its vectors A and B). Units below
+// `turned` hold pairs of the rotation.
+template <int VEC>
+__device__ __forceinline__ void unit_channels(int u, int turned, int rot, int inter, int& a, int& b) {
+    if (!inter && u < turned) {
+        a = u * VEC;
+        b = a + rot / 2;
+    } else {
+        a = 2 * u * VEC;
+        b = a + VEC;
+    }
+}
+
+// Turns the pairs of one unit by (co, si); SIGN -1 turns back.
+template <int VEC>
+__device__ __forceinline__ void turn(float* a, float* b, const float* co, const float* si, int inter, float sign) {
+    if (!inter || VEC == 1) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const float s = si[j] * sign, x = a[j], y = b[j];
+            a[j] = x * co[j] - y * s;
+            b[j] = y * co[j] + x * s;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j + 1 < VEC; j += 2) {
+            const float s0 = si[j / 2] * sign, x0 = a[j], y0 = a[j + 1], c0 = co[j / 2];
+            a[j] = x0 * c0 - y0 * s0;
+            a[j + 1] = y0 * c0 + x0 * s0;
+            const int i = VEC / 2 + j / 2;
+            const float s1 = si[i] * sign, x1 = b[j], y1 = b[j + 1], c1 = co[i];
+            b[j] = x1 * c1 - y1 * s1;
+            b[j + 1] = y1 * c1 + x1 * s1;
+        }
+    }
+}
+
+enum RowOut : int { OUT_DENSE = 0, OUT_SAME = 1, OUT_I8 = 2, OUT_E4M3 = 3 };
+
+// One vector of a cache row in the cache's format.
+template <typename T, int VEC, int OUT>
+__device__ __forceinline__ void store_code(void* base, int64_t at, const float* x, float scale) {
+    if constexpr (OUT == OUT_I8 || OUT == OUT_E4M3) {
+        Pack<uint8_t, VEC> p;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) p.v[j] = OUT == OUT_I8 ? code_i8(x[j], scale) : code_e4m3(x[j], scale);
+        *reinterpret_cast<Pack<uint8_t, VEC>*>(static_cast<uint8_t*>(base) + at) = p;
+    } else {
+        store_vec<T, VEC>(static_cast<T*>(base) + at, x);
+    }
+}
+
+// Rows in: q heads (normed, rotated, dense out), k heads (the same, dense out
+// or into the cache), v heads (into the cache). ROPE false: k and v heads go
+// to the cache as they are.
+template <typename T, int VEC, int UPL, int OUT, bool ROPE>
+__global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ RowArgs a) {
+    const int lanes = 1 << a.lanes_log2;
+    const int lane = threadIdx.x & (lanes - 1);
+    const unsigned mask = group_mask(lanes);
+    uint32_t row = blockIdx.x * (kThreads >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2);
+    const bool live = row < a.rows;
+    if (!live) row = a.rows - 1;
+    uint32_t hh, t, b;
+    const uint32_t tok = a.heads.divmod(row, hh);
+    const uint32_t nb = a.tdiv.divmod(tok, t);
+    const uint32_t i = a.bdiv.divmod(nb, b);
+    const bool is_q = (int)hh < a.hq;
+    const bool is_v = (int)hh >= a.hq + a.hk;
+    const int h = is_q ? (int)hh : (is_v ? (int)hh - a.hq - a.hk : (int)hh - a.hq);
+    const Strides st = is_q ? a.sq : (is_v ? a.sv : a.sk);
+    const T* src = static_cast<const T*>(is_q ? a.q : (is_v ? a.v : a.k)) + i * st.n + b * st.b + t * st.t + h * st.h;
+    const int pos = load_index(a.pos, i * a.pos_n + b * a.pos_b + t * a.pos_t, a.pos64);
+
+    const int turned = ROPE ? a.rot / 2 / VEC : 0;
+    float xa[UPL][VEC], xb[UPL][VEC];
+#pragma unroll
+    for (int s = 0; s < UPL; ++s) {
+        int ca, cb;
+        unit_channels<VEC>(lane + s * lanes, turned, a.rot, a.inter, ca, cb);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) xa[s][j] = xb[s][j] = 0.f;
+        if (ca < a.d) load_vec<T, VEC>(src + ca, xa[s]);
+        if (cb < a.d) load_vec<T, VEC>(src + cb, xb[s]);
+    }
+
+    bool keep = pos >= 0;
+    if (ROPE && !is_v) {
+        if (pos >= a.table_rows) {
+            keep = false;
+            if (live && lane == 0) raise_device_error(a.err, DEV_ERR_INDEX);
+        }
+        float ss = 0.f;
+#pragma unroll
+        for (int s = 0; s < UPL; ++s)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) ss += xa[s][j] * xa[s][j] + xb[s][j] * xb[s][j];
+        const float r = rsqrtf(group_sum(ss, lanes, mask) / (float)a.d + a.eps);
+        const T* w = static_cast<const T*>(is_q ? a.qw : a.kw) + (int64_t)i * a.d;
+        const int64_t trow = (int64_t)(keep ? pos : 0) * (a.rot / 2);
+#pragma unroll
+        for (int s = 0; s < UPL; ++s) {
+            const int u = lane + s * lanes;
+            int ca, cb;
+            unit_channels<VEC>(u, turned, a.rot, a.inter, ca, cb);
+            float wv[VEC];
+            if (ca < a.d) {
+                load_vec<T, VEC>(w + ca, wv);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) xa[s][j] *= r * wv[j];
+            }
+            if (cb < a.d) {
+                load_vec<T, VEC>(w + cb, wv);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) xb[s][j] *= r * wv[j];
+            }
+            if (u < turned && keep) {
+                float co[VEC], si[VEC];
+                load_table<VEC>(a.cs + trow + u * VEC, co);
+                load_table<VEC>(a.sn + trow + u * VEC, si);
+                turn<VEC>(xa[s], xb[s], co, si, a.inter, 1.f);
+            }
+        }
+    }
+
+    if (is_q || OUT == OUT_DENSE) {
+        T* y = static_cast<T*>(is_q ? a.yq : a.yk) + ((int64_t)tok * (is_q ? a.hq : a.hk) + h) * a.d;
+        if (!live) return;
+#pragma unroll
+        for (int s = 0; s < UPL; ++s) {
+            int ca, cb;
+            unit_channels<VEC>(lane + s * lanes, turned, a.rot, a.inter, ca, cb);
+            if (!keep) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) xa[s][j] = xb[s][j] = 0.f;
+            }
+            if (ca < a.d) store_vec<T, VEC>(y + ca, xa[s]);
+            if (cb < a.d) store_vec<T, VEC>(y + cb, xb[s]);
+        }
+        return;
+    }
+    if constexpr (OUT != OUT_DENSE) {
+        float scale = 1.f;
+        if constexpr (OUT == OUT_I8 || OUT == OUT_E4M3) {
+            float m = 0.f;
+#pragma unroll
+            for (int s = 0; s < UPL; ++s)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) m = amax2(m, amax2(fabsf(xa[s][j]), fabsf(xb[s][j])));
+            for (int o = lanes >> 1; o > 0; o >>= 1) m = amax2(m, __shfl_xor_sync(mask, m, o));
+            scale = code_scale(m, OUT == OUT_I8);
+        }
+        if (!live || !keep) return;
+        const int slot = a.c.row(i, b, a.hk, h, pos);
+        if (slot < 0) {
+            if (lane == 0) raise_device_error(a.err, DEV_ERR_INDEX);
+            return;
+        }
+        const int64_t at = (int64_t)i * a.c.pages * a.hk * a.c.page + slot;
+        void* base = is_v ? a.c.v : a.c.k;
+        if constexpr (OUT == OUT_I8 || OUT == OUT_E4M3) {
+            if (lane == 0) (is_v ? a.c.vs : a.c.ks)[at] = scale;
+        }
+#pragma unroll
+        for (int s = 0; s < UPL; ++s) {
+            int ca, cb;
+            unit_channels<VEC>(lane + s * lanes, turned, a.rot, a.inter, ca, cb);
+            if (ca < a.d) store_code<T, VEC, OUT>(base, at * a.d + ca, xa[s], scale);
+            if (cb < a.d) store_code<T, VEC, OUT>(base, at * a.d + cb, xb[s], scale);
+        }
+    }
+}
+
+// Cache rows out: value = code * scale, rounded once to T; k and v heads of
+// the tokens at `pos`, zeros for padding.
+template <typename T, int VEC, int UPL, int IN>
+__global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_constant__ RowArgs a) {
+    const int lanes = 1 << a.lanes_log2;
+    const int lane = threadIdx.x & (lanes - 1);
+    const uint32_t row = blockIdx.x * (kThreads >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2);
+    if (row >= a.rows) return;
+    uint32_t hh, t, b;
+    const uint32_t tok = a.heads.divmod(row, hh);
+    const uint32_t nb = a.tdiv.divmod(tok, t);
+    const uint32_t i = a.bdiv.divmod(nb, b);
+    const bool is_v = (int)hh >= a.hk;
+    const int h = is_v ? (int)hh - a.hk : (int)hh;
+    const int pos = load_index(a.pos, i * a.pos_n + b * a.pos_b + t * a.pos_t, a.pos64);
+    const int slot = pos < 0 ? -1 : a.c.row(i, b, a.hk, h, pos);
+    if (pos >= 0 && slot < 0 && lane == 0) raise_device_error(a.err, DEV_ERR_INDEX);
+    const int64_t at = (int64_t)i * a.c.pages * a.hk * a.c.page + (slot < 0 ? 0 : slot);
+    const void* base = is_v ? a.c.v : a.c.k;
+    float scale = 1.f;
+    if constexpr (IN == OUT_I8 || IN == OUT_E4M3) {
+        if (slot >= 0) scale = (is_v ? a.c.vs : a.c.ks)[at];
+    }
+    T* y = static_cast<T*>(is_v ? a.yv : a.yk) + ((int64_t)tok * a.hk + h) * a.d;
+#pragma unroll
+    for (int s = 0; s < 2 * UPL; ++s) {
+        const int c = (lane + s * lanes) * VEC;
+        if (c >= a.d) continue;
+        float x[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) x[j] = 0.f;
+        if (slot >= 0) {
+            if constexpr (IN == OUT_I8 || IN == OUT_E4M3) {
+                const Pack<uint8_t, VEC> p =
+                    *reinterpret_cast<const Pack<uint8_t, VEC>*>(static_cast<const uint8_t*>(base) + at * a.d + c);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    x[j] = (IN == OUT_I8 ? (float)(int8_t)p.v[j] : value_e4m3(p.v[j])) * scale;
+            } else {
+                load_vec<T, VEC>(static_cast<const T*>(base) + at * a.d + c, x);
+            }
+        }
+        store_vec<T, VEC>(y + c, x);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Gradients of the norm + rotation
+// ---------------------------------------------------------------------------
+struct GradArgs {
+    RowArgs r;                  // q, k, weights, tables, positions as in the forward; yq / yk = dq / dk
+    const void *dyq, *dyk;      // dense
+    float* part;                // [n, chunks, d] fp32: one row of partial weight gradients per block
+    void *dqw, *dkw;            // [n, d], nullable
+    int cq, ck;                 // blocks per model for the q rows and the k rows
+    uint32_t per_q, per_k;      // rows of one block
+    FastDiv hq_div, hk_div;
+};
+
+// A block takes consecutive rows of one model's q (or k) heads, and each of
+// its groups of lanes every 256/lanes-th of them, keeping the weight gradient
+// of its channels in registers; groups, warps and blocks are joined in a
+// fixed order, so the sums do not depend on timing.
+template <typename T, int VEC, int UPL>
+__global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const __grid_constant__ GradArgs g) {
+    const RowArgs& a = g.r;
+    __shared__ float red[kThreads / 32][256];
+    const int lanes = 1 << a.lanes_log2;
+    const int lane = threadIdx.x & (lanes - 1);
+    const unsigned mask = group_mask(lanes);
+    const int groups = kThreads >> a.lanes_log2;
+    const int chunks = g.cq + g.ck;
+    const int i = blockIdx.x / chunks;
+    const int chunk = blockIdx.x - i * chunks;
+    const bool is_q = chunk < g.cq;
+    const uint32_t heads = is_q ? a.hq : a.hk;
+    const uint32_t all = (uint32_t)a.b * a.t * heads;
+    const uint32_t per = is_q ? g.per_q : g.per_k;
+    const uint32_t first = (is_q ? chunk : chunk - g.cq) * per;
+    const uint32_t last = min(all, first + per);
+    const FastDiv hd = is_q ? g.hq_div : g.hk_div;
+    const Strides st = is_q ? a.sq : a.sk;
+    const T* x0 = static_cast<const T*>(is_q ? a.q : a.k) + (int64_t)i * st.n;
+    const int64_t dense0 = (int64_t)i * all;
+    const T* dy0 = static_cast<const T*>(is_q ? g.dyq : g.dyk);
+    T* dx0 = static_cast<T*>(is_q ? a.yq : a.yk);
+    const T* w = static_cast<const T*>(is_q ? a.qw : a.kw) + (int64_t)i * a.d;
+    const int turned = a.rot / 2 / VEC;
+
+    int ca[UPL], cb[UPL];
+    float wa[UPL][VEC], wb[UPL][VEC], da[UPL][VEC], db[UPL][VEC];
+#pragma unroll
+    for (int s = 0; s < UPL; ++s) {
+        unit_channels<VEC>(lane + s * lanes, turned, a.rot, a.inter, ca[s], cb[s]);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) wa[s][j] = wb[s][j] = da[s][j] = db[s][j] = 0.f;
+        if (ca[s] < a.d) load_vec<T, VEC>(w + ca[s], wa[s]);
+        if (cb[s] < a.d) load_vec<T, VEC>(w + cb[s], wb[s]);
+    }
+    const float inv_d = 1.f / (float)a.d;
+    for (uint32_t base = first; base < last; base += groups) {
+        uint32_t row = base + (threadIdx.x >> a.lanes_log2);
+        const bool live = row < last;
+        if (!live) row = last - 1;
+        uint32_t h, t;
+        const uint32_t bt = hd.divmod(row, h);
+        const uint32_t b = a.tdiv.divmod(bt, t);
+        const int pos = load_index(a.pos, i * a.pos_n + b * a.pos_b + t * a.pos_t, a.pos64);
+        const bool keep = pos >= 0 && pos < a.table_rows;
+        const T* x = x0 + b * st.b + t * st.t + h * st.h;
+        const T* dy = dy0 + (dense0 + row) * a.d;
+        T* dx = dx0 + (dense0 + row) * a.d;
+        float xa[UPL][VEC], xb[UPL][VEC], ga[UPL][VEC], gb[UPL][VEC];
+#pragma unroll
+        for (int s = 0; s < UPL; ++s) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) xa[s][j] = xb[s][j] = ga[s][j] = gb[s][j] = 0.f;
+            if (ca[s] < a.d) {
+                load_vec<T, VEC>(x + ca[s], xa[s]);
+                load_vec<T, VEC>(dy + ca[s], ga[s]);
+            }
+            if (cb[s] < a.d) {
+                load_vec<T, VEC>(x + cb[s], xb[s]);
+                load_vec<T, VEC>(dy + cb[s], gb[s]);
+            }
+        }
+        const int64_t trow = (int64_t)(keep ? pos : 0) * (a.rot / 2);
+        float ss = 0.f;
+#pragma unroll
+        for (int s = 0; s < UPL; ++s) {
+            const int u = lane + s * lanes;
+            if (u < turned && keep) {
+                float co[VEC], si[VEC];
+                load_table<VEC>(a.cs + trow + u * VEC, co);
+                load_table<VEC>(a.sn + trow + u * VEC, si);
+                turn<VEC>(ga[s], gb[s], co, si, a.inter, -1.f);
+            }
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) ss += xa[s][j] * xa[s][j] + xb[s][j] * xb[s][j];
+        }
+        const float r = rsqrtf(group_sum(ss, lanes, mask) * inv_d + a.eps);
+        // padding rows add nothing, not even a NaN that they hold
+        float gx = 0.f;
+#pragma unroll
+        for (int s = 0; s < UPL; ++s)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                if (live && keep) {
+                    da[s][j] += ga[s][j] * xa[s][j] * r;
+                    db[s][j] += gb[s][j] * xb[s][j] * r;
+                }
+                ga[s][j] *= wa[s][j];
+                gb[s][j] *= wb[s][j];
+                gx += ga[s][j] * xa[s][j] + gb[s][j] * xb[s][j];
+            }
+        const float m = group_sum(gx, lanes, mask) * inv_d * r * r;
+        if (live) {
+#pragma unroll
+            for (int s = 0; s < UPL; ++s) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    ga[s][j] = keep ? r * (ga[s][j] - xa[s][j] * m) : 0.f;
+                    gb[s][j] = keep ? r * (gb[s][j] - xb[s][j] * m) : 0.f;
+                }
+                if (ca[s] < a.d) store_vec<T, VEC>(dx + ca[s], ga[s]);
+                if (cb[s] < a.d) store_vec<T, VEC>(dx + cb[s], gb[s]);
+            }
+        }
+    }
+    // groups of a warp, then the warps
+#pragma unroll
+    for (int s = 0; s < UPL; ++s)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            for (int o = lanes; o < 32; o <<= 1) {
+                da[s][j] += __shfl_xor_sync(0xffffffffu, da[s][j], o);
+                db[s][j] += __shfl_xor_sync(0xffffffffu, db[s][j], o);
+            }
+    if ((threadIdx.x & 31) < lanes) {
+#pragma unroll
+        for (int s = 0; s < UPL; ++s)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                if (ca[s] < a.d) red[threadIdx.x >> 5][ca[s] + j] = da[s][j];
+                if (cb[s] < a.d) red[threadIdx.x >> 5][cb[s] + j] = db[s][j];
+            }
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < a.d) {
+        float sum = 0.f;
+#pragma unroll
+        for (int wp = 0; wp < kThreads / 32; ++wp) sum += red[wp][threadIdx.x];
+        g.part[(int64_t)blockIdx.x * a.d + threadIdx.x] = sum;
+    }
+}
+
+// Weight gradients: the blocks' partial rows of one model and side, in order.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) rope_bwd_join_kernel(const float* part, T* dqw, T* dkw, int cq, int ck,
+                                                                 int d) {
+    __shared__ float red[kThreads / 32][33];
+    const int i = blockIdx.x >> 1;
+    const bool is_q = (blockIdx.x & 1) == 0;
+    T* out = is_q ? dqw : dkw;
+    const int c = blockIdx.y * 32 + (threadIdx.x & 31);
+    const float* p = part + ((int64_t)i * (cq + ck) + (is_q ? 0 : cq)) * d;
+    float sum = 0.f;
+    if (c < d)
+        for (int r = threadIdx.x >> 5; r < (is_q ? cq : ck); r += kThreads / 32) sum += p[(int64_t)r * d + c];
+    red[threadIdx.x >> 5][threadIdx.x & 31] = sum;
+    __syncthreads();
+    if (threadIdx.x < 32 && c < d && out) {
+        sum = 0.f;
+#pragma unroll
+        for (int wp = 0; wp < kThreads / 32; ++wp) sum += red[wp][threadIdx.x];
+        out[(int64_t)i * d + c] = from_f<T>(sum);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+inline bool strides_fit(const Strides& s, int vec) {
+    return s.n % vec == 0 && s.b % vec == 0 && s.t % vec == 0 && s.h % vec == 0;
+}
+
+// Widest vector (elements) that every row address allows: 16 bytes, else 2
+// elements, else 1. The halves of a rotation have to start on one too.
+int row_vec(const RowArgs& a, size_t esz, std::initializer_list<const void*> dense, bool cache_same) {
+    for (int vec : {(int)(16 / esz), 2}) {
+        bool ok = a.d % vec == 0 && (a.rot / 2) % vec == 0;
+        ok = ok && (!a.q || (aligned_to(a.q, vec * esz) && strides_fit(a.sq, vec)));
+        ok = ok && (!a.k || (aligned_to(a.k, vec * esz) && strides_fit(a.sk, vec)));
+        ok = ok && (!a.v || (aligned_to(a.v, vec * esz) && strides_fit(a.sv, vec)));
+        for (const void* p : dense) ok = ok && (!p || aligned_to(p, vec * esz));
+        for (const void* p : {(const void*)a.cs, (const void*)a.sn}) ok = ok && (!p || aligned_to(p, vec < 4 ? 4 * vec : 16));
+        for (const void* p : {(const void*)a.c.k, (const void*)a.c.v})
+            ok = ok && (!p || aligned_to(p, cache_same ? vec * esz : vec));
+        if (ok) return vec;
+    }
+    return 1;
+}
+
+int lanes_log2(int d, int vec) {
+    const int units = ((d + vec - 1) / vec + 1) / 2;
+    int l = 0;
+    while ((1 << l) < units && l < 5) ++l;
+    return l;
+}
+
+// geom: n, b, t, hq, hk, d, rot, table rows, strides (n, b, t, head) of q, k
+// and v, strides (n, b, t) of the positions.
+int row_args(RowArgs& a, const char* what, const int64_t* g, int pos64) {
+    if (!g) return set_error(WIDEK_ERR_INVALID, "%s: null geometry", what);
+    for (int i = 0; i < 8; ++i)
+        if (g[i] < 0 || g[i] > 0x7fffffff)
+            return set_error(WIDEK_ERR_INVALID, "%s: size %d out of range (%lld)", what, i, (long long)g[i]);
+    if (g[5] > 256) return set_error(WIDEK_ERR_UNSUPPORTED, "%s: head size %lld above 256", what, (long long)g[5]);
+    if (g[6] > g[5] || g[6] % 2 != 0)
+        return set_error(WIDEK_ERR_INVALID, "%s: %lld rotated channels of %lld (an even number of at most the head)",
+                         what, (long long)g[6], (long long)g[5]);
+    a = RowArgs{};
+    a.n = (int)g[0], a.b = (int)g[1], a.t = (int)g[2], a.hq = (int)g[3], a.hk = (int)g[4], a.d = (int)g[5];
+    a.rot = (int)g[6], a.table_rows = (int)g[7];
+    a.sq = Strides{g[8], g[9], g[10], g[11]};
+    a.sk = Strides{g[12], g[13], g[14], g[15]};
+    a.sv = Strides{g[16], g[17], g[18], g[19]};
+    a.pos_n = g[20], a.pos_b = g[21], a.pos_t = g[22];
+    a.pos64 = pos64;
+    a.err = device_error_ptr();
+    return WIDEK_OK;
+}
+
+int row_count(RowArgs& a, const char* what, int64_t heads) {
+    const double rows = (double)a.n * a.b * a.t * (double)heads;
+    if (rows > 2147483647.0)
+        return set_error(WIDEK_ERR_INVALID, "%s: over 2^31 rows (%.0f)", what, rows);
+    a.rows = (uint32_t)rows;
+    if (a.rows == 0) return WIDEK_OK;
+    a.heads = FastDiv::make((uint32_t)heads);
+    a.tdiv = FastDiv::make((uint32_t)a.t);
+    a.bdiv = FastDiv::make((uint32_t)a.b);
+    return WIDEK_OK;
+}
+
+template <int OUT, bool ROPE>
+struct RowLaunch {
+    RowArgs a;
+    int vec;
+    const char* what;
+    cudaStream_t st;
+    template <typename T>
+    int run() {
+        constexpr int W = 16 / sizeof(T);
+        a.lanes_log2 = lanes_log2(a.d, vec);
+        const uint32_t per = kThreads >> a.lanes_log2;
+        const unsigned blocks = (a.rows + per - 1) / per;
+        if (vec == W) rows_kernel<T, W, 1, OUT, ROPE><<<blocks, kThreads, 0, st>>>(a);
+        else if (vec == 2) rows_kernel<T, 2, 2, OUT, ROPE><<<blocks, kThreads, 0, st>>>(a);
+        else rows_kernel<T, 1, 4, OUT, ROPE><<<blocks, kThreads, 0, st>>>(a);
+        return check_launch(what);
+    }
+};
+
+template <int IN>
+struct ReadLaunch {
+    RowArgs a;
+    int vec;
+    cudaStream_t st;
+    template <typename T>
+    int run() {
+        constexpr int W = 16 / sizeof(T);
+        a.lanes_log2 = lanes_log2(a.d, vec);
+        const uint32_t per = kThreads >> a.lanes_log2;
+        const unsigned blocks = (a.rows + per - 1) / per;
+        if (vec == W) cache_read_kernel<T, W, 1, IN><<<blocks, kThreads, 0, st>>>(a);
+        else if (vec == 2) cache_read_kernel<T, 2, 2, IN><<<blocks, kThreads, 0, st>>>(a);
+        else cache_read_kernel<T, 1, 4, IN><<<blocks, kThreads, 0, st>>>(a);
+        return check_launch("widek_cache_read_fwd");
+    }
+};
+
+template <int OUT, bool ROPE>
+int launch_rows(const RowArgs& a, int vec, const char* what, int dtype, cudaStream_t st) {
+    RowLaunch<OUT, ROPE> L{a, vec, what, st};
+    return dispatch_dtype(dtype, L);
+}
+
+template <bool ROPE>
+int launch_rows_fmt(const RowArgs& a, int vec, const char* what, int fmt, int dtype, cudaStream_t st) {
+    if (fmt == WIDEK_I8) return launch_rows<OUT_I8, ROPE>(a, vec, what, dtype, st);
+    if (fmt == WIDEK_E4M3) return launch_rows<OUT_E4M3, ROPE>(a, vec, what, dtype, st);
+    return launch_rows<OUT_SAME, ROPE>(a, vec, what, dtype, st);
+}
+
+// Blocks per model of the backward: about three blocks for each SM over all
+// models and both sides, none with fewer rows than its groups of lanes.
+void grad_chunks(const RowArgs& a, int vec, int& cq, int& ck, uint32_t& per_q, uint32_t& per_k) {
+    const int groups = kThreads >> lanes_log2(a.d, vec);
+    const int64_t tokens = (int64_t)a.b * a.t;
+    auto split = [&](int64_t heads, int& c, uint32_t& per) {
+        const int64_t rows = tokens * heads;
+        int64_t want = (int64_t)444 * heads / ((int64_t)a.n * (a.hq + a.hk));
+        const int64_t most = (rows + groups - 1) / groups;
+        want = want < 1 ? 1 : (want > most ? most : want);
+        per = (uint32_t)(((rows + want - 1) / want + groups - 1) / groups * groups);
+        c = (int)((rows + per - 1) / per);
+    };
+    split(a.hq, cq, per_q);
+    split(a.hk, ck, per_k);
+}
+
+struct GradLaunch {
+    GradArgs g;
+    int vec;
+    cudaStream_t st;
+    template <typename T>
+    int run() {
+        constexpr int W = 16 / sizeof(T);
+        g.r.lanes_log2 = lanes_log2(g.r.d, vec);
+        const unsigned blocks = (unsigned)g.r.n * (g.cq + g.ck);
+        if (vec == W) rope_bwd_kernel<T, W, 1><<<blocks, kThreads, 0, st>>>(g);
+        else if (vec == 2) rope_bwd_kernel<T, 2, 2><<<blocks, kThreads, 0, st>>>(g);
+        else rope_bwd_kernel<T, 1, 4><<<blocks, kThreads, 0, st>>>(g);
+        int rc = check_launch("widek_qk_norm_rope_bwd");
+        if (rc != WIDEK_OK || (!g.dqw && !g.dkw)) return rc;
+        const dim3 grid(2 * g.r.n, (g.r.d + 31) / 32);
+        rope_bwd_join_kernel<T><<<grid, kThreads, 0, st>>>(g.part, static_cast<T*>(g.dqw), static_cast<T*>(g.dkw), g.cq,
+                                                           g.ck, g.r.d);
+        return check_launch("widek_qk_norm_rope_bwd (join)");
+    }
+};
+
+int rope_pointers(const RowArgs& a, const char* what) {
+    if (a.hq < 1 || a.hk < 1) return set_error(WIDEK_ERR_INVALID, "%s: no heads (hq=%d, hk=%d)", what, a.hq, a.hk);
+    if (a.rows > 0 && a.d > 0 &&
+        (!a.q || !a.k || !a.qw || !a.kw || !a.pos || !a.yq || (a.rot > 0 && a.table_rows > 0 && (!a.cs || !a.sn))))
+        return set_error(WIDEK_ERR_INVALID, "%s: null pointer", what);
+    return WIDEK_OK;
+}
+
+}  // namespace
+}  // namespace widek
+
+using namespace widek;
+
+extern "C" int widek_qk_norm_rope_fwd(const void* q, const void* k, const void* qw, const void* kw, const float* cos,
+                                      const float* sin, const void* positions, void* yq, void* yk,
+                                      const int64_t* geom, double eps, int interleaved, int pos64, int dtype,
+                                      void* stream) {
+    const char* what = "widek_qk_norm_rope_fwd";
+    RowArgs a;
+    int rc = row_args(a, what, geom, pos64);
+    if (rc != WIDEK_OK) return rc;
+    rc = row_count(a, what, (int64_t)a.hq + a.hk);
+    if (rc != WIDEK_OK) return rc;
+    a.q = q, a.k = k, a.qw = qw, a.kw = kw, a.cs = cos, a.sn = sin, a.pos = positions, a.yq = yq, a.yk = yk;
+    a.eps = (float)eps, a.inter = interleaved;
+    rc = rope_pointers(a, what);
+    if (rc != WIDEK_OK) return rc;
+    if (a.rows == 0 || a.d == 0) return WIDEK_OK;
+    if (!yk) return set_error(WIDEK_ERR_INVALID, "%s: null pointer", what);
+    const int vec = row_vec(a, dtype_size(dtype) ? dtype_size(dtype) : 4, {qw, kw, yq, yk}, false);
+    return launch_rows<OUT_DENSE, true>(a, vec, what, dtype, (cudaStream_t)stream);
+}
+
+extern "C" int widek_qk_norm_rope_write_fwd(const void* q, const void* k, const void* v, const void* qw,
+                                            const void* kw, const float* cos, const float* sin, const void* positions,
+                                            void* yq, void* kc, void* vc, float* ks, float* vs, const void* table,
+                                            const int64_t* geom, const int64_t* cgeom, double eps, int interleaved,
+                                            int pos64, int fmt, int dtype, void* stream) {
+    const char* what = "widek_qk_norm_rope_write_fwd";
+    RowArgs a;
+    int rc = row_args(a, what, geom, pos64);
+    if (rc != WIDEK_OK) return rc;
+    rc = row_count(a, what, (int64_t)a.hq + 2 * a.hk);
+    if (rc != WIDEK_OK) return rc;
+    rc = cache_args(a.c, what, kc, vc, ks, vs, table, cgeom, a.rows, a.hk, a.d, fmt, dtype);
+    if (rc != WIDEK_OK) return rc;
+    a.q = q, a.k = k, a.v = v, a.qw = qw, a.kw = kw, a.cs = cos, a.sn = sin, a.pos = positions, a.yq = yq;
+    a.eps = (float)eps, a.inter = interleaved;
+    rc = rope_pointers(a, what);
+    if (rc != WIDEK_OK) return rc;
+    if (a.rows == 0 || a.d == 0) return WIDEK_OK;
+    if (!v) return set_error(WIDEK_ERR_INVALID, "%s: null pointer", what);
+    const int vec = row_vec(a, dtype_size(dtype) ? dtype_size(dtype) : 4, {qw, kw, yq}, !cache_fmt_8bit(fmt));
+    return launch_rows_fmt<true>(a, vec, what, fmt, dtype, (cudaStream_t)stream);
+}
+
+extern "C" int widek_cache_write_fwd(const void* k, const void* v, const void* positions, void* kc, void* vc,
+                                     float* ks, float* vs, const void* table, const int64_t* geom,
+                                     const int64_t* cgeom, int pos64, int fmt, int dtype, void* stream) {
+    const char* what = "widek_cache_write_fwd";
+    RowArgs a;
+    int rc = row_args(a, what, geom, pos64);
+    if (rc != WIDEK_OK) return rc;
+    a.hq = 0, a.rot = 0;
+    rc = row_count(a, what, 2 * (int64_t)a.hk);
+    if (rc != WIDEK_OK) return rc;
+    rc = cache_args(a.c, what, kc, vc, ks, vs, table, cgeom, a.rows, a.hk, a.d, fmt, dtype);
+    if (rc != WIDEK_OK) return rc;
+    if (a.rows == 0 || a.d == 0) return WIDEK_OK;
+    if (!k || !v || !positions) return set_error(WIDEK_ERR_INVALID, "%s: null pointer", what);
+    a.k = k, a.v = v, a.pos = positions;
+    const int vec = row_vec(a, dtype_size(dtype) ? dtype_size(dtype) : 4, {}, !cache_fmt_8bit(fmt));
+    return launch_rows_fmt<false>(a, vec, what, fmt, dtype, (cudaStream_t)stream);
+}
+
+extern "C" int widek_cache_read_fwd(const void* kc, const void* vc, const float* ks, const float* vs,
+                                    const void* table, const void* positions, void* k, void* v, const int64_t* geom,
+                                    const int64_t* cgeom, int pos64, int fmt, int dtype, void* stream) {
+    const char* what = "widek_cache_read_fwd";
+    RowArgs a;
+    int rc = row_args(a, what, geom, pos64);
+    if (rc != WIDEK_OK) return rc;
+    a.hq = 0, a.rot = 0;
+    rc = row_count(a, what, 2 * (int64_t)a.hk);
+    if (rc != WIDEK_OK) return rc;
+    rc = cache_args(a.c, what, const_cast<void*>(kc), const_cast<void*>(vc), const_cast<float*>(ks),
+                    const_cast<float*>(vs), table, cgeom, a.rows, a.hk, a.d, fmt, dtype);
+    if (rc != WIDEK_OK) return rc;
+    if (a.rows == 0 || a.d == 0) return WIDEK_OK;
+    if (!k || !v || !positions) return set_error(WIDEK_ERR_INVALID, "%s: null pointer", what);
+    a.yk = k, a.yv = v, a.pos = positions;
+    const int vec = row_vec(a, dtype_size(dtype) ? dtype_size(dtype) : 4, {k, v}, !cache_fmt_8bit(fmt));
+    cudaStream_t st = (cudaStream_t)stream;
+    if (fmt == WIDEK_I8) {
+        ReadLaunch<OUT_I8> L{a, vec, st};
+        return dispatch_dtype(dtype, L);
+    }
+    if (fmt == WIDEK_E4M3) {
+        ReadLaunch<OUT_E4M3> L{a, vec, st};
+        return dispatch_dtype(dtype, L);
+    }
+    ReadLaunch<OUT_SAME> L{a, vec, st};
+    return dispatch_dtype(dtype, L);
+}
+
+extern "C" int64_t widek_qk_norm_rope_bwd_workspace(const int64_t* geom) {
+    RowArgs a;
+    if (row_args(a, "widek_qk_norm_rope_bwd_workspace", geom, 0) != WIDEK_OK || a.hq < 1 || a.hk < 1) return -1;
+    if (row_count(a, "widek_qk_norm_rope_bwd_workspace", (int64_t)a.hq + a.hk) != WIDEK_OK) return -1;
+    if (a.rows == 0 || a.d == 0) return 0;
+    // the most blocks of any vector width
+    int64_t blocks = 0;
+    for (int vec : {8, 4, 2, 1}) {
+        int cq, ck;
+        uint32_t pq, pk;
+        grad_chunks(a, vec, cq, ck, pq, pk);
+        if (cq + ck > blocks) blocks = cq + ck;
+    }
+    return blocks * a.n * a.d * (int64_t)sizeof(float);
+}
+
+extern "C" int widek_qk_norm_rope_bwd(const void* q, const void* k, const void* qw, const void* kw, const float* cos,
+                                      const float* sin, const void* positions, const void* dyq, const void* dyk,
+                                      void* dq, void* dk, void* dqw, void* dkw, const int64_t* geom, double eps,
+                                      int interleaved, int pos64, int dtype, void* workspace,
+                                      int64_t workspace_bytes, void* stream) {
+    const char* what = "widek_qk_norm_rope_bwd";
+    GradArgs g{};
+    RowArgs& a = g.r;
+    int rc = row_args(a, what, geom, pos64);
+    if (rc != WIDEK_OK) return rc;
+    rc = row_count(a, what, (int64_t)a.hq + a.hk);
+    if (rc != WIDEK_OK) return rc;
+    a.q = q, a.k = k, a.qw = qw, a.kw = kw, a.cs = cos, a.sn = sin, a.pos = positions, a.yq = dq, a.yk = dk;
+    a.eps = (float)eps, a.inter = interleaved;
+    rc = rope_pointers(a, what);
+    if (rc != WIDEK_OK) return rc;
+    if (a.rows == 0 || a.d == 0) return WIDEK_OK;
+    if (!dk || !dyq || !dyk) return set_error(WIDEK_ERR_INVALID, "%s: null pointer", what);
+    const int64_t need = widek_qk_norm_rope_bwd_workspace(geom);
+    if (!workspace || workspace_bytes < need)
+        return set_error(WIDEK_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed", what,
+                         (long long)workspace_bytes, (long long)need);
+    g.dyq = dyq, g.dyk = dyk, g.dqw = dqw, g.dkw = dkw, g.part = static_cast<float*>(workspace);
+    const int vec = row_vec(a, dtype_size(dtype) ? dtype_size(dtype) : 4, {qw, kw, dyq, dyk, dq, dk}, false);
+    grad_chunks(a, vec, g.cq, g.ck, g.per_q, g.per_k);
+    g.hq_div = FastDiv::make((uint32_t)a.hq);
+    g.hk_div = FastDiv::make((uint32_t)a.hk);
+    GradLaunch L{g, vec, (cudaStream_t)stream};
+    return dispatch_dtype(dtype, L);
+}

@@ -18,6 +18,7 @@ from .core.config import WideConfig, get_default_config, set_default_config
 from .core.registry import register, unregister, get_registry, list_registered
 from .core.traced_wide import TracedWideModel, FunctionalOp, BinaryOp, print_trace
 from .core.ensemble_util import pack_inputs, unpack_outputs
+from .core.paged_cache import WidePagedCache
 from .core.primitives import (WideLinear, WideConv1d, WideConv2d, WideConv3d, WideBatchNorm1d, WideBatchNorm2d,
                               WideLayerNorm, WideGroupNorm, WideInstanceNorm1d, WideInstanceNorm2d, WideEmbedding,
                               WideAttention, WideGRU, WideLSTM)
@@ -40,7 +41,7 @@ __all__ = [
     'TracedWideModel', 'FunctionalOp', 'BinaryOp', 'print_trace', 'pack_inputs', 'unpack_outputs',
     'WideLinear', 'WideConv1d', 'WideConv2d', 'WideConv3d', 'WideBatchNorm1d', 'WideBatchNorm2d',
     'WideLayerNorm', 'WideGroupNorm', 'WideInstanceNorm1d', 'WideInstanceNorm2d', 'WideEmbedding',
-    'WideAttention', 'WideGRU', 'WideLSTM',
+    'WideAttention', 'WideGRU', 'WideLSTM', 'WidePagedCache',
     'benchmark_primitive', 'benchmark_multi', 'benchmark_all', 'benchmark_custom', 'list_benchmark_primitives',
     'BenchmarkResult', 'SweepParams',
 ]

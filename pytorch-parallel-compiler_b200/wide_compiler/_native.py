@@ -33,6 +33,7 @@ DEV_ERR_GEMM_TIMEOUT, DEV_ERR_RNN_TIMEOUT, DEV_ERR_ATTN_TIMEOUT = 101, 102, 103
 DEV_ERR_CONV_TIMEOUT, DEV_ERR_NORM_TIMEOUT, DEV_ERR_WAIT_PROBE, DEV_ERR_INDEX = 104, 105, 106, 110
 
 F32, BF16, F16 = 0, 1, 2
+I8, E4M3 = 3, 4                        # cache formats with one fp32 scale per (token, head)
 ACT_NONE, ACT_RELU, ACT_GELU = 0, 1, 2
 
 _DTYPE_CODES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
@@ -104,11 +105,23 @@ SIGNATURES = {
     "widek_act_bwd": [_c_void_p] * 3 + [_i64, _int, _int, _c_void_p],
     "widek_layernorm_bwd_workspace": [_i64] * 3,
     "widek_layernorm_bwd": [_c_void_p] * 6 + [_i64] * 3 + [_dbl, _int, _c_void_p, _i64, _c_void_p],
+    "widek_qk_norm_rope_fwd": [_c_void_p] * 9 + [ctypes.POINTER(_i64), _dbl, _int, _int, _int, _c_void_p],
+    "widek_qk_norm_rope_write_fwd": [_c_void_p] * 14 + [ctypes.POINTER(_i64)] * 2 + [_dbl] + [_int] * 4
+                                    + [_c_void_p],
+    "widek_qk_norm_rope_bwd_workspace": [ctypes.POINTER(_i64)],
+    "widek_qk_norm_rope_bwd": [_c_void_p] * 13 + [ctypes.POINTER(_i64), _dbl, _int, _int, _int, _c_void_p, _i64,
+                                                  _c_void_p],
+    "widek_cache_write_fwd": [_c_void_p] * 8 + [ctypes.POINTER(_i64)] * 2 + [_int] * 3 + [_c_void_p],
+    "widek_cache_read_fwd": [_c_void_p] * 8 + [ctypes.POINTER(_i64)] * 2 + [_int] * 3 + [_c_void_p],
+    "widek_decode_attention_workspace": [ctypes.POINTER(_i64)] * 2 + [_i64],
+    "widek_decode_attention_fwd": [_c_void_p] * 8 + [ctypes.POINTER(_i64)] * 2 + [_dbl, _i64, _int, _int, _int,
+                                                                                  _c_void_p, _i64, _c_void_p],
 }
 RESTYPES = {"widek_batchnorm_train_workspace": ctypes.c_size_t, "widek_conv_workspace": ctypes.c_size_t,
             "widek_rnn_workspace": ctypes.c_size_t, "widek_conv_packed_weight_elems": _i64,
             "widek_launch_count": ctypes.c_longlong, "widek_linear_bwd_workspace": _i64,
-            "widek_layernorm_bwd_workspace": _i64, "widek_groupnorm_bwd_workspace": _i64}
+            "widek_layernorm_bwd_workspace": _i64, "widek_groupnorm_bwd_workspace": _i64,
+            "widek_qk_norm_rope_bwd_workspace": _i64, "widek_decode_attention_workspace": _i64}
 
 
 class WideKernelError(RuntimeError):

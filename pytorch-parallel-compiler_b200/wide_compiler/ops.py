@@ -944,6 +944,261 @@ def attention_dropout(mod, query: Tensor, key: Tensor, value: Tensor, attn_mask:
 
 
 # ---------------------------------------------------------------------------
+# Decoder attention: norm + rotation of queries and keys, the paged
+# key-value cache, attention of one new token
+# ---------------------------------------------------------------------------
+
+_INDEX = (torch.int32, torch.int64)
+
+
+def _row_strides(t: Tensor, what: str):
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{what}: the channels of a head must be dense (stride {t.stride(-1)})")
+    return t.stride()[:-1]
+
+
+def _index_strides(t: Tensor, shape, what: str, name: str):
+    """Strides of an index tensor over ``shape`` = [N, B(, T)]; it may leave
+    out leading dims (shared by the models, or by the sequences)."""
+    if t.dtype not in _INDEX:
+        raise TypeError(f"{what}: {name} must be int32 or int64, got {t.dtype}")
+    lead = len(shape) - t.dim()
+    if lead < 0 or t.dim() < 1 or tuple(t.shape) != tuple(shape[lead:]):
+        raise ValueError(f"{what}: {name} {tuple(t.shape)} is not {list(shape)} or its last dims")
+    return (0,) * lead + t.stride()
+
+
+def _row_geom(what: str, q: Optional[Tensor], k: Tensor, v: Optional[Tensor], positions: Tensor, rot: int = 0,
+              rows: int = 0):
+    """Checks the head tensors and builds the geometry array of the row
+    kernels (include/widek.h)."""
+    if k.dim() != 5 or (v is not None and v.shape != k.shape):
+        raise ValueError(f"{what}: k and v must be [N, B, T, Hk, D], got {tuple(k.shape)}"
+                         + ("" if v is None else f" and {tuple(v.shape)}"))
+    n, b, t, hk, d = k.shape
+    if q is not None and (q.dim() != 5 or q.shape[:3] != k.shape[:3] or q.shape[4] != d):
+        raise ValueError(f"{what}: q {tuple(q.shape)} does not match k {tuple(k.shape)}")
+    sk = _row_strides(k, what)
+    sq = sk if q is None else _row_strides(q, what)
+    sv = sk if v is None else _row_strides(v, what)
+    return (ctypes.c_int64 * 23)(n, b, t, 0 if q is None else q.shape[3], hk, d, rot, rows, *sq, *sk, *sv,
+                                 *_index_strides(positions, (n, b, t), what, "positions"))
+
+
+def _rope_args(what: str, q: Tensor, k: Tensor, v: Optional[Tensor], q_weight: Tensor, k_weight: Tensor, cos: Tensor,
+               sin: Tensor, positions: Tensor):
+    dev = N.require_cuda(q, k, v, q_weight, k_weight, cos, sin, positions, what=what)
+    _same_dtype(what, q, k, v, q_weight, k_weight)
+    if cos.dim() != 2 or sin.shape != cos.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise ValueError(f"{what}: cos and sin must be float32 [positions, rotated / 2], got {tuple(cos.shape)} "
+                         f"{cos.dtype} and {tuple(sin.shape)} {sin.dtype}")
+    geom = _row_geom(what, q, k, v, positions, 2 * cos.shape[1], cos.shape[0])
+    want = (k.shape[0], k.shape[4])
+    if tuple(q_weight.shape) != want or tuple(k_weight.shape) != want:
+        raise ValueError(f"{what}: the norm weights must be [N, D] = {list(want)}, got {tuple(q_weight.shape)} and "
+                         f"{tuple(k_weight.shape)}")
+    if 2 * cos.shape[1] > k.shape[4]:
+        raise ValueError(f"{what}: {2 * cos.shape[1]} rotated channels of heads of {k.shape[4]}")
+    return dev, geom, (_dense(q_weight), _dense(k_weight), _dense(cos), _dense(sin))
+
+
+def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, cos: Tensor, sin: Tensor,
+                 positions: Tensor, eps: float = 1e-6, interleaved: bool = False):
+    """RMS norm of every query and key head, then the position rotation, in
+    one pass (widek_qk_norm_rope_fwd; differentiable).
+
+    q [N, B, T, Hq, D], k [N, B, T, Hk, D] (views of a fused projection are
+    read in place), norm weights [N, D], cos / sin float32 [P, R/2] tables:
+    the first R channels turn, pairs (i, i + R/2) or, interleaved, (2i, 2i+1).
+    positions int32/int64 [T], [B, T] or [N, B, T]; a negative one marks a
+    padding row, whose output and gradient are zero. Returns dense (q', k')."""
+    if _compiling():
+        return torch.ops.widek.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    if _AG.needs_grad(q, k, q_weight, k_weight):
+        return _AG.QkNormRopeFn.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    dev, geom, (qw, kw, co, si) = _rope_args("qk_norm_rope", q, k, None, q_weight, k_weight, cos, sin, positions)
+    yq = torch.empty(q.shape, device=dev, dtype=q.dtype)
+    yk = torch.empty(k.shape, device=dev, dtype=k.dtype)
+    with _guard(dev):
+        rc = N.lib().widek_qk_norm_rope_fwd(q.data_ptr(), k.data_ptr(), qw.data_ptr(), kw.data_ptr(), co.data_ptr(),
+                                            si.data_ptr(), positions.data_ptr(), yq.data_ptr(), yk.data_ptr(), geom,
+                                            float(eps), int(interleaved), int(positions.dtype == torch.int64),
+                                            N.dtype_code(q), N.stream_ptr(dev))
+    N.check(rc, "widek_qk_norm_rope_fwd")
+    return yq, yk
+
+
+def qk_norm_rope_bwd(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, cos: Tensor, sin: Tensor,
+                     positions: Tensor, dyq: Tensor, dyk: Tensor, eps: float = 1e-6, interleaved: bool = False,
+                     need_dw: bool = True):
+    """Gradients of ``qk_norm_rope``: (dq, dk, dq_weight, dk_weight), the last
+    two None unless asked for (widek_qk_norm_rope_bwd)."""
+    what = "qk_norm_rope backward"
+    dev, geom, (qw, kw, co, si) = _rope_args(what, q, k, None, q_weight, k_weight, cos, sin, positions)
+    N.require_cuda(q, dyq, dyk, what=what)
+    _same_dtype(what, q, dyq, dyk)
+    if dyq.shape != q.shape or dyk.shape != k.shape:
+        raise ValueError(f"{what}: gradients {tuple(dyq.shape)}, {tuple(dyk.shape)} do not match the heads")
+    dyq, dyk = _dense(dyq), _dense(dyk)
+    dq = torch.empty(q.shape, device=dev, dtype=q.dtype)
+    dk = torch.empty(k.shape, device=dev, dtype=k.dtype)
+    if k.numel() == 0 or q.numel() == 0:
+        return dq, dk, *((torch.zeros_like(qw), torch.zeros_like(kw)) if need_dw else (None, None))
+    dqw, dkw = (torch.empty_like(qw), torch.empty_like(kw)) if need_dw else (None, None)
+    ws_bytes = N.lib().widek_qk_norm_rope_bwd_workspace(geom)
+    if ws_bytes < 0:
+        raise ValueError(f"{what}: {N.last_error()}")
+    ws = torch.empty(max(ws_bytes, 1), device=dev, dtype=torch.uint8)
+    with _guard(dev):
+        rc = N.lib().widek_qk_norm_rope_bwd(q.data_ptr(), k.data_ptr(), qw.data_ptr(), kw.data_ptr(), co.data_ptr(),
+                                            si.data_ptr(), positions.data_ptr(), dyq.data_ptr(), dyk.data_ptr(),
+                                            dq.data_ptr(), dk.data_ptr(), N.ptr(dqw), N.ptr(dkw), geom, float(eps),
+                                            int(interleaved), int(positions.dtype == torch.int64), N.dtype_code(q),
+                                            ws.data_ptr(), ws_bytes, N.stream_ptr(dev))
+    N.check(rc, "widek_qk_norm_rope_bwd")
+    return dq, dk, dqw, dkw
+
+
+def _cache_args(what: str, cache, n: int, b: int, hk: int, d: int, *tensors: Optional[Tensor]) -> torch.device:
+    dev = N.require_cuda(cache.k, cache.v, cache.table, cache.k_scale, cache.v_scale, *tensors, what=what)
+    if (cache.n, cache.batch, cache.kv_heads, cache.head_dim) != (n, b, hk, d):
+        raise ValueError(f"{what}: N={n}, B={b}, Hk={hk}, D={d} do not match {cache!r}")
+    return dev
+
+
+def _no_grad(what: str, *tensors: Optional[Tensor]) -> None:
+    if _AG.needs_grad(*tensors):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
+
+
+def _cache_type(what: str, cache, dtype: torch.dtype) -> None:
+    if not cache.quantized and cache.k.dtype != dtype:
+        raise TypeError(f"{what}: dtype mismatch ({dtype} vs a cache of {cache.k.dtype})")
+
+
+def qk_norm_rope_write(q: Tensor, k: Tensor, v: Tensor, q_weight: Tensor, k_weight: Tensor, cos: Tensor, sin: Tensor,
+                       positions: Tensor, cache, eps: float = 1e-6, interleaved: bool = False) -> Tensor:
+    """``qk_norm_rope`` whose keys go, with the values, straight into the
+    cache at their positions: one launch for a decoder step
+    (widek_qk_norm_rope_write_fwd). An 8-bit cache is quantised from the fp32
+    keys. Padding rows (negative positions) write nothing. Returns q'."""
+    what = "qk_norm_rope_write"
+    _no_grad(what, q, k, v, q_weight, k_weight)
+    if _compiling():
+        return torch.ops.widek.qk_norm_rope_write(q, k, v, q_weight, k_weight, cos, sin, positions, cache.k, cache.v,
+                                                  cache.table, cache.k_scale, cache.v_scale, eps, interleaved)
+    dev, geom, (qw, kw, co, si) = _rope_args(what, q, k, v, q_weight, k_weight, cos, sin, positions)
+    n, b, _, hk, d = k.shape
+    _cache_args(what, cache, n, b, hk, d, q)
+    _cache_type(what, cache, q.dtype)
+    yq = torch.empty(q.shape, device=dev, dtype=q.dtype)
+    with _guard(dev):
+        rc = N.lib().widek_qk_norm_rope_write_fwd(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), qw.data_ptr(), kw.data_ptr(), co.data_ptr(), si.data_ptr(),
+            positions.data_ptr(), yq.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), N.ptr(cache.k_scale),
+            N.ptr(cache.v_scale), cache.table.data_ptr(), geom, cache.geom, float(eps), int(interleaved),
+            int(positions.dtype == torch.int64), cache.fmt, N.dtype_code(q), N.stream_ptr(dev))
+    N.check(rc, "widek_qk_norm_rope_write_fwd")
+    return yq
+
+
+def cache_write(cache, k: Tensor, v: Tensor, positions: Tensor) -> None:
+    """Writes k, v [N, B, T, Hk, D] to the cache at ``positions`` ([T],
+    [B, T] or [N, B, T]; negative: not written), quantising each (token, head)
+    row for an 8-bit cache (widek_cache_write_fwd)."""
+    what = "cache_write"
+    _no_grad(what, k, v)
+    if _compiling():
+        torch.ops.widek.cache_write(cache.k, cache.v, cache.table, cache.k_scale, cache.v_scale, k, v, positions)
+        return
+    geom = _row_geom(what, None, k, v, positions)
+    n, b, _, hk, d = k.shape
+    dev = _cache_args(what, cache, n, b, hk, d, k, v, positions)
+    _same_dtype(what, k, v)
+    _cache_type(what, cache, k.dtype)
+    with _guard(dev):
+        rc = N.lib().widek_cache_write_fwd(k.data_ptr(), v.data_ptr(), positions.data_ptr(), cache.k.data_ptr(),
+                                           cache.v.data_ptr(), N.ptr(cache.k_scale), N.ptr(cache.v_scale),
+                                           cache.table.data_ptr(), geom, cache.geom,
+                                           int(positions.dtype == torch.int64), cache.fmt, N.dtype_code(k),
+                                           N.stream_ptr(dev))
+    N.check(rc, "widek_cache_write_fwd")
+
+
+def cache_read(cache, positions: Tensor, dtype: Optional[torch.dtype] = None):
+    """The cached keys and values of the tokens at ``positions`` ([B, T] or
+    [N, B, T], or [T] for all sequences; negative: zeros) as dense
+    (k, v) [N, B, T, Hk, D] (widek_cache_read_fwd). ``dtype``: the result's
+    type for an 8-bit cache (default bfloat16), rounded once from
+    code * scale; else the cache's own."""
+    what = "cache_read"
+    if _compiling():
+        return torch.ops.widek.cache_read(cache.k, cache.v, cache.table, cache.k_scale, cache.v_scale, positions,
+                                          dtype)
+    dev = N.require_cuda(cache.k, cache.v, cache.table, cache.k_scale, cache.v_scale, positions, what=what)
+    if dtype is None:
+        dtype = torch.bfloat16 if cache.quantized else cache.k.dtype
+    _cache_type(what, cache, dtype)
+    n, b, hk, d = cache.n, cache.batch, cache.kv_heads, cache.head_dim
+    if positions.dim() < 1:
+        raise ValueError(f"{what}: positions must be [T], [B, T] or [N, B, T]")
+    t = positions.shape[-1]
+    k = torch.empty((n, b, t, hk, d), device=dev, dtype=dtype)
+    v = torch.empty_like(k)
+    geom = _row_geom(what, None, k, v, positions)
+    with _guard(dev):
+        rc = N.lib().widek_cache_read_fwd(cache.k.data_ptr(), cache.v.data_ptr(), N.ptr(cache.k_scale),
+                                          N.ptr(cache.v_scale), cache.table.data_ptr(), positions.data_ptr(),
+                                          k.data_ptr(), v.data_ptr(), geom, cache.geom,
+                                          int(positions.dtype == torch.int64), cache.fmt, N.dtype_code(k),
+                                          N.stream_ptr(dev))
+    N.check(rc, "widek_cache_read_fwd")
+    return k, v
+
+
+def decode_attention(q: Tensor, cache, lengths: Tensor, scale: Optional[float] = None, window: int = 0) -> Tensor:
+    """Attention of one new token of every sequence over its cached tokens
+    (widek_decode_attention_fwd).
+
+    q [N, B, Hq, D], Hq a multiple of the cache's Hk (query head h reads key
+    head h // (Hq / Hk)); lengths int32/int64 [B] or [N, B]: tokens visible,
+    the new one included; scale defaults to 1/sqrt(D); window > 0: only the
+    last ``window`` of them. Returns [N, B, Hq, D]; zeros for a sequence
+    without tokens."""
+    what = "decode_attention"
+    _no_grad(what, q)
+    if scale is None:
+        scale = 1.0 / math.sqrt(max(q.shape[-1], 1))
+    if _compiling():
+        return torch.ops.widek.decode_attention(q, cache.k, cache.v, cache.table, cache.k_scale, cache.v_scale,
+                                                lengths, scale, window)
+    if q.dim() != 4:
+        raise ValueError(f"{what}: q must be [N, B, Hq, D], got {tuple(q.shape)}")
+    n, b, hq, d = q.shape
+    hk = cache.kv_heads
+    dev = _cache_args(what, cache, n, b, hk, d, q, lengths)
+    _cache_type(what, cache, q.dtype)
+    if hk < 1 or hq % hk != 0:
+        raise ValueError(f"{what}: {hq} query heads over {hk} key heads")
+    geom = (ctypes.c_int64 * 10)(n, b, hq, hk, d, *_row_strides(q, what),
+                                 *_index_strides(lengths, (n, b), what, "lengths"))
+    lib = N.lib()
+    ws_bytes = lib.widek_decode_attention_workspace(geom, cache.geom, window)
+    if ws_bytes < 0:
+        raise ValueError(f"{what}: {N.last_error()}")
+    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
+    out = torch.empty((n, b, hq, d), device=dev, dtype=q.dtype)
+    with _guard(dev):
+        rc = lib.widek_decode_attention_fwd(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(),
+                                            N.ptr(cache.k_scale), N.ptr(cache.v_scale), cache.table.data_ptr(),
+                                            lengths.data_ptr(), out.data_ptr(), geom, cache.geom, float(scale),
+                                            int(window), int(lengths.dtype == torch.int64), cache.fmt,
+                                            N.dtype_code(q), N.ptr(ws), ws_bytes, N.stream_ptr(dev))
+    N.check(rc, "widek_decode_attention_fwd")
+    return out
+
+
+# ---------------------------------------------------------------------------
 # Convolutions
 # ---------------------------------------------------------------------------
 
