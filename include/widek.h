@@ -709,7 +709,7 @@ WIDEK_API int widek_cache_read_fwd(const void* kc, const void* vc, const float* 
 
 /* Workspace bytes widek_decode_attention_fwd needs (-1 for bad arguments). */
 WIDEK_API int64_t widek_decode_attention_workspace(const int64_t* geom, const int64_t* cgeom,
-                                                   int64_t window);
+                                                   int64_t window, int fmt);
 
 /* Attention of one new token of every sequence over its cache: query head h
  * reads key head h / (hq / hk), softmax(scale * q k^T) v over the tokens p

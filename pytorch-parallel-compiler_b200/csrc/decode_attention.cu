@@ -1,127 +1,66 @@
-// Attention of one new token of every sequence over a paged key-value cache.
-//
-//   z_p = scale q . k_p,  out = sum_p exp(z_p - m) v_p / sum_p exp(z_p - m),
-//   m = max z, over the tokens max(0, len - window) <= p < len; zeros where
-//   there is none.
-//
-// One block per query head, one token per warp at a time, the running maximum
-// and sum of each warp joined at the end.
-#include "paged_cache.cuh"
+// Attention of one new token of every sequence over a paged key-value cache:
+// the argument checks, the choice of how often a sequence is split, and the
+// join of its ranges. The kernel is in decode_attention.cuh.
+#include "decode_attention.cuh"
+
+#include <algorithm>
 
 namespace widek {
 namespace {
 
-struct DecodeArgs {
-    const void* q;
-    const void* lengths;
-    void* out;
-    int64_t q_n, q_b, q_h, len_n, len_b;
-    int n, b, hq, hk, d, group, len64, window;
-    float scale_log2;            // scale * log2(e)
-    PagedCache c;
-    int* err;
-};
+constexpr int kJoinWarps = 8;
+constexpr int kMostSplits = 512;
 
-constexpr int kWarps = 4;
-
-enum CacheIn : int { IN_SAME = 1, IN_I8 = 2, IN_E4M3 = 3 };
-
-template <typename T, int IN>
-__device__ __forceinline__ float cache_value(const void* base, int64_t at) {
-    if constexpr (IN == IN_I8) return (float)static_cast<const int8_t*>(base)[at];
-    if constexpr (IN == IN_E4M3) return value_e4m3(static_cast<const uint8_t*>(base)[at]);
-    return to_f<T>(static_cast<const T*>(base)[at]);
-}
-
-template <typename T, int IN>
-__global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_constant__ DecodeArgs a) {
-    constexpr int CH = 8;        // channels of a lane: lane + 32 j, up to 256
-    __shared__ float sm[kWarps], sl[kWarps], so[kWarps][256];
+// out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s over a sequence's ranges,
+// in a fixed order; one block per query head, its warps every 8th range.
+// Sequences of one range were finished by the attention itself.
+__global__ void __launch_bounds__(32 * kJoinWarps) decode_join_kernel(const __grid_constant__ DecodeArgs a) {
+    __shared__ float factor[kMostSplits];
+    __shared__ float red[kJoinWarps][256];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int h = blockIdx.x % a.hq;
-    const int b = (blockIdx.x / a.hq) % a.b;
-    const int64_t i = blockIdx.x / a.hq / a.b;
-    const int kh = h / a.group;
-    int len = load_index(a.lengths, i * a.len_n + b * a.len_b, a.len64);
-    if ((int64_t)len > (int64_t)a.c.cols * a.c.page) {
-        len = a.c.cols * a.c.page;
-        if (threadIdx.x == 0) raise_device_error(a.err, DEV_ERR_INDEX);
-    }
-    const int start = a.window > 0 && len > a.window ? len - a.window : 0;
-    const T* q = static_cast<const T*>(a.q) + i * a.q_n + b * a.q_b + h * a.q_h;
-    float qv[CH], acc[CH];
-#pragma unroll
-    for (int j = 0; j < CH; ++j) {
-        qv[j] = lane + 32 * j < a.d ? to_f<T>(q[lane + 32 * j]) * a.scale_log2 : 0.f;
-        acc[j] = 0.f;
-    }
-    float m = -INFINITY, l = 0.f;
-    for (int p = start + warp; p < len; p += kWarps) {
-        const int slot = a.c.row(i, b, a.hk, kh, p);
-        if (slot < 0) {
-            if (lane == 0) raise_device_error(a.err, DEV_ERR_INDEX);
-            continue;
-        }
-        const int64_t at = i * a.c.pages * a.hk * a.c.page + slot;
-        float z = 0.f;
-#pragma unroll
-        for (int j = 0; j < CH; ++j)
-            if (lane + 32 * j < a.d) z += qv[j] * cache_value<T, IN>(a.c.k, at * a.d + lane + 32 * j);
-        z = warp_sum(z);
-        float vs = 1.f;
-        if constexpr (IN != IN_SAME) {
-            z *= a.c.ks[at];
-            vs = a.c.vs[at];
-        }
-        const float top = fmaxf(m, z);
-        const float ref = top == -INFINITY ? 0.f : top;
-        const float keep = exp2f(m - ref), w = exp2f(z - ref);
-        m = top;
-        l = l * keep + w;
-#pragma unroll
-        for (int j = 0; j < CH; ++j)
-            if (lane + 32 * j < a.d)
-                acc[j] = acc[j] * keep + w * vs * cache_value<T, IN>(a.c.v, at * a.d + lane + 32 * j);
-    }
-    if (lane == 0) sm[warp] = m, sl[warp] = l;
-#pragma unroll
-    for (int j = 0; j < CH; ++j) so[warp][lane + 32 * j] = acc[j];
-    __syncthreads();
+    const int64_t row = blockIdx.x, nb = row / a.hq;
+    const DecodeRange rg(a, nb / a.b, nb % a.b);
+    if (rg.active <= 1) return;
+    const float2* ml = a.part_ml + row * a.splits;
     float top = -INFINITY;
+    for (int s = lane; s < rg.active; s += 32) top = fmaxf(top, ml[s].x);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w]);
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float ref = top == -INFINITY ? 0.f : top;
-    float total = 0.f, f[kWarps];
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        f[w] = exp2f(sm[w] - ref);
-        total += f[w] * sl[w];
+    float total = 0.f;
+    for (int s = lane; s < rg.active; s += 32) {
+        const float2 x = ml[s];
+        const float f = ex2(x.x - ref);
+        total += f * x.y;
+        if (warp == 0) factor[s] = f;
     }
-    T* out = static_cast<T*>(a.out) + (int64_t)blockIdx.x * a.d;
-    for (int c = threadIdx.x; c < a.d; c += 32 * kWarps) {
+    total = warp_sum(total);
+    __syncthreads();
+    float acc[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+    const float* po = a.part_o + row * a.splits * a.d;
+#pragma unroll 4
+    for (int s = warp; s < rg.active; s += kJoinWarps) {
+        const float f = factor[s];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (lane + 32 * j < a.d) acc[j] += f * po[(int64_t)s * a.d + lane + 32 * j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) red[warp][lane + 32 * j] = acc[j];
+    __syncthreads();
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    for (int ch = threadIdx.x; ch < a.d; ch += 32 * kJoinWarps) {
         float o = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) o += f[w] * so[w][c];
-        out[c] = from_f<T>(total == 0.f ? 0.f : o / total);
+        for (int w = 0; w < kJoinWarps; ++w) o += red[w][ch];
+        store_out(a.out, row * a.d + ch, o * inv, a.dtype);
     }
 }
 
-struct DecodeLaunch {
-    DecodeArgs a;
-    int fmt;
-    cudaStream_t st;
-    template <typename T>
-    int run() {
-        const unsigned blocks = (unsigned)a.n * a.b * a.hq;
-        if (fmt == WIDEK_I8) decode_kernel<T, IN_I8><<<blocks, 32 * kWarps, 0, st>>>(a);
-        else if (fmt == WIDEK_E4M3) decode_kernel<T, IN_E4M3><<<blocks, 32 * kWarps, 0, st>>>(a);
-        else decode_kernel<T, IN_SAME><<<blocks, 32 * kWarps, 0, st>>>(a);
-        return check_launch("widek_decode_attention_fwd");
-    }
-};
-
-int decode_args(DecodeArgs& a, const char* what, const int64_t* g, int64_t window) {
-    if (!g) return set_error(WIDEK_ERR_INVALID, "%s: null geometry", what);
+int decode_args(DecodeArgs& a, const char* what, const int64_t* g, const int64_t* cgeom, int64_t window, int fmt) {
+    if (!g || !cgeom) return set_error(WIDEK_ERR_INVALID, "%s: null geometry", what);
     for (int i = 0; i < 5; ++i)
         if (g[i] < 0 || g[i] > 0x7fffffff)
             return set_error(WIDEK_ERR_INVALID, "%s: size %d out of range (%lld)", what, i, (long long)g[i]);
@@ -137,8 +76,30 @@ int decode_args(DecodeArgs& a, const char* what, const int64_t* g, int64_t windo
     a.q_n = g[5], a.q_b = g[6], a.q_h = g[7], a.len_n = g[8], a.len_b = g[9];
     a.group = a.hq / a.hk;
     a.window = window > 0x7fffffff ? 0x7fffffff : (int)window;
+    a.fmt = fmt;
     a.err = device_error_ptr();
+    const int nt = decode_nt(a.group, a.d, fmt);
+    a.tiles = (a.group + 8 * nt - 1) / (8 * nt);
+    // Ranges of a sequence. The host does not know the lengths, only the most
+    // tokens that a table row holds. Fewer blocks than the GPU has places (3 of
+    // an SM): as many ranges as fill them once, of one tile for each warp or
+    // more. More blocks: ranges for six rounds, which evens out ragged lengths
+    // and the last round, as long as they keep 1024 tokens to start up for.
+    const int64_t blocks = (int64_t)a.n * a.b * a.hk * a.tiles;
+    const int64_t places = 3 * (int64_t)sm_count(current_device());
+    const double span = (double)cgeom[1] * (double)cgeom[2];
+    int64_t tokens = span > 2147418112.0 ? 2147418112 : (int64_t)span;
+    if (a.window > 0 && a.window < tokens) tokens = a.window;
+    a.unit = decode_unit(a.d, fmt);
+    int64_t splits = 1;
+    if (blocks > 0 && blocks < places) splits = std::min(places / blocks, (tokens + a.unit - 1) / a.unit);
+    else if (blocks > 0) splits = std::min((6 * places + blocks - 1) / blocks, tokens / 1024);
+    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(splits, kMostSplits));
     return WIDEK_OK;
+}
+
+int64_t part_rows(const DecodeArgs& a) {
+    return a.splits > 1 ? (int64_t)a.n * a.b * a.hq * a.splits : 0;
 }
 
 }  // namespace
@@ -146,10 +107,11 @@ int decode_args(DecodeArgs& a, const char* what, const int64_t* g, int64_t windo
 
 using namespace widek;
 
-extern "C" int64_t widek_decode_attention_workspace(const int64_t* geom, const int64_t* cgeom, int64_t window) {
+extern "C" int64_t widek_decode_attention_workspace(const int64_t* geom, const int64_t* cgeom, int64_t window,
+                                                    int fmt) {
     DecodeArgs a;
-    if (!cgeom || decode_args(a, "widek_decode_attention_workspace", geom, window) != WIDEK_OK) return -1;
-    return 0;
+    if (decode_args(a, "widek_decode_attention_workspace", geom, cgeom, window, fmt) != WIDEK_OK) return -1;
+    return part_rows(a) * (int64_t)(sizeof(float2) + a.d * sizeof(float));
 }
 
 extern "C" int widek_decode_attention_fwd(const void* q, const void* kc, const void* vc, const float* ks,
@@ -159,15 +121,34 @@ extern "C" int widek_decode_attention_fwd(const void* q, const void* kc, const v
                                           void* stream) {
     const char* what = "widek_decode_attention_fwd";
     DecodeArgs a;
-    int rc = decode_args(a, what, geom, window);
+    int rc = decode_args(a, what, geom, cgeom, window, fmt);
     if (rc != WIDEK_OK) return rc;
+    if (dtype_size(dtype) == 0) return set_error(WIDEK_ERR_INVALID, "%s: unknown dtype code %d", what, dtype);
     rc = cache_args(a.c, what, const_cast<void*>(kc), const_cast<void*>(vc), const_cast<float*>(ks),
                     const_cast<float*>(vs), table, cgeom, (int64_t)a.n * a.b, a.hk, a.d, fmt, dtype);
     if (rc != WIDEK_OK) return rc;
     if (a.n == 0 || a.b == 0 || a.d == 0) return WIDEK_OK;
     if (!q || !lengths || !out) return set_error(WIDEK_ERR_INVALID, "%s: null pointer", what);
-    a.q = q, a.lengths = lengths, a.out = out, a.len64 = len64;
+    const int64_t rows = part_rows(a), need = rows * (int64_t)(sizeof(float2) + a.d * sizeof(float));
+    if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 7)))
+        return set_error(WIDEK_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed", what,
+                         (long long)workspace_bytes, (long long)need);
+    a.part_ml = static_cast<float2*>(workspace);
+    a.part_o = reinterpret_cast<float*>(a.part_ml + rows);
+    a.q = q, a.lengths = lengths, a.out = out, a.len64 = len64, a.dtype = dtype;
     a.scale_log2 = (float)(scale * 1.4426950408889634);
-    DecodeLaunch L{a, fmt, (cudaStream_t)stream};
-    return dispatch_dtype(dtype, L);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (fmt == WIDEK_I8)
+        rc = dtype == WIDEK_F32 ? launch_decode<DK_I8, true>(a, st) : launch_decode<DK_I8, false>(a, st);
+    else if (fmt == WIDEK_E4M3)
+        rc = dtype == WIDEK_F32 ? launch_decode<DK_E4M3, true>(a, st) : launch_decode<DK_E4M3, false>(a, st);
+    else if (fmt == WIDEK_BF16)
+        rc = launch_decode<DK_BF16, false>(a, st);
+    else if (fmt == WIDEK_F16)
+        rc = launch_decode<DK_F16, false>(a, st);
+    else
+        rc = launch_decode<DK_F32, false>(a, st);
+    if (rc != WIDEK_OK || a.splits == 1) return rc;
+    decode_join_kernel<<<(unsigned)((int64_t)a.n * a.b * a.hq), 32 * kJoinWarps, 0, st>>>(a);
+    return check_launch("widek_decode_attention_fwd (join)");
 }

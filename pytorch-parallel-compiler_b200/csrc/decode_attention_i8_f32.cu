@@ -1,0 +1,6 @@
+// Single-token attention over a paged cache: the i8_f32 instantiations.
+#include "decode_attention.cuh"
+
+namespace widek {
+template int launch_decode<DK_I8, true>(const DecodeArgs&, cudaStream_t);
+}  // namespace widek

@@ -113,7 +113,7 @@ SIGNATURES = {
                                                   _c_void_p],
     "widek_cache_write_fwd": [_c_void_p] * 8 + [ctypes.POINTER(_i64)] * 2 + [_int] * 3 + [_c_void_p],
     "widek_cache_read_fwd": [_c_void_p] * 8 + [ctypes.POINTER(_i64)] * 2 + [_int] * 3 + [_c_void_p],
-    "widek_decode_attention_workspace": [ctypes.POINTER(_i64)] * 2 + [_i64],
+    "widek_decode_attention_workspace": [ctypes.POINTER(_i64)] * 2 + [_i64, _int],
     "widek_decode_attention_fwd": [_c_void_p] * 8 + [ctypes.POINTER(_i64)] * 2 + [_dbl, _i64, _int, _int, _int,
                                                                                   _c_void_p, _i64, _c_void_p],
 }

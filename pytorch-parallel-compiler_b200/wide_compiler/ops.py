@@ -1183,7 +1183,7 @@ def decode_attention(q: Tensor, cache, lengths: Tensor, scale: Optional[float] =
     geom = (ctypes.c_int64 * 10)(n, b, hq, hk, d, *_row_strides(q, what),
                                  *_index_strides(lengths, (n, b), what, "lengths"))
     lib = N.lib()
-    ws_bytes = lib.widek_decode_attention_workspace(geom, cache.geom, window)
+    ws_bytes = lib.widek_decode_attention_workspace(geom, cache.geom, window, cache.fmt)
     if ws_bytes < 0:
         raise ValueError(f"{what}: {N.last_error()}")
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
