@@ -8,55 +8,43 @@
 namespace widek {
 namespace {
 
-constexpr int kJoinWarps = 8;
+constexpr int kJoinWarps = 4;
 constexpr int kMostSplits = 512;
 
-// out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s over a sequence's ranges,
-// in a fixed order; one block per query head, its warps every 8th range.
-// Sequences of one range were finished by the attention itself.
+// out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s over the groups of a
+// sequence's ranges, in their order; one warp per query head. Sequences of one
+// group were finished by the attention itself.
 __global__ void __launch_bounds__(32 * kJoinWarps) decode_join_kernel(const __grid_constant__ DecodeArgs a) {
-    __shared__ float factor[kMostSplits];
-    __shared__ float red[kJoinWarps][256];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t row = blockIdx.x, nb = row / a.hq;
+    sm100::grid_dep_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t row = (int64_t)blockIdx.x * kJoinWarps + (threadIdx.x >> 5), nb = row / a.hq;
+    if (row >= (int64_t)a.n * a.b * a.hq) return;
     const DecodeRange rg(a, nb / a.b, nb % a.b);
-    if (rg.active <= 1) return;
-    const float2* ml = a.part_ml + row * a.splits;
+    if (rg.active <= a.cluster) return;
+    const int groups = (rg.active + a.cluster - 1) / a.cluster;
+    const float2* ml = a.part_ml + row * a.groups;
     float top = -INFINITY;
-    for (int s = lane; s < rg.active; s += 32) top = fmaxf(top, ml[s].x);
+    for (int s = lane; s < groups; s += 32) top = fmaxf(top, ml[s].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float ref = top == -INFINITY ? 0.f : top;
-    float total = 0.f;
-    for (int s = lane; s < rg.active; s += 32) {
+    float total = 0.f, acc[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+    const float* po = a.part_o + row * a.groups * a.d;
+#pragma unroll 8
+    for (int s = 0; s < groups; ++s) {
         const float2 x = ml[s];
         const float f = ex2(x.x - ref);
         total += f * x.y;
-        if (warp == 0) factor[s] = f;
-    }
-    total = warp_sum(total);
-    __syncthreads();
-    float acc[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-    const float* po = a.part_o + row * a.splits * a.d;
-#pragma unroll 4
-    for (int s = warp; s < rg.active; s += kJoinWarps) {
-        const float f = factor[s];
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (lane + 32 * j < a.d) acc[j] += f * po[(int64_t)s * a.d + lane + 32 * j];
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) red[warp][lane + 32 * j] = acc[j];
-    __syncthreads();
     const float inv = total == 0.f ? 0.f : 1.f / total;
-    for (int ch = threadIdx.x; ch < a.d; ch += 32 * kJoinWarps) {
-        float o = 0.f;
 #pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) o += red[w][ch];
-        store_out(a.out, row * a.d + ch, o * inv, a.dtype);
-    }
+    for (int j = 0; j < 8; ++j)
+        if (lane + 32 * j < a.d) store_out(a.out, row * a.d + lane + 32 * j, acc[j] * inv, a.dtype);
 }
 
 int decode_args(DecodeArgs& a, const char* what, const int64_t* g, const int64_t* cgeom, int64_t window, int fmt) {
@@ -81,25 +69,27 @@ int decode_args(DecodeArgs& a, const char* what, const int64_t* g, const int64_t
     const int nt = decode_nt(a.group, a.d, fmt);
     a.tiles = (a.group + 8 * nt - 1) / (8 * nt);
     // Ranges of a sequence. The host does not know the lengths, only the most
-    // tokens that a table row holds. Fewer blocks than the GPU has places (3 of
-    // an SM): as many ranges as fill them once, of one tile for each warp or
+    // tokens that a table row holds. Fewer blocks than the GPU has places: as many ranges as fill them once, of one tile for each warp or
     // more. More blocks: ranges for six rounds, which evens out ragged lengths
     // and the last round, as long as they keep 1024 tokens to start up for.
     const int64_t blocks = (int64_t)a.n * a.b * a.hk * a.tiles;
-    const int64_t places = 3 * (int64_t)sm_count(current_device());
+    const int64_t places = decode_places(a.d, fmt, nt) * (int64_t)sm_count(current_device());
     const double span = (double)cgeom[1] * (double)cgeom[2];
-    int64_t tokens = span > 2147418112.0 ? 2147418112 : (int64_t)span;
+    int64_t tokens = span > 2147418112.0 ? 2147418112 : (int64_t)span;      // the cache's own check refuses such a span
     if (a.window > 0 && a.window < tokens) tokens = a.window;
     a.unit = decode_unit(a.d, fmt);
     int64_t splits = 1;
     if (blocks > 0 && blocks < places) splits = std::min(places / blocks, (tokens + a.unit - 1) / a.unit);
     else if (blocks > 0) splits = std::min((6 * places + blocks - 1) / blocks, tokens / 1024);
-    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(splits, kMostSplits));
+    splits = std::max<int64_t>(1, std::min<int64_t>(splits, kMostSplits));
+    a.cluster = (int)std::min<int64_t>(splits, kMostCluster);
+    a.groups = (int)(splits / a.cluster);
+    a.splits = a.groups * a.cluster;
     return WIDEK_OK;
 }
 
 int64_t part_rows(const DecodeArgs& a) {
-    return a.splits > 1 ? (int64_t)a.n * a.b * a.hq * a.splits : 0;
+    return a.groups > 1 ? (int64_t)a.n * a.b * a.hq * a.groups : 0;
 }
 
 }  // namespace
@@ -137,6 +127,8 @@ extern "C" int widek_decode_attention_fwd(const void* q, const void* kc, const v
     a.part_o = reinterpret_cast<float*>(a.part_ml + rows);
     a.q = q, a.lengths = lengths, a.out = out, a.len64 = len64, a.dtype = dtype;
     a.scale_log2 = (float)(scale * 1.4426950408889634);
+    const int64_t in16 = 16 / (int64_t)dtype_size(dtype);
+    a.q_vec = aligned16(q) && a.q_n % in16 == 0 && a.q_b % in16 == 0 && a.q_h % in16 == 0;
     cudaStream_t st = (cudaStream_t)stream;
     if (fmt == WIDEK_I8)
         rc = dtype == WIDEK_F32 ? launch_decode<DK_I8, true>(a, st) : launch_decode<DK_I8, false>(a, st);
@@ -148,7 +140,17 @@ extern "C" int widek_decode_attention_fwd(const void* q, const void* kc, const v
         rc = launch_decode<DK_F16, false>(a, st);
     else
         rc = launch_decode<DK_F32, false>(a, st);
-    if (rc != WIDEK_OK || a.splits == 1) return rc;
-    decode_join_kernel<<<(unsigned)((int64_t)a.n * a.b * a.hq), 32 * kJoinWarps, 0, st>>>(a);
+    if (rc != WIDEK_OK || a.groups == 1) return rc;
+    // the join's blocks are set up while the attention's last ones run
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(((int64_t)a.n * a.b * a.hq + kJoinWarps - 1) / kJoinWarps));
+    cfg.blockDim = dim3(32 * kJoinWarps);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, decode_join_kernel, a);
     return check_launch("widek_decode_attention_fwd (join)");
 }

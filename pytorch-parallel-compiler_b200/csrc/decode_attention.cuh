@@ -43,6 +43,7 @@
 #pragma once
 
 #include "paged_cache.cuh"
+#include "sm100_ptx.cuh"
 
 #include <atomic>
 
@@ -52,17 +53,20 @@ struct DecodeArgs {
     const void* q;
     const void* lengths;
     void* out;
-    float* part_o;               // [n b hq, splits, d] partial outputs (relative to their own maximum)
-    float2* part_ml;             // [n b hq, splits] maximum and sum
+    float* part_o;               // [n b hq, groups, d] partial outputs (relative to their own maximum)
+    float2* part_ml;             // [n b hq, groups] maximum and sum
     int64_t q_n, q_b, q_h, len_n, len_b;
     int n, b, hq, hk, d, group, len64, window, dtype, fmt;
-    int tiles, splits, unit;     // query-head tiles of a group, ranges of a sequence, tokens of the block's tiles
+    int tiles, unit;             // query-head tiles of a group, tokens of a block's tiles
+    int splits, cluster, groups; // ranges of a sequence, joined in clusters of blocks, groups = splits / cluster
+    int q_vec;                   // query rows start at multiples of 16 bytes
     float scale_log2;            // scale * log2(e)
     PagedCache c;
     int* err;
 };
 
 constexpr int kDecodeWarps = 4;
+constexpr int kMostCluster = 8;       // blocks of a cluster that any GPU of the architecture takes
 
 // Visible tokens of a sequence and its cut into ranges: the same for the
 // attention and the join.
@@ -94,6 +98,21 @@ __device__ __forceinline__ void store_out(void* p, int64_t at, float v, int dtyp
     if (dtype == WIDEK_F32) static_cast<float*>(p)[at] = v;
     else if (dtype == WIDEK_BF16) static_cast<__nv_bfloat16*>(p)[at] = __float2bfloat16_rn(v);
     else static_cast<__half*>(p)[at] = __float2half_rn(v);
+}
+
+// N queries' channels from `at` on, in 16-byte loads.
+template <int N>
+__device__ __forceinline__ void load_in16(const void* p, int64_t at, int dtype, float (&x)[N]) {
+    if (dtype == WIDEK_F32) {
+#pragma unroll
+        for (int e = 0; e < N; e += 4) load16<float>(static_cast<const float*>(p) + at + e, x + e);
+    } else if constexpr (N % 8 == 0) {
+#pragma unroll
+        for (int e = 0; e < N; e += 8) {
+            if (dtype == WIDEK_BF16) load16<__nv_bfloat16>(static_cast<const __nv_bfloat16*>(p) + at + e, x + e);
+            else load16<__half>(static_cast<const __half*>(p) + at + e, x + e);
+        }
+    }
 }
 
 __device__ __forceinline__ float load_in(const void* p, int64_t at, int dtype) {
@@ -209,21 +228,25 @@ __device__ __forceinline__ uint32_t code_word(uint32_t w) {
     return KIND == DK_I8 ? w ^ 0x80808080u : w;
 }
 
+// How cached rows lie: of any size and place, of multiples of 16 bytes, or
+// those with exactly the channels of the tiles.
+enum RowsAre : int { ROWS_ANY, ROWS_16, ROWS_FULL };
+
 // Copies W words at byte `off` of a cached row (of `bytes`) to shared memory
-// without waiting; zeros past the row, or all of them unless `live`. ALIGNED:
-// rows start at multiples of 16 bytes, so a piece lies inside the row or
-// outside; else rows of whole words, or single elements.
-template <int W, int SIZE, bool ALIGNED>
+// without waiting; zeros past the row, or all of them unless `live`. Rows of
+// 16 bytes' multiples have a piece inside or outside; others come as words
+// (cp.async of 4 bytes) or, where even these are not aligned, as elements.
+template <int W, int SIZE, int ROWS>
 __device__ __forceinline__ void copy_piece(uint32_t dst, const uint8_t* row, int off, int bytes, bool words,
                                            bool live) {
-    if constexpr (ALIGNED) {
-        const int n = live && off < bytes ? 4 * W : 0;
-        const uint8_t* p = row + (n ? off : 0);
+    if constexpr (ROWS != ROWS_ANY) {
+        const int n = live && (ROWS == ROWS_FULL || off < bytes) ? 4 * W : 0;
         if constexpr (W == 4)
-            asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(p), "r"(n) : "memory");
-        else
-            asm volatile("cp.async.ca.shared.global.L2::256B [%0], [%1], %2, %3;" ::"r"(dst), "l"(p), "n"(4 * W), "r"(n)
+            asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(row + off), "r"(n)
                          : "memory");
+        else
+            asm volatile("cp.async.ca.shared.global.L2::256B [%0], [%1], %2, %3;" ::"r"(dst), "l"(row + off),
+                         "n"(4 * W), "r"(n) : "memory");
         return;
     }
     if (words) {
@@ -271,7 +294,7 @@ __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group 
 //   MT     tiles of 16 tokens a warp has in registers at a time
 //   SPLITQ the queries need two f16 pieces (8-bit cache, fp32 queries)
 // ---------------------------------------------------------------------------
-template <int KIND, int DP, int NT, bool ALIGNED, bool SPLITQ>
+template <int KIND, int DP, int NT, int ROWS, bool SPLITQ>
 struct DecodeShape {
     static constexpr int size = Kind<KIND>::size;
     static constexpr int row_bytes = DP * size;
@@ -284,26 +307,34 @@ struct DecodeShape {
     static constexpr int KW = KD * size / 4, VW = VD * size / 4;            // words of a piece
     static constexpr int KR = Kind<KIND>::f32 ? KD : KD / 2;                // MMA registers of a K piece
     static constexpr int QR = KP * KR;                                      // MMA registers of a query row
+    // pieces read back from the ring at a time: 32 words, so that their latencies overlap
+    static constexpr int KB = 16 / (MT * KW) < KP ? 16 / (MT * KW) : KP;
+    static constexpr int VB = 8 / (MT * VW) < 1 ? 1 : (8 / (MT * VW) < VP ? 8 / (MT * VW) : VP);
     static constexpr int NR = (TOK + 31) / 32;                              // token slots a lane looks up
-    // ring: `stages` tiles of K and as many of V for each thread; blocks of an SM
-    static constexpr int unit = 32 * kDecodeWarps * TOK * row_bytes / 32;   // bytes of a block's K (or V) tiles
-    static constexpr int stages = row_bytes <= 256 ? 2 : 1;
-    static constexpr int ring = 2 * stages * unit;
-    static constexpr int blocks = row_bytes <= 512 ? (NT == 2 || SPLITQ || DP == 256 || row_bytes > 256 ? 2 : 3) : 1;
+    // Ring of `units` units, a unit being a tile of K or of V of each warp.
+    // Unit 2 i is K of tile i, unit 2 i + 1 its V; unit j lies in place
+    // j % units, and j + units is copied as soon as j has been read.
+    static constexpr int unit = 32 * kDecodeWarps * TOK * row_bytes / 32;   // bytes
+    static constexpr int units = row_bytes <= 256 ? 3 : 2;
+    static constexpr int ring = units * unit;
+    static constexpr int blocks =                                           // of an SM
+        row_bytes > 512 ? 1 : (row_bytes > 256 || NT == 2 || SPLITQ || DP == 256 ? 2 : (Kind<KIND>::f32 ? 3 : 4));
     static constexpr int joined = kDecodeWarps * 8 * NT * (DP + 2) * 4;     // the warps' sums, over the ring
     static constexpr int smem = ring > joined ? ring : joined;
 };
 
-template <int KIND, int DP, int NT, bool ALIGNED, bool SPLITQ>
-__global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, ALIGNED, SPLITQ>::blocks)
+template <int KIND, int DP, int NT, int ROWS, bool SPLITQ>
+__global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, ROWS, SPLITQ>::blocks)
     decode_kernel(const __grid_constant__ DecodeArgs a) {
-    using S = DecodeShape<KIND, DP, NT, ALIGNED, SPLITQ>;
+    using S = DecodeShape<KIND, DP, NT, ROWS, SPLITQ>;
     using K = Kind<KIND>;
     constexpr int MT = S::MT, TOK = S::TOK;
-    extern __shared__ __align__(16) uint8_t ring[];
+    extern __shared__ __align__(16) uint8_t decode_ring[];
+    uint8_t* const ring = decode_ring;
     __shared__ float sm_m[kDecodeWarps][8 * NT], sm_l[kDecodeWarps][8 * NT];
-    // scales of a tile's key and value rows
-    __shared__ float sm_s[K::code ? S::stages : 1][kDecodeWarps][2][K::code ? TOK : 1];
+    __shared__ float2 sm_ml[8 * NT], sm_all[kMostCluster][8 * NT];
+    // scales of the key and value rows of a tile and the next
+    __shared__ float sm_s[2][kDecodeWarps][2][K::code ? TOK : 1];
     float(*sm_o)[8 * NT][DP + 2] = reinterpret_cast<float(*)[8 * NT][DP + 2]>(ring);
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -313,8 +344,11 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, A
     const int64_t nb = blockIdx.x / a.tiles / a.hk;
     const int64_t i = nb / a.b, b = nb % a.b;
     const DecodeRange rg(a, i, b);
+    if (a.groups > 1) sm100::grid_dep_launch_dependents();     // the join waits for this grid's end by itself
     const int split = blockIdx.y;
-    if (split > 0 && split >= rg.active) return;
+    // ranges that a short sequence does not have: their blocks are needed only
+    // by a cluster that has others
+    if (split >= rg.active && split / a.cluster * a.cluster >= max(rg.active, 1)) return;
     const int first = rg.start + split * rg.chunk;
     const int end = min(rg.len, first + rg.chunk);
     const int h0 = tile * 8 * NT;                        // first query head of the group here
@@ -336,15 +370,14 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, A
         }
     };
     const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring);
-    auto k_place = [&](int stage, int mt, int hf, int p) {
-        return mine + 2 * stage * S::unit + (((mt * 2 + hf) * S::KP + p) * 32 * kDecodeWarps + threadIdx.x) * S::KW * 4;
+    auto k_place = [&](int place, int mt, int hf, int p) {
+        return mine + place * S::unit + (((mt * 2 + hf) * S::KP + p) * 32 * kDecodeWarps + threadIdx.x) * S::KW * 4;
     };
-    auto v_place = [&](int stage, int mt, int t, int p) {
-        return mine + (2 * stage + 1) * S::unit +
-               (((mt * 4 + t) * S::VP + p) * 32 * kDecodeWarps + threadIdx.x) * S::VW * 4;
+    auto v_place = [&](int place, int mt, int t, int p) {
+        return mine + place * S::unit + (((mt * 4 + t) * S::VP + p) * 32 * kDecodeWarps + threadIdx.x) * S::VW * 4;
     };
     // K pieces of tokens g and g + 8 of every 16, the tile's scales, and a bit for each token that is there
-    auto copy_k = [&](int stage, const int (&rows)[S::NR], uint32_t (&seen)[S::NR]) {
+    auto copy_k = [&](int place, int turn, const int (&rows)[S::NR], uint32_t (&seen)[S::NR]) {
 #pragma unroll
         for (int r = 0; r < S::NR; ++r) {
             seen[r] = __ballot_sync(0xffffffffu, rows[r] >= 0);
@@ -353,10 +386,10 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, A
                 const int64_t at = pool + (rows[r] < 0 ? 0 : rows[r]);
                 const int n = rows[r] >= 0 ? 4 : 0, t = TOK < 32 ? lane & (TOK - 1) : lane + 32 * r;
                 asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
-                                 (uint32_t)__cvta_generic_to_shared(&sm_s[stage][warp][0][t])),
+                                 (uint32_t)__cvta_generic_to_shared(&sm_s[turn][warp][0][t])),
                              "l"(a.c.ks + at), "r"(n) : "memory");
                 asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
-                                 (uint32_t)__cvta_generic_to_shared(&sm_s[stage][warp][1][t])),
+                                 (uint32_t)__cvta_generic_to_shared(&sm_s[turn][warp][1][t])),
                              "l"(a.c.vs + at), "r"(n) : "memory");
             }
         }
@@ -369,11 +402,11 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, A
                 const uint8_t* row = kbase + (int64_t)max(r, 0) * bytes;
 #pragma unroll
                 for (int p = 0; p < S::KP; ++p)
-                    copy_piece<S::KW, S::size, ALIGNED>(k_place(stage, mt, hf, p), row, (p * 4 + c) * S::KD * S::size,
+                    copy_piece<S::KW, S::size, ROWS>(k_place(place, mt, hf, p), row, (p * 4 + c) * S::KD * S::size,
                                                         bytes, words, r >= 0);
             }
     };
-    auto copy_v = [&](int stage, const int (&rows)[S::NR]) {
+    auto copy_v = [&](int place, const int (&rows)[S::NR]) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -384,25 +417,26 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, A
                 const uint8_t* row = vbase + (int64_t)max(r, 0) * bytes;
 #pragma unroll
                 for (int p = 0; p < S::VP; ++p)
-                    copy_piece<S::VW, S::size, ALIGNED>(v_place(stage, mt, t, p), row, (p * 8 + g) * S::VD * S::size,
+                    copy_piece<S::VW, S::size, ROWS>(v_place(place, mt, t, p), row, (p * 8 + g) * S::VD * S::size,
                                                         bytes, words, r >= 0);
             }
     };
 
     constexpr int STEP = kDecodeWarps * TOK;
     int tb = first + warp * TOK;
-    int rows[S::NR];
-    uint32_t seen[S::stages][S::NR];         // of the tiles in flight, the current one first
+    int r1[S::NR], r2[S::NR];                // slots of the next tile and of the one after it
+    uint32_t seen[2][S::NR];                 // tokens that are there, of the current tile and the next
     {
-        int ahead[S::stages][S::NR];
-#pragma unroll
-        for (int st = 0; st < S::stages; ++st) look_up(ahead[st], tb + st * STEP);
-        look_up(rows, tb + S::stages * STEP);
-#pragma unroll
-        for (int st = 0; st < S::stages; ++st) {
-            copy_k(st, ahead[st], seen[st]);
-            copy_commit();
-            copy_v(st, ahead[st]);
+        int r0[S::NR];
+        look_up(r0, tb);
+        look_up(r1, tb + STEP);
+        if constexpr (S::units == 3) look_up(r2, tb + 2 * STEP);
+        copy_k(0, 0, r0, seen[0]);
+        copy_commit();
+        copy_v(1, r0);
+        copy_commit();
+        if constexpr (S::units == 3) {
+            copy_k(2, 1, r1, seen[1]);
             copy_commit();
         }
     }
@@ -417,13 +451,20 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, A
         float x[S::KP][S::KD];
         float top = 0.f;
 #pragma unroll
-        for (int p = 0; p < S::KP; ++p)
+        for (int p = 0; p < S::KP; ++p) {
+            const int ch = (p * 4 + c) * S::KD;
 #pragma unroll
-            for (int e = 0; e < S::KD; ++e) {
-                const int ch = (p * 4 + c) * S::KD + e;
-                x[p][e] = h < heads && ch < a.d ? load_in(a.q, at + ch, a.dtype) : 0.f;
-                top = fmaxf(top, fabsf(x[p][e]));
+            for (int e = 0; e < S::KD; ++e) x[p][e] = 0.f;
+            if (ROWS != ROWS_ANY && a.q_vec) {
+                if (h < heads && ch < a.d) load_in16<S::KD>(a.q, at + ch, a.dtype, x[p]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < S::KD; ++e)
+                    if (h < heads && ch + e < a.d) x[p][e] = load_in(a.q, at + ch + e, a.dtype);
             }
+#pragma unroll
+            for (int e = 0; e < S::KD; ++e) top = fmaxf(top, fabsf(x[p][e]));
+        }
         zs[t][0] = zs[t][1] = a.scale_log2;
         float up = 1.f;
         if constexpr (K::code) {
@@ -465,14 +506,21 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, A
 
     // S^T += K q^T over the pieces in registers
     float s[NT][MT][4];
-    auto scores = [&](int stage) {
+    auto scores = [&](int place) {
+        uint32_t batch[MT][S::KB][2][S::KW];
+#pragma unroll
+        for (int p0 = 0; p0 < S::KP; p0 += S::KB) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int p = 0; p < S::KP; ++p) {
-                uint32_t kr[2][S::KW];
-                read_piece<S::KW>(kr[0], k_place(stage, mt, 0, p));
-                read_piece<S::KW>(kr[1], k_place(stage, mt, 1, p));
+            for (int p = 0; p < S::KB; ++p)
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) read_piece<S::KW>(batch[mt][p][hf], k_place(place, mt, hf, p0 + p));
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int p = p0; p < p0 + S::KB; ++p) {
+                const uint32_t(&kr)[2][S::KW] = batch[mt][p - p0];
                 if constexpr (K::f32) {
                     // the tensor core's sums round towards zero: chains of 6, added up in fp32
                     float part[NT][4];
@@ -527,9 +575,30 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, A
                         }
                 }
             }
+        }
     };
     // Running maxima and sums; s becomes the weights that meet V.
     auto softmax = [&](const uint32_t (&seen)[S::NR], const float (&kt)[MT][2], const float (&vt)[MT][2]) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    s[t][mt][e] *= K::code ? zs[t][e & 1] * kt[mt][e >> 1] : zs[t][e & 1];
+        bool all = true;
+#pragma unroll
+        for (int r = 0; r < S::NR; ++r) all = all && seen[r] == 0xffffffffu;
+        if (!all) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!((seen[S::NR == 1 ? 0 : mt >> 1] >> ((16 * mt + 8 * (e >> 1) + g) & 31)) & 1))
+                            s[t][mt][e] = -INFINITY;
+        }
         float f[NT][2];
         bool same = true;
 #pragma unroll
@@ -537,17 +606,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, A
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 float top = -INFINITY;
-                float z[MT][2];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int hf = 0; hf < 2; ++hf) {
-                        float x = s[t][mt][2 * hf + e] * zs[t][e];
-                        if constexpr (K::code) x *= kt[mt][hf];
-                        x = (seen[S::NR == 1 ? 0 : mt >> 1] >> ((16 * mt + 8 * hf + g) & 31)) & 1 ? x : -INFINITY;
-                        z[mt][hf] = x;
-                        top = fmaxf(top, x);
-                    }
+                for (int mt = 0; mt < MT; ++mt) top = fmaxf(top, fmaxf(s[t][mt][e], s[t][mt][2 + e]));
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                 top = fmaxf(top, m[t][e]);
@@ -559,7 +619,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, A
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int hf = 0; hf < 2; ++hf) {
-                        const float w = ex2(z[mt][hf] - ref);
+                        const float w = ex2(s[t][mt][2 * hf + e] - ref);
                         sum += w;
                         s[t][mt][2 * hf + e] = K::code ? w * vt[mt][hf] : (K::lift > 0.f ? w * 32768.f : w);
                     }
@@ -603,14 +663,21 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, A
             }
     };
     // O^T += V^T P^T over the pieces in registers
-    auto values = [&](int stage) {
+    auto values = [&](int place) {
+        uint32_t batch[MT][S::VB][4][S::VW];
+#pragma unroll
+        for (int p0 = 0; p0 < S::VP; p0 += S::VB) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int p = 0; p < S::VP; ++p) {
-                uint32_t vr[4][S::VW];
+            for (int p = 0; p < S::VB; ++p)
 #pragma unroll
-                for (int t = 0; t < 4; ++t) read_piece<S::VW>(vr[t], v_place(stage, mt, t, p));
+                for (int t = 0; t < 4; ++t) read_piece<S::VW>(batch[mt][p][t], v_place(place, mt, t, p0 + p));
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int p = p0; p < p0 + S::VB; ++p) {
+                const uint32_t(&vr)[4][S::VW] = batch[mt][p - p0];
                 if constexpr (K::f32) {
 #pragma unroll
                     for (int e = 0; e < S::VD; e += 2) {
@@ -677,6 +744,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, A
                         }
                 }
             }
+        }
     };
     auto clear_scores = [&]() {
 #pragma unroll
@@ -687,8 +755,9 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, A
                 for (int e = 0; e < 4; ++e) s[t][mt][e] = 0.f;
     };
 
-    for (int stage = 0; tb < end; tb += STEP, stage = S::stages == 1 ? 0 : (stage + 1 == S::stages ? 0 : stage + 1)) {
-        copy_wait<2 * S::stages - 1>();
+    int place = 0, turn = 0;
+    for (; tb < end; tb += STEP) {
+        copy_wait<S::units - 1>();
         float kt[MT][2], vt[MT][2];
         if constexpr (K::code) {
             __syncwarp();
@@ -696,30 +765,41 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, A
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    kt[mt][hf] = sm_s[stage][warp][0][16 * mt + 8 * hf + g];
-                    vt[mt][hf] = sm_s[stage][warp][1][16 * mt + 8 * hf + g];
+                    kt[mt][hf] = sm_s[turn][warp][0][16 * mt + 8 * hf + g];
+                    vt[mt][hf] = sm_s[turn][warp][1][16 * mt + 8 * hf + g];
                 }
             __syncwarp();
         }
         clear_scores();
-        scores(stage);
+        scores(place);
+        const int second = S::units == 3 && place == 2 ? 0 : place + 1;
         uint32_t now[S::NR];
 #pragma unroll
-        for (int r = 0; r < S::NR; ++r) {
-            now[r] = seen[0][r];
-#pragma unroll
-            for (int st = 0; st + 1 < S::stages; ++st) seen[st][r] = seen[st + 1][r];
+        for (int r = 0; r < S::NR; ++r) now[r] = seen[0][r], seen[0][r] = seen[1][r];
+        if constexpr (S::units == 3) {
+            if (tb + STEP < end) copy_v(place, r1);
+            copy_commit();
+        } else {
+            if (tb + STEP < end) copy_k(place, 0, r1, seen[0]);
+            copy_commit();
         }
-        const bool more = tb + S::stages * STEP < end;
-        if (more) copy_k(stage, rows, seen[S::stages - 1]);
-        copy_commit();
         softmax(now, kt, vt);
         turn_weights();
-        copy_wait<2 * S::stages - 1>();
-        values(stage);
-        if (more) copy_v(stage, rows);
-        copy_commit();
-        look_up(rows, tb + (S::stages + 1) * STEP);
+        copy_wait<S::units - 1>();
+        values(second);
+        if constexpr (S::units == 3) {
+            if (tb + 2 * STEP < end) copy_k(second, turn, r2, seen[1]);
+            copy_commit();
+#pragma unroll
+            for (int r = 0; r < S::NR; ++r) r1[r] = r2[r];
+            look_up(r2, tb + 3 * STEP);
+            turn ^= 1;
+            place = place == 0 ? 2 : place - 1;          // (place + 2) % 3
+        } else {
+            if (tb + STEP < end) copy_v(second, r1);
+            copy_commit();
+            look_up(r1, tb + 2 * STEP);
+        }
     }
     copy_wait<0>();
     __syncthreads();             // the ring now takes the warps' sums
@@ -744,6 +824,13 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, A
         }
     __syncthreads();
     const int64_t row0 = (i * a.b + b) * a.hq + (int64_t)kh * a.group + h0;
+    const bool last = a.cluster == 1;                 // nothing to join within a cluster
+    const bool whole = rg.active <= a.cluster;        // nothing to join after it
+    const int group = split / a.cluster;
+    auto put = [&](int h, int ch, float o, float total) {
+        if (whole) store_out(a.out, (row0 + h) * a.d + ch, total == 0.f ? 0.f : o / total, a.dtype);
+        else a.part_o[((row0 + h) * a.groups + group) * a.d + ch] = o;
+    };
     for (int h = warp; h < heads; h += kDecodeWarps) {
         float top = sm_m[0][h];
 #pragma unroll
@@ -755,23 +842,59 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, A
             total += ex2(sm_m[w][h] - ref) * sm_l[w][h];
             f[w] = ex2(sm_m[w][h] - ref - K::lift);
         }
-        const bool whole = rg.active <= 1;
-        const float inv = whole ? (total == 0.f ? 0.f : 1.f / total) : 1.f;
         for (int ch = lane; ch < a.d; ch += 32) {
             float o = 0.f;
 #pragma unroll
             for (int w = 0; w < kDecodeWarps; ++w) o += f[w] * sm_o[w][h][ch];
-            if (whole) store_out(a.out, (row0 + h) * a.d + ch, o * inv, a.dtype);
-            else a.part_o[((row0 + h) * a.splits + split) * a.d + ch] = o;
+            if (last) put(h, ch, o, total);
+            else sm_o[0][h][ch] = o;                  // in place: this thread alone reads and writes it
         }
-        if (!whole && lane == 0) a.part_ml[(row0 + h) * a.splits + split] = make_float2(top, total);
+        if (lane == 0) {
+            if (last && !whole) a.part_ml[(row0 + h) * a.groups + group] = make_float2(top, total);
+            sm_ml[h] = make_float2(top, total);
+        }
     }
+    if (last) return;
+    __syncwarp();
+
+    // --- join the cluster's ranges: each block reads its share of the
+    // channels from all blocks' shared memory, in the order of the ranges
+    sm100::cluster_sync_all();
+    const int rank = split % a.cluster;
+    const int ranks = min(a.cluster, rg.active - group * a.cluster);
+    for (int e = threadIdx.x; e < ranks * 8 * NT; e += 32 * kDecodeWarps) {
+        const uint32_t at = sm100::map_to_rank(sm100::smem_addr(&sm_ml[e % (8 * NT)]), e / (8 * NT));
+        float x, y;
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x), "=f"(y) : "r"(at) : "memory");
+        sm_all[e / (8 * NT)][e % (8 * NT)] = make_float2(x, y);
+    }
+    __syncthreads();
+    for (int e = rank * 32 * kDecodeWarps + threadIdx.x; e < heads * a.d; e += a.cluster * 32 * kDecodeWarps) {
+        const int h = e / a.d, ch = e - h * a.d;
+        float top = -INFINITY;
+        for (int r = 0; r < ranks; ++r) top = fmaxf(top, sm_all[r][h].x);
+        const float ref = top == -INFINITY ? 0.f : top;
+        const uint32_t at = sm100::smem_addr(&sm_o[0][h][ch]);
+        float o = 0.f, total = 0.f;
+#pragma unroll 4
+        for (int r = 0; r < ranks; ++r) {
+            float x;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(sm100::map_to_rank(at, r)) : "memory");
+            const float f = ex2(sm_all[r][h].x - ref);
+            o += f * x;
+            total += f * sm_all[r][h].y;
+        }
+        put(h, ch, o, total);
+        if (!whole && ch == 0) a.part_ml[(row0 + h) * a.groups + group] = make_float2(top, total);
+    }
+    __syncwarp();
+    sm100::cluster_sync_all();           // no block leaves while others read its sums
 }
 
-template <int KIND, int DP, int NT, bool ALIGNED, bool SPLITQ>
+template <int KIND, int DP, int NT, int ROWS, bool SPLITQ>
 int launch_decode_shape(const DecodeArgs& a, cudaStream_t st) {
-    using S = DecodeShape<KIND, DP, NT, ALIGNED, SPLITQ>;
-    auto kernel = decode_kernel<KIND, DP, NT, ALIGNED, SPLITQ>;
+    using S = DecodeShape<KIND, DP, NT, ROWS, SPLITQ>;
+    auto kernel = decode_kernel<KIND, DP, NT, ROWS, SPLITQ>;
     static std::atomic<uint64_t> allowed{0};      // devices whose limit is raised
     const uint64_t bit = 1ull << (current_device() & 63);
     if (!(allowed.load(std::memory_order_relaxed) & bit)) {
@@ -781,8 +904,19 @@ int launch_decode_shape(const DecodeArgs& a, cudaStream_t st) {
                              cudaGetErrorString(e));
         allowed.fetch_or(bit, std::memory_order_relaxed);
     }
-    const dim3 grid((unsigned)((int64_t)a.n * a.b * a.hk * a.tiles), (unsigned)a.splits);
-    kernel<<<grid, 32 * kDecodeWarps, S::smem, st>>>(a);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)((int64_t)a.n * a.b * a.hk * a.tiles), (unsigned)a.splits);
+    cfg.blockDim = dim3(32 * kDecodeWarps);
+    cfg.dynamicSmemBytes = S::smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = (unsigned)a.cluster;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.cluster > 1 ? 1 : 0;
+    cudaLaunchKernelEx(&cfg, kernel, a);
     return check_launch("widek_decode_attention_fwd");
 }
 
@@ -797,13 +931,20 @@ inline int decode_unit(int d, int fmt) {
     return kDecodeWarps * 16 * (bytes >= 256 ? 1 : 256 / bytes);
 }
 
+// Blocks of an SM, as DecodeShape has them (fp32 queries over codes: 2, not 4).
+inline int decode_places(int d, int fmt, int nt) {
+    const int bytes = (d <= 64 ? 64 : (d <= 128 ? 128 : 256)) * (int)cache_fmt_size(fmt);
+    return bytes > 512 ? 1 : (bytes > 256 || nt == 2 || d > 128 ? 2 : (fmt == WIDEK_F32 ? 3 : 4));
+}
+
 template <int KIND, bool SPLITQ>
 int launch_decode(const DecodeArgs& a, cudaStream_t st) {
     const bool aligned = (a.d * Kind<KIND>::size) % 16 == 0 && aligned16(a.c.k) && aligned16(a.c.v);
     const int nt = decode_nt(a.group, a.d, a.fmt);
-#define WIDEK_DECODE(DP, NT)                                                     \
-    return aligned ? launch_decode_shape<KIND, DP, NT, true, SPLITQ>(a, st)      \
-                   : launch_decode_shape<KIND, DP, NT, false, SPLITQ>(a, st)
+#define WIDEK_DECODE(DP, NT)                                                             \
+    return !aligned    ? launch_decode_shape<KIND, DP, NT, ROWS_ANY, SPLITQ>(a, st)      \
+           : a.d == DP ? launch_decode_shape<KIND, DP, NT, ROWS_FULL, SPLITQ>(a, st)     \
+                       : launch_decode_shape<KIND, DP, NT, ROWS_16, SPLITQ>(a, st)
     if constexpr (KIND != DK_F32) {
         if (nt == 2 && a.d <= 64) WIDEK_DECODE(64, 2);
         if (nt == 2) WIDEK_DECODE(128, 2);

@@ -40,7 +40,7 @@ int cache_args(PagedCache& c, const char* what, void* k, void* v, float* ks, flo
     if (page > 0x7fffffff || cols > 0x7fffffff || (hk > 0 && pages > 0x7fffffff / hk / page))
         return set_error(WIDEK_ERR_INVALID, "%s: one model's pool holds over 2^31 rows (pages=%lld, heads=%lld, "
                          "page=%lld)", what, (long long)pages, (long long)hk, (long long)page);
-    if (cols * page > 0x7fff0000)       // positions and the tiles past them stay 32-bit numbers
+    if (cols * page > 0x7f000000)       // positions and the tiles past them stay 32-bit numbers
         return set_error(WIDEK_ERR_INVALID, "%s: a sequence spans about 2^31 tokens or more", what);
     if (calls > 0 && hk > 0 && d > 0 && pages > 0 && cols > 0 && (!k || !v || !table || (cache_fmt_8bit(fmt) && (!ks || !vs))))
         return set_error(WIDEK_ERR_INVALID, "%s: null cache pointer", what);
