@@ -8,43 +8,82 @@
 namespace widek {
 namespace {
 
-constexpr int kJoinWarps = 4;
-constexpr int kMostSplits = 512;
+constexpr int kJoinWarps = 8;
+// Sequences whose steps every block adds up to find its place in line (32 for
+// each thread).
+constexpr int kMostInLine = 4096;
 
-// out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s over the groups of a
-// sequence's ranges, in their order; one warp per query head. Sequences of one
-// group were finished by the attention itself.
+// out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c over the blocks c that a
+// segment lies in, in their order; W warps for each query head. Segments that
+// lie in one block were finished by the attention itself.
+template <int W>
 __global__ void __launch_bounds__(32 * kJoinWarps) decode_join_kernel(const __grid_constant__ DecodeArgs a) {
+    __shared__ float red[W > 1 ? W : 1][W > 1 ? 256 : 1];
+    __shared__ float2 red_ml[W > 1 ? W : 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = W > 1 ? warp : 0;
+    const int64_t last = (int64_t)a.n * a.b * a.hq - 1;
+    const int64_t row = min((int64_t)blockIdx.x * (kJoinWarps / W) + warp / W, last);     // the same for a head's warps
+    // the segment's place in line, while the attention still runs
+    const int nb = (int)(row / a.hq), h = (int)(row - (int64_t)nb * a.hq), in_group = h % a.group;
+    const int sequences = a.n * a.b, per_seq = a.hk * a.tiles;
+    const int hp = h / a.group * a.tiles + in_group / (8 * a.nt);
+    long long before = 0, all = 0;
+    for (int s = lane; s < sequences; s += 32) {
+        const int n = DecodeRange(a, s).steps(a.step);
+        all += n;
+        if (s < nb) before += n;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        all += __shfl_xor_sync(0xffffffffu, all, o);
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+    }
+    const long long per = (all * per_seq + a.blocks - 1) / a.blocks;
+    const int n = DecodeRange(a, nb).steps(a.step);
+    const long long f0 = before * per_seq + (long long)hp * n;
+    const int c0 = (int)(f0 / per), c1 = (int)((f0 + n - 1) / per);
     sm100::grid_dep_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * kJoinWarps + (threadIdx.x >> 5), nb = row / a.hq;
-    if (row >= (int64_t)a.n * a.b * a.hq) return;
-    const DecodeRange rg(a, nb / a.b, nb % a.b);
-    if (rg.active <= a.cluster) return;
-    const int groups = (rg.active + a.cluster - 1) / a.cluster;
-    const float2* ml = a.part_ml + row * a.groups;
+    if (c0 == c1 || (W == 1 && (int64_t)blockIdx.x * kJoinWarps + warp > last)) return;
+    // a block's part 0 is the segment it starts in
+    const int late = f0 > c0 * per ? 1 : 0;
+    auto place = [&](int c) {
+        return ((int64_t)c * 2 + (c == c0 ? late : 0)) * 8 * a.nt + in_group % (8 * a.nt);
+    };
     float top = -INFINITY;
-    for (int s = lane; s < groups; s += 32) top = fmaxf(top, ml[s].x);
+    for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, a.part_ml[place(c)].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float ref = top == -INFINITY ? 0.f : top;
     float total = 0.f, acc[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-    const float* po = a.part_o + row * a.groups * a.d;
-#pragma unroll 8
-    for (int s = 0; s < groups; ++s) {
-        const float2 x = ml[s];
+#pragma unroll 4
+    for (int c = c0 + part; c <= c1; c += W) {
+        const int64_t at = place(c);
+        const float2 x = a.part_ml[at];
         const float f = ex2(x.x - ref);
         total += f * x.y;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (lane + 32 * j < a.d) acc[j] += f * po[(int64_t)s * a.d + lane + 32 * j];
+            if (lane + 32 * j < a.d) acc[j] += f * a.part_o[at * a.d + lane + 32 * j];
     }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
+    if constexpr (W > 1) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (lane + 32 * j < a.d) store_out(a.out, row * a.d + lane + 32 * j, acc[j] * inv, a.dtype);
+        for (int j = 0; j < 8; ++j) red[warp][lane + 32 * j] = acc[j];
+        if (lane == 0) red_ml[warp] = make_float2(0.f, total);
+        __syncthreads();
+        for (int ch = threadIdx.x; ch < a.d; ch += 32 * W) {
+            float o = 0.f, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) o += red[w][ch], sum += red_ml[w].y;
+            store_out(a.out, row * a.d + ch, sum == 0.f ? 0.f : o / sum, a.dtype);
+        }
+    } else {
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (lane + 32 * j < a.d) store_out(a.out, row * a.d + lane + 32 * j, acc[j] * inv, a.dtype);
+    }
 }
 
 int decode_args(DecodeArgs& a, const char* what, const int64_t* g, const int64_t* cgeom, int64_t window, int fmt) {
@@ -66,31 +105,24 @@ int decode_args(DecodeArgs& a, const char* what, const int64_t* g, const int64_t
     a.window = window > 0x7fffffff ? 0x7fffffff : (int)window;
     a.fmt = fmt;
     a.err = device_error_ptr();
-    const int nt = decode_nt(a.group, a.d, fmt);
-    a.tiles = (a.group + 8 * nt - 1) / (8 * nt);
-    // Ranges of a sequence. The host does not know the lengths, only the most
-    // tokens that a table row holds. Fewer blocks than the GPU has places: as many ranges as fill them once, of one tile for each warp or
-    // more. More blocks: ranges for six rounds, which evens out ragged lengths
-    // and the last round, as long as they keep 1024 tokens to start up for.
-    const int64_t blocks = (int64_t)a.n * a.b * a.hk * a.tiles;
-    const int64_t places = decode_places(a.d, fmt, nt) * (int64_t)sm_count(current_device());
+    a.nt = decode_nt(a.group, a.d, fmt);
+    a.tiles = (a.group + 8 * a.nt - 1) / (8 * a.nt);
+    a.step = decode_step(a.d, fmt);
+    // As many blocks as the GPU holds, or as there can be steps: the host does
+    // not know the lengths, only the most tokens that a table row holds.
     const double span = (double)cgeom[1] * (double)cgeom[2];
-    int64_t tokens = span > 2147418112.0 ? 2147418112 : (int64_t)span;      // the cache's own check refuses such a span
+    int64_t tokens = span > 2130706432.0 ? 2130706432 : (int64_t)span;      // the cache's check refuses larger ones
     if (a.window > 0 && a.window < tokens) tokens = a.window;
-    a.unit = decode_unit(a.d, fmt);
-    int64_t splits = 1;
-    if (blocks > 0 && blocks < places) splits = std::min(places / blocks, (tokens + a.unit - 1) / a.unit);
-    else if (blocks > 0) splits = std::min((6 * places + blocks - 1) / blocks, tokens / 1024);
-    splits = std::max<int64_t>(1, std::min<int64_t>(splits, kMostSplits));
-    a.cluster = (int)std::min<int64_t>(splits, kMostCluster);
-    a.groups = (int)(splits / a.cluster);
-    a.splits = a.groups * a.cluster;
+    const int64_t segments = (int64_t)a.n * a.b * a.hk * a.tiles;
+    const int64_t steps = std::max<int64_t>(1, (tokens + a.step - 1) / a.step);
+    const int64_t places = (int64_t)decode_places(a.d, fmt, a.nt) * sm_count(current_device());
+    a.blocks = (int)(segments < places && segments * steps < places ? std::max<int64_t>(segments * steps, 1) : places);
+    // nothing to divide when every segment is one step, or too much to add up
+    a.in_turn = steps == 1 || (int64_t)a.n * a.b > kMostInLine;
     return WIDEK_OK;
 }
 
-int64_t part_rows(const DecodeArgs& a) {
-    return a.groups > 1 ? (int64_t)a.n * a.b * a.hq * a.groups : 0;
-}
+int64_t part_rows(const DecodeArgs& a) { return a.in_turn ? 0 : (int64_t)a.blocks * 2 * 8 * a.nt; }
 
 }  // namespace
 }  // namespace widek
@@ -140,10 +172,13 @@ extern "C" int widek_decode_attention_fwd(const void* q, const void* kc, const v
         rc = launch_decode<DK_F16, false>(a, st);
     else
         rc = launch_decode<DK_F32, false>(a, st);
-    if (rc != WIDEK_OK || a.groups == 1) return rc;
-    // the join's blocks are set up while the attention's last ones run
+    if (rc != WIDEK_OK || a.in_turn) return rc;
+    // The join is set up while the attention runs. A segment lies in about
+    // blocks / segments of them: more than 8, and its heads take 8 warps each.
+    const int64_t heads = (int64_t)a.n * a.b * a.hq;
+    const bool wide = a.blocks > 8 * (int64_t)a.n * a.b * a.hk * a.tiles;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(((int64_t)a.n * a.b * a.hq + kJoinWarps - 1) / kJoinWarps));
+    cfg.gridDim = dim3((unsigned)(wide ? heads : (heads + kJoinWarps - 1) / kJoinWarps));
     cfg.blockDim = dim3(32 * kJoinWarps);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -151,6 +186,7 @@ extern "C" int widek_decode_attention_fwd(const void* q, const void* kc, const v
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, decode_join_kernel, a);
+    if (wide) cudaLaunchKernelEx(&cfg, decode_join_kernel<kJoinWarps>, a);
+    else cudaLaunchKernelEx(&cfg, decode_join_kernel<1>, a);
     return check_launch("widek_decode_attention_fwd (join)");
 }

@@ -13,10 +13,19 @@
 // tcgen05 would be mostly padding, and the operands would have to pass through
 // shared memory, which the layout below avoids).
 //
-// Mapping. A block takes one key head of one sequence and up to 8 NT of its
-// query heads, over a range of tokens; its 4 warps take every 4th tile of
-// 16 MT tokens each, with their own running maxima and sums. Both products put
-// tokens or channels on the MMA's 16 rows and the query heads on its 8 columns:
+// Work. A segment is one key head of one sequence with up to 8 NT of its query
+// heads; it is walked in steps, a step being a tile of 16 MT tokens for each of
+// a block's 4 warps. All segments' steps stand in one line, which the blocks
+// (as many as the GPU holds) divide evenly: a block walks through segments of
+// any length without a pause, the copies running ahead of the products over
+// their borders. A segment that lies in several blocks leaves partial results,
+// at most two for each block, which a second kernel joins in their order. (One
+// block for each segment or fixed range lost 6.5 us of every block's life to
+// its start and end, 45 of 328 us at 1.6 GB of bf16 pages.) With more
+// sequences than are worth adding up, blocks take whole segments in turn.
+//
+// Mapping. Both products put tokens or channels on the MMA's 16 rows and the
+// query heads on its 8 columns, each warp with its own running maxima and sums:
 //   S^T [tokens, heads] = K q^T, O^T [channels, heads] += V^T P^T.
 // The channel order of a dot product is free, and so is the row order of O^T,
 // so each lane's operands are whole 16-byte pieces of cached rows: for K rows g
@@ -53,12 +62,12 @@ struct DecodeArgs {
     const void* q;
     const void* lengths;
     void* out;
-    float* part_o;               // [n b hq, groups, d] partial outputs (relative to their own maximum)
-    float2* part_ml;             // [n b hq, groups] maximum and sum
+    float* part_o;               // [blocks, 2, 8 NT, d] partial outputs (relative to their own maximum)
+    float2* part_ml;             // [blocks, 2, 8 NT] maximum and sum
     int64_t q_n, q_b, q_h, len_n, len_b;
     int n, b, hq, hk, d, group, len64, window, dtype, fmt;
-    int tiles, unit;             // query-head tiles of a group, tokens of a block's tiles
-    int splits, cluster, groups; // ranges of a sequence, joined in clusters of blocks, groups = splits / cluster
+    int nt, tiles, step;         // 8 nt query heads of a segment, tiles of a group, tokens of a step
+    int blocks, in_turn;         // blocks of the launch; whole segments in turn
     int q_vec;                   // query rows start at multiples of 16 bytes
     float scale_log2;            // scale * log2(e)
     PagedCache c;
@@ -66,26 +75,23 @@ struct DecodeArgs {
 };
 
 constexpr int kDecodeWarps = 4;
-constexpr int kMostCluster = 8;       // blocks of a cluster that any GPU of the architecture takes
 
-// Visible tokens of a sequence and its cut into ranges: the same for the
-// attention and the join.
+// Visible tokens of sequence nb.
 struct DecodeRange {
-    int start, len, chunk, active;
-    __device__ __forceinline__ DecodeRange(const DecodeArgs& a, int64_t i, int64_t b) {
+    int start, len;
+    __device__ __forceinline__ DecodeRange(const DecodeArgs& a, int nb) {
+        const int i = nb / a.b, b = nb - i * a.b;
         len = load_index(a.lengths, i * a.len_n + b * a.len_b, a.len64);
         const int most = a.c.cols * a.c.page;
         if (len > most) {
             len = most;
-            if (threadIdx.x == 0) raise_device_error(a.err, DEV_ERR_INDEX);
+            raise_device_error(a.err, DEV_ERR_INDEX);
         }
         if (len < 0) len = 0;
         start = a.window > 0 && len > a.window ? len - a.window : 0;
-        const int range = len - start;
-        chunk = (range + a.splits - 1) / a.splits;
-        chunk = max(1, (chunk + a.unit - 1) / a.unit) * a.unit;
-        active = (range + chunk - 1) / chunk;
     }
+    // Steps of one of its segments; an empty one has one, which writes zeros.
+    __device__ __forceinline__ int steps(int step) const { return max(1, (len - start + step - 1) / step); }
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -272,15 +278,9 @@ __device__ __forceinline__ void copy_piece(uint32_t dst, const uint8_t* row, int
     }
 }
 
-template <int W>
-__device__ __forceinline__ void read_piece(uint32_t (&r)[W], uint32_t src) {
-    if constexpr (W == 4)
-        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(src) : "memory");
-    else if constexpr (W == 2)
-        asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(src) : "memory");
-    else
-        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r[0]) : "r"(src) : "memory");
+__device__ __forceinline__ void read_piece(uint32_t (&r)[4], uint32_t src) {
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(src) : "memory");
 }
 
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -305,6 +305,7 @@ struct DecodeShape {
     static constexpr int VD = 16 / size < DP / 8 ? 16 / size : DP / 8;      // and of its V piece
     static constexpr int KP = DP / 4 / KD, VP = DP / 8 / VD;                // pieces of a row per lane
     static constexpr int KW = KD * size / 4, VW = VD * size / 4;            // words of a piece
+    static_assert(KW == 4 && (VW == 4 || (VW == 2 && VP == 1)), "pieces fill 16-byte places");
     static constexpr int KR = Kind<KIND>::f32 ? KD : KD / 2;                // MMA registers of a K piece
     static constexpr int QR = KP * KR;                                      // MMA registers of a query row
     // pieces read back from the ring at a time: 32 words, so that their latencies overlap
@@ -319,8 +320,7 @@ struct DecodeShape {
     static constexpr int ring = units * unit;
     static constexpr int blocks =                                           // of an SM
         row_bytes > 512 ? 1 : (row_bytes > 256 || NT == 2 || SPLITQ || DP == 256 ? 2 : (Kind<KIND>::f32 ? 3 : 4));
-    static constexpr int joined = kDecodeWarps * 8 * NT * (DP + 2) * 4;     // the warps' sums, over the ring
-    static constexpr int smem = ring > joined ? ring : joined;
+    static constexpr int JC = DP > 64 ? 2 : 1;                              // 16-channel tiles joined at a time
 };
 
 template <int KIND, int DP, int NT, int ROWS, bool SPLITQ>
@@ -330,61 +330,134 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
     using K = Kind<KIND>;
     constexpr int MT = S::MT, TOK = S::TOK;
     extern __shared__ __align__(16) uint8_t decode_ring[];
-    uint8_t* const ring = decode_ring;
     __shared__ float sm_m[kDecodeWarps][8 * NT], sm_l[kDecodeWarps][8 * NT];
-    __shared__ float2 sm_ml[8 * NT], sm_all[kMostCluster][8 * NT];
+    __shared__ float2 sm_t[8 * NT];
+    __shared__ float sm_o[kDecodeWarps][8 * NT][16 * S::JC + 2];
     // scales of the key and value rows of a tile and the next
     __shared__ float sm_s[2][kDecodeWarps][2][K::code ? TOK : 1];
-    float(*sm_o)[8 * NT][DP + 2] = reinterpret_cast<float(*)[8 * NT][DP + 2]>(ring);
+    __shared__ long long sm_sum[kDecodeWarps];
+    __shared__ int sm_at[3];
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, c = lane & 3;
-    const int tile = blockIdx.x % a.tiles;
-    const int kh = blockIdx.x / a.tiles % a.hk;
-    const int64_t nb = blockIdx.x / a.tiles / a.hk;
-    const int64_t i = nb / a.b, b = nb % a.b;
-    const DecodeRange rg(a, i, b);
-    if (a.groups > 1) sm100::grid_dep_launch_dependents();     // the join waits for this grid's end by itself
-    const int split = blockIdx.y;
-    // ranges that a short sequence does not have: their blocks are needed only
-    // by a cluster that has others
-    if (split >= rg.active && split / a.cluster * a.cluster >= max(rg.active, 1)) return;
-    const int first = rg.start + split * rg.chunk;
-    const int end = min(rg.len, first + rg.chunk);
-    const int h0 = tile * 8 * NT;                        // first query head of the group here
-    const int heads = min(8 * NT, a.group - h0);
+    constexpr int STEP = kDecodeWarps * TOK;
     const int bytes = a.d * S::size;
-    const int64_t pool = i * a.c.pages * a.hk * a.c.page;     // first row of this model's pool
-    const uint8_t* kbase = static_cast<const uint8_t*>(a.c.k) + pool * bytes;
-    const uint8_t* vbase = static_cast<const uint8_t*>(a.c.v) + pool * bytes;
+    const int64_t pool_rows = (int64_t)a.c.pages * a.hk * a.c.page;      // rows of one model's pool
     const bool words = ((bytes | reinterpret_cast<uintptr_t>(a.c.k) | reinterpret_cast<uintptr_t>(a.c.v)) & 3) == 0;
+    const int sequences = a.n * a.b, per_seq = a.hk * a.tiles;           // per_seq: segments of a sequence
+    if (!a.in_turn) sm100::grid_dep_launch_dependents();                 // the join waits for this grid's end by itself
+
+    // --- where this block's steps begin
+    struct Walk {
+        int nb, hp, pos, start, len, left;       // segment (nb, hp), token of the step, its range; steps still to do
+    };
+    Walk front;
+    if (a.in_turn) {
+        front.nb = blockIdx.x / per_seq;
+        front.hp = blockIdx.x - front.nb * per_seq;
+        front.left = front.nb < sequences ? 0x7fffffff : 0;
+    } else {
+        const int each = (sequences + 32 * kDecodeWarps - 1) / (32 * kDecodeWarps);
+        const int s0 = min(sequences, (int)threadIdx.x * each), s1 = min(sequences, s0 + each);
+        long long mine = 0;
+        for (int s = s0; s < s1; ++s) mine += DecodeRange(a, s).steps(STEP);
+        long long upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        if (lane == 31) sm_sum[warp] = upto;
+        __syncthreads();
+        long long all = 0;
+#pragma unroll
+        for (int w = 0; w < kDecodeWarps; ++w) {
+            if (w < warp) upto += sm_sum[w];
+            all += sm_sum[w];
+        }
+        all *= per_seq;
+        const long long per = (all + a.blocks - 1) / a.blocks, begin = per * blockIdx.x;
+        long long before = (upto - mine) * per_seq;
+        if (begin >= before && begin < upto * per_seq) {
+            for (int s = s0; s < s1; ++s) {
+                const int n = DecodeRange(a, s).steps(STEP);
+                if (begin < before + (long long)n * per_seq) {
+                    const int off = (int)(begin - before);
+                    sm_at[0] = s, sm_at[1] = off / n, sm_at[2] = off % n;
+                    break;
+                }
+                before += (long long)n * per_seq;
+            }
+        }
+        __syncthreads();
+        front.left = (int)max(0ll, min(per, all - begin));
+        front.nb = sm_at[0], front.hp = sm_at[1];
+    }
+    if (front.left <= 0) return;
+    auto enter = [&](Walk& w) {
+        const DecodeRange r(a, w.nb);
+        w.start = w.pos = r.start;
+        w.len = r.len;
+    };
+    enter(front);
+    if (!a.in_turn) front.pos += sm_at[2] * STEP;
+    Walk at = front;                             // the step whose products are next; `front` the one to look up
+    auto next_segment = [&](Walk& w) {
+        w.hp += a.in_turn ? a.blocks : 1;
+        if (w.hp >= per_seq) {
+            w.nb += w.hp / per_seq;
+            w.hp %= per_seq;
+        }
+        if (w.nb >= sequences) w.left = 0;
+        if (w.left > 0) enter(w);
+    };
 
     // --- token slots: lane holds those of tokens (lane + 32 r) of a tile; -1
     // past the end, -2 where the table names no page of the pool
-    auto look_up = [&](int (&rows)[S::NR], int tb) {
+    struct Slots {
+        int row[S::NR];
+        int model;
+    };
+    auto look_up = [&](Slots& x) {               // the step at `front`, which moves on
+        const int i = front.left > 0 ? front.nb / a.b : 0, kh = front.hp / a.tiles;
+        x.model = i;
 #pragma unroll
         for (int r = 0; r < S::NR; ++r) {
-            const int p = tb + (TOK < 32 ? lane & (TOK - 1) : lane + 32 * r);
-            rows[r] = p < end ? a.c.row(i, b, a.hk, kh, p) : -1;
-            if (p < end && rows[r] < 0) rows[r] = -2;
+            const int p = front.pos + warp * TOK + (TOK < 32 ? lane & (TOK - 1) : lane + 32 * r);
+            x.row[r] = -1;
+            if (front.left > 0 && p < front.len) {
+                x.row[r] = a.c.row(i, front.nb - i * a.b, a.hk, kh, p);
+                if (x.row[r] < 0) x.row[r] = -2;
+            }
+        }
+        if (front.left > 0) {
+            --front.left;
+            front.pos += STEP;
+            if (front.pos >= front.len) next_segment(front);
         }
     };
-    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring);
+    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(decode_ring);
     auto k_place = [&](int place, int mt, int hf, int p) {
         return mine + place * S::unit + (((mt * 2 + hf) * S::KP + p) * 32 * kDecodeWarps + threadIdx.x) * S::KW * 4;
     };
+    // the same 16-byte places as K's: a unit's space changes hands between the
+    // two without a barrier, so a thread's must be its own in both. V pieces of
+    // 8 bytes (64 channels of 8 bits) share one, those of tokens t and t + 1.
     auto v_place = [&](int place, int mt, int t, int p) {
-        return mine + place * S::unit + (((mt * 4 + t) * S::VP + p) * 32 * kDecodeWarps + threadIdx.x) * S::VW * 4;
+        const int word = ((mt * 4 + t) * S::VP + p) * S::VW;
+        return mine + place * S::unit + ((word / 4) * 32 * kDecodeWarps + threadIdx.x) * 16 + word % 4 * 4;
     };
     // K pieces of tokens g and g + 8 of every 16, the tile's scales, and a bit for each token that is there
-    auto copy_k = [&](int place, int turn, const int (&rows)[S::NR], uint32_t (&seen)[S::NR]) {
+    auto copy_k = [&](int place, int turn, const Slots& x, uint32_t (&seen)[S::NR]) {
+        const int64_t pool = x.model * pool_rows;
+        const uint8_t* kbase = static_cast<const uint8_t*>(a.c.k) + pool * bytes;
 #pragma unroll
         for (int r = 0; r < S::NR; ++r) {
-            seen[r] = __ballot_sync(0xffffffffu, rows[r] >= 0);
-            if (rows[r] == -2) raise_device_error(a.err, DEV_ERR_INDEX);
+            seen[r] = __ballot_sync(0xffffffffu, x.row[r] >= 0);
+            if (x.row[r] == -2) raise_device_error(a.err, DEV_ERR_INDEX);
             if constexpr (K::code) {
-                const int64_t at = pool + (rows[r] < 0 ? 0 : rows[r]);
-                const int n = rows[r] >= 0 ? 4 : 0, t = TOK < 32 ? lane & (TOK - 1) : lane + 32 * r;
+                const int64_t at = pool + (x.row[r] < 0 ? 0 : x.row[r]);
+                const int n = x.row[r] >= 0 ? 4 : 0, t = TOK < 32 ? lane & (TOK - 1) : lane + 32 * r;
                 asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
                                  (uint32_t)__cvta_generic_to_shared(&sm_s[turn][warp][0][t])),
                              "l"(a.c.ks + at), "r"(n) : "memory");
@@ -398,7 +471,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
                 // token 16 mt + 8 hf + g: the register that holds it is known at compile time, the lane is not
-                const int r = __shfl_sync(0xffffffffu, rows[S::NR == 1 ? 0 : mt >> 1], (16 * mt + 8 * hf + g) & 31);
+                const int r = __shfl_sync(0xffffffffu, x.row[S::NR == 1 ? 0 : mt >> 1], (16 * mt + 8 * hf + g) & 31);
                 const uint8_t* row = kbase + (int64_t)max(r, 0) * bytes;
 #pragma unroll
                 for (int p = 0; p < S::KP; ++p)
@@ -406,14 +479,15 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
                                                         bytes, words, r >= 0);
             }
     };
-    auto copy_v = [&](int place, const int (&rows)[S::NR]) {
+    auto copy_v = [&](int place, const Slots& x) {
+        const uint8_t* vbase = static_cast<const uint8_t*>(a.c.v) + x.model * pool_rows * bytes;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 // the k index of lane c: tokens 2c, 2c + 1, 2c + 8, 2c + 9; tf32 c, c + 4, c + 8, c + 12
                 const int tok = K::f32 ? c + 4 * t : 2 * c + (t & 1) + 8 * (t >> 1);
-                const int r = __shfl_sync(0xffffffffu, rows[S::NR == 1 ? 0 : mt >> 1], (16 * mt + tok) & 31);
+                const int r = __shfl_sync(0xffffffffu, x.row[S::NR == 1 ? 0 : mt >> 1], (16 * mt + tok) & 31);
                 const uint8_t* row = vbase + (int64_t)max(r, 0) * bytes;
 #pragma unroll
                 for (int p = 0; p < S::VP; ++p)
@@ -422,32 +496,34 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
             }
     };
 
-    constexpr int STEP = kDecodeWarps * TOK;
-    int tb = first + warp * TOK;
-    int r1[S::NR], r2[S::NR];                // slots of the next tile and of the one after it
-    uint32_t seen[2][S::NR];                 // tokens that are there, of the current tile and the next
+    Slots x1, x2;                            // slots of the next step and of the one after it
+    uint32_t seen[2][S::NR];                 // tokens that are there, of the current step and the next
     {
-        int r0[S::NR];
-        look_up(r0, tb);
-        look_up(r1, tb + STEP);
-        if constexpr (S::units == 3) look_up(r2, tb + 2 * STEP);
-        copy_k(0, 0, r0, seen[0]);
+        Slots x0;
+        look_up(x0);
+        look_up(x1);
+        if constexpr (S::units == 3) look_up(x2);
+        copy_k(0, 0, x0, seen[0]);
         copy_commit();
-        copy_v(1, r0);
+        copy_v(1, x0);
         copy_commit();
         if constexpr (S::units == 3) {
-            copy_k(2, 1, r1, seen[1]);
+            copy_k(2, 1, x1, seen[1]);
             copy_commit();
         }
     }
 
-    // --- query fragments: lane (g, c) holds head g's channels of its K pieces
+    // --- query fragments of a segment: lane (g, c) holds head g's channels of its K pieces
     uint32_t q[NT][S::QR], ql[SPLITQ ? NT : 1][SPLITQ ? S::QR : 1];
     float zs[NT][2];                                     // what a score is multiplied by, heads 2c and 2c + 1
+    auto load_queries = [&]() {
+        const int i = at.nb / a.b, kh = at.hp / a.tiles, h0 = (at.hp - kh * a.tiles) * 8 * NT;
+        const int heads = min(8 * NT, a.group - h0);
+        const int64_t base = i * a.q_n + (at.nb - i * a.b) * a.q_b + (int64_t)(kh * a.group + h0) * a.q_h;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const int h = t * 8 + g;
-        const int64_t at = i * a.q_n + b * a.q_b + (int64_t)(kh * a.group + h0 + (h < heads ? h : 0)) * a.q_h;
+        const int64_t at = base + (h < heads ? h : 0) * a.q_h;
         float x[S::KP][S::KD];
         float top = 0.f;
 #pragma unroll
@@ -492,17 +568,10 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
             }
     }
 
+    };
+
     float acc[NT][DP / 16][4];
     float m[NT][2], l[NT][2];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-#pragma unroll
-        for (int j = 0; j < DP / 16; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[t][j][e] = 0.f;
-        m[t][0] = m[t][1] = -INFINITY;
-        l[t][0] = l[t][1] = 0.f;
-    }
 
     // S^T += K q^T over the pieces in registers
     float s[NT][MT][4];
@@ -515,7 +584,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
 #pragma unroll
             for (int p = 0; p < S::KB; ++p)
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) read_piece<S::KW>(batch[mt][p][hf], k_place(place, mt, hf, p0 + p));
+                for (int hf = 0; hf < 2; ++hf) read_piece(batch[mt][p][hf], k_place(place, mt, hf, p0 + p));
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -672,7 +741,16 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
 #pragma unroll
             for (int p = 0; p < S::VB; ++p)
 #pragma unroll
-                for (int t = 0; t < 4; ++t) read_piece<S::VW>(batch[mt][p][t], v_place(place, mt, t, p0 + p));
+                for (int t = 0; t < 4; ++t) {
+                    if constexpr (S::VW == 4) {
+                        read_piece(batch[mt][p][t], v_place(place, mt, t, p0 + p));
+                    } else if (t % 2 == 0) {
+                        uint32_t two[4];
+                        read_piece(two, v_place(place, mt, t, p0 + p));
+                        batch[mt][p][t][0] = two[0], batch[mt][p][t][1] = two[1];
+                        batch[mt][p][t + 1][0] = two[2], batch[mt][p][t + 1][1] = two[3];
+                    }
+                }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -755,140 +833,134 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
                 for (int e = 0; e < 4; ++e) s[t][mt][e] = 0.f;
     };
 
-    int place = 0, turn = 0;
-    for (; tb < end; tb += STEP) {
-        copy_wait<S::units - 1>();
-        float kt[MT][2], vt[MT][2];
-        if constexpr (K::code) {
-            __syncwarp();
+    // --- the end of a segment (or of this block's part of it): join the warps
+    auto finish = [&](bool whole, int part) {
+        const int kh = at.hp / a.tiles, h0 = (at.hp - kh * a.tiles) * 8 * NT;
+        const int heads = min(8 * NT, a.group - h0);
+        const int64_t row0 = (int64_t)at.nb * a.hq + kh * a.group + h0;
+        const int64_t part0 = ((int64_t)blockIdx.x * 2 + part) * 8 * NT;
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    kt[mt][hf] = sm_s[turn][warp][0][16 * mt + 8 * hf + g];
-                    vt[mt][hf] = sm_s[turn][warp][1][16 * mt + 8 * hf + g];
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], o);
+                if (g == 0) {
+                    sm_m[warp][t * 8 + 2 * c + e] = m[t][e];
+                    sm_l[warp][t * 8 + 2 * c + e] = l[t][e];
                 }
-            __syncwarp();
-        }
-        clear_scores();
-        scores(place);
-        const int second = S::units == 3 && place == 2 ? 0 : place + 1;
-        uint32_t now[S::NR];
+            }
+        __syncthreads();
+        float f[NT][2];
 #pragma unroll
-        for (int r = 0; r < S::NR; ++r) now[r] = seen[0][r], seen[0][r] = seen[1][r];
-        if constexpr (S::units == 3) {
-            if (tb + STEP < end) copy_v(place, r1);
-            copy_commit();
-        } else {
-            if (tb + STEP < end) copy_k(place, 0, r1, seen[0]);
-            copy_commit();
-        }
-        softmax(now, kt, vt);
-        turn_weights();
-        copy_wait<S::units - 1>();
-        values(second);
-        if constexpr (S::units == 3) {
-            if (tb + 2 * STEP < end) copy_k(second, turn, r2, seen[1]);
-            copy_commit();
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int r = 0; r < S::NR; ++r) r1[r] = r2[r];
-            look_up(r2, tb + 3 * STEP);
-            turn ^= 1;
-            place = place == 0 ? 2 : place - 1;          // (place + 2) % 3
-        } else {
-            if (tb + STEP < end) copy_v(second, r1);
-            copy_commit();
-            look_up(r1, tb + 2 * STEP);
+            for (int e = 0; e < 2; ++e) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kDecodeWarps; ++w) top = fmaxf(top, sm_m[w][t * 8 + 2 * c + e]);
+                f[t][e] = ex2(m[t][e] - (top == -INFINITY ? 0.f : top) - K::lift);
+            }
+        if (threadIdx.x < heads) {
+            float top = -INFINITY, total = 0.f;
+#pragma unroll
+            for (int w = 0; w < kDecodeWarps; ++w) top = fmaxf(top, sm_m[w][threadIdx.x]);
+#pragma unroll
+            for (int w = 0; w < kDecodeWarps; ++w)
+                total += ex2(sm_m[w][threadIdx.x] - (top == -INFINITY ? 0.f : top)) * sm_l[w][threadIdx.x];
+            sm_t[threadIdx.x] = make_float2(top, total);
+            if (!whole) a.part_ml[part0 + threadIdx.x] = make_float2(top, total);
         }
+#pragma unroll
+        for (int j0 = 0; j0 < DP / 16; j0 += S::JC) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int jj = 0; jj < S::JC; ++jj)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        *reinterpret_cast<float2*>(&sm_o[warp][t * 8 + 2 * c + e][jj * 16 + 2 * g]) =
+                            make_float2(acc[t][j0 + jj][e] * f[t][e], acc[t][j0 + jj][e + 2] * f[t][e]);
+            __syncthreads();
+            for (int e = threadIdx.x; e < heads * 16 * S::JC; e += 32 * kDecodeWarps) {
+                const int h = e / (16 * S::JC), x = e % (16 * S::JC), j = j0 + x / 16;
+                const int ch = j / (S::VD / 2) * 8 * S::VD + x % 16 / 2 * S::VD + j % (S::VD / 2) * 2 + (x & 1);
+                if (ROWS != ROWS_FULL && ch >= a.d) continue;
+                float o = 0.f;
+#pragma unroll
+                for (int w = 0; w < kDecodeWarps; ++w) o += sm_o[w][h][x];
+                const float total = sm_t[h].y;
+                if (whole) store_out(a.out, (row0 + h) * a.d + ch, total == 0.f ? 0.f : o / total, a.dtype);
+                else a.part_o[(part0 + h) * a.d + ch] = o;
+            }
+            __syncthreads();
+        }
+    };
+
+    int place = 0, turn = 0, part = 0;
+    while (at.left > 0) {
+        load_queries();
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int j = 0; j < DP / 16; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[t][j][e] = 0.f;
+            m[t][0] = m[t][1] = -INFINITY;
+            l[t][0] = l[t][1] = 0.f;
+        }
+        const int entered = at.pos;
+        do {
+            copy_wait<S::units - 1>();
+            float kt[MT][2], vt[MT][2];
+            if constexpr (K::code) {
+                __syncwarp();
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        kt[mt][hf] = sm_s[turn][warp][0][16 * mt + 8 * hf + g];
+                        vt[mt][hf] = sm_s[turn][warp][1][16 * mt + 8 * hf + g];
+                    }
+                __syncwarp();
+            }
+            uint32_t now[S::NR], any = 0;
+#pragma unroll
+            for (int r = 0; r < S::NR; ++r) now[r] = seen[0][r], any |= now[r], seen[0][r] = seen[1][r];
+            const int second = S::units == 3 && place == 2 ? 0 : place + 1;
+            if (any) {
+                clear_scores();
+                scores(place);
+            }
+            if constexpr (S::units == 3) copy_v(place, x1);
+            else copy_k(place, 0, x1, seen[0]);
+            copy_commit();
+            if (any) {
+                softmax(now, kt, vt);
+                turn_weights();
+            }
+            copy_wait<S::units - 1>();
+            if (any) values(second);
+            if constexpr (S::units == 3) {
+                copy_k(second, turn, x2, seen[1]);
+                copy_commit();
+                x1 = x2;
+                look_up(x2);
+                turn ^= 1;
+                place = place == 0 ? 2 : place - 1;          // (place + 2) % 3
+            } else {
+                copy_v(second, x1);
+                copy_commit();
+                look_up(x1);
+            }
+            --at.left;
+            at.pos += STEP;
+        } while (at.pos < at.len && at.left > 0);
+        finish(entered == at.start && at.pos >= at.len, part);
+        part = 1;
+        if (at.left > 0) next_segment(at);
     }
     copy_wait<0>();
-    __syncthreads();             // the ring now takes the warps' sums
-
-    // --- join the warps
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], o);
-            if (g == 0) {
-                const int h = t * 8 + 2 * c + e;
-                sm_m[warp][h] = m[t][e];
-                sm_l[warp][h] = l[t][e];
-            }
-#pragma unroll
-            for (int j = 0; j < DP / 16; ++j) {
-                const int ch = j / (S::VD / 2) * 8 * S::VD + g * S::VD + j % (S::VD / 2) * 2;
-                *reinterpret_cast<float2*>(&sm_o[warp][t * 8 + 2 * c + e][ch]) = make_float2(acc[t][j][e], acc[t][j][e + 2]);
-            }
-        }
-    __syncthreads();
-    const int64_t row0 = (i * a.b + b) * a.hq + (int64_t)kh * a.group + h0;
-    const bool last = a.cluster == 1;                 // nothing to join within a cluster
-    const bool whole = rg.active <= a.cluster;        // nothing to join after it
-    const int group = split / a.cluster;
-    auto put = [&](int h, int ch, float o, float total) {
-        if (whole) store_out(a.out, (row0 + h) * a.d + ch, total == 0.f ? 0.f : o / total, a.dtype);
-        else a.part_o[((row0 + h) * a.groups + group) * a.d + ch] = o;
-    };
-    for (int h = warp; h < heads; h += kDecodeWarps) {
-        float top = sm_m[0][h];
-#pragma unroll
-        for (int w = 1; w < kDecodeWarps; ++w) top = fmaxf(top, sm_m[w][h]);
-        const float ref = top == -INFINITY ? 0.f : top;
-        float total = 0.f, f[kDecodeWarps];
-#pragma unroll
-        for (int w = 0; w < kDecodeWarps; ++w) {
-            total += ex2(sm_m[w][h] - ref) * sm_l[w][h];
-            f[w] = ex2(sm_m[w][h] - ref - K::lift);
-        }
-        for (int ch = lane; ch < a.d; ch += 32) {
-            float o = 0.f;
-#pragma unroll
-            for (int w = 0; w < kDecodeWarps; ++w) o += f[w] * sm_o[w][h][ch];
-            if (last) put(h, ch, o, total);
-            else sm_o[0][h][ch] = o;                  // in place: this thread alone reads and writes it
-        }
-        if (lane == 0) {
-            if (last && !whole) a.part_ml[(row0 + h) * a.groups + group] = make_float2(top, total);
-            sm_ml[h] = make_float2(top, total);
-        }
-    }
-    if (last) return;
-    __syncwarp();
-
-    // --- join the cluster's ranges: each block reads its share of the
-    // channels from all blocks' shared memory, in the order of the ranges
-    sm100::cluster_sync_all();
-    const int rank = split % a.cluster;
-    const int ranks = min(a.cluster, rg.active - group * a.cluster);
-    for (int e = threadIdx.x; e < ranks * 8 * NT; e += 32 * kDecodeWarps) {
-        const uint32_t at = sm100::map_to_rank(sm100::smem_addr(&sm_ml[e % (8 * NT)]), e / (8 * NT));
-        float x, y;
-        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x), "=f"(y) : "r"(at) : "memory");
-        sm_all[e / (8 * NT)][e % (8 * NT)] = make_float2(x, y);
-    }
-    __syncthreads();
-    for (int e = rank * 32 * kDecodeWarps + threadIdx.x; e < heads * a.d; e += a.cluster * 32 * kDecodeWarps) {
-        const int h = e / a.d, ch = e - h * a.d;
-        float top = -INFINITY;
-        for (int r = 0; r < ranks; ++r) top = fmaxf(top, sm_all[r][h].x);
-        const float ref = top == -INFINITY ? 0.f : top;
-        const uint32_t at = sm100::smem_addr(&sm_o[0][h][ch]);
-        float o = 0.f, total = 0.f;
-#pragma unroll 4
-        for (int r = 0; r < ranks; ++r) {
-            float x;
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(sm100::map_to_rank(at, r)) : "memory");
-            const float f = ex2(sm_all[r][h].x - ref);
-            o += f * x;
-            total += f * sm_all[r][h].y;
-        }
-        put(h, ch, o, total);
-        if (!whole && ch == 0) a.part_ml[(row0 + h) * a.groups + group] = make_float2(top, total);
-    }
-    __syncwarp();
-    sm100::cluster_sync_all();           // no block leaves while others read its sums
 }
 
 template <int KIND, int DP, int NT, int ROWS, bool SPLITQ>
@@ -898,25 +970,13 @@ int launch_decode_shape(const DecodeArgs& a, cudaStream_t st) {
     static std::atomic<uint64_t> allowed{0};      // devices whose limit is raised
     const uint64_t bit = 1ull << (current_device() & 63);
     if (!(allowed.load(std::memory_order_relaxed) & bit)) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::ring);
         if (e != cudaSuccess)
-            return set_error(WIDEK_ERR_CUDA, "widek_decode_attention_fwd: shared memory of %d bytes: %s", S::smem,
+            return set_error(WIDEK_ERR_CUDA, "widek_decode_attention_fwd: shared memory of %d bytes: %s", S::ring,
                              cudaGetErrorString(e));
         allowed.fetch_or(bit, std::memory_order_relaxed);
     }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)((int64_t)a.n * a.b * a.hk * a.tiles), (unsigned)a.splits);
-    cfg.blockDim = dim3(32 * kDecodeWarps);
-    cfg.dynamicSmemBytes = S::smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1;
-    attr[0].val.clusterDim.y = (unsigned)a.cluster;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = a.cluster > 1 ? 1 : 0;
-    cudaLaunchKernelEx(&cfg, kernel, a);
+    kernel<<<(unsigned)a.blocks, 32 * kDecodeWarps, S::ring, st>>>(a);
     return check_launch("widek_decode_attention_fwd");
 }
 
@@ -925,8 +985,8 @@ int launch_decode_shape(const DecodeArgs& a, cudaStream_t st) {
 // split operands of fp32, their sums would not fit in registers beside the tile.
 inline int decode_nt(int group, int d, int fmt) { return group > 8 && d <= 128 && fmt != WIDEK_F32 ? 2 : 1; }
 
-// Tokens that the 4 warps of a block have in registers at a time.
-inline int decode_unit(int d, int fmt) {
+// Tokens of a step.
+inline int decode_step(int d, int fmt) {
     const int bytes = (d <= 64 ? 64 : (d <= 128 ? 128 : 256)) * (int)cache_fmt_size(fmt);
     return kDecodeWarps * 16 * (bytes >= 256 ? 1 : 256 / bytes);
 }
@@ -940,14 +1000,13 @@ inline int decode_places(int d, int fmt, int nt) {
 template <int KIND, bool SPLITQ>
 int launch_decode(const DecodeArgs& a, cudaStream_t st) {
     const bool aligned = (a.d * Kind<KIND>::size) % 16 == 0 && aligned16(a.c.k) && aligned16(a.c.v);
-    const int nt = decode_nt(a.group, a.d, a.fmt);
-#define WIDEK_DECODE(DP, NT)                                                             \
+    #define WIDEK_DECODE(DP, NT)                                                             \
     return !aligned    ? launch_decode_shape<KIND, DP, NT, ROWS_ANY, SPLITQ>(a, st)      \
            : a.d == DP ? launch_decode_shape<KIND, DP, NT, ROWS_FULL, SPLITQ>(a, st)     \
                        : launch_decode_shape<KIND, DP, NT, ROWS_16, SPLITQ>(a, st)
     if constexpr (KIND != DK_F32) {
-        if (nt == 2 && a.d <= 64) WIDEK_DECODE(64, 2);
-        if (nt == 2) WIDEK_DECODE(128, 2);
+        if (a.nt == 2 && a.d <= 64) WIDEK_DECODE(64, 2);
+        if (a.nt == 2) WIDEK_DECODE(128, 2);
     }
     if (a.d <= 64) WIDEK_DECODE(64, 1);
     if (a.d <= 128) WIDEK_DECODE(128, 1);
