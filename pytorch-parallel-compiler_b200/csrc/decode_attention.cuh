@@ -30,12 +30,14 @@
 // The channel order of a dot product is free, and so is the row order of O^T,
 // so each lane's operands are whole 16-byte pieces of cached rows: for K rows g
 // and g + 8 of the tile (g = lane / 4), 4 lanes side by side; for V 4 tokens, 8
-// lanes side by side, token pairs joined by byte permutes. Each thread copies
-// its own pieces into its own places of shared memory (cp.async, zeros for
-// tokens and channels that are not there) and reads them back itself, so the
-// ring needs no barrier and no swizzle: it only holds what is in flight, about
-// 190 KB on an SM. Held in registers instead, one tile ahead, the same loop
-// reached 3.5 of 6.5 TB/s: other instructions waited on the loads' scoreboards.
+// lanes side by side, token pairs joined by byte permutes: no ldmatrix, no
+// transposed copy. Each warp copies its own tiles into its own part of a ring
+// in shared memory (cp.async of whole lines, zeros for tokens and channels that
+// are not there), so the ring needs no barrier beyond the warp; it holds what
+// is in flight, 128 KB and more on an SM. (Held in registers, one tile ahead,
+// the loop reached 3.5 of 6.5 TB/s: other instructions waited on the loads'
+// scoreboards. Copied by each lane for itself, 64 bytes of a row in a request,
+// it stopped at 4.4 to 5.2 TB/s: the SM's requests in flight ran out.)
 // The weights change layout (tokens from rows to the contraction) by 8x8
 // transposes within the warp.
 //
@@ -238,33 +240,28 @@ __device__ __forceinline__ uint32_t code_word(uint32_t w) {
 // those with exactly the channels of the tiles.
 enum RowsAre : int { ROWS_ANY, ROWS_16, ROWS_FULL };
 
-// Copies W words at byte `off` of a cached row (of `bytes`) to shared memory
+// Copies 16 bytes at byte `off` of a cached row (of `bytes`) to shared memory
 // without waiting; zeros past the row, or all of them unless `live`. Rows of
-// 16 bytes' multiples have a piece inside or outside; others come as words
+// 16 bytes' multiples have the place inside or outside; others come as words
 // (cp.async of 4 bytes) or, where even these are not aligned, as elements.
-template <int W, int SIZE, int ROWS>
-__device__ __forceinline__ void copy_piece(uint32_t dst, const uint8_t* row, int off, int bytes, bool words,
+template <int SIZE, int ROWS>
+__device__ __forceinline__ void copy_place(uint32_t dst, const uint8_t* row, int off, int bytes, bool words,
                                            bool live) {
     if constexpr (ROWS != ROWS_ANY) {
-        const int n = live && (ROWS == ROWS_FULL || off < bytes) ? 4 * W : 0;
-        if constexpr (W == 4)
-            asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(row + off), "r"(n)
-                         : "memory");
-        else
-            asm volatile("cp.async.ca.shared.global.L2::256B [%0], [%1], %2, %3;" ::"r"(dst), "l"(row + off),
-                         "n"(4 * W), "r"(n) : "memory");
+        const int n = live && (ROWS == ROWS_FULL || off < bytes) ? 16 : 0;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(row + off), "r"(n) : "memory");
         return;
     }
     if (words) {
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
+        for (int w = 0; w < 4; ++w) {
             const int n = live && off + 4 * w < bytes ? 4 : 0;
             asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + 4 * w),
                          "l"(row + (n ? off + 4 * w : 0)), "r"(n) : "memory");
         }
     } else {
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
+        for (int w = 0; w < 4; ++w) {
             uint32_t x = 0;
 #pragma unroll
             for (int e = 0; e < 4 / SIZE; ++e) {
@@ -278,9 +275,13 @@ __device__ __forceinline__ void copy_piece(uint32_t dst, const uint8_t* row, int
     }
 }
 
-__device__ __forceinline__ void read_piece(uint32_t (&r)[4], uint32_t src) {
-    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(src) : "memory");
+template <int W>
+__device__ __forceinline__ void read_piece(uint32_t (&r)[W], uint32_t src) {
+    if constexpr (W == 4)
+        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(src) : "memory");
+    else
+        asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(src) : "memory");
 }
 
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -305,7 +306,19 @@ struct DecodeShape {
     static constexpr int VD = 16 / size < DP / 8 ? 16 / size : DP / 8;      // and of its V piece
     static constexpr int KP = DP / 4 / KD, VP = DP / 8 / VD;                // pieces of a row per lane
     static constexpr int KW = KD * size / 4, VW = VD * size / 4;            // words of a piece
-    static_assert(KW == 4 && (VW == 4 || (VW == 2 && VP == 1)), "pieces fill 16-byte places");
+    static_assert(KW == 4 && (VW == 4 || VW == 2), "pieces of 16 bytes, or halves");
+    // A tile in shared memory: rows of row_bytes, their 16-byte places permuted
+    // within every 128 bytes so that the 8 lanes of a quarter warp read from
+    // different banks, for K (rows g, g + 1 side by side) as for V (4 tokens).
+    static constexpr int places = row_bytes / 16;                           // of a row
+    static constexpr int copies = TOK * places / 32;                        // of a lane for a tile
+    static __device__ __forceinline__ int at(int row, int place) {
+        if (row_bytes == 64) {               // two rows in 128 bytes
+            const int p = ((row & 1) * 4 + place) ^ (((row >> 1) & 3) << 1);
+            return (row >> 1) * 128 + p * 16;
+        }
+        return row * row_bytes + ((place ^ (((row >> 1) & 3) << 1) ^ ((row & 1) << 2)) * 16);
+    }
     static constexpr int KR = Kind<KIND>::f32 ? KD : KD / 2;                // MMA registers of a K piece
     static constexpr int QR = KP * KR;                                      // MMA registers of a query row
     // pieces read back from the ring at a time: 32 words, so that their latencies overlap
@@ -417,6 +430,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
     struct Slots {
         int row[S::NR];
         int model;
+        bool run;                            // all there and one after the other
     };
     auto look_up = [&](Slots& x) {               // the step at `front`, which moves on
         const int i = front.left > 0 ? front.nb / a.b : 0, kh = front.hp / a.tiles;
@@ -436,28 +450,45 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
             if (front.pos >= front.len) next_segment(front);
         }
     };
-    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(decode_ring);
-    auto k_place = [&](int place, int mt, int hf, int p) {
-        return mine + place * S::unit + (((mt * 2 + hf) * S::KP + p) * 32 * kDecodeWarps + threadIdx.x) * S::KW * 4;
+    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(decode_ring) + warp * (S::unit / kDecodeWarps);
+    // One unit: the rows of a tile, whole rows side by side in each instruction
+    // (every memory request is a full line); from one address on where the
+    // slots follow one another, as they do inside a page.
+    auto copy_rows = [&](int place, const void* pages, const Slots& x) {
+        const uint8_t* base = static_cast<const uint8_t*>(pages) + x.model * pool_rows * bytes;
+        const uint32_t dst = mine + place * S::unit;
+        if (x.run) {
+            const uint8_t* from = base + (int64_t)__shfl_sync(0xffffffffu, x.row[0], 0) * bytes;
+#pragma unroll
+            for (int j = 0; j < S::copies; ++j) {
+                const int n = j * 32 + lane, row = n / S::places, p = n % S::places;
+                copy_place<S::size, ROWS>(dst + S::at(row, p), from + row * bytes, p * 16, bytes, words, true);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < S::copies; ++j) {
+                const int n = j * 32 + lane, row = n / S::places, p = n % S::places;
+                // the register that holds the row's slot is known at compile time, its lane is not
+                const int r = __shfl_sync(0xffffffffu, x.row[S::NR == 1 ? 0 : (j * 32 / S::places) >> 5], row & 31);
+                copy_place<S::size, ROWS>(dst + S::at(row, p), base + (int64_t)max(r, 0) * bytes, p * 16, bytes, words,
+                                          r >= 0);
+            }
+        }
     };
-    // the same 16-byte places as K's: a unit's space changes hands between the
-    // two without a barrier, so a thread's must be its own in both. V pieces of
-    // 8 bytes (64 channels of 8 bits) share one, those of tokens t and t + 1.
-    auto v_place = [&](int place, int mt, int t, int p) {
-        const int word = ((mt * 4 + t) * S::VP + p) * S::VW;
-        return mine + place * S::unit + ((word / 4) * 32 * kDecodeWarps + threadIdx.x) * 16 + word % 4 * 4;
-    };
-    // K pieces of tokens g and g + 8 of every 16, the tile's scales, and a bit for each token that is there
-    auto copy_k = [&](int place, int turn, const Slots& x, uint32_t (&seen)[S::NR]) {
+    // K of a tile with its scales, and a bit for each token that is there
+    auto copy_k = [&](int place, int turn, Slots& x, uint32_t (&seen)[S::NR]) {
         const int64_t pool = x.model * pool_rows;
-        const uint8_t* kbase = static_cast<const uint8_t*>(a.c.k) + pool * bytes;
+        const int first = __shfl_sync(0xffffffffu, x.row[0], 0);
+        bool run = first >= 0;
 #pragma unroll
         for (int r = 0; r < S::NR; ++r) {
+            const int t = TOK < 32 ? lane & (TOK - 1) : lane + 32 * r;
             seen[r] = __ballot_sync(0xffffffffu, x.row[r] >= 0);
+            run = run && x.row[r] == first + t;
             if (x.row[r] == -2) raise_device_error(a.err, DEV_ERR_INDEX);
             if constexpr (K::code) {
                 const int64_t at = pool + (x.row[r] < 0 ? 0 : x.row[r]);
-                const int n = x.row[r] >= 0 ? 4 : 0, t = TOK < 32 ? lane & (TOK - 1) : lane + 32 * r;
+                const int n = x.row[r] >= 0 ? 4 : 0;
                 asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
                                  (uint32_t)__cvta_generic_to_shared(&sm_s[turn][warp][0][t])),
                              "l"(a.c.ks + at), "r"(n) : "memory");
@@ -466,35 +497,10 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
                              "l"(a.c.vs + at), "r"(n) : "memory");
             }
         }
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                // token 16 mt + 8 hf + g: the register that holds it is known at compile time, the lane is not
-                const int r = __shfl_sync(0xffffffffu, x.row[S::NR == 1 ? 0 : mt >> 1], (16 * mt + 8 * hf + g) & 31);
-                const uint8_t* row = kbase + (int64_t)max(r, 0) * bytes;
-#pragma unroll
-                for (int p = 0; p < S::KP; ++p)
-                    copy_piece<S::KW, S::size, ROWS>(k_place(place, mt, hf, p), row, (p * 4 + c) * S::KD * S::size,
-                                                        bytes, words, r >= 0);
-            }
+        x.run = __all_sync(0xffffffffu, run);
+        copy_rows(place, a.c.k, x);
     };
-    auto copy_v = [&](int place, const Slots& x) {
-        const uint8_t* vbase = static_cast<const uint8_t*>(a.c.v) + x.model * pool_rows * bytes;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                // the k index of lane c: tokens 2c, 2c + 1, 2c + 8, 2c + 9; tf32 c, c + 4, c + 8, c + 12
-                const int tok = K::f32 ? c + 4 * t : 2 * c + (t & 1) + 8 * (t >> 1);
-                const int r = __shfl_sync(0xffffffffu, x.row[S::NR == 1 ? 0 : mt >> 1], (16 * mt + tok) & 31);
-                const uint8_t* row = vbase + (int64_t)max(r, 0) * bytes;
-#pragma unroll
-                for (int p = 0; p < S::VP; ++p)
-                    copy_piece<S::VW, S::size, ROWS>(v_place(place, mt, t, p), row, (p * 8 + g) * S::VD * S::size,
-                                                        bytes, words, r >= 0);
-            }
-    };
+    auto copy_v = [&](int place, const Slots& x) { copy_rows(place, a.c.v, x); };
 
     Slots x1, x2;                            // slots of the next step and of the one after it
     uint32_t seen[2][S::NR];                 // tokens that are there, of the current step and the next
@@ -576,6 +582,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
     // S^T += K q^T over the pieces in registers
     float s[NT][MT][4];
     auto scores = [&](int place) {
+        const uint32_t from = mine + place * S::unit;
         uint32_t batch[MT][S::KB][2][S::KW];
 #pragma unroll
         for (int p0 = 0; p0 < S::KP; p0 += S::KB) {
@@ -584,7 +591,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
 #pragma unroll
             for (int p = 0; p < S::KB; ++p)
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) read_piece(batch[mt][p][hf], k_place(place, mt, hf, p0 + p));
+                for (int hf = 0; hf < 2; ++hf) read_piece(batch[mt][p][hf], from + S::at(16 * mt + 8 * hf + g, (p0 + p) * 4 + c));
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -733,6 +740,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
     };
     // O^T += V^T P^T over the pieces in registers
     auto values = [&](int place) {
+        const uint32_t from = mine + place * S::unit;
         uint32_t batch[MT][S::VB][4][S::VW];
 #pragma unroll
         for (int p0 = 0; p0 < S::VP; p0 += S::VB) {
@@ -742,14 +750,10 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
             for (int p = 0; p < S::VB; ++p)
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
-                    if constexpr (S::VW == 4) {
-                        read_piece(batch[mt][p][t], v_place(place, mt, t, p0 + p));
-                    } else if (t % 2 == 0) {
-                        uint32_t two[4];
-                        read_piece(two, v_place(place, mt, t, p0 + p));
-                        batch[mt][p][t][0] = two[0], batch[mt][p][t][1] = two[1];
-                        batch[mt][p][t + 1][0] = two[2], batch[mt][p][t + 1][1] = two[3];
-                    }
+                    // the k index of lane c: tokens 2c, 2c + 1, 2c + 8, 2c + 9; tf32 c, c + 4, c + 8, c + 12
+                    const int row = 16 * mt + (K::f32 ? c + 4 * t : 2 * c + (t & 1) + 8 * (t >> 1));
+                    if constexpr (S::VW == 4) read_piece(batch[mt][p][t], from + S::at(row, (p0 + p) * 8 + g));
+                    else read_piece(batch[mt][p][t], from + S::at(row, (p0 + p) * 4 + g / 2) + g % 2 * 8);
                 }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -912,9 +916,9 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
         const int entered = at.pos;
         do {
             copy_wait<S::units - 1>();
+            __syncwarp();                        // what the other lanes copied
             float kt[MT][2], vt[MT][2];
             if constexpr (K::code) {
-                __syncwarp();
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -922,7 +926,6 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
                         kt[mt][hf] = sm_s[turn][warp][0][16 * mt + 8 * hf + g];
                         vt[mt][hf] = sm_s[turn][warp][1][16 * mt + 8 * hf + g];
                     }
-                __syncwarp();
             }
             uint32_t now[S::NR], any = 0;
 #pragma unroll
@@ -932,6 +935,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
                 clear_scores();
                 scores(place);
             }
+            __syncwarp();                        // all lanes have read the unit
             if constexpr (S::units == 3) copy_v(place, x1);
             else copy_k(place, 0, x1, seen[0]);
             copy_commit();
@@ -940,7 +944,9 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
                 turn_weights();
             }
             copy_wait<S::units - 1>();
+            __syncwarp();
             if (any) values(second);
+            __syncwarp();
             if constexpr (S::units == 3) {
                 copy_k(second, turn, x2, seen[1]);
                 copy_commit();
