@@ -144,6 +144,10 @@ struct Kind {
     // then keep 16 bits of a weight down to 2^-24 of the largest, and reach
     // to 2^-40 of it (bf16 and tf32 have fp32's exponents).
     static constexpr float lift = KIND == DK_F16 ? 15.f : 0.f;
+    // The running maximum follows the scores only when they pass it by more:
+    // weights up to 2^8 cost nothing where the exponents are fp32's, and the
+    // sums then are rescaled a few times in a segment, not in most tiles.
+    static constexpr float slack = KIND == DK_F16 ? 0.f : 8.f;
 };
 
 // D (16 x 8) += A (16 x 16, or 16 x 8 of tf32) B, fp32 sums.
@@ -363,6 +367,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
     // --- where this block's steps begin
     struct Walk {
         int nb, hp, pos, start, len, left;       // segment (nb, hp), token of the step, its range; steps still to do
+        const int* table;                        // of the sequence
     };
     Walk front;
     if (a.in_turn) {
@@ -409,8 +414,10 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
     if (front.left <= 0) return;
     auto enter = [&](Walk& w) {
         const DecodeRange r(a, w.nb);
+        const int i = w.nb / a.b;
         w.start = w.pos = r.start;
         w.len = r.len;
+        w.table = a.c.table + i * a.c.table_n + (w.nb - i * a.b) * a.c.table_b;
     };
     enter(front);
     if (!a.in_turn) front.pos += sm_at[2] * STEP;
@@ -425,29 +432,39 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
         if (w.left > 0) enter(w);
     };
 
-    // --- token slots: lane holds those of tokens (lane + 32 r) of a tile; -1
-    // past the end, -2 where the table names no page of the pool
+    // --- token slots: lane holds those of tokens (lane + 32 r) of a tile.
+    // look_up only asks for the pages; `resolve`, an iteration later, waits for them.
     struct Slots {
-        int row[S::NR];
+        int row[S::NR];                      // the page, then the row; -1 past the end, -2 where the pool has no such page
+        int off[S::NR];                      // of the token in a page's rows of all heads, -1 past the end
         int model;
         bool run;                            // all there and one after the other
     };
     auto look_up = [&](Slots& x) {               // the step at `front`, which moves on
-        const int i = front.left > 0 ? front.nb / a.b : 0, kh = front.hp / a.tiles;
-        x.model = i;
+        const int kh = front.hp / a.tiles;
+        x.model = front.left > 0 ? front.nb / a.b : 0;
 #pragma unroll
         for (int r = 0; r < S::NR; ++r) {
             const int p = front.pos + warp * TOK + (TOK < 32 ? lane & (TOK - 1) : lane + 32 * r);
-            x.row[r] = -1;
-            if (front.left > 0 && p < front.len) {
-                x.row[r] = a.c.row(i, front.nb - i * a.b, a.hk, kh, p);
-                if (x.row[r] < 0) x.row[r] = -2;
+            x.row[r] = x.off[r] = -1;
+            if (front.left > 0 && p < front.len) {       // the length never passes the table's columns
+                uint32_t off;
+                const uint32_t col = a.c.page_div.divmod((uint32_t)p, off);
+                x.row[r] = __ldg(front.table + col);
+                x.off[r] = kh * a.c.page + (int)off;
             }
         }
         if (front.left > 0) {
             --front.left;
             front.pos += STEP;
             if (front.pos >= front.len) next_segment(front);
+        }
+    };
+    auto resolve = [&](Slots& x) {
+#pragma unroll
+        for (int r = 0; r < S::NR; ++r) {
+            const bool there = (uint32_t)x.row[r] < (uint32_t)a.c.pages;
+            x.row[r] = x.off[r] < 0 ? -1 : (there ? x.row[r] * (a.hk * a.c.page) + x.off[r] : -2);
         }
     };
     const uint32_t mine = (uint32_t)__cvta_generic_to_shared(decode_ring) + warp * (S::unit / kDecodeWarps);
@@ -477,6 +494,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
     };
     // K of a tile with its scales, and a bit for each token that is there
     auto copy_k = [&](int place, int turn, Slots& x, uint32_t (&seen)[S::NR]) {
+        resolve(x);
         const int64_t pool = x.model * pool_rows;
         const int first = __shfl_sync(0xffffffffu, x.row[0], 0);
         bool run = first >= 0;
@@ -686,7 +704,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
                 for (int mt = 0; mt < MT; ++mt) top = fmaxf(top, fmaxf(s[t][mt][e], s[t][mt][2 + e]));
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                top = fmaxf(top, m[t][e]);
+                top = top > m[t][e] + K::slack ? top : m[t][e];
                 const float ref = top == -INFINITY ? 0.f : top;
                 f[t][e] = ex2(m[t][e] - ref);
                 m[t][e] = top;
