@@ -8,21 +8,24 @@
 namespace widek {
 namespace {
 
-constexpr int kJoinWarps = 8;
+constexpr int kJoinThreads = 256;
+constexpr int kMostBlocks = 1024;
 // Sequences whose steps every block adds up to find its place in line (32 for
 // each thread).
 constexpr int kMostInLine = 4096;
 
 // out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c over the blocks c that a
-// segment lies in, in their order; W warps for each query head. Segments that
-// lie in one block were finished by the attention itself.
-template <int W>
-__global__ void __launch_bounds__(32 * kJoinWarps) decode_join_kernel(const __grid_constant__ DecodeArgs a) {
-    __shared__ float red[W > 1 ? W : 1][W > 1 ? 256 : 1];
-    __shared__ float2 red_ml[W > 1 ? W : 1];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = W > 1 ? warp : 0;
+// segment lies in, in a fixed order. WIDE: a block for 32 channels of a query
+// head, its 8 warps taking every 8th c; else a warp for each head. Segments
+// that lie in one block were finished by the attention itself.
+template <bool WIDE>
+__global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_constant__ DecodeArgs a) {
+    constexpr int kWarps = kJoinThreads / 32;
+    __shared__ float factor[WIDE ? kMostBlocks : 1];
+    __shared__ float red[WIDE ? kWarps : 1][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t last = (int64_t)a.n * a.b * a.hq - 1;
-    const int64_t row = min((int64_t)blockIdx.x * (kJoinWarps / W) + warp / W, last);     // the same for a head's warps
+    const int64_t row = WIDE ? blockIdx.x : min((int64_t)blockIdx.x * kWarps + warp, last);
     // the segment's place in line, while the attention still runs
     const int nb = (int)(row / a.hq), h = (int)(row - (int64_t)nb * a.hq), in_group = h % a.group;
     const int sequences = a.n * a.b, per_seq = a.hk * a.tiles;
@@ -43,42 +46,54 @@ __global__ void __launch_bounds__(32 * kJoinWarps) decode_join_kernel(const __gr
     const long long f0 = before * per_seq + (long long)hp * n;
     const int c0 = (int)(f0 / per), c1 = (int)((f0 + n - 1) / per);
     sm100::grid_dep_wait();
-    if (c0 == c1 || (W == 1 && (int64_t)blockIdx.x * kJoinWarps + warp > last)) return;
+    if (c0 == c1 || (!WIDE && (int64_t)blockIdx.x * kWarps + warp > last)) return;
     // a block's part 0 is the segment it starts in
     const int late = f0 > c0 * per ? 1 : 0;
     auto place = [&](int c) {
         return ((int64_t)c * 2 + (c == c0 ? late : 0)) * 8 * a.nt + in_group % (8 * a.nt);
     };
-    float top = -INFINITY;
+    float top = -INFINITY, total = 0.f;
     for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, a.part_ml[place(c)].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float ref = top == -INFINITY ? 0.f : top;
-    float total = 0.f, acc[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-#pragma unroll 4
-    for (int c = c0 + part; c <= c1; c += W) {
-        const int64_t at = place(c);
-        const float2 x = a.part_ml[at];
-        const float f = ex2(x.x - ref);
-        total += f * x.y;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (lane + 32 * j < a.d) acc[j] += f * a.part_o[at * a.d + lane + 32 * j];
-    }
-    if constexpr (W > 1) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) red[warp][lane + 32 * j] = acc[j];
-        if (lane == 0) red_ml[warp] = make_float2(0.f, total);
+    if constexpr (WIDE) {
+        for (int c = c0 + lane; c <= c1; c += 32) {
+            const float2 x = a.part_ml[place(c)];
+            const float f = ex2(x.x - ref);
+            total += f * x.y;
+            if (warp == 0) factor[c - c0] = f;
+        }
+        total = warp_sum(total);
         __syncthreads();
-        for (int ch = threadIdx.x; ch < a.d; ch += 32 * W) {
-            float o = 0.f, sum = 0.f;
+        const int ch = blockIdx.y * 32 + lane;
+        float o = 0.f;
+        if (ch < a.d) {
+#pragma unroll 8
+            for (int c = c0 + warp; c <= c1; c += kWarps) o += factor[c - c0] * a.part_o[place(c) * a.d + ch];
+        }
+        red[warp][lane] = o;
+        __syncthreads();
+        if (warp == 0 && ch < a.d) {
+            o = 0.f;
 #pragma unroll
-            for (int w = 0; w < W; ++w) o += red[w][ch], sum += red_ml[w].y;
-            store_out(a.out, row * a.d + ch, sum == 0.f ? 0.f : o / sum, a.dtype);
+            for (int w = 0; w < kWarps; ++w) o += red[w][lane];
+            store_out(a.out, row * a.d + ch, total == 0.f ? 0.f : o / total, a.dtype);
         }
     } else {
+        float acc[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+#pragma unroll 4
+        for (int c = c0; c <= c1; ++c) {
+            const int64_t at = place(c);
+            const float2 x = a.part_ml[at];
+            const float f = ex2(x.x - ref);
+            total += f * x.y;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (lane + 32 * j < a.d) acc[j] += f * a.part_o[at * a.d + lane + 32 * j];
+        }
         const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -115,7 +130,8 @@ int decode_args(DecodeArgs& a, const char* what, const int64_t* g, const int64_t
     if (a.window > 0 && a.window < tokens) tokens = a.window;
     const int64_t segments = (int64_t)a.n * a.b * a.hk * a.tiles;
     const int64_t steps = std::max<int64_t>(1, (tokens + a.step - 1) / a.step);
-    const int64_t places = (int64_t)decode_places(a.d, fmt, a.nt) * sm_count(current_device());
+    const int64_t places =
+        std::min<int64_t>(decode_places(a.d, fmt, a.nt) * sm_count(current_device()), kMostBlocks);
     a.blocks = (int)(segments < places && segments * steps < places ? std::max<int64_t>(segments * steps, 1) : places);
     // nothing to divide when every segment is one step, or too much to add up
     a.in_turn = steps == 1 || (int64_t)a.n * a.b > kMostInLine;
@@ -174,19 +190,20 @@ extern "C" int widek_decode_attention_fwd(const void* q, const void* kc, const v
         rc = launch_decode<DK_F32, false>(a, st);
     if (rc != WIDEK_OK || a.in_turn) return rc;
     // The join is set up while the attention runs. A segment lies in about
-    // blocks / segments of them: more than 8, and its heads take 8 warps each.
+    // blocks / segments of them: with more than 8 its heads are spread out.
     const int64_t heads = (int64_t)a.n * a.b * a.hq;
     const bool wide = a.blocks > 8 * (int64_t)a.n * a.b * a.hk * a.tiles;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(wide ? heads : (heads + kJoinWarps - 1) / kJoinWarps));
-    cfg.blockDim = dim3(32 * kJoinWarps);
+    cfg.gridDim = wide ? dim3((unsigned)heads, (unsigned)((a.d + 31) / 32))
+                       : dim3((unsigned)((heads + kJoinThreads / 32 - 1) / (kJoinThreads / 32)));
+    cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (wide) cudaLaunchKernelEx(&cfg, decode_join_kernel<kJoinWarps>, a);
-    else cudaLaunchKernelEx(&cfg, decode_join_kernel<1>, a);
+    if (wide) cudaLaunchKernelEx(&cfg, decode_join_kernel<true>, a);
+    else cudaLaunchKernelEx(&cfg, decode_join_kernel<false>, a);
     return check_launch("widek_decode_attention_fwd (join)");
 }

@@ -303,8 +303,9 @@ template <int KIND, int DP, int NT, int ROWS, bool SPLITQ>
 struct DecodeShape {
     static constexpr int size = Kind<KIND>::size;
     static constexpr int row_bytes = DP * size;
-    // tiles of a warp: 4 KB of K and 4 KB of V, more where 16 tokens already are
-    static constexpr int MT = row_bytes >= 256 ? 1 : 256 / row_bytes;
+    // tiles of a warp: 8 KB of K and 8 KB of V where rows are 256 bytes or
+    // more, 4 KB below (measured against twice and half as much)
+    static constexpr int MT = row_bytes >= 512 ? 1 : (row_bytes == 256 ? 2 : 256 / row_bytes);
     static constexpr int TOK = 16 * MT;
     static constexpr int KD = 16 / size < DP / 4 ? 16 / size : DP / 4;      // channels of a lane's K piece
     static constexpr int VD = 16 / size < DP / 8 ? 16 / size : DP / 8;      // and of its V piece
@@ -336,7 +337,7 @@ struct DecodeShape {
     static constexpr int units = row_bytes <= 256 ? 3 : 2;
     static constexpr int ring = units * unit;
     static constexpr int blocks =                                           // of an SM
-        row_bytes > 512 ? 1 : (row_bytes > 256 || NT == 2 || SPLITQ || DP == 256 ? 2 : (Kind<KIND>::f32 ? 3 : 4));
+        row_bytes > 512 ? 1 : (row_bytes >= 256 || NT == 2 || SPLITQ || DP == 256 ? 2 : 3);
     static constexpr int JC = DP > 64 ? 2 : 1;                              // 16-channel tiles joined at a time
 };
 
@@ -1012,13 +1013,13 @@ inline int decode_nt(int group, int d, int fmt) { return group > 8 && d <= 128 &
 // Tokens of a step.
 inline int decode_step(int d, int fmt) {
     const int bytes = (d <= 64 ? 64 : (d <= 128 ? 128 : 256)) * (int)cache_fmt_size(fmt);
-    return kDecodeWarps * 16 * (bytes >= 256 ? 1 : 256 / bytes);
+    return kDecodeWarps * 16 * (bytes >= 512 ? 1 : (bytes == 256 ? 2 : 256 / bytes));
 }
 
-// Blocks of an SM, as DecodeShape has them (fp32 queries over codes: 2, not 4).
+// Blocks of an SM, as DecodeShape has them (fp32 queries over codes: 2, not 3).
 inline int decode_places(int d, int fmt, int nt) {
     const int bytes = (d <= 64 ? 64 : (d <= 128 ? 128 : 256)) * (int)cache_fmt_size(fmt);
-    return bytes > 512 ? 1 : (bytes > 256 || nt == 2 || d > 128 ? 2 : (fmt == WIDEK_F32 ? 3 : 4));
+    return bytes > 512 ? 1 : (bytes >= 256 || nt == 2 || d > 128 ? 2 : 3);
 }
 
 template <int KIND, bool SPLITQ>
