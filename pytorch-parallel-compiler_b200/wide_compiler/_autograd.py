@@ -360,8 +360,7 @@ class QkNormRopeFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
         from . import ops
-        with torch.no_grad():
-            y = ops.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+        y = ops._qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
         ctx.eps, ctx.interleaved = eps, interleaved
         ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
         return y
@@ -371,9 +370,8 @@ class QkNormRopeFn(torch.autograd.Function):
         from . import ops
         q, k, qw, kw, cos, sin, positions = ctx.saved_tensors
         need = ctx.needs_input_grad
-        with torch.no_grad():
-            grads = ops.qk_norm_rope_bwd(q, k, qw, kw, cos, sin, positions, dyq.to(q.dtype), dyk.to(k.dtype), ctx.eps,
-                                         ctx.interleaved, need_dw=need[2] or need[3])
+        grads = ops.qk_norm_rope_bwd(q, k, qw, kw, cos, sin, positions, dyq, dyk, ctx.eps, ctx.interleaved,
+                                     need_dw=need[2] or need[3])
         return (*(g if want else None for g, want in zip(grads, need[:4])), None, None, None, None, None)
 
 

@@ -42,6 +42,7 @@ _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _dbl = ctypes.c_double
+_geom = ctypes.c_char_p                 # int64 array on the host, packed into bytes
 
 # name -> argtypes (restype is always c_int). Mirrors include/widek.h.
 SIGNATURES = {
@@ -105,17 +106,15 @@ SIGNATURES = {
     "widek_act_bwd": [_c_void_p] * 3 + [_i64, _int, _int, _c_void_p],
     "widek_layernorm_bwd_workspace": [_i64] * 3,
     "widek_layernorm_bwd": [_c_void_p] * 6 + [_i64] * 3 + [_dbl, _int, _c_void_p, _i64, _c_void_p],
-    "widek_qk_norm_rope_fwd": [_c_void_p] * 9 + [ctypes.POINTER(_i64), _dbl, _int, _int, _int, _c_void_p],
-    "widek_qk_norm_rope_write_fwd": [_c_void_p] * 14 + [ctypes.POINTER(_i64)] * 2 + [_dbl] + [_int] * 4
-                                    + [_c_void_p],
-    "widek_qk_norm_rope_bwd_workspace": [ctypes.POINTER(_i64)],
-    "widek_qk_norm_rope_bwd": [_c_void_p] * 13 + [ctypes.POINTER(_i64), _dbl, _int, _int, _int, _c_void_p, _i64,
-                                                  _c_void_p],
-    "widek_cache_write_fwd": [_c_void_p] * 8 + [ctypes.POINTER(_i64)] * 2 + [_int] * 3 + [_c_void_p],
-    "widek_cache_read_fwd": [_c_void_p] * 8 + [ctypes.POINTER(_i64)] * 2 + [_int] * 3 + [_c_void_p],
-    "widek_decode_attention_workspace": [ctypes.POINTER(_i64)] * 2 + [_i64, _int],
-    "widek_decode_attention_fwd": [_c_void_p] * 8 + [ctypes.POINTER(_i64)] * 2 + [_dbl, _i64, _int, _int, _int,
-                                                                                  _c_void_p, _i64, _c_void_p],
+    "widek_qk_norm_rope_fwd": [_c_void_p] * 9 + [_geom, _dbl, _int, _int, _int, _c_void_p],
+    "widek_qk_norm_rope_write_fwd": [_c_void_p] * 14 + [_geom, _geom, _dbl] + [_int] * 4 + [_c_void_p],
+    "widek_qk_norm_rope_bwd_workspace": [_geom],
+    "widek_qk_norm_rope_bwd": [_c_void_p] * 13 + [_geom, _dbl, _int, _int, _int, _c_void_p, _i64, _c_void_p],
+    "widek_cache_write_fwd": [_c_void_p] * 8 + [_geom, _geom] + [_int] * 3 + [_c_void_p],
+    "widek_cache_read_fwd": [_c_void_p] * 8 + [_geom, _geom] + [_int] * 3 + [_c_void_p],
+    "widek_decode_attention_workspace": [_geom, _geom, _i64, _int],
+    "widek_decode_attention_fwd": [_c_void_p] * 8 + [_geom, _geom, _dbl, _i64, _int, _int, _int, _c_void_p, _i64,
+                                                     _c_void_p],
 }
 RESTYPES = {"widek_batchnorm_train_workspace": ctypes.c_size_t, "widek_conv_workspace": ctypes.c_size_t,
             "widek_rnn_workspace": ctypes.c_size_t, "widek_conv_packed_weight_elems": _i64,
@@ -281,6 +280,11 @@ def stream_ptr(device: torch.device) -> int:
         idx = device.index if device.index is not None else torch.cuda.current_device()
         return _raw_stream(idx)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def raw_stream(index: int) -> int:
+    """Handle of torch's current stream on device ``index``."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

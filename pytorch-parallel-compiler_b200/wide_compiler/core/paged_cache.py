@@ -11,7 +11,7 @@ and ``ops.qk_norm_rope_write`` fill it, ``ops.cache_read`` reads tokens back and
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 from typing import Optional
 
 import torch
@@ -19,39 +19,50 @@ from torch import Tensor
 
 from .. import _native as N
 
+_pack = struct.Struct('=5q').pack
 CODE_DTYPES = {torch.int8: N.I8, torch.float8_e4m3fn: N.E4M3}
 
 
 class WidePagedCache:
+    __slots__ = ('k', 'v', 'table', 'k_scale', 'v_scale', 'fmt', 'quantized', 'sizes', 'geom')
+
     def __init__(self, k: Tensor, v: Tensor, table: Tensor, k_scale: Optional[Tensor] = None,
                  v_scale: Optional[Tensor] = None):
         what = "WidePagedCache"
-        if k.dim() != 5 or v.shape != k.shape or v.dtype != k.dtype:
-            raise ValueError(f"{what}: k and v must be alike, [N, pages, Hk, page, D]; got {tuple(k.shape)} "
-                             f"{k.dtype} and {tuple(v.shape)} {v.dtype}")
+        shape, dtype = k.shape, k.dtype
+        if len(shape) != 5 or v.shape != shape or v.dtype != dtype:
+            raise ValueError(f"{what}: k and v must be alike, [N, pages, Hk, page, D]; got {tuple(shape)} "
+                             f"{dtype} and {tuple(v.shape)} {v.dtype}")
         if not (k.is_contiguous() and v.is_contiguous()):
             raise ValueError(f"{what}: the pages must be contiguous")
-        self.fmt = CODE_DTYPES.get(k.dtype)
+        self.fmt = CODE_DTYPES.get(dtype)
         self.quantized = self.fmt is not None
         if self.quantized:
             for s in (k_scale, v_scale):
-                if s is None or s.shape != k.shape[:4] or s.dtype != torch.float32 or not s.is_contiguous():
-                    raise ValueError(f"{what}: {k.dtype} pages need contiguous float32 scales {tuple(k.shape[:4])}")
+                if s is None or s.shape != shape[:4] or s.dtype != torch.float32 or not s.is_contiguous():
+                    raise ValueError(f"{what}: {dtype} pages need contiguous float32 scales {tuple(shape[:4])}")
         else:
             self.fmt = N.dtype_code(k)
             if k_scale is not None or v_scale is not None:
-                raise ValueError(f"{what}: scales belong to int8 and float8_e4m3fn pages, not {k.dtype}")
-        self.n, self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
-        if self.page_size < 1 and k.shape[1] > 0:
-            raise ValueError(f"{what}: pages of {self.page_size} tokens")
-        if table.dtype != torch.int32 or table.dim() not in (2, 3) or (table.dim() == 3 and table.shape[0] != self.n) \
-                or (table.shape[-1] > 1 and table.stride(-1) != 1):
-            raise ValueError(f"{what}: the table must be int32 [B, M] or [N={self.n}, B, M] with dense rows, got "
-                             f"{tuple(table.shape)} {table.dtype}")
+                raise ValueError(f"{what}: scales belong to int8 and float8_e4m3fn pages, not {dtype}")
+        n, pages, kv_heads, page_size, head_dim = shape
+        if page_size < 1 and pages > 0:
+            raise ValueError(f"{what}: pages of {page_size} tokens")
+        ts, st = table.shape, table.stride()
+        if table.dtype != torch.int32 or len(ts) not in (2, 3) or (len(ts) == 3 and ts[0] != n) \
+                or (ts[-1] > 1 and st[-1] != 1):
+            raise ValueError(f"{what}: the table must be int32 [B, M] or [N={n}, B, M] with dense rows, got "
+                             f"{tuple(ts)} {table.dtype}")
         self.k, self.v, self.table, self.k_scale, self.v_scale = k, v, table, k_scale, v_scale
-        self.batch = table.shape[-2]
-        self.geom = (ctypes.c_int64 * 5)(self.pages, max(self.page_size, 1), table.shape[-1],
-                                         table.stride(0) if table.dim() == 3 else 0, table.stride(-2))
+        self.sizes = (n, ts[-2], kv_heads, head_dim)              # N, B, Hk, D
+        self.geom = _pack(pages, max(page_size, 1), ts[-1], st[0] if len(ts) == 3 else 0, st[-2])
+
+    n = property(lambda self: self.sizes[0])
+    batch = property(lambda self: self.sizes[1])
+    kv_heads = property(lambda self: self.sizes[2])
+    head_dim = property(lambda self: self.sizes[3])
+    pages = property(lambda self: self.k.shape[1])
+    page_size = property(lambda self: self.k.shape[3])
 
     @property
     def max_len(self) -> int:

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import math
+import struct
 from typing import List, Optional, Sequence
 
 import ctypes
@@ -948,58 +949,111 @@ def attention_dropout(mod, query: Tensor, key: Tensor, value: Tensor, attn_mask:
 # key-value cache, attention of one new token
 # ---------------------------------------------------------------------------
 
-_INDEX = (torch.int32, torch.int64)
+# A decoder step is a handful of calls of a few microseconds on the device:
+# these wrappers keep to the checks that need no new objects (get_device, packed
+# geometry arrays, workspace sizes remembered by geometry).
+_INDEX = {torch.int32: 0, torch.int64: 1}
+_pack_rows = struct.Struct('=23q').pack
+_pack_decode = struct.Struct('=10q').pack
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, '_cuda_getDevice') else torch.cuda.current_device
+_WS_BYTES: dict = {}
 
 
-def _row_strides(t: Tensor, what: str):
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{what}: the channels of a head must be dense (stride {t.stride(-1)})")
-    return t.stride()[:-1]
+def _device(what: str, ref: Tensor, *others: Optional[Tensor]) -> int:
+    """Index of the one CUDA device that holds all the tensors."""
+    idx = ref.get_device()
+    for t in others:
+        if t is not None and t.get_device() != idx:
+            idx = -1
+            break
+    if idx < 0:
+        N.require_cuda(ref, *others, what=what)
+    return idx
+
+
+def _launch(idx: int, name: str, *args) -> None:
+    """Calls the entry point on device ``idx`` (its stream is torch's current one)."""
+    fn = getattr(N.lib(), name)
+    if idx == _current_device():
+        rc = fn(*args, N.raw_stream(idx))
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*args, N.raw_stream(idx))
+    if rc:
+        N.check(rc, name)
+
+
+def _workspace(name: str, key, *args) -> int:
+    """Workspace bytes by the library's own query, remembered by its arguments."""
+    size = _WS_BYTES.get(key)
+    if size is None:
+        size = int(getattr(N.lib(), name)(*args))
+        if size < 0:
+            raise ValueError(f"{name}: {N.last_error()}")
+        if len(_WS_BYTES) > 4096:
+            _WS_BYTES.clear()
+        _WS_BYTES[key] = size
+    return size
+
+
+def _head_strides(t: Tensor, what: str):
+    s = t.stride()
+    if s[-1] != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{what}: the channels of a head must be dense (stride {s[-1]})")
+    return s[:-1]
 
 
 def _index_strides(t: Tensor, shape, what: str, name: str):
-    """Strides of an index tensor over ``shape`` = [N, B(, T)]; it may leave
+    """Strides of an index tensor over ``shape`` = (N, B[, T]); it may leave
     out leading dims (shared by the models, or by the sequences)."""
     if t.dtype not in _INDEX:
         raise TypeError(f"{what}: {name} must be int32 or int64, got {t.dtype}")
     lead = len(shape) - t.dim()
-    if lead < 0 or t.dim() < 1 or tuple(t.shape) != tuple(shape[lead:]):
+    if lead < 0 or lead == len(shape) or tuple(t.shape) != shape[lead:]:
         raise ValueError(f"{what}: {name} {tuple(t.shape)} is not {list(shape)} or its last dims")
     return (0,) * lead + t.stride()
 
 
 def _row_geom(what: str, q: Optional[Tensor], k: Tensor, v: Optional[Tensor], positions: Tensor, rot: int = 0,
-              rows: int = 0):
+              rows: int = 0) -> bytes:
     """Checks the head tensors and builds the geometry array of the row
     kernels (include/widek.h)."""
-    if k.dim() != 5 or (v is not None and v.shape != k.shape):
-        raise ValueError(f"{what}: k and v must be [N, B, T, Hk, D], got {tuple(k.shape)}"
+    ks = k.shape
+    if len(ks) != 5 or (v is not None and v.shape != ks):
+        raise ValueError(f"{what}: k and v must be [N, B, T, Hk, D], got {tuple(ks)}"
                          + ("" if v is None else f" and {tuple(v.shape)}"))
-    n, b, t, hk, d = k.shape
-    if q is not None and (q.dim() != 5 or q.shape[:3] != k.shape[:3] or q.shape[4] != d):
-        raise ValueError(f"{what}: q {tuple(q.shape)} does not match k {tuple(k.shape)}")
-    sk = _row_strides(k, what)
-    sq = sk if q is None else _row_strides(q, what)
-    sv = sk if v is None else _row_strides(v, what)
-    return (ctypes.c_int64 * 23)(n, b, t, 0 if q is None else q.shape[3], hk, d, rot, rows, *sq, *sk, *sv,
-                                 *_index_strides(positions, (n, b, t), what, "positions"))
+    n, b, t, hk, d = ks
+    hq = 0
+    sk = _head_strides(k, what)
+    sq = sv = sk
+    if q is not None:
+        qs = q.shape
+        if len(qs) != 5 or qs[:3] != ks[:3] or qs[4] != d:
+            raise ValueError(f"{what}: q {tuple(qs)} does not match k {tuple(ks)}")
+        hq = qs[3]
+        sq = _head_strides(q, what)
+    if v is not None:
+        sv = _head_strides(v, what)
+    return _pack_rows(n, b, t, hq, hk, d, rot, rows, *sq, *sk, *sv,
+                      *_index_strides(positions, (n, b, t), what, "positions"))
 
 
 def _rope_args(what: str, q: Tensor, k: Tensor, v: Optional[Tensor], q_weight: Tensor, k_weight: Tensor, cos: Tensor,
                sin: Tensor, positions: Tensor):
-    dev = N.require_cuda(q, k, v, q_weight, k_weight, cos, sin, positions, what=what)
+    idx = _device(what, q, k, v, q_weight, k_weight, cos, sin, positions)
     _same_dtype(what, q, k, v, q_weight, k_weight)
-    if cos.dim() != 2 or sin.shape != cos.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
-        raise ValueError(f"{what}: cos and sin must be float32 [positions, rotated / 2], got {tuple(cos.shape)} "
+    cs = cos.shape
+    if len(cs) != 2 or sin.shape != cs or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise ValueError(f"{what}: cos and sin must be float32 [positions, rotated / 2], got {tuple(cs)} "
                          f"{cos.dtype} and {tuple(sin.shape)} {sin.dtype}")
-    geom = _row_geom(what, q, k, v, positions, 2 * cos.shape[1], cos.shape[0])
+    geom = _row_geom(what, q, k, v, positions, 2 * cs[1], cs[0])
     want = (k.shape[0], k.shape[4])
-    if tuple(q_weight.shape) != want or tuple(k_weight.shape) != want:
+    if q_weight.shape != want or k_weight.shape != want:
         raise ValueError(f"{what}: the norm weights must be [N, D] = {list(want)}, got {tuple(q_weight.shape)} and "
                          f"{tuple(k_weight.shape)}")
-    if 2 * cos.shape[1] > k.shape[4]:
-        raise ValueError(f"{what}: {2 * cos.shape[1]} rotated channels of heads of {k.shape[4]}")
-    return dev, geom, (_dense(q_weight), _dense(k_weight), _dense(cos), _dense(sin))
+    if 2 * cs[1] > want[1]:
+        raise ValueError(f"{what}: {2 * cs[1]} rotated channels of heads of {want[1]}")
+    return idx, geom, _dense(q_weight), _dense(k_weight), _dense(cos), _dense(sin)
 
 
 def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, cos: Tensor, sin: Tensor,
@@ -1016,15 +1070,15 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, cos: 
         return torch.ops.widek.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
     if _AG.needs_grad(q, k, q_weight, k_weight):
         return _AG.QkNormRopeFn.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
-    dev, geom, (qw, kw, co, si) = _rope_args("qk_norm_rope", q, k, None, q_weight, k_weight, cos, sin, positions)
-    yq = torch.empty(q.shape, device=dev, dtype=q.dtype)
-    yk = torch.empty(k.shape, device=dev, dtype=k.dtype)
-    with _guard(dev):
-        rc = N.lib().widek_qk_norm_rope_fwd(q.data_ptr(), k.data_ptr(), qw.data_ptr(), kw.data_ptr(), co.data_ptr(),
-                                            si.data_ptr(), positions.data_ptr(), yq.data_ptr(), yk.data_ptr(), geom,
-                                            float(eps), int(interleaved), int(positions.dtype == torch.int64),
-                                            N.dtype_code(q), N.stream_ptr(dev))
-    N.check(rc, "widek_qk_norm_rope_fwd")
+    return _qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+
+
+def _qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+    idx, geom, qw, kw, co, si = _rope_args("qk_norm_rope", q, k, None, q_weight, k_weight, cos, sin, positions)
+    yq, yk = q.new_empty(q.shape), k.new_empty(k.shape)
+    _launch(idx, "widek_qk_norm_rope_fwd", q.data_ptr(), k.data_ptr(), qw.data_ptr(), kw.data_ptr(), co.data_ptr(),
+            si.data_ptr(), positions.data_ptr(), yq.data_ptr(), yk.data_ptr(), geom, eps, interleaved,
+            _INDEX[positions.dtype], N.dtype_code(q))
     return yq, yk
 
 
@@ -1034,46 +1088,37 @@ def qk_norm_rope_bwd(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, c
     """Gradients of ``qk_norm_rope``: (dq, dk, dq_weight, dk_weight), the last
     two None unless asked for (widek_qk_norm_rope_bwd)."""
     what = "qk_norm_rope backward"
-    dev, geom, (qw, kw, co, si) = _rope_args(what, q, k, None, q_weight, k_weight, cos, sin, positions)
-    N.require_cuda(q, dyq, dyk, what=what)
+    idx, geom, qw, kw, co, si = _rope_args(what, q, k, None, q_weight, k_weight, cos, sin, positions)
+    _device(what, q, dyq, dyk)
     _same_dtype(what, q, dyq, dyk)
     if dyq.shape != q.shape or dyk.shape != k.shape:
         raise ValueError(f"{what}: gradients {tuple(dyq.shape)}, {tuple(dyk.shape)} do not match the heads")
     dyq, dyk = _dense(dyq), _dense(dyk)
-    dq = torch.empty(q.shape, device=dev, dtype=q.dtype)
-    dk = torch.empty(k.shape, device=dev, dtype=k.dtype)
+    dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
     if k.numel() == 0 or q.numel() == 0:
         return dq, dk, *((torch.zeros_like(qw), torch.zeros_like(kw)) if need_dw else (None, None))
     dqw, dkw = (torch.empty_like(qw), torch.empty_like(kw)) if need_dw else (None, None)
-    ws_bytes = N.lib().widek_qk_norm_rope_bwd_workspace(geom)
-    if ws_bytes < 0:
-        raise ValueError(f"{what}: {N.last_error()}")
-    ws = torch.empty(max(ws_bytes, 1), device=dev, dtype=torch.uint8)
-    with _guard(dev):
-        rc = N.lib().widek_qk_norm_rope_bwd(q.data_ptr(), k.data_ptr(), qw.data_ptr(), kw.data_ptr(), co.data_ptr(),
-                                            si.data_ptr(), positions.data_ptr(), dyq.data_ptr(), dyk.data_ptr(),
-                                            dq.data_ptr(), dk.data_ptr(), N.ptr(dqw), N.ptr(dkw), geom, float(eps),
-                                            int(interleaved), int(positions.dtype == torch.int64), N.dtype_code(q),
-                                            ws.data_ptr(), ws_bytes, N.stream_ptr(dev))
-    N.check(rc, "widek_qk_norm_rope_bwd")
+    ws_bytes = _workspace("widek_qk_norm_rope_bwd_workspace", geom, geom)
+    ws = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8)
+    _launch(idx, "widek_qk_norm_rope_bwd", q.data_ptr(), k.data_ptr(), qw.data_ptr(), kw.data_ptr(), co.data_ptr(),
+            si.data_ptr(), positions.data_ptr(), dyq.data_ptr(), dyk.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+            N.ptr(dqw), N.ptr(dkw), geom, eps, interleaved, _INDEX[positions.dtype], N.dtype_code(q), ws.data_ptr(),
+            ws_bytes)
     return dq, dk, dqw, dkw
 
 
-def _cache_args(what: str, cache, n: int, b: int, hk: int, d: int, *tensors: Optional[Tensor]) -> torch.device:
-    dev = N.require_cuda(cache.k, cache.v, cache.table, cache.k_scale, cache.v_scale, *tensors, what=what)
-    if (cache.n, cache.batch, cache.kv_heads, cache.head_dim) != (n, b, hk, d):
+def _cache_args(what: str, cache, n: int, b: int, hk: int, d: int, ref: Tensor, *others: Optional[Tensor]) -> int:
+    idx = _device(what, ref, cache.k, cache.v, cache.table, cache.k_scale, cache.v_scale, *others)
+    if cache.sizes != (n, b, hk, d):
         raise ValueError(f"{what}: N={n}, B={b}, Hk={hk}, D={d} do not match {cache!r}")
-    return dev
+    if not cache.quantized and cache.k.dtype != ref.dtype:
+        raise TypeError(f"{what}: dtype mismatch ({ref.dtype} vs a cache of {cache.k.dtype})")
+    return idx
 
 
 def _no_grad(what: str, *tensors: Optional[Tensor]) -> None:
     if _AG.needs_grad(*tensors):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
-
-
-def _cache_type(what: str, cache, dtype: torch.dtype) -> None:
-    if not cache.quantized and cache.k.dtype != dtype:
-        raise TypeError(f"{what}: dtype mismatch ({dtype} vs a cache of {cache.k.dtype})")
 
 
 def qk_norm_rope_write(q: Tensor, k: Tensor, v: Tensor, q_weight: Tensor, k_weight: Tensor, cos: Tensor, sin: Tensor,
@@ -1087,18 +1132,14 @@ def qk_norm_rope_write(q: Tensor, k: Tensor, v: Tensor, q_weight: Tensor, k_weig
     if _compiling():
         return torch.ops.widek.qk_norm_rope_write(q, k, v, q_weight, k_weight, cos, sin, positions, cache.k, cache.v,
                                                   cache.table, cache.k_scale, cache.v_scale, eps, interleaved)
-    dev, geom, (qw, kw, co, si) = _rope_args(what, q, k, v, q_weight, k_weight, cos, sin, positions)
+    idx, geom, qw, kw, co, si = _rope_args(what, q, k, v, q_weight, k_weight, cos, sin, positions)
     n, b, _, hk, d = k.shape
     _cache_args(what, cache, n, b, hk, d, q)
-    _cache_type(what, cache, q.dtype)
-    yq = torch.empty(q.shape, device=dev, dtype=q.dtype)
-    with _guard(dev):
-        rc = N.lib().widek_qk_norm_rope_write_fwd(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), qw.data_ptr(), kw.data_ptr(), co.data_ptr(), si.data_ptr(),
-            positions.data_ptr(), yq.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), N.ptr(cache.k_scale),
-            N.ptr(cache.v_scale), cache.table.data_ptr(), geom, cache.geom, float(eps), int(interleaved),
-            int(positions.dtype == torch.int64), cache.fmt, N.dtype_code(q), N.stream_ptr(dev))
-    N.check(rc, "widek_qk_norm_rope_write_fwd")
+    yq = q.new_empty(q.shape)
+    _launch(idx, "widek_qk_norm_rope_write_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), qw.data_ptr(),
+            kw.data_ptr(), co.data_ptr(), si.data_ptr(), positions.data_ptr(), yq.data_ptr(), cache.k.data_ptr(),
+            cache.v.data_ptr(), N.ptr(cache.k_scale), N.ptr(cache.v_scale), cache.table.data_ptr(), geom, cache.geom,
+            eps, interleaved, _INDEX[positions.dtype], cache.fmt, N.dtype_code(q))
     return yq
 
 
@@ -1113,16 +1154,11 @@ def cache_write(cache, k: Tensor, v: Tensor, positions: Tensor) -> None:
         return
     geom = _row_geom(what, None, k, v, positions)
     n, b, _, hk, d = k.shape
-    dev = _cache_args(what, cache, n, b, hk, d, k, v, positions)
     _same_dtype(what, k, v)
-    _cache_type(what, cache, k.dtype)
-    with _guard(dev):
-        rc = N.lib().widek_cache_write_fwd(k.data_ptr(), v.data_ptr(), positions.data_ptr(), cache.k.data_ptr(),
-                                           cache.v.data_ptr(), N.ptr(cache.k_scale), N.ptr(cache.v_scale),
-                                           cache.table.data_ptr(), geom, cache.geom,
-                                           int(positions.dtype == torch.int64), cache.fmt, N.dtype_code(k),
-                                           N.stream_ptr(dev))
-    N.check(rc, "widek_cache_write_fwd")
+    idx = _cache_args(what, cache, n, b, hk, d, k, v, positions)
+    _launch(idx, "widek_cache_write_fwd", k.data_ptr(), v.data_ptr(), positions.data_ptr(), cache.k.data_ptr(),
+            cache.v.data_ptr(), N.ptr(cache.k_scale), N.ptr(cache.v_scale), cache.table.data_ptr(), geom, cache.geom,
+            _INDEX[positions.dtype], cache.fmt, N.dtype_code(k))
 
 
 def cache_read(cache, positions: Tensor, dtype: Optional[torch.dtype] = None):
@@ -1135,24 +1171,18 @@ def cache_read(cache, positions: Tensor, dtype: Optional[torch.dtype] = None):
     if _compiling():
         return torch.ops.widek.cache_read(cache.k, cache.v, cache.table, cache.k_scale, cache.v_scale, positions,
                                           dtype)
-    dev = N.require_cuda(cache.k, cache.v, cache.table, cache.k_scale, cache.v_scale, positions, what=what)
     if dtype is None:
         dtype = torch.bfloat16 if cache.quantized else cache.k.dtype
-    _cache_type(what, cache, dtype)
-    n, b, hk, d = cache.n, cache.batch, cache.kv_heads, cache.head_dim
+    n, b, hk, d = cache.sizes
     if positions.dim() < 1:
         raise ValueError(f"{what}: positions must be [T], [B, T] or [N, B, T]")
-    t = positions.shape[-1]
-    k = torch.empty((n, b, t, hk, d), device=dev, dtype=dtype)
+    k = torch.empty((n, b, positions.shape[-1], hk, d), device=cache.k.device, dtype=dtype)
     v = torch.empty_like(k)
     geom = _row_geom(what, None, k, v, positions)
-    with _guard(dev):
-        rc = N.lib().widek_cache_read_fwd(cache.k.data_ptr(), cache.v.data_ptr(), N.ptr(cache.k_scale),
-                                          N.ptr(cache.v_scale), cache.table.data_ptr(), positions.data_ptr(),
-                                          k.data_ptr(), v.data_ptr(), geom, cache.geom,
-                                          int(positions.dtype == torch.int64), cache.fmt, N.dtype_code(k),
-                                          N.stream_ptr(dev))
-    N.check(rc, "widek_cache_read_fwd")
+    idx = _cache_args(what, cache, n, b, hk, d, k, positions)
+    _launch(idx, "widek_cache_read_fwd", cache.k.data_ptr(), cache.v.data_ptr(), N.ptr(cache.k_scale),
+            N.ptr(cache.v_scale), cache.table.data_ptr(), positions.data_ptr(), k.data_ptr(), v.data_ptr(), geom,
+            cache.geom, _INDEX[positions.dtype], cache.fmt, N.dtype_code(k))
     return k, v
 
 
@@ -1172,29 +1202,22 @@ def decode_attention(q: Tensor, cache, lengths: Tensor, scale: Optional[float] =
     if _compiling():
         return torch.ops.widek.decode_attention(q, cache.k, cache.v, cache.table, cache.k_scale, cache.v_scale,
                                                 lengths, scale, window)
-    if q.dim() != 4:
-        raise ValueError(f"{what}: q must be [N, B, Hq, D], got {tuple(q.shape)}")
-    n, b, hq, d = q.shape
+    qs = q.shape
+    if len(qs) != 4:
+        raise ValueError(f"{what}: q must be [N, B, Hq, D], got {tuple(qs)}")
+    n, b, hq, d = qs
     hk = cache.kv_heads
-    dev = _cache_args(what, cache, n, b, hk, d, q, lengths)
-    _cache_type(what, cache, q.dtype)
+    idx = _cache_args(what, cache, n, b, hk, d, q, lengths)
     if hk < 1 or hq % hk != 0:
         raise ValueError(f"{what}: {hq} query heads over {hk} key heads")
-    geom = (ctypes.c_int64 * 10)(n, b, hq, hk, d, *_row_strides(q, what),
-                                 *_index_strides(lengths, (n, b), what, "lengths"))
-    lib = N.lib()
-    ws_bytes = lib.widek_decode_attention_workspace(geom, cache.geom, window, cache.fmt)
-    if ws_bytes < 0:
-        raise ValueError(f"{what}: {N.last_error()}")
-    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
-    out = torch.empty((n, b, hq, d), device=dev, dtype=q.dtype)
-    with _guard(dev):
-        rc = lib.widek_decode_attention_fwd(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(),
-                                            N.ptr(cache.k_scale), N.ptr(cache.v_scale), cache.table.data_ptr(),
-                                            lengths.data_ptr(), out.data_ptr(), geom, cache.geom, float(scale),
-                                            int(window), int(lengths.dtype == torch.int64), cache.fmt,
-                                            N.dtype_code(q), N.ptr(ws), ws_bytes, N.stream_ptr(dev))
-    N.check(rc, "widek_decode_attention_fwd")
+    geom = _pack_decode(n, b, hq, hk, d, *_head_strides(q, what), *_index_strides(lengths, (n, b), what, "lengths"))
+    ws_bytes = _workspace("widek_decode_attention_workspace", (geom, cache.geom, window, cache.fmt, idx), geom,
+                          cache.geom, window, cache.fmt)
+    ws = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8) if ws_bytes else None
+    out = q.new_empty(qs)
+    _launch(idx, "widek_decode_attention_fwd", q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(),
+            N.ptr(cache.k_scale), N.ptr(cache.v_scale), cache.table.data_ptr(), lengths.data_ptr(), out.data_ptr(),
+            geom, cache.geom, scale, window, _INDEX[lengths.dtype], cache.fmt, N.dtype_code(q), N.ptr(ws), ws_bytes)
     return out
 
 
