@@ -103,6 +103,7 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
 
 int decode_args(DecodeArgs& a, const char* what, const int64_t* g, const int64_t* cgeom, int64_t window, int fmt) {
     if (!g || !cgeom) return set_error(WIDEK_ERR_INVALID, "%s: null geometry", what);
+    if (cache_fmt_size(fmt) == 0) return set_error(WIDEK_ERR_INVALID, "%s: unknown cache format %d", what, fmt);
     for (int i = 0; i < 5; ++i)
         if (g[i] < 0 || g[i] > 0x7fffffff)
             return set_error(WIDEK_ERR_INVALID, "%s: size %d out of range (%lld)", what, i, (long long)g[i]);

@@ -83,19 +83,133 @@ __device__ __forceinline__ float code_scale(float amax, bool is_i8) {
     return __fdiv_rn(m, is_i8 ? 127.f : 448.f);
 }
 
-__device__ __forceinline__ uint8_t code_i8(float x, float scale) {
-    const int q = __float2int_rn(__fdiv_rn(x, scale));
-    return (uint8_t)(int8_t)(q > 127 ? 127 : (q < -127 ? -127 : q));
+// Two fp32 operations in one instruction, each rounded as usual.
+__device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, float b0, float b1, float c0, float c1) {
+    asm("{.reg .b64 a, b, c, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c; mov.b64 {%0, %1}, d;}"
+        : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void mul2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+    asm("{.reg .b64 a, b, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mul.rn.f32x2 d, a, b; mov.b64 {%0, %1}, d;}"
+        : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void add2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+    asm("{.reg .b64 a, b, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; add.rn.f32x2 d, a, b; mov.b64 {%0, %1}, d;}"
+        : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+// d = a b + c, d = a b and d = a b with one b, over VEC elements.
+template <int VEC>
+__device__ __forceinline__ void fma_vec(float* d, const float* a, const float* b, const float* c) {
+    if constexpr (VEC == 1) d[0] = fmaf(a[0], b[0], c[0]);
+#pragma unroll
+    for (int j = 0; j + 1 < VEC; j += 2) fma2(d[j], d[j + 1], a[j], a[j + 1], b[j], b[j + 1], c[j], c[j + 1]);
+}
+template <int VEC>
+__device__ __forceinline__ void mul_vec(float* d, const float* a, const float* b) {
+    if constexpr (VEC == 1) d[0] = a[0] * b[0];
+#pragma unroll
+    for (int j = 0; j + 1 < VEC; j += 2) mul2(d[j], d[j + 1], a[j], a[j + 1], b[j], b[j + 1]);
+}
+template <int VEC>
+__device__ __forceinline__ void scale_vec(float* d, const float* a, float b) {
+    if constexpr (VEC == 1) d[0] = a[0] * b;
+#pragma unroll
+    for (int j = 0; j + 1 < VEC; j += 2) mul2(d[j], d[j + 1], a[j], a[j + 1], b, b);
+}
+// Sum of a b over VEC elements, two partial sums.
+template <int VEC>
+__device__ __forceinline__ float dot_vec(const float* a, const float* b) {
+    if constexpr (VEC == 1) return a[0] * b[0];
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int j = 0; j + 1 < VEC; j += 2) fma2(s0, s1, a[j], a[j + 1], b[j], b[j + 1], s0, s1);
+    return s0 + s1;
 }
 
-__device__ __forceinline__ uint8_t code_e4m3(float x, float scale) {
-    return (uint8_t)__nv_cvt_float_to_fp8(__fdiv_rn(x, scale), __NV_SATFINITE, __NV_E4M3);
+// The larger of two magnitudes, NaN if either is (fmaxf would drop it).
+__device__ __forceinline__ float amax2(float x, float y) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(fabsf(x)), "f"(fabsf(y)));
+    return m;
 }
 
-__device__ __forceinline__ float value_e4m3(uint8_t c) {
-    __nv_fp8_e4m3 f;
-    f.__x = c;
-    return (float)f;
+// Codes of VEC values. The division is rounded once and its result then to a
+// code: x * (1 / scale) gives the same code unless it lies within a few units
+// in the last place of a tie, and only there (and in rows that are not finite)
+// the divisions are done.
+template <int VEC>
+__device__ __forceinline__ void codes_i8(const float* x, float scale, uint8_t* out) {
+    const float inv = __fdiv_rn(1.f, scale);
+    float q[VEC], r[VEC], off[VEC];
+    scale_vec<VEC>(q, x, inv);
+    // 1.5 * 2^23: the sum's low bits are q rounded half to even
+    if constexpr (VEC == 1) {
+        r[0] = q[0] + 12582912.f;
+        off[0] = q[0] - (r[0] - 12582912.f);
+    }
+#pragma unroll
+    for (int j = 0; j + 1 < VEC; j += 2) {
+        float t0, t1;
+        add2(r[j], r[j + 1], q[j], q[j + 1], 12582912.f, 12582912.f);
+        add2(t0, t1, r[j], r[j + 1], -12582912.f, -12582912.f);
+        fma2(off[j], off[j + 1], t0, t1, -1.f, -1.f, q[j], q[j + 1]);
+    }
+    bool sure = true;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        out[j] = (uint8_t)__float_as_uint(r[j]);
+        sure = sure && fabsf(off[j]) < 0.4999f;      // false for NaN
+    }
+    if (!sure) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const int k = __float2int_rn(__fdiv_rn(x[j], scale));
+            out[j] = (uint8_t)(int8_t)(k > 127 ? 127 : (k < -127 ? -127 : k));
+        }
+    }
+}
+
+template <int VEC>
+__device__ __forceinline__ void codes_e4m3(const float* x, float scale, uint8_t* out) {
+    const float inv = __fdiv_rn(1.f, scale);
+    bool sure = scale < 3e38f;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        // the codes just below and just above the product agree: no tie between
+        const float q = x[j] * inv;
+        const float2 pair = make_float2(q * (1.f - 2e-6f), q * (1.f + 2e-6f));
+        const uint16_t c = __nv_cvt_float2_to_fp8x2(pair, __NV_SATFINITE, __NV_E4M3);
+        out[j] = (uint8_t)c;
+        sure = sure && (c & 0xff) == (c >> 8);
+    }
+    if (!sure) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            out[j] = (uint8_t)__nv_cvt_float_to_fp8(__fdiv_rn(x[j], scale), __NV_SATFINITE, __NV_E4M3);
+    }
+}
+
+// Values of VEC codes (unscaled). An int8 by way of the fp32 number
+// 2^23 + (code + 128): integer conversions run at a quarter of that rate.
+template <int VEC>
+__device__ __forceinline__ void values_i8(const uint8_t* c, float* x) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) x[j] = __uint_as_float(0x4b000000u | (uint32_t)(c[j] ^ 0x80)) - 8388736.f;
+}
+template <int VEC>
+__device__ __forceinline__ void values_e4m3(const uint8_t* c, float* x) {
+    if constexpr (VEC == 1) {
+        __nv_fp8_e4m3 f;
+        f.__x = c[0];
+        x[0] = (float)f;
+    }
+#pragma unroll
+    for (int j = 0; j + 1 < VEC; j += 2) {
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c[j] | (c[j + 1] << 8)), __NV_E4M3);
+        const float2 f = __half22float2(__half2(h));
+        x[j] = f.x;
+        x[j + 1] = f.y;
+    }
 }
 
 }  // namespace widek

@@ -24,6 +24,7 @@
 #include "paged_cache.cuh"
 
 #include <initializer_list>
+#include <type_traits>
 
 namespace widek {
 
@@ -65,9 +66,10 @@ struct RowArgs {
     Strides sq, sk, sv;
     int64_t pos_n, pos_b, pos_t;
     int pos64, n, b, t, hq, hk, d, rot, table_rows, inter, lanes_log2;
-    uint32_t rows;
+    uint32_t units;               // a unit: HPT heads of one kind of a token, one group of lanes
+    int parts_q, parts_k;         // units of a token's q heads and k heads (and as many of v)
     float eps;
-    FastDiv heads, tdiv, bdiv;
+    FastDiv parts, tdiv, bdiv;
     PagedCache c;
     int* err;
 };
@@ -79,10 +81,23 @@ struct alignas(sizeof(T) * VEC) Pack {
 };
 
 template <typename T, int VEC>
-__device__ __forceinline__ void load_vec(const T* p, float* out) {
-    const Pack<T, VEC> r = *reinterpret_cast<const Pack<T, VEC>*>(p);
+__device__ __forceinline__ void unpack(const Pack<T, VEC>& r, float* out) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) out[i] = to_f<T>(r.v[i]);
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T* p, float* out) {
+    const Pack<T, VEC> r = *reinterpret_cast<const Pack<T, VEC>*>(p);
+    unpack<T, VEC>(r, out);
+}
+
+// Loads that belong together are issued without branches around them (places
+// outside a row read its first vector and are zeroed later): a branch around
+// each kept them from being in flight at the same time.
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> load_pack(const T* p) {
+    return *reinterpret_cast<const Pack<T, VEC>*>(p);
 }
 
 template <typename T, int VEC>
@@ -107,14 +122,6 @@ __device__ __forceinline__ unsigned group_mask(int lanes) {
     return lanes == 32 ? 0xffffffffu : ((1u << lanes) - 1u) << (threadIdx.x & 31 & ~(lanes - 1));
 }
 
-__device__ __forceinline__ float group_sum(float v, int lanes, unsigned mask) {
-    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
-    return v;
-}
-
-// The larger of two magnitudes, NaN if either is (fmaxf would drop it).
-__device__ __forceinline__ float amax2(float x, float y) { return (x != x || y != y) ? x + y : fmaxf(x, y); }
-
 // Channels of unit u (first elements of its vectors A and B). Units below
 // `turned` hold pairs of the rotation.
 template <int VEC>
@@ -128,29 +135,45 @@ __device__ __forceinline__ void unit_channels(int u, int turned, int rot, int in
     }
 }
 
-// Turns the pairs of one unit by (co, si); SIGN -1 turns back.
+// The rotation of one unit as y_a = x_a ca + p_a sa, y_b = x_b cb + p_b sb with
+// each channel's partner p: the coefficients, the norm's weights folded in
+// (w_p belongs to the partner), from the angles' cosines and sines. SIGN -1
+// turns back; then the weights apply after the turn and are left out.
 template <int VEC>
-__device__ __forceinline__ void turn(float* a, float* b, const float* co, const float* si, int inter, float sign) {
-    if (!inter || VEC == 1) {
+struct Turn {
+    float ca[VEC], sa[VEC], cb[VEC], sb[VEC];
+    __device__ __forceinline__ void set(const float* co, const float* si, const float* wa, const float* wb, int inter) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            const float s = si[j] * sign, x = a[j], y = b[j];
-            a[j] = x * co[j] - y * s;
-            b[j] = y * co[j] + x * s;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j + 1 < VEC; j += 2) {
-            const float s0 = si[j / 2] * sign, x0 = a[j], y0 = a[j + 1], c0 = co[j / 2];
-            a[j] = x0 * c0 - y0 * s0;
-            a[j + 1] = y0 * c0 + x0 * s0;
-            const int i = VEC / 2 + j / 2;
-            const float s1 = si[i] * sign, x1 = b[j], y1 = b[j + 1], c1 = co[i];
-            b[j] = x1 * c1 - y1 * s1;
-            b[j + 1] = y1 * c1 + x1 * s1;
+            if (!inter || VEC == 1) {
+                ca[j] = co[j] * wa[j];
+                sa[j] = -si[j] * wb[j];
+                cb[j] = co[j] * wb[j];
+                sb[j] = si[j] * wa[j];
+            } else {
+                const int p = j / 2, q = VEC / 2 + j / 2;
+                ca[j] = co[p] * wa[j];
+                sa[j] = (j & 1 ? si[p] : -si[p]) * wa[j ^ 1];
+                cb[j] = co[q] * wb[j];
+                sb[j] = (j & 1 ? si[q] : -si[q]) * wb[j ^ 1];
+            }
         }
     }
-}
+    __device__ __forceinline__ void apply(float* a, float* b, int inter) const {
+        float pa[VEC], pb[VEC];
+        if (!inter || VEC == 1) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) pa[j] = b[j], pb[j] = a[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) pa[j] = a[VEC == 1 ? 0 : j ^ 1], pb[j] = b[VEC == 1 ? 0 : j ^ 1];
+        }
+        mul_vec<VEC>(a, a, ca);
+        mul_vec<VEC>(b, b, cb);
+        fma_vec<VEC>(a, pa, sa, a);
+        fma_vec<VEC>(b, pb, sb, b);
+    }
+};
 
 enum RowOut : int { OUT_DENSE = 0, OUT_SAME = 1, OUT_I8 = 2, OUT_E4M3 = 3 };
 
@@ -159,8 +182,8 @@ template <typename T, int VEC, int OUT>
 __device__ __forceinline__ void store_code(void* base, int64_t at, const float* x, float scale) {
     if constexpr (OUT == OUT_I8 || OUT == OUT_E4M3) {
         Pack<uint8_t, VEC> p;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) p.v[j] = OUT == OUT_I8 ? code_i8(x[j], scale) : code_e4m3(x[j], scale);
+        if constexpr (OUT == OUT_I8) codes_i8<VEC>(x, scale, p.v);
+        else codes_e4m3<VEC>(x, scale, p.v);
         *reinterpret_cast<Pack<uint8_t, VEC>*>(static_cast<uint8_t*>(base) + at) = p;
     } else {
         store_vec<T, VEC>(static_cast<T*>(base) + at, x);
@@ -169,168 +192,215 @@ __device__ __forceinline__ void store_code(void* base, int64_t at, const float* 
 
 // Rows in: q heads (normed, rotated, dense out), k heads (the same, dense out
 // or into the cache), v heads (into the cache). ROPE false: k and v heads go
-// to the cache as they are.
-template <typename T, int VEC, int UPL, int OUT, bool ROPE>
+// to the cache as they are. A group of lanes takes HPT heads of one token and
+// kind at once: its loads are in flight together, and the angles and weights
+// are read once (one row at a time reached 3.8 of 6.5 TB/s).
+template <typename T, int VEC, int UPL, int HPT, int OUT, bool ROPE>
 __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ RowArgs a) {
     const int lanes = 1 << a.lanes_log2;
     const int lane = threadIdx.x & (lanes - 1);
     const unsigned mask = group_mask(lanes);
-    uint32_t row = blockIdx.x * (kThreads >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2);
-    const bool live = row < a.rows;
-    if (!live) row = a.rows - 1;
-    uint32_t hh, t, b;
-    const uint32_t tok = a.heads.divmod(row, hh);
+    uint32_t unit = blockIdx.x * (kThreads >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2);
+    if (unit >= a.units) return;
+    uint32_t part, t, b;
+    const uint32_t tok = a.parts.divmod(unit, part);
     const uint32_t nb = a.tdiv.divmod(tok, t);
     const uint32_t i = a.bdiv.divmod(nb, b);
-    const bool is_q = (int)hh < a.hq;
-    const bool is_v = (int)hh >= a.hq + a.hk;
-    const int h = is_q ? (int)hh : (is_v ? (int)hh - a.hq - a.hk : (int)hh - a.hq);
+    const bool is_q = (int)part < a.parts_q;
+    const bool is_v = (int)part >= a.parts_q + a.parts_k;
+    const int h0 = HPT * (is_q ? (int)part : (is_v ? (int)part - a.parts_q - a.parts_k : (int)part - a.parts_q));
+    const int nh = min(HPT, (is_q ? a.hq : a.hk) - h0);
     const Strides st = is_q ? a.sq : (is_v ? a.sv : a.sk);
-    const T* src = static_cast<const T*>(is_q ? a.q : (is_v ? a.v : a.k)) + i * st.n + b * st.b + t * st.t + h * st.h;
+    const T* src = static_cast<const T*>(is_q ? a.q : (is_v ? a.v : a.k)) + i * st.n + b * st.b + t * st.t + h0 * st.h;
     const int pos = load_index(a.pos, i * a.pos_n + b * a.pos_b + t * a.pos_t, a.pos64);
 
     const int turned = ROPE ? a.rot / 2 / VEC : 0;
-    float xa[UPL][VEC], xb[UPL][VEC];
+    int ca[UPL], cb[UPL];
+    Pack<T, VEC> ra[HPT][UPL], rb[HPT][UPL];
 #pragma unroll
-    for (int s = 0; s < UPL; ++s) {
-        int ca, cb;
-        unit_channels<VEC>(lane + s * lanes, turned, a.rot, a.inter, ca, cb);
+    for (int s = 0; s < UPL; ++s) unit_channels<VEC>(lane + s * lanes, turned, a.rot, a.inter, ca[s], cb[s]);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) xa[s][j] = xb[s][j] = 0.f;
-        if (ca < a.d) load_vec<T, VEC>(src + ca, xa[s]);
-        if (cb < a.d) load_vec<T, VEC>(src + cb, xb[s]);
-    }
+    for (int r = 0; r < HPT; ++r)
+#pragma unroll
+        for (int s = 0; s < UPL; ++s) {
+            const T* row = src + min(r, nh - 1) * st.h;
+            ra[r][s] = load_pack<T, VEC>(row + (ca[s] < a.d ? ca[s] : 0));
+            rb[r][s] = load_pack<T, VEC>(row + (cb[s] < a.d ? cb[s] : 0));
+        }
 
     bool keep = pos >= 0;
-    if (ROPE && !is_v) {
-        if (pos >= a.table_rows) {
-            keep = false;
-            if (live && lane == 0) raise_device_error(a.err, DEV_ERR_INDEX);
-        }
-        float ss = 0.f;
-#pragma unroll
-        for (int s = 0; s < UPL; ++s)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) ss += xa[s][j] * xa[s][j] + xb[s][j] * xb[s][j];
-        const float r = rsqrtf(group_sum(ss, lanes, mask) / (float)a.d + a.eps);
+    const bool rope = ROPE && !is_v;
+    if (rope && pos >= a.table_rows) {
+        keep = false;
+        if (lane == 0) raise_device_error(a.err, DEV_ERR_INDEX);
+    }
+    Turn<VEC> turn[UPL];                  // channels that do not turn: ca and cb are the weights
+    float norm[HPT];
+    if (ROPE && rope) {
         const T* w = static_cast<const T*>(is_q ? a.qw : a.kw) + (int64_t)i * a.d;
         const int64_t trow = (int64_t)(keep ? pos : 0) * (a.rot / 2);
 #pragma unroll
         for (int s = 0; s < UPL; ++s) {
             const int u = lane + s * lanes;
-            int ca, cb;
-            unit_channels<VEC>(u, turned, a.rot, a.inter, ca, cb);
-            float wv[VEC];
-            if (ca < a.d) {
-                load_vec<T, VEC>(w + ca, wv);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) xa[s][j] *= r * wv[j];
-            }
-            if (cb < a.d) {
-                load_vec<T, VEC>(w + cb, wv);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) xb[s][j] *= r * wv[j];
-            }
-            if (u < turned && keep) {
+            float wa[VEC], wb[VEC];
+            load_vec<T, VEC>(w + (ca[s] < a.d ? ca[s] : 0), wa);
+            load_vec<T, VEC>(w + (cb[s] < a.d ? cb[s] : 0), wb);
+            if (u < turned && a.table_rows > 0) {
                 float co[VEC], si[VEC];
                 load_table<VEC>(a.cs + trow + u * VEC, co);
                 load_table<VEC>(a.sn + trow + u * VEC, si);
-                turn<VEC>(xa[s], xb[s], co, si, a.inter, 1.f);
+                turn[s].set(co, si, wa, wb, a.inter);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) turn[s].ca[j] = wa[j], turn[s].cb[j] = wb[j];
             }
         }
+#pragma unroll
+        for (int r = 0; r < HPT; ++r) {
+            norm[r] = 0.f;
+#pragma unroll
+            for (int s = 0; s < UPL; ++s) {
+                float x[VEC];
+                unpack<T, VEC>(ra[r][s], x);
+                norm[r] += ca[s] < a.d ? dot_vec<VEC>(x, x) : 0.f;
+                unpack<T, VEC>(rb[r][s], x);
+                norm[r] += cb[s] < a.d ? dot_vec<VEC>(x, x) : 0.f;
+            }
+        }
+        for (int o = lanes >> 1; o > 0; o >>= 1)
+#pragma unroll
+            for (int r = 0; r < HPT; ++r) norm[r] += __shfl_xor_sync(mask, norm[r], o);
+        const float inv_d = 1.f / (float)a.d;
+#pragma unroll
+        for (int r = 0; r < HPT; ++r) norm[r] = rsqrtf(norm[r] * inv_d + a.eps);
     }
 
-    if (is_q || OUT == OUT_DENSE) {
-        T* y = static_cast<T*>(is_q ? a.yq : a.yk) + ((int64_t)tok * (is_q ? a.hq : a.hk) + h) * a.d;
-        if (!live) return;
-#pragma unroll
-        for (int s = 0; s < UPL; ++s) {
-            int ca, cb;
-            unit_channels<VEC>(lane + s * lanes, turned, a.rot, a.inter, ca, cb);
-            if (!keep) {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) xa[s][j] = xb[s][j] = 0.f;
-            }
-            if (ca < a.d) store_vec<T, VEC>(y + ca, xa[s]);
-            if (cb < a.d) store_vec<T, VEC>(y + cb, xb[s]);
-        }
-        return;
+    int slot = -1;
+    if (OUT != OUT_DENSE && !is_q && keep) {
+        slot = a.c.row(i, b, a.hk, h0, pos);
+        if (slot < 0 && lane == 0) raise_device_error(a.err, DEV_ERR_INDEX);
     }
-    if constexpr (OUT != OUT_DENSE) {
-        float scale = 1.f;
-        if constexpr (OUT == OUT_I8 || OUT == OUT_E4M3) {
-            float m = 0.f;
 #pragma unroll
-            for (int s = 0; s < UPL; ++s)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) m = amax2(m, amax2(fabsf(xa[s][j]), fabsf(xb[s][j])));
-            for (int o = lanes >> 1; o > 0; o >>= 1) m = amax2(m, __shfl_xor_sync(mask, m, o));
-            scale = code_scale(m, OUT == OUT_I8);
-        }
-        if (!live || !keep) return;
-        const int slot = a.c.row(i, b, a.hk, h, pos);
-        if (slot < 0) {
-            if (lane == 0) raise_device_error(a.err, DEV_ERR_INDEX);
-            return;
-        }
-        const int64_t at = (int64_t)i * a.c.pages * a.hk * a.c.page + slot;
-        void* base = is_v ? a.c.v : a.c.k;
-        if constexpr (OUT == OUT_I8 || OUT == OUT_E4M3) {
-            if (lane == 0) (is_v ? a.c.vs : a.c.ks)[at] = scale;
-        }
+    for (int r = 0; r < HPT; ++r) {
+        float xa[UPL][VEC], xb[UPL][VEC];
 #pragma unroll
         for (int s = 0; s < UPL; ++s) {
-            int ca, cb;
-            unit_channels<VEC>(lane + s * lanes, turned, a.rot, a.inter, ca, cb);
-            if (ca < a.d) store_code<T, VEC, OUT>(base, at * a.d + ca, xa[s], scale);
-            if (cb < a.d) store_code<T, VEC, OUT>(base, at * a.d + cb, xb[s], scale);
+            unpack<T, VEC>(ra[r][s], xa[s]);
+            unpack<T, VEC>(rb[r][s], xb[s]);
+            if (ROPE && rope) {
+                scale_vec<VEC>(xa[s], xa[s], norm[r]);
+                scale_vec<VEC>(xb[s], xb[s], norm[r]);
+                if (lane + s * lanes < turned) {
+                    turn[s].apply(xa[s], xb[s], a.inter);
+                } else {
+                    mul_vec<VEC>(xa[s], xa[s], turn[s].ca);
+                    mul_vec<VEC>(xb[s], xb[s], turn[s].cb);
+                }
+            }
+        }
+        if (is_q || OUT == OUT_DENSE) {
+            if (r >= nh) break;
+            T* y = static_cast<T*>(is_q ? a.yq : a.yk) + ((int64_t)tok * (is_q ? a.hq : a.hk) + h0 + r) * a.d;
+#pragma unroll
+            for (int s = 0; s < UPL; ++s) {
+                if (!keep) {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) xa[s][j] = xb[s][j] = 0.f;
+                }
+                if (ca[s] < a.d) store_vec<T, VEC>(y + ca[s], xa[s]);
+                if (cb[s] < a.d) store_vec<T, VEC>(y + cb[s], xb[s]);
+            }
+        } else if constexpr (OUT != OUT_DENSE) {
+            float scale = 1.f;
+            if constexpr (OUT == OUT_I8 || OUT == OUT_E4M3) {
+                float m = 0.f;
+#pragma unroll
+                for (int s = 0; s < UPL; ++s) {
+                    float ma = 0.f, mb = 0.f;
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) ma = amax2(ma, xa[s][j]), mb = amax2(mb, xb[s][j]);
+                    if (ca[s] < a.d) m = amax2(m, ma);
+                    if (cb[s] < a.d) m = amax2(m, mb);
+                }
+                for (int o = lanes >> 1; o > 0; o >>= 1) m = amax2(m, __shfl_xor_sync(mask, m, o));
+                scale = code_scale(m, OUT == OUT_I8);
+            }
+            if (r >= nh || slot < 0) break;               // the same for all lanes of the group
+            const int64_t at = (int64_t)i * a.c.pages * a.hk * a.c.page + slot + (int64_t)r * a.c.page;
+            void* base = is_v ? a.c.v : a.c.k;
+            if constexpr (OUT == OUT_I8 || OUT == OUT_E4M3) {
+                if (lane == 0) (is_v ? a.c.vs : a.c.ks)[at] = scale;
+            }
+#pragma unroll
+            for (int s = 0; s < UPL; ++s) {
+                if (ca[s] < a.d) store_code<T, VEC, OUT>(base, at * a.d + ca[s], xa[s], scale);
+                if (cb[s] < a.d) store_code<T, VEC, OUT>(base, at * a.d + cb[s], xb[s], scale);
+            }
         }
     }
 }
 
 // Cache rows out: value = code * scale, rounded once to T; k and v heads of
-// the tokens at `pos`, zeros for padding.
-template <typename T, int VEC, int UPL, int IN>
+// the tokens at `pos`, zeros for padding. HPT heads of a token at once.
+template <typename T, int VEC, int UPL, int HPT, int IN>
 __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_constant__ RowArgs a) {
+    constexpr bool CODE = IN == OUT_I8 || IN == OUT_E4M3;
+    using C = typename std::conditional<CODE, uint8_t, T>::type;
     const int lanes = 1 << a.lanes_log2;
     const int lane = threadIdx.x & (lanes - 1);
-    const uint32_t row = blockIdx.x * (kThreads >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2);
-    if (row >= a.rows) return;
-    uint32_t hh, t, b;
-    const uint32_t tok = a.heads.divmod(row, hh);
+    const uint32_t unit = blockIdx.x * (kThreads >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2);
+    if (unit >= a.units) return;
+    uint32_t part, t, b;
+    const uint32_t tok = a.parts.divmod(unit, part);
     const uint32_t nb = a.tdiv.divmod(tok, t);
     const uint32_t i = a.bdiv.divmod(nb, b);
-    const bool is_v = (int)hh >= a.hk;
-    const int h = is_v ? (int)hh - a.hk : (int)hh;
+    const bool is_v = (int)part >= a.parts_k;
+    const int h0 = HPT * (is_v ? (int)part - a.parts_k : (int)part);
+    const int nh = min(HPT, a.hk - h0);
     const int pos = load_index(a.pos, i * a.pos_n + b * a.pos_b + t * a.pos_t, a.pos64);
-    const int slot = pos < 0 ? -1 : a.c.row(i, b, a.hk, h, pos);
+    const int slot = pos < 0 ? -1 : a.c.row(i, b, a.hk, h0, pos);
     if (pos >= 0 && slot < 0 && lane == 0) raise_device_error(a.err, DEV_ERR_INDEX);
-    const int64_t at = (int64_t)i * a.c.pages * a.hk * a.c.page + (slot < 0 ? 0 : slot);
-    const void* base = is_v ? a.c.v : a.c.k;
-    float scale = 1.f;
-    if constexpr (IN == OUT_I8 || IN == OUT_E4M3) {
-        if (slot >= 0) scale = (is_v ? a.c.vs : a.c.ks)[at];
-    }
-    T* y = static_cast<T*>(is_v ? a.yv : a.yk) + ((int64_t)tok * a.hk + h) * a.d;
+    Pack<C, VEC> raw[HPT][2 * UPL];
+    float scale[HPT];
+    if (slot >= 0) {
+        const int64_t at = (int64_t)i * a.c.pages * a.hk * a.c.page + slot;
+        const C* base = static_cast<const C*>(is_v ? a.c.v : a.c.k);
 #pragma unroll
-    for (int s = 0; s < 2 * UPL; ++s) {
-        const int c = (lane + s * lanes) * VEC;
-        if (c >= a.d) continue;
-        float x[VEC];
+        for (int r = 0; r < HPT; ++r) {
+            const int64_t row = at + (int64_t)min(r, nh - 1) * a.c.page;
+            scale[r] = CODE ? __ldg((is_v ? a.c.vs : a.c.ks) + row) : 1.f;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) x[j] = 0.f;
-        if (slot >= 0) {
-            if constexpr (IN == OUT_I8 || IN == OUT_E4M3) {
-                const Pack<uint8_t, VEC> p =
-                    *reinterpret_cast<const Pack<uint8_t, VEC>*>(static_cast<const uint8_t*>(base) + at * a.d + c);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    x[j] = (IN == OUT_I8 ? (float)(int8_t)p.v[j] : value_e4m3(p.v[j])) * scale;
-            } else {
-                load_vec<T, VEC>(static_cast<const T*>(base) + at * a.d + c, x);
+            for (int s = 0; s < 2 * UPL; ++s) {
+                const int c = (lane + s * lanes) * VEC;
+                raw[r][s] = load_pack<C, VEC>(base + row * a.d + (c < a.d ? c : 0));
             }
         }
-        store_vec<T, VEC>(y + c, x);
+    } else {
+#pragma unroll
+        for (int r = 0; r < HPT; ++r) {
+            scale[r] = 0.f;
+#pragma unroll
+            for (int s = 0; s < 2 * UPL; ++s) raw[r][s] = Pack<C, VEC>{};
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < HPT; ++r) {
+        if (r >= nh) break;
+        T* y = static_cast<T*>(is_v ? a.yv : a.yk) + ((int64_t)tok * a.hk + h0 + r) * a.d;
+#pragma unroll
+        for (int s = 0; s < 2 * UPL; ++s) {
+            const int c = (lane + s * lanes) * VEC;
+            if (c >= a.d) continue;
+            if constexpr (CODE) {
+                float x[VEC];
+                if constexpr (IN == OUT_I8) values_i8<VEC>(raw[r][s].v, x);
+                else values_e4m3<VEC>(raw[r][s].v, x);
+                scale_vec<VEC>(x, x, scale[r]);
+                store_vec<T, VEC>(y + c, x);
+            } else {
+                *reinterpret_cast<Pack<T, VEC>*>(y + c) = raw[r][s];
+            }
+        }
     }
 }
 
@@ -343,15 +413,15 @@ struct GradArgs {
     float* part;                // [n, chunks, d] fp32: one row of partial weight gradients per block
     void *dqw, *dkw;            // [n, d], nullable
     int cq, ck;                 // blocks per model for the q rows and the k rows
-    uint32_t per_q, per_k;      // rows of one block
-    FastDiv hq_div, hk_div;
+    uint32_t per_q, per_k;      // units of one block
+    FastDiv q_parts, k_parts;
 };
 
-// A block takes consecutive rows of one model's q (or k) heads, and each of
-// its groups of lanes every 256/lanes-th of them, keeping the weight gradient
-// of its channels in registers; groups, warps and blocks are joined in a
-// fixed order, so the sums do not depend on timing.
-template <typename T, int VEC, int UPL>
+// A block takes consecutive units (HPT heads of a token) of one model's q (or
+// k) side, and each of its groups of lanes every 256/lanes-th of them, keeping
+// the weight gradient of its channels in registers; groups, warps and blocks
+// are joined in a fixed order, so the sums do not depend on timing.
+template <typename T, int VEC, int UPL, int HPT>
 __global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const __grid_constant__ GradArgs g) {
     const RowArgs& a = g.r;
     __shared__ float red[kThreads / 32][256];
@@ -363,15 +433,15 @@ __global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const __grid_constan
     const int i = blockIdx.x / chunks;
     const int chunk = blockIdx.x - i * chunks;
     const bool is_q = chunk < g.cq;
-    const uint32_t heads = is_q ? a.hq : a.hk;
-    const uint32_t all = (uint32_t)a.b * a.t * heads;
+    const int heads = is_q ? a.hq : a.hk;
+    const uint32_t all = (uint32_t)a.b * a.t * (is_q ? a.parts_q : a.parts_k);
     const uint32_t per = is_q ? g.per_q : g.per_k;
     const uint32_t first = (is_q ? chunk : chunk - g.cq) * per;
     const uint32_t last = min(all, first + per);
-    const FastDiv hd = is_q ? g.hq_div : g.hk_div;
+    const FastDiv parts = is_q ? g.q_parts : g.k_parts;
     const Strides st = is_q ? a.sq : a.sk;
     const T* x0 = static_cast<const T*>(is_q ? a.q : a.k) + (int64_t)i * st.n;
-    const int64_t dense0 = (int64_t)i * all;
+    const int64_t dense0 = (int64_t)i * a.b * a.t * heads;
     const T* dy0 = static_cast<const T*>(is_q ? g.dyq : g.dyk);
     T* dx0 = static_cast<T*>(is_q ? a.yq : a.yk);
     const T* w = static_cast<const T*>(is_q ? a.qw : a.kw) + (int64_t)i * a.d;
@@ -388,75 +458,100 @@ __global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const __grid_constan
         if (cb[s] < a.d) load_vec<T, VEC>(w + cb[s], wb[s]);
     }
     const float inv_d = 1.f / (float)a.d;
-    for (uint32_t base = first; base < last; base += groups) {
-        uint32_t row = base + (threadIdx.x >> a.lanes_log2);
-        const bool live = row < last;
-        if (!live) row = last - 1;
-        uint32_t h, t;
-        const uint32_t bt = hd.divmod(row, h);
+    for (uint32_t unit = first + (threadIdx.x >> a.lanes_log2); unit < last; unit += groups) {
+        uint32_t part, t;
+        const uint32_t bt = parts.divmod(unit, part);
         const uint32_t b = a.tdiv.divmod(bt, t);
+        const int h0 = (int)part * HPT, nh = min(HPT, heads - h0);
         const int pos = load_index(a.pos, i * a.pos_n + b * a.pos_b + t * a.pos_t, a.pos64);
         const bool keep = pos >= 0 && pos < a.table_rows;
-        const T* x = x0 + b * st.b + t * st.t + h * st.h;
-        const T* dy = dy0 + (dense0 + row) * a.d;
-        T* dx = dx0 + (dense0 + row) * a.d;
-        float xa[UPL][VEC], xb[UPL][VEC], ga[UPL][VEC], gb[UPL][VEC];
+        const T* x = x0 + b * st.b + t * st.t + h0 * st.h;
+        const int64_t dense = (dense0 + (int64_t)bt * heads + h0) * a.d;
+        const T* dy = dy0 + dense;
+        T* dx = dx0 + dense;
+        Pack<T, VEC> ra[HPT][UPL], rb[HPT][UPL], sa[HPT][UPL], sb[HPT][UPL];
 #pragma unroll
-        for (int s = 0; s < UPL; ++s) {
+        for (int r = 0; r < HPT; ++r)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) xa[s][j] = xb[s][j] = ga[s][j] = gb[s][j] = 0.f;
-            if (ca[s] < a.d) {
-                load_vec<T, VEC>(x + ca[s], xa[s]);
-                load_vec<T, VEC>(dy + ca[s], ga[s]);
+            for (int s = 0; s < UPL; ++s) {
+                // places outside the row are read from its first vector and left out of the sums
+                const int at = min(r, nh - 1), pa = ca[s] < a.d ? ca[s] : 0, pb = cb[s] < a.d ? cb[s] : 0;
+                ra[r][s] = load_pack<T, VEC>(x + at * st.h + pa);
+                sa[r][s] = load_pack<T, VEC>(dy + at * a.d + pa);
+                rb[r][s] = load_pack<T, VEC>(x + at * st.h + pb);
+                sb[r][s] = load_pack<T, VEC>(dy + at * a.d + pb);
             }
-            if (cb[s] < a.d) {
-                load_vec<T, VEC>(x + cb[s], xb[s]);
-                load_vec<T, VEC>(dy + cb[s], gb[s]);
-            }
-        }
         const int64_t trow = (int64_t)(keep ? pos : 0) * (a.rot / 2);
-        float ss = 0.f;
+        Turn<VEC> turn[UPL];                 // back: the sines negated, no weights
 #pragma unroll
         for (int s = 0; s < UPL; ++s) {
             const int u = lane + s * lanes;
-            if (u < turned && keep) {
-                float co[VEC], si[VEC];
+            if (u < turned && a.table_rows > 0) {
+                float co[VEC], si[VEC], one[VEC];
                 load_table<VEC>(a.cs + trow + u * VEC, co);
                 load_table<VEC>(a.sn + trow + u * VEC, si);
-                turn<VEC>(ga[s], gb[s], co, si, a.inter, -1.f);
-            }
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) ss += xa[s][j] * xa[s][j] + xb[s][j] * xb[s][j];
+                for (int j = 0; j < VEC; ++j) si[j] = -si[j], one[j] = 1.f;
+                turn[s].set(co, si, one, one, a.inter);
+            }
         }
-        const float r = rsqrtf(group_sum(ss, lanes, mask) * inv_d + a.eps);
-        // padding rows add nothing, not even a NaN that they hold
-        float gx = 0.f;
+        // du, and the sums over the row of x^2 and of g x with g = w du
+        float ss[HPT], gx[HPT], ua[HPT][UPL][VEC], ub[HPT][UPL][VEC];
 #pragma unroll
-        for (int s = 0; s < UPL; ++s)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                if (live && keep) {
-                    da[s][j] += ga[s][j] * xa[s][j] * r;
-                    db[s][j] += gb[s][j] * xb[s][j] * r;
-                }
-                ga[s][j] *= wa[s][j];
-                gb[s][j] *= wb[s][j];
-                gx += ga[s][j] * xa[s][j] + gb[s][j] * xb[s][j];
-            }
-        const float m = group_sum(gx, lanes, mask) * inv_d * r * r;
-        if (live) {
+        for (int r = 0; r < HPT; ++r) {
+            ss[r] = gx[r] = 0.f;
 #pragma unroll
             for (int s = 0; s < UPL; ++s) {
+                float x[VEC], g[VEC];
+                unpack<T, VEC>(sa[r][s], ua[r][s]);
+                unpack<T, VEC>(sb[r][s], ub[r][s]);
+                if (lane + s * lanes < turned) turn[s].apply(ua[r][s], ub[r][s], a.inter);
+                unpack<T, VEC>(ra[r][s], x);
+                mul_vec<VEC>(g, ua[r][s], wa[s]);
+                if (ca[s] < a.d) ss[r] += dot_vec<VEC>(x, x), gx[r] += dot_vec<VEC>(g, x);
+                unpack<T, VEC>(rb[r][s], x);
+                mul_vec<VEC>(g, ub[r][s], wb[s]);
+                if (cb[s] < a.d) ss[r] += dot_vec<VEC>(x, x), gx[r] += dot_vec<VEC>(g, x);
+            }
+        }
+        for (int o = lanes >> 1; o > 0; o >>= 1)
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    ga[s][j] = keep ? r * (ga[s][j] - xa[s][j] * m) : 0.f;
-                    gb[s][j] = keep ? r * (gb[s][j] - xb[s][j] * m) : 0.f;
-                }
-                if (ca[s] < a.d) store_vec<T, VEC>(dx + ca[s], ga[s]);
-                if (cb[s] < a.d) store_vec<T, VEC>(dx + cb[s], gb[s]);
+            for (int r = 0; r < HPT; ++r) {
+                ss[r] += __shfl_xor_sync(mask, ss[r], o);
+                gx[r] += __shfl_xor_sync(mask, gx[r], o);
+            }
+#pragma unroll
+        for (int r = 0; r < HPT; ++r) {
+            if (r >= nh) break;
+            const float rs = rsqrtf(ss[r] * inv_d + a.eps);
+            const float m = -gx[r] * inv_d * rs * rs;
+#pragma unroll
+            for (int s = 0; s < UPL; ++s) {
+                // t = x r; dw += du t; dx = r (w du) - t m
+                auto one = [&](const Pack<T, VEC>& raw, float* u, const float* w, float* dw, int ch) {
+                    float t[VEC], mt[VEC];
+                    unpack<T, VEC>(raw, t);
+                    scale_vec<VEC>(t, t, rs);
+                    if (keep) {                  // padding rows add nothing, not even a NaN that they hold
+                        fma_vec<VEC>(dw, u, t, dw);
+                        scale_vec<VEC>(mt, t, m);
+                        mul_vec<VEC>(u, u, w);
+                        float rr[VEC];
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) rr[j] = rs;
+                        fma_vec<VEC>(u, u, rr, mt);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) u[j] = 0.f;
+                    }
+                    if (ch < a.d) store_vec<T, VEC>(dx + r * a.d + ch, u);
+                };
+                one(ra[r][s], ua[r][s], wa[s], da[s], ca[s]);
+                one(rb[r][s], ub[r][s], wb[s], db[s], cb[s]);
             }
         }
     }
+    __syncwarp();
     // groups of a warp, then the warps
 #pragma unroll
     for (int s = 0; s < UPL; ++s)
@@ -563,17 +658,35 @@ int row_args(RowArgs& a, const char* what, const int64_t* g, int pos64) {
     return WIDEK_OK;
 }
 
-int row_count(RowArgs& a, const char* what, int64_t heads) {
-    const double rows = (double)a.n * a.b * a.t * (double)heads;
-    if (rows > 2147483647.0)
-        return set_error(WIDEK_ERR_INVALID, "%s: over 2^31 rows (%.0f)", what, rows);
-    a.rows = (uint32_t)rows;
-    if (a.rows == 0) return WIDEK_OK;
-    a.heads = FastDiv::make((uint32_t)heads);
+// Heads that a group of lanes takes at once: 4 with 16-byte vectors, one in
+// the narrow paths, whose rows take more registers.
+#ifndef HPT_F
+#define HPT_F 4
+#endif
+#ifndef HPT_B
+#define HPT_B 2
+#endif
+constexpr int heads_at_once(int vec, size_t esz) { return vec == (int)(16 / esz) ? HPT_F : 1; }
+
+// Units of a call with `vec`-wide accesses; sides: 1 (k) or 2 (k and v).
+int row_units(RowArgs& a, const char* what, int vec, size_t esz, int sides) {
+    const int hpt = heads_at_once(vec, esz);
+    a.parts_q = (a.hq + hpt - 1) / hpt;
+    a.parts_k = (a.hk + hpt - 1) / hpt;
+    const int64_t parts = (int64_t)a.parts_q + (int64_t)sides * a.parts_k;
+    const double units = (double)a.n * a.b * a.t * (double)parts;
+    if (units > 2147483647.0) return set_error(WIDEK_ERR_INVALID, "%s: over 2^31 rows (%.0f)", what, units);
+    a.units = (uint32_t)units;
+    if (a.units == 0) return WIDEK_OK;
+    a.parts = FastDiv::make((uint32_t)parts);
     a.tdiv = FastDiv::make((uint32_t)a.t);
     a.bdiv = FastDiv::make((uint32_t)a.b);
+    a.lanes_log2 = lanes_log2(a.d, vec);
     return WIDEK_OK;
 }
+
+// Whether the call has no rows at all.
+bool no_rows(const RowArgs& a, int heads) { return a.n == 0 || a.b == 0 || a.t == 0 || heads == 0 || a.d == 0; }
 
 template <int OUT, bool ROPE>
 struct RowLaunch {
@@ -584,12 +697,11 @@ struct RowLaunch {
     template <typename T>
     int run() {
         constexpr int W = 16 / sizeof(T);
-        a.lanes_log2 = lanes_log2(a.d, vec);
         const uint32_t per = kThreads >> a.lanes_log2;
-        const unsigned blocks = (a.rows + per - 1) / per;
-        if (vec == W) rows_kernel<T, W, 1, OUT, ROPE><<<blocks, kThreads, 0, st>>>(a);
-        else if (vec == 2) rows_kernel<T, 2, 2, OUT, ROPE><<<blocks, kThreads, 0, st>>>(a);
-        else rows_kernel<T, 1, 4, OUT, ROPE><<<blocks, kThreads, 0, st>>>(a);
+        const unsigned blocks = (a.units + per - 1) / per;
+        if (vec == W) rows_kernel<T, W, 1, heads_at_once(W, sizeof(T)), OUT, ROPE><<<blocks, kThreads, 0, st>>>(a);
+        else if (vec == 2) rows_kernel<T, 2, 2, 1, OUT, ROPE><<<blocks, kThreads, 0, st>>>(a);
+        else rows_kernel<T, 1, 4, 1, OUT, ROPE><<<blocks, kThreads, 0, st>>>(a);
         return check_launch(what);
     }
 };
@@ -602,12 +714,11 @@ struct ReadLaunch {
     template <typename T>
     int run() {
         constexpr int W = 16 / sizeof(T);
-        a.lanes_log2 = lanes_log2(a.d, vec);
         const uint32_t per = kThreads >> a.lanes_log2;
-        const unsigned blocks = (a.rows + per - 1) / per;
-        if (vec == W) cache_read_kernel<T, W, 1, IN><<<blocks, kThreads, 0, st>>>(a);
-        else if (vec == 2) cache_read_kernel<T, 2, 2, IN><<<blocks, kThreads, 0, st>>>(a);
-        else cache_read_kernel<T, 1, 4, IN><<<blocks, kThreads, 0, st>>>(a);
+        const unsigned blocks = (a.units + per - 1) / per;
+        if (vec == W) cache_read_kernel<T, W, 1, heads_at_once(W, sizeof(T)), IN><<<blocks, kThreads, 0, st>>>(a);
+        else if (vec == 2) cache_read_kernel<T, 2, 2, 1, IN><<<blocks, kThreads, 0, st>>>(a);
+        else cache_read_kernel<T, 1, 4, 1, IN><<<blocks, kThreads, 0, st>>>(a);
         return check_launch("widek_cache_read_fwd");
     }
 };
@@ -625,18 +736,21 @@ int launch_rows_fmt(const RowArgs& a, int vec, const char* what, int fmt, int dt
     return launch_rows<OUT_SAME, ROPE>(a, vec, what, dtype, st);
 }
 
+constexpr int kGradHeads = HPT_B;     // heads at once in the backward, whose rows take twice the registers
+constexpr int grad_heads(int vec, size_t esz) { return vec == (int)(16 / esz) ? kGradHeads : 1; }
+
 // Blocks per model of the backward: about three blocks for each SM over all
-// models and both sides, none with fewer rows than its groups of lanes.
-void grad_chunks(const RowArgs& a, int vec, int& cq, int& ck, uint32_t& per_q, uint32_t& per_k) {
+// models and both sides, none with fewer units than its groups of lanes.
+void grad_chunks(const RowArgs& a, int vec, int hpt, int& cq, int& ck, uint32_t& per_q, uint32_t& per_k) {
     const int groups = kThreads >> lanes_log2(a.d, vec);
     const int64_t tokens = (int64_t)a.b * a.t;
     auto split = [&](int64_t heads, int& c, uint32_t& per) {
-        const int64_t rows = tokens * heads;
-        int64_t want = (int64_t)444 * heads / ((int64_t)a.n * (a.hq + a.hk));
-        const int64_t most = (rows + groups - 1) / groups;
+        const int64_t units = tokens * ((heads + hpt - 1) / hpt);
+        int64_t want = (int64_t)444 * heads / ((int64_t)a.n * ((int64_t)a.hq + a.hk));
+        const int64_t most = (units + groups - 1) / groups;
         want = want < 1 ? 1 : (want > most ? most : want);
-        per = (uint32_t)(((rows + want - 1) / want + groups - 1) / groups * groups);
-        c = (int)((rows + per - 1) / per);
+        per = (uint32_t)(((units + want - 1) / want + groups - 1) / groups * groups);
+        c = (int)((units + per - 1) / per);
     };
     split(a.hq, cq, per_q);
     split(a.hk, ck, per_k);
@@ -649,11 +763,10 @@ struct GradLaunch {
     template <typename T>
     int run() {
         constexpr int W = 16 / sizeof(T);
-        g.r.lanes_log2 = lanes_log2(g.r.d, vec);
         const unsigned blocks = (unsigned)g.r.n * (g.cq + g.ck);
-        if (vec == W) rope_bwd_kernel<T, W, 1><<<blocks, kThreads, 0, st>>>(g);
-        else if (vec == 2) rope_bwd_kernel<T, 2, 2><<<blocks, kThreads, 0, st>>>(g);
-        else rope_bwd_kernel<T, 1, 4><<<blocks, kThreads, 0, st>>>(g);
+        if (vec == W) rope_bwd_kernel<T, W, 1, grad_heads(W, sizeof(T))><<<blocks, kThreads, 0, st>>>(g);
+        else if (vec == 2) rope_bwd_kernel<T, 2, 2, 1><<<blocks, kThreads, 0, st>>>(g);
+        else rope_bwd_kernel<T, 1, 4, 1><<<blocks, kThreads, 0, st>>>(g);
         int rc = check_launch("widek_qk_norm_rope_bwd");
         if (rc != WIDEK_OK || (!g.dqw && !g.dkw)) return rc;
         const dim3 grid(2 * g.r.n, (g.r.d + 31) / 32);
@@ -665,7 +778,7 @@ struct GradLaunch {
 
 int rope_pointers(const RowArgs& a, const char* what) {
     if (a.hq < 1 || a.hk < 1) return set_error(WIDEK_ERR_INVALID, "%s: no heads (hq=%d, hk=%d)", what, a.hq, a.hk);
-    if (a.rows > 0 && a.d > 0 &&
+    if (!no_rows(a, a.hq) &&
         (!a.q || !a.k || !a.qw || !a.kw || !a.pos || !a.yq || (a.rot > 0 && a.table_rows > 0 && (!a.cs || !a.sn))))
         return set_error(WIDEK_ERR_INVALID, "%s: null pointer", what);
     return WIDEK_OK;
@@ -684,15 +797,17 @@ extern "C" int widek_qk_norm_rope_fwd(const void* q, const void* k, const void* 
     RowArgs a;
     int rc = row_args(a, what, geom, pos64);
     if (rc != WIDEK_OK) return rc;
-    rc = row_count(a, what, (int64_t)a.hq + a.hk);
-    if (rc != WIDEK_OK) return rc;
     a.q = q, a.k = k, a.qw = qw, a.kw = kw, a.cs = cos, a.sn = sin, a.pos = positions, a.yq = yq, a.yk = yk;
     a.eps = (float)eps, a.inter = interleaved;
     rc = rope_pointers(a, what);
     if (rc != WIDEK_OK) return rc;
-    if (a.rows == 0 || a.d == 0) return WIDEK_OK;
+    if (no_rows(a, a.hq)) return WIDEK_OK;
     if (!yk) return set_error(WIDEK_ERR_INVALID, "%s: null pointer", what);
-    const int vec = row_vec(a, dtype_size(dtype) ? dtype_size(dtype) : 4, {qw, kw, yq, yk}, false);
+    const size_t esz = dtype_size(dtype);
+    if (esz == 0) return set_error(WIDEK_ERR_INVALID, "%s: unknown dtype code %d", what, dtype);
+    const int vec = row_vec(a, esz, {qw, kw, yq, yk}, false);
+    rc = row_units(a, what, vec, esz, 1);
+    if (rc != WIDEK_OK) return rc;
     return launch_rows<OUT_DENSE, true>(a, vec, what, dtype, (cudaStream_t)stream);
 }
 
@@ -705,17 +820,19 @@ extern "C" int widek_qk_norm_rope_write_fwd(const void* q, const void* k, const 
     RowArgs a;
     int rc = row_args(a, what, geom, pos64);
     if (rc != WIDEK_OK) return rc;
-    rc = row_count(a, what, (int64_t)a.hq + 2 * a.hk);
-    if (rc != WIDEK_OK) return rc;
-    rc = cache_args(a.c, what, kc, vc, ks, vs, table, cgeom, a.rows, a.hk, a.d, fmt, dtype);
+    rc = cache_args(a.c, what, kc, vc, ks, vs, table, cgeom, (int64_t)a.n * a.b * a.t, a.hk, a.d, fmt, dtype);
     if (rc != WIDEK_OK) return rc;
     a.q = q, a.k = k, a.v = v, a.qw = qw, a.kw = kw, a.cs = cos, a.sn = sin, a.pos = positions, a.yq = yq;
     a.eps = (float)eps, a.inter = interleaved;
     rc = rope_pointers(a, what);
     if (rc != WIDEK_OK) return rc;
-    if (a.rows == 0 || a.d == 0) return WIDEK_OK;
+    if (no_rows(a, a.hq)) return WIDEK_OK;
     if (!v) return set_error(WIDEK_ERR_INVALID, "%s: null pointer", what);
-    const int vec = row_vec(a, dtype_size(dtype) ? dtype_size(dtype) : 4, {qw, kw, yq}, !cache_fmt_8bit(fmt));
+    const size_t esz = dtype_size(dtype);
+    if (esz == 0) return set_error(WIDEK_ERR_INVALID, "%s: unknown dtype code %d", what, dtype);
+    const int vec = row_vec(a, esz, {qw, kw, yq}, !cache_fmt_8bit(fmt));
+    rc = row_units(a, what, vec, esz, 2);
+    if (rc != WIDEK_OK) return rc;
     return launch_rows_fmt<true>(a, vec, what, fmt, dtype, (cudaStream_t)stream);
 }
 
@@ -727,14 +844,16 @@ extern "C" int widek_cache_write_fwd(const void* k, const void* v, const void* p
     int rc = row_args(a, what, geom, pos64);
     if (rc != WIDEK_OK) return rc;
     a.hq = 0, a.rot = 0;
-    rc = row_count(a, what, 2 * (int64_t)a.hk);
+    rc = cache_args(a.c, what, kc, vc, ks, vs, table, cgeom, (int64_t)a.n * a.b * a.t, a.hk, a.d, fmt, dtype);
     if (rc != WIDEK_OK) return rc;
-    rc = cache_args(a.c, what, kc, vc, ks, vs, table, cgeom, a.rows, a.hk, a.d, fmt, dtype);
-    if (rc != WIDEK_OK) return rc;
-    if (a.rows == 0 || a.d == 0) return WIDEK_OK;
+    if (no_rows(a, a.hk)) return WIDEK_OK;
     if (!k || !v || !positions) return set_error(WIDEK_ERR_INVALID, "%s: null pointer", what);
     a.k = k, a.v = v, a.pos = positions;
-    const int vec = row_vec(a, dtype_size(dtype) ? dtype_size(dtype) : 4, {}, !cache_fmt_8bit(fmt));
+    const size_t esz = dtype_size(dtype);
+    if (esz == 0) return set_error(WIDEK_ERR_INVALID, "%s: unknown dtype code %d", what, dtype);
+    const int vec = row_vec(a, esz, {}, !cache_fmt_8bit(fmt));
+    rc = row_units(a, what, vec, esz, 2);
+    if (rc != WIDEK_OK) return rc;
     return launch_rows_fmt<false>(a, vec, what, fmt, dtype, (cudaStream_t)stream);
 }
 
@@ -746,15 +865,17 @@ extern "C" int widek_cache_read_fwd(const void* kc, const void* vc, const float*
     int rc = row_args(a, what, geom, pos64);
     if (rc != WIDEK_OK) return rc;
     a.hq = 0, a.rot = 0;
-    rc = row_count(a, what, 2 * (int64_t)a.hk);
-    if (rc != WIDEK_OK) return rc;
     rc = cache_args(a.c, what, const_cast<void*>(kc), const_cast<void*>(vc), const_cast<float*>(ks),
-                    const_cast<float*>(vs), table, cgeom, a.rows, a.hk, a.d, fmt, dtype);
+                    const_cast<float*>(vs), table, cgeom, (int64_t)a.n * a.b * a.t, a.hk, a.d, fmt, dtype);
     if (rc != WIDEK_OK) return rc;
-    if (a.rows == 0 || a.d == 0) return WIDEK_OK;
+    if (no_rows(a, a.hk)) return WIDEK_OK;
     if (!k || !v || !positions) return set_error(WIDEK_ERR_INVALID, "%s: null pointer", what);
     a.yk = k, a.yv = v, a.pos = positions;
-    const int vec = row_vec(a, dtype_size(dtype) ? dtype_size(dtype) : 4, {k, v}, !cache_fmt_8bit(fmt));
+    const size_t esz = dtype_size(dtype);
+    if (esz == 0) return set_error(WIDEK_ERR_INVALID, "%s: unknown dtype code %d", what, dtype);
+    const int vec = row_vec(a, esz, {k, v}, !cache_fmt_8bit(fmt));
+    rc = row_units(a, what, vec, esz, 2);
+    if (rc != WIDEK_OK) return rc;
     cudaStream_t st = (cudaStream_t)stream;
     if (fmt == WIDEK_I8) {
         ReadLaunch<OUT_I8> L{a, vec, st};
@@ -771,16 +892,16 @@ extern "C" int widek_cache_read_fwd(const void* kc, const void* vc, const float*
 extern "C" int64_t widek_qk_norm_rope_bwd_workspace(const int64_t* geom) {
     RowArgs a;
     if (row_args(a, "widek_qk_norm_rope_bwd_workspace", geom, 0) != WIDEK_OK || a.hq < 1 || a.hk < 1) return -1;
-    if (row_count(a, "widek_qk_norm_rope_bwd_workspace", (int64_t)a.hq + a.hk) != WIDEK_OK) return -1;
-    if (a.rows == 0 || a.d == 0) return 0;
+    if (no_rows(a, a.hq)) return 0;
     // the most blocks of any vector width
     int64_t blocks = 0;
-    for (int vec : {8, 4, 2, 1}) {
-        int cq, ck;
-        uint32_t pq, pk;
-        grad_chunks(a, vec, cq, ck, pq, pk);
-        if (cq + ck > blocks) blocks = cq + ck;
-    }
+    for (int vec : {8, 4, 2, 1})
+        for (int hpt : {1, kGradHeads}) {
+            int cq, ck;
+            uint32_t pq, pk;
+            grad_chunks(a, vec, hpt, cq, ck, pq, pk);
+            if (cq + ck > blocks) blocks = cq + ck;
+        }
     return blocks * a.n * a.d * (int64_t)sizeof(float);
 }
 
@@ -794,23 +915,29 @@ extern "C" int widek_qk_norm_rope_bwd(const void* q, const void* k, const void* 
     RowArgs& a = g.r;
     int rc = row_args(a, what, geom, pos64);
     if (rc != WIDEK_OK) return rc;
-    rc = row_count(a, what, (int64_t)a.hq + a.hk);
-    if (rc != WIDEK_OK) return rc;
     a.q = q, a.k = k, a.qw = qw, a.kw = kw, a.cs = cos, a.sn = sin, a.pos = positions, a.yq = dq, a.yk = dk;
     a.eps = (float)eps, a.inter = interleaved;
     rc = rope_pointers(a, what);
     if (rc != WIDEK_OK) return rc;
-    if (a.rows == 0 || a.d == 0) return WIDEK_OK;
+    if (no_rows(a, a.hq)) return WIDEK_OK;
     if (!dk || !dyq || !dyk) return set_error(WIDEK_ERR_INVALID, "%s: null pointer", what);
     const int64_t need = widek_qk_norm_rope_bwd_workspace(geom);
     if (!workspace || workspace_bytes < need)
         return set_error(WIDEK_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed", what,
                          (long long)workspace_bytes, (long long)need);
     g.dyq = dyq, g.dyk = dyk, g.dqw = dqw, g.dkw = dkw, g.part = static_cast<float*>(workspace);
-    const int vec = row_vec(a, dtype_size(dtype) ? dtype_size(dtype) : 4, {qw, kw, dyq, dyk, dq, dk}, false);
-    grad_chunks(a, vec, g.cq, g.ck, g.per_q, g.per_k);
-    g.hq_div = FastDiv::make((uint32_t)a.hq);
-    g.hk_div = FastDiv::make((uint32_t)a.hk);
+    const size_t esz = dtype_size(dtype);
+    if (esz == 0) return set_error(WIDEK_ERR_INVALID, "%s: unknown dtype code %d", what, dtype);
+    const int vec = row_vec(a, esz, {qw, kw, dyq, dyk, dq, dk}, false);
+    const int hpt = grad_heads(vec, esz);
+    rc = row_units(a, what, 1, esz, 1);          // the narrowest: units of one head, for the size check
+    if (rc != WIDEK_OK) return rc;
+    grad_chunks(a, vec, hpt, g.cq, g.ck, g.per_q, g.per_k);
+    a.lanes_log2 = lanes_log2(a.d, vec);
+    a.parts_q = (a.hq + hpt - 1) / hpt;
+    a.parts_k = (a.hk + hpt - 1) / hpt;
+    g.q_parts = FastDiv::make((uint32_t)a.parts_q);
+    g.k_parts = FastDiv::make((uint32_t)a.parts_k);
     GradLaunch L{g, vec, (cudaStream_t)stream};
     return dispatch_dtype(dtype, L);
 }
