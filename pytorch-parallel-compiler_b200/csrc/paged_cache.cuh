@@ -154,11 +154,19 @@ __device__ __forceinline__ void codes_i8(const float* x, float scale, uint8_t* o
         add2(t0, t1, r[j], r[j + 1], -12582912.f, -12582912.f);
         fma2(off[j], off[j + 1], t0, t1, -1.f, -1.f, q[j], q[j + 1]);
     }
-    bool sure = true;
+    int sure = 1;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-        out[j] = (uint8_t)__float_as_uint(r[j]);
-        sure = sure && fabsf(off[j]) < 0.4999f;      // false for NaN
+    for (int j = 0; j < VEC; ++j) sure &= fabsf(off[j]) < 0.4999f;      // false for NaN
+    if constexpr (VEC % 4 == 0) {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 4) {
+            const uint32_t lo = __byte_perm(__float_as_uint(r[j]), __float_as_uint(r[j + 1]), 0x0040);
+            const uint32_t hi = __byte_perm(__float_as_uint(r[j + 2]), __float_as_uint(r[j + 3]), 0x0040);
+            reinterpret_cast<uint32_t*>(out)[j / 4] = __byte_perm(lo, hi, 0x5410);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) out[j] = (uint8_t)__float_as_uint(r[j]);
     }
     if (!sure) {
 #pragma unroll
@@ -172,7 +180,7 @@ __device__ __forceinline__ void codes_i8(const float* x, float scale, uint8_t* o
 template <int VEC>
 __device__ __forceinline__ void codes_e4m3(const float* x, float scale, uint8_t* out) {
     const float inv = __fdiv_rn(1.f, scale);
-    bool sure = scale < 3e38f;
+    int sure = scale < 3e38f;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
         // the codes just below and just above the product agree: no tie between
@@ -180,7 +188,7 @@ __device__ __forceinline__ void codes_e4m3(const float* x, float scale, uint8_t*
         const float2 pair = make_float2(q * (1.f - 2e-6f), q * (1.f + 2e-6f));
         const uint16_t c = __nv_cvt_float2_to_fp8x2(pair, __NV_SATFINITE, __NV_E4M3);
         out[j] = (uint8_t)c;
-        sure = sure && (c & 0xff) == (c >> 8);
+        sure &= (c & 0xff) == (c >> 8);
     }
     if (!sure) {
 #pragma unroll
@@ -193,8 +201,19 @@ __device__ __forceinline__ void codes_e4m3(const float* x, float scale, uint8_t*
 // 2^23 + (code + 128): integer conversions run at a quarter of that rate.
 template <int VEC>
 __device__ __forceinline__ void values_i8(const uint8_t* c, float* x) {
+    if constexpr (VEC % 4 == 0) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) x[j] = __uint_as_float(0x4b000000u | (uint32_t)(c[j] ^ 0x80)) - 8388736.f;
+        for (int j = 0; j < VEC; j += 4) {
+            const uint32_t w = reinterpret_cast<const uint32_t*>(c)[j / 4] ^ 0x80808080u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[j + e] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540 | e));
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) add2(x[j], x[j + 1], x[j], x[j + 1], -8388736.f, -8388736.f);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) x[j] = __uint_as_float(0x4b000000u | (uint32_t)(c[j] ^ 0x80)) - 8388736.f;
+    }
 }
 template <int VEC>
 __device__ __forceinline__ void values_e4m3(const uint8_t* c, float* x) {

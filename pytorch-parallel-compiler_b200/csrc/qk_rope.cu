@@ -124,9 +124,9 @@ __device__ __forceinline__ unsigned group_mask(int lanes) {
 
 // Channels of unit u (first elements of its vectors A and B). Units below
 // `turned` hold pairs of the rotation.
-template <int VEC>
-__device__ __forceinline__ void unit_channels(int u, int turned, int rot, int inter, int& a, int& b) {
-    if (!inter && u < turned) {
+template <int VEC, bool INTER>
+__device__ __forceinline__ void unit_channels(int u, int turned, int rot, int& a, int& b) {
+    if (!INTER && u < turned) {
         a = u * VEC;
         b = a + rot / 2;
     } else {
@@ -139,13 +139,13 @@ __device__ __forceinline__ void unit_channels(int u, int turned, int rot, int in
 // each channel's partner p: the coefficients, the norm's weights folded in
 // (w_p belongs to the partner), from the angles' cosines and sines. SIGN -1
 // turns back; then the weights apply after the turn and are left out.
-template <int VEC>
+template <int VEC, bool INTER>
 struct Turn {
     float ca[VEC], sa[VEC], cb[VEC], sb[VEC];
-    __device__ __forceinline__ void set(const float* co, const float* si, const float* wa, const float* wb, int inter) {
+    __device__ __forceinline__ void set(const float* co, const float* si, const float* wa, const float* wb) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            if (!inter || VEC == 1) {
+            if constexpr (!INTER || VEC == 1) {
                 ca[j] = co[j] * wa[j];
                 sa[j] = -si[j] * wb[j];
                 cb[j] = co[j] * wb[j];
@@ -159,14 +159,17 @@ struct Turn {
             }
         }
     }
-    __device__ __forceinline__ void apply(float* a, float* b, int inter) const {
+    // Channels that do not turn.
+    __device__ __forceinline__ void keep(const float* wa, const float* wb) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) ca[j] = wa[j], cb[j] = wb[j], sa[j] = sb[j] = 0.f;
+    }
+    __device__ __forceinline__ void apply(float* a, float* b) const {
         float pa[VEC], pb[VEC];
-        if (!inter || VEC == 1) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) pa[j] = b[j], pb[j] = a[j];
-        } else {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) pa[j] = a[VEC == 1 ? 0 : j ^ 1], pb[j] = b[VEC == 1 ? 0 : j ^ 1];
+        for (int j = 0; j < VEC; ++j) {
+            pa[j] = !INTER || VEC == 1 ? b[j] : a[VEC == 1 ? 0 : j ^ 1];
+            pb[j] = !INTER || VEC == 1 ? a[j] : b[VEC == 1 ? 0 : j ^ 1];
         }
         mul_vec<VEC>(a, a, ca);
         mul_vec<VEC>(b, b, cb);
@@ -179,14 +182,14 @@ enum RowOut : int { OUT_DENSE = 0, OUT_SAME = 1, OUT_I8 = 2, OUT_E4M3 = 3 };
 
 // One vector of a cache row in the cache's format.
 template <typename T, int VEC, int OUT>
-__device__ __forceinline__ void store_code(void* base, int64_t at, const float* x, float scale) {
+__device__ __forceinline__ void store_code(void* base, int64_t at, const float* x, float scale, bool live) {
     if constexpr (OUT == OUT_I8 || OUT == OUT_E4M3) {
         Pack<uint8_t, VEC> p;
         if constexpr (OUT == OUT_I8) codes_i8<VEC>(x, scale, p.v);
         else codes_e4m3<VEC>(x, scale, p.v);
-        *reinterpret_cast<Pack<uint8_t, VEC>*>(static_cast<uint8_t*>(base) + at) = p;
+        if (live) *reinterpret_cast<Pack<uint8_t, VEC>*>(static_cast<uint8_t*>(base) + at) = p;
     } else {
-        store_vec<T, VEC>(static_cast<T*>(base) + at, x);
+        if (live) store_vec<T, VEC>(static_cast<T*>(base) + at, x);
     }
 }
 
@@ -195,7 +198,7 @@ __device__ __forceinline__ void store_code(void* base, int64_t at, const float* 
 // to the cache as they are. A group of lanes takes HPT heads of one token and
 // kind at once: its loads are in flight together, and the angles and weights
 // are read once (one row at a time reached 3.8 of 6.5 TB/s).
-template <typename T, int VEC, int UPL, int HPT, int OUT, bool ROPE>
+template <typename T, int VEC, int UPL, int HPT, int OUT, bool ROPE, bool INTER>
 __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ RowArgs a) {
     const int lanes = 1 << a.lanes_log2;
     const int lane = threadIdx.x & (lanes - 1);
@@ -218,7 +221,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ 
     int ca[UPL], cb[UPL];
     Pack<T, VEC> ra[HPT][UPL], rb[HPT][UPL];
 #pragma unroll
-    for (int s = 0; s < UPL; ++s) unit_channels<VEC>(lane + s * lanes, turned, a.rot, a.inter, ca[s], cb[s]);
+    for (int s = 0; s < UPL; ++s) unit_channels<VEC, INTER>(lane + s * lanes, turned, a.rot, ca[s], cb[s]);
 #pragma unroll
     for (int r = 0; r < HPT; ++r)
 #pragma unroll
@@ -234,7 +237,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ 
         keep = false;
         if (lane == 0) raise_device_error(a.err, DEV_ERR_INDEX);
     }
-    Turn<VEC> turn[UPL];                  // channels that do not turn: ca and cb are the weights
+    Turn<VEC, INTER> turn[UPL];
     float norm[HPT];
     if (ROPE && rope) {
         const T* w = static_cast<const T*>(is_q ? a.qw : a.kw) + (int64_t)i * a.d;
@@ -249,10 +252,9 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ 
                 float co[VEC], si[VEC];
                 load_table<VEC>(a.cs + trow + u * VEC, co);
                 load_table<VEC>(a.sn + trow + u * VEC, si);
-                turn[s].set(co, si, wa, wb, a.inter);
+                turn[s].set(co, si, wa, wb);
             } else {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) turn[s].ca[j] = wa[j], turn[s].cb[j] = wb[j];
+                turn[s].keep(wa, wb);
             }
         }
 #pragma unroll
@@ -275,6 +277,17 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ 
         for (int r = 0; r < HPT; ++r) norm[r] = rsqrtf(norm[r] * inv_d + a.eps);
     }
 
+    if ((is_q || OUT == OUT_DENSE) && !keep) {       // a padding row: zeros
+        for (int r = 0; r < nh; ++r) {
+            T* y = static_cast<T*>(is_q ? a.yq : a.yk) + ((int64_t)tok * (is_q ? a.hq : a.hk) + h0 + r) * a.d;
+#pragma unroll
+            for (int s = 0; s < UPL; ++s) {
+                if (ca[s] < a.d) *reinterpret_cast<Pack<T, VEC>*>(y + ca[s]) = Pack<T, VEC>{};
+                if (cb[s] < a.d) *reinterpret_cast<Pack<T, VEC>*>(y + cb[s]) = Pack<T, VEC>{};
+            }
+        }
+        return;
+    }
     int slot = -1;
     if (OUT != OUT_DENSE && !is_q && keep) {
         slot = a.c.row(i, b, a.hk, h0, pos);
@@ -290,25 +303,15 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ 
             if (ROPE && rope) {
                 scale_vec<VEC>(xa[s], xa[s], norm[r]);
                 scale_vec<VEC>(xb[s], xb[s], norm[r]);
-                if (lane + s * lanes < turned) {
-                    turn[s].apply(xa[s], xb[s], a.inter);
-                } else {
-                    mul_vec<VEC>(xa[s], xa[s], turn[s].ca);
-                    mul_vec<VEC>(xb[s], xb[s], turn[s].cb);
-                }
+                turn[s].apply(xa[s], xb[s]);
             }
         }
         if (is_q || OUT == OUT_DENSE) {
-            if (r >= nh) break;
             T* y = static_cast<T*>(is_q ? a.yq : a.yk) + ((int64_t)tok * (is_q ? a.hq : a.hk) + h0 + r) * a.d;
 #pragma unroll
             for (int s = 0; s < UPL; ++s) {
-                if (!keep) {
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) xa[s][j] = xb[s][j] = 0.f;
-                }
-                if (ca[s] < a.d) store_vec<T, VEC>(y + ca[s], xa[s]);
-                if (cb[s] < a.d) store_vec<T, VEC>(y + cb[s], xb[s]);
+                if (r < nh && ca[s] < a.d) store_vec<T, VEC>(y + ca[s], xa[s]);
+                if (r < nh && cb[s] < a.d) store_vec<T, VEC>(y + cb[s], xb[s]);
             }
         } else if constexpr (OUT != OUT_DENSE) {
             float scale = 1.f;
@@ -319,22 +322,21 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ 
                     float ma = 0.f, mb = 0.f;
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) ma = amax2(ma, xa[s][j]), mb = amax2(mb, xb[s][j]);
-                    if (ca[s] < a.d) m = amax2(m, ma);
-                    if (cb[s] < a.d) m = amax2(m, mb);
+                    m = amax2(m, amax2(ca[s] < a.d ? ma : 0.f, cb[s] < a.d ? mb : 0.f));
                 }
                 for (int o = lanes >> 1; o > 0; o >>= 1) m = amax2(m, __shfl_xor_sync(mask, m, o));
                 scale = code_scale(m, OUT == OUT_I8);
             }
-            if (r >= nh || slot < 0) break;               // the same for all lanes of the group
+            const bool live = r < nh && slot >= 0;
             const int64_t at = (int64_t)i * a.c.pages * a.hk * a.c.page + slot + (int64_t)r * a.c.page;
             void* base = is_v ? a.c.v : a.c.k;
             if constexpr (OUT == OUT_I8 || OUT == OUT_E4M3) {
-                if (lane == 0) (is_v ? a.c.vs : a.c.ks)[at] = scale;
+                if (live && lane == 0) (is_v ? a.c.vs : a.c.ks)[at] = scale;
             }
 #pragma unroll
             for (int s = 0; s < UPL; ++s) {
-                if (ca[s] < a.d) store_code<T, VEC, OUT>(base, at * a.d + ca[s], xa[s], scale);
-                if (cb[s] < a.d) store_code<T, VEC, OUT>(base, at * a.d + cb[s], xb[s], scale);
+                store_code<T, VEC, OUT>(base, at * a.d + ca[s], xa[s], scale, live && ca[s] < a.d);
+                store_code<T, VEC, OUT>(base, at * a.d + cb[s], xb[s], scale, live && cb[s] < a.d);
             }
         }
     }
@@ -385,19 +387,18 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_const
     }
 #pragma unroll
     for (int r = 0; r < HPT; ++r) {
-        if (r >= nh) break;
         T* y = static_cast<T*>(is_v ? a.yv : a.yk) + ((int64_t)tok * a.hk + h0 + r) * a.d;
 #pragma unroll
         for (int s = 0; s < 2 * UPL; ++s) {
             const int c = (lane + s * lanes) * VEC;
-            if (c >= a.d) continue;
+            const bool live = r < nh && c < a.d;
             if constexpr (CODE) {
                 float x[VEC];
                 if constexpr (IN == OUT_I8) values_i8<VEC>(raw[r][s].v, x);
                 else values_e4m3<VEC>(raw[r][s].v, x);
                 scale_vec<VEC>(x, x, scale[r]);
-                store_vec<T, VEC>(y + c, x);
-            } else {
+                if (live) store_vec<T, VEC>(y + c, x);
+            } else if (live) {
                 *reinterpret_cast<Pack<T, VEC>*>(y + c) = raw[r][s];
             }
         }
@@ -421,7 +422,7 @@ struct GradArgs {
 // k) side, and each of its groups of lanes every 256/lanes-th of them, keeping
 // the weight gradient of its channels in registers; groups, warps and blocks
 // are joined in a fixed order, so the sums do not depend on timing.
-template <typename T, int VEC, int UPL, int HPT>
+template <typename T, int VEC, int UPL, int HPT, bool INTER>
 __global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const __grid_constant__ GradArgs g) {
     const RowArgs& a = g.r;
     __shared__ float red[kThreads / 32][256];
@@ -451,7 +452,7 @@ __global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const __grid_constan
     float wa[UPL][VEC], wb[UPL][VEC], da[UPL][VEC], db[UPL][VEC];
 #pragma unroll
     for (int s = 0; s < UPL; ++s) {
-        unit_channels<VEC>(lane + s * lanes, turned, a.rot, a.inter, ca[s], cb[s]);
+        unit_channels<VEC, INTER>(lane + s * lanes, turned, a.rot, ca[s], cb[s]);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) wa[s][j] = wb[s][j] = da[s][j] = db[s][j] = 0.f;
         if (ca[s] < a.d) load_vec<T, VEC>(w + ca[s], wa[s]);
@@ -482,7 +483,7 @@ __global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const __grid_constan
                 sb[r][s] = load_pack<T, VEC>(dy + at * a.d + pb);
             }
         const int64_t trow = (int64_t)(keep ? pos : 0) * (a.rot / 2);
-        Turn<VEC> turn[UPL];                 // back: the sines negated, no weights
+        Turn<VEC, INTER> turn[UPL];                 // back: the sines negated, no weights
 #pragma unroll
         for (int s = 0; s < UPL; ++s) {
             const int u = lane + s * lanes;
@@ -492,7 +493,12 @@ __global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const __grid_constan
                 load_table<VEC>(a.sn + trow + u * VEC, si);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) si[j] = -si[j], one[j] = 1.f;
-                turn[s].set(co, si, one, one, a.inter);
+                turn[s].set(co, si, one, one);
+            } else {
+                float one[VEC];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) one[j] = 1.f;
+                turn[s].keep(one, one);
             }
         }
         // du, and the sums over the row of x^2 and of g x with g = w du
@@ -505,13 +511,15 @@ __global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const __grid_constan
                 float x[VEC], g[VEC];
                 unpack<T, VEC>(sa[r][s], ua[r][s]);
                 unpack<T, VEC>(sb[r][s], ub[r][s]);
-                if (lane + s * lanes < turned) turn[s].apply(ua[r][s], ub[r][s], a.inter);
+                turn[s].apply(ua[r][s], ub[r][s]);
                 unpack<T, VEC>(ra[r][s], x);
                 mul_vec<VEC>(g, ua[r][s], wa[s]);
-                if (ca[s] < a.d) ss[r] += dot_vec<VEC>(x, x), gx[r] += dot_vec<VEC>(g, x);
+                ss[r] += ca[s] < a.d ? dot_vec<VEC>(x, x) : 0.f;
+                gx[r] += ca[s] < a.d ? dot_vec<VEC>(g, x) : 0.f;
                 unpack<T, VEC>(rb[r][s], x);
                 mul_vec<VEC>(g, ub[r][s], wb[s]);
-                if (cb[s] < a.d) ss[r] += dot_vec<VEC>(x, x), gx[r] += dot_vec<VEC>(g, x);
+                ss[r] += cb[s] < a.d ? dot_vec<VEC>(x, x) : 0.f;
+                gx[r] += cb[s] < a.d ? dot_vec<VEC>(g, x) : 0.f;
             }
         }
         for (int o = lanes >> 1; o > 0; o >>= 1)
@@ -520,31 +528,36 @@ __global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const __grid_constan
                 ss[r] += __shfl_xor_sync(mask, ss[r], o);
                 gx[r] += __shfl_xor_sync(mask, gx[r], o);
             }
+        if (!keep) {                         // padding adds nothing, not even a NaN that it holds
+            for (int r = 0; r < nh; ++r)
+#pragma unroll
+                for (int s = 0; s < UPL; ++s) {
+                    if (ca[s] < a.d) *reinterpret_cast<Pack<T, VEC>*>(dx + r * a.d + ca[s]) = Pack<T, VEC>{};
+                    if (cb[s] < a.d) *reinterpret_cast<Pack<T, VEC>*>(dx + r * a.d + cb[s]) = Pack<T, VEC>{};
+                }
+            continue;
+        }
 #pragma unroll
         for (int r = 0; r < HPT; ++r) {
-            if (r >= nh) break;
+            const bool live = r < nh;
             const float rs = rsqrtf(ss[r] * inv_d + a.eps);
             const float m = -gx[r] * inv_d * rs * rs;
 #pragma unroll
             for (int s = 0; s < UPL; ++s) {
                 // t = x r; dw += du t; dx = r (w du) - t m
                 auto one = [&](const Pack<T, VEC>& raw, float* u, const float* w, float* dw, int ch) {
-                    float t[VEC], mt[VEC];
+                    float t[VEC], mt[VEC], td[VEC];
                     unpack<T, VEC>(raw, t);
                     scale_vec<VEC>(t, t, rs);
-                    if (keep) {                  // padding rows add nothing, not even a NaN that they hold
-                        fma_vec<VEC>(dw, u, t, dw);
-                        scale_vec<VEC>(mt, t, m);
-                        mul_vec<VEC>(u, u, w);
-                        float rr[VEC];
+                    scale_vec<VEC>(td, t, live ? 1.f : 0.f);      // a head read twice counts once
+                    fma_vec<VEC>(dw, u, td, dw);
+                    scale_vec<VEC>(mt, t, m);
+                    mul_vec<VEC>(u, u, w);
+                    float rr[VEC];
 #pragma unroll
-                        for (int j = 0; j < VEC; ++j) rr[j] = rs;
-                        fma_vec<VEC>(u, u, rr, mt);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < VEC; ++j) u[j] = 0.f;
-                    }
-                    if (ch < a.d) store_vec<T, VEC>(dx + r * a.d + ch, u);
+                    for (int j = 0; j < VEC; ++j) rr[j] = rs;
+                    fma_vec<VEC>(u, u, rr, mt);
+                    if (live && ch < a.d) store_vec<T, VEC>(dx + r * a.d + ch, u);
                 };
                 one(ra[r][s], ua[r][s], wa[s], da[s], ca[s]);
                 one(rb[r][s], ub[r][s], wb[s], db[s], cb[s]);
@@ -694,14 +707,23 @@ struct RowLaunch {
     int vec;
     const char* what;
     cudaStream_t st;
-    template <typename T>
-    int run() {
-        constexpr int W = 16 / sizeof(T);
+    template <typename T, bool INTER>
+    void go() {
+        constexpr int W = 16 / sizeof(T), H = heads_at_once(W, sizeof(T));
         const uint32_t per = kThreads >> a.lanes_log2;
         const unsigned blocks = (a.units + per - 1) / per;
-        if (vec == W) rows_kernel<T, W, 1, heads_at_once(W, sizeof(T)), OUT, ROPE><<<blocks, kThreads, 0, st>>>(a);
-        else if (vec == 2) rows_kernel<T, 2, 2, 1, OUT, ROPE><<<blocks, kThreads, 0, st>>>(a);
-        else rows_kernel<T, 1, 4, 1, OUT, ROPE><<<blocks, kThreads, 0, st>>>(a);
+        if (vec == W) rows_kernel<T, W, 1, H, OUT, ROPE, INTER><<<blocks, kThreads, 0, st>>>(a);
+        else if (vec == 2) rows_kernel<T, 2, 2, 1, OUT, ROPE, INTER><<<blocks, kThreads, 0, st>>>(a);
+        else rows_kernel<T, 1, 4, 1, OUT, ROPE, INTER><<<blocks, kThreads, 0, st>>>(a);
+    }
+    template <typename T>
+    int run() {
+        if constexpr (ROPE) {
+            if (a.inter) go<T, true>();
+            else go<T, false>();
+        } else {
+            go<T, false>();
+        }
         return check_launch(what);
     }
 };
@@ -760,13 +782,18 @@ struct GradLaunch {
     GradArgs g;
     int vec;
     cudaStream_t st;
+    template <typename T, bool INTER>
+    void go(unsigned blocks) {
+        constexpr int W = 16 / sizeof(T);
+        if (vec == W) rope_bwd_kernel<T, W, 1, grad_heads(W, sizeof(T)), INTER><<<blocks, kThreads, 0, st>>>(g);
+        else if (vec == 2) rope_bwd_kernel<T, 2, 2, 1, INTER><<<blocks, kThreads, 0, st>>>(g);
+        else rope_bwd_kernel<T, 1, 4, 1, INTER><<<blocks, kThreads, 0, st>>>(g);
+    }
     template <typename T>
     int run() {
-        constexpr int W = 16 / sizeof(T);
         const unsigned blocks = (unsigned)g.r.n * (g.cq + g.ck);
-        if (vec == W) rope_bwd_kernel<T, W, 1, grad_heads(W, sizeof(T))><<<blocks, kThreads, 0, st>>>(g);
-        else if (vec == 2) rope_bwd_kernel<T, 2, 2, 1><<<blocks, kThreads, 0, st>>>(g);
-        else rope_bwd_kernel<T, 1, 4, 1><<<blocks, kThreads, 0, st>>>(g);
+        if (g.r.inter) go<T, true>(blocks);
+        else go<T, false>(blocks);
         int rc = check_launch("widek_qk_norm_rope_bwd");
         if (rc != WIDEK_OK || (!g.dqw && !g.dkw)) return rc;
         const dim3 grid(2 * g.r.n, (g.r.d + 31) / 32);
