@@ -18,9 +18,16 @@
 // after the other for the interleaved order, the channels past R and rows
 // without a rotation), so that the rotation needs no exchange between lanes
 // and the norm one reduction. Every channel is read once and written once,
-// in 16-byte vectors where sizes and strides allow it. All of it is bound by
-// memory: 2 D bytes in and out per row of a 16-bit type against ~10 flops a
-// channel.
+// in 16-byte vectors where sizes and strides allow it.
+//
+// Bound by memory (2 D bytes in and out per row of a 16-bit type) but near the
+// instructions' bound: at the copy rate there is time for about 7 of them a
+// channel. So four heads of a token share its angles, weights and addresses,
+// the weights are folded into the angles' coefficients, fp32 arithmetic runs
+// two to an instruction, and codes and values change form by byte permutes.
+// Measured (B200, floor at the measured copy rate): norm + rotation of 168 M
+// bf16 values 135 us (103), its backward over 84 M 119 us (77), int8 write of
+// 268 M 183 us (124), read 127 us (125).
 #include "paged_cache.cuh"
 
 #include <initializer_list>
@@ -52,7 +59,7 @@ int cache_args(PagedCache& c, const char* what, void* k, void* v, float* ks, flo
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
 struct Strides {
     int64_t n, b, t, h;
@@ -226,7 +233,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ 
     for (int r = 0; r < HPT; ++r)
 #pragma unroll
         for (int s = 0; s < UPL; ++s) {
-            const T* row = src + min(r, nh - 1) * st.h;
+            const T* row = src + (r < nh ? r : 0) * (int64_t)(int)st.h;
             ra[r][s] = load_pack<T, VEC>(row + (ca[s] < a.d ? ca[s] : 0));
             rb[r][s] = load_pack<T, VEC>(row + (cb[s] < a.d ? cb[s] : 0));
         }
@@ -419,7 +426,7 @@ struct GradArgs {
 };
 
 // A block takes consecutive units (HPT heads of a token) of one model's q (or
-// k) side, and each of its groups of lanes every 256/lanes-th of them, keeping
+// k) side, and each of its groups of lanes every (threads / lanes)-th of them, keeping
 // the weight gradient of its channels in registers; groups, warps and blocks
 // are joined in a fixed order, so the sums do not depend on timing.
 template <typename T, int VEC, int UPL, int HPT, bool INTER>
@@ -476,10 +483,11 @@ __global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const __grid_constan
 #pragma unroll
             for (int s = 0; s < UPL; ++s) {
                 // places outside the row are read from its first vector and left out of the sums
-                const int at = min(r, nh - 1), pa = ca[s] < a.d ? ca[s] : 0, pb = cb[s] < a.d ? cb[s] : 0;
-                ra[r][s] = load_pack<T, VEC>(x + at * st.h + pa);
+                const int at = r < nh ? r : 0, pa = ca[s] < a.d ? ca[s] : 0, pb = cb[s] < a.d ? cb[s] : 0;
+                const T* row = x + at * (int64_t)(int)st.h;
+                ra[r][s] = load_pack<T, VEC>(row + pa);
                 sa[r][s] = load_pack<T, VEC>(dy + at * a.d + pa);
-                rb[r][s] = load_pack<T, VEC>(x + at * st.h + pb);
+                rb[r][s] = load_pack<T, VEC>(row + pb);
                 sb[r][s] = load_pack<T, VEC>(dy + at * a.d + pb);
             }
         const int64_t trow = (int64_t)(keep ? pos : 0) * (a.rot / 2);
@@ -584,11 +592,11 @@ __global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const __grid_constan
             }
     }
     __syncthreads();
-    if ((int)threadIdx.x < a.d) {
+    for (int c = threadIdx.x; c < a.d; c += kThreads) {
         float sum = 0.f;
 #pragma unroll
-        for (int wp = 0; wp < kThreads / 32; ++wp) sum += red[wp][threadIdx.x];
-        g.part[(int64_t)blockIdx.x * a.d + threadIdx.x] = sum;
+        for (int wp = 0; wp < kThreads / 32; ++wp) sum += red[wp][c];
+        g.part[(int64_t)blockIdx.x * a.d + c] = sum;
     }
 }
 
@@ -666,24 +674,30 @@ int row_args(RowArgs& a, const char* what, const int64_t* g, int pos64) {
     a.sk = Strides{g[12], g[13], g[14], g[15]};
     a.sv = Strides{g[16], g[17], g[18], g[19]};
     a.pos_n = g[20], a.pos_b = g[21], a.pos_t = g[22];
+    for (int64_t h : {a.sq.h, a.sk.h, a.sv.h})
+        if (h > 0x7fffffff || h < -0x7fffffff)
+            return set_error(WIDEK_ERR_UNSUPPORTED, "%s: heads %lld elements apart", what, (long long)h);
     a.pos64 = pos64;
     a.err = device_error_ptr();
     return WIDEK_OK;
 }
 
-// Heads that a group of lanes takes at once: 4 with 16-byte vectors, one in
-// the narrow paths, whose rows take more registers.
-#ifndef HPT_F
-#define HPT_F 4
-#endif
-#ifndef HPT_B
-#define HPT_B 2
-#endif
-constexpr int heads_at_once(int vec, size_t esz) { return vec == (int)(16 / esz) ? HPT_F : 1; }
+// Heads that a group of lanes takes at once. 4 with 16-byte vectors (1, 2 and 8
+// took 228, 194 and 193 us where 4 took 145, at 168 M values), one in the
+// narrow paths, whose rows take more registers, and where there are so few
+// rows that one each does not fill the GPU (a decoder step of 6144 rows: 4.8
+// us, not 7.2).
+constexpr int kHeadsAtOnce = 4;
 
-// Units of a call with `vec`-wide accesses; sides: 1 (k) or 2 (k and v).
-int row_units(RowArgs& a, const char* what, int vec, size_t esz, int sides) {
-    const int hpt = heads_at_once(vec, esz);
+int heads_at_once(const RowArgs& a, int vec, size_t esz, int sides) {
+    if (vec != (int)(16 / esz)) return 1;
+    const double lanes = (double)a.n * a.b * a.t * ((double)a.hq + (double)sides * a.hk) * (1 << lanes_log2(a.d, vec));
+    return lanes > 2048.0 * sm_count(current_device()) ? kHeadsAtOnce : 1;
+}
+
+// Units of a call with `vec`-wide accesses, hpt heads at once; sides: 1 (k) or
+// 2 (k and v).
+int row_units(RowArgs& a, const char* what, int vec, int hpt, int sides) {
     a.parts_q = (a.hq + hpt - 1) / hpt;
     a.parts_k = (a.hk + hpt - 1) / hpt;
     const int64_t parts = (int64_t)a.parts_q + (int64_t)sides * a.parts_k;
@@ -704,15 +718,16 @@ bool no_rows(const RowArgs& a, int heads) { return a.n == 0 || a.b == 0 || a.t =
 template <int OUT, bool ROPE>
 struct RowLaunch {
     RowArgs a;
-    int vec;
+    int vec, hpt;
     const char* what;
     cudaStream_t st;
     template <typename T, bool INTER>
     void go() {
-        constexpr int W = 16 / sizeof(T), H = heads_at_once(W, sizeof(T));
+        constexpr int W = 16 / sizeof(T), H = kHeadsAtOnce;
         const uint32_t per = kThreads >> a.lanes_log2;
         const unsigned blocks = (a.units + per - 1) / per;
-        if (vec == W) rows_kernel<T, W, 1, H, OUT, ROPE, INTER><<<blocks, kThreads, 0, st>>>(a);
+        if (vec == W && hpt == H) rows_kernel<T, W, 1, H, OUT, ROPE, INTER><<<blocks, kThreads, 0, st>>>(a);
+        else if (vec == W) rows_kernel<T, W, 1, 1, OUT, ROPE, INTER><<<blocks, kThreads, 0, st>>>(a);
         else if (vec == 2) rows_kernel<T, 2, 2, 1, OUT, ROPE, INTER><<<blocks, kThreads, 0, st>>>(a);
         else rows_kernel<T, 1, 4, 1, OUT, ROPE, INTER><<<blocks, kThreads, 0, st>>>(a);
     }
@@ -731,14 +746,15 @@ struct RowLaunch {
 template <int IN>
 struct ReadLaunch {
     RowArgs a;
-    int vec;
+    int vec, hpt;
     cudaStream_t st;
     template <typename T>
     int run() {
         constexpr int W = 16 / sizeof(T);
         const uint32_t per = kThreads >> a.lanes_log2;
         const unsigned blocks = (a.units + per - 1) / per;
-        if (vec == W) cache_read_kernel<T, W, 1, heads_at_once(W, sizeof(T)), IN><<<blocks, kThreads, 0, st>>>(a);
+        if (vec == W && hpt > 1) cache_read_kernel<T, W, 1, kHeadsAtOnce, IN><<<blocks, kThreads, 0, st>>>(a);
+        else if (vec == W) cache_read_kernel<T, W, 1, 1, IN><<<blocks, kThreads, 0, st>>>(a);
         else if (vec == 2) cache_read_kernel<T, 2, 2, 1, IN><<<blocks, kThreads, 0, st>>>(a);
         else cache_read_kernel<T, 1, 4, 1, IN><<<blocks, kThreads, 0, st>>>(a);
         return check_launch("widek_cache_read_fwd");
@@ -746,19 +762,20 @@ struct ReadLaunch {
 };
 
 template <int OUT, bool ROPE>
-int launch_rows(const RowArgs& a, int vec, const char* what, int dtype, cudaStream_t st) {
-    RowLaunch<OUT, ROPE> L{a, vec, what, st};
+int launch_rows(const RowArgs& a, int vec, int hpt, const char* what, int dtype, cudaStream_t st) {
+    RowLaunch<OUT, ROPE> L{a, vec, hpt, what, st};
     return dispatch_dtype(dtype, L);
 }
 
 template <bool ROPE>
-int launch_rows_fmt(const RowArgs& a, int vec, const char* what, int fmt, int dtype, cudaStream_t st) {
-    if (fmt == WIDEK_I8) return launch_rows<OUT_I8, ROPE>(a, vec, what, dtype, st);
-    if (fmt == WIDEK_E4M3) return launch_rows<OUT_E4M3, ROPE>(a, vec, what, dtype, st);
-    return launch_rows<OUT_SAME, ROPE>(a, vec, what, dtype, st);
+int launch_rows_fmt(const RowArgs& a, int vec, int hpt, const char* what, int fmt, int dtype, cudaStream_t st) {
+    if (fmt == WIDEK_I8) return launch_rows<OUT_I8, ROPE>(a, vec, hpt, what, dtype, st);
+    if (fmt == WIDEK_E4M3) return launch_rows<OUT_E4M3, ROPE>(a, vec, hpt, what, dtype, st);
+    return launch_rows<OUT_SAME, ROPE>(a, vec, hpt, what, dtype, st);
 }
 
-constexpr int kGradHeads = HPT_B;     // heads at once in the backward, whose rows take twice the registers
+constexpr int kGradBlocks = 444;  // of the backward over all models, 3 for each SM: twice as many cost the join what they gave
+constexpr int kGradHeads = 2;     // heads at once in the backward, whose rows take twice the registers
 constexpr int grad_heads(int vec, size_t esz) { return vec == (int)(16 / esz) ? kGradHeads : 1; }
 
 // Blocks per model of the backward: about three blocks for each SM over all
@@ -768,7 +785,7 @@ void grad_chunks(const RowArgs& a, int vec, int hpt, int& cq, int& ck, uint32_t&
     const int64_t tokens = (int64_t)a.b * a.t;
     auto split = [&](int64_t heads, int& c, uint32_t& per) {
         const int64_t units = tokens * ((heads + hpt - 1) / hpt);
-        int64_t want = (int64_t)444 * heads / ((int64_t)a.n * ((int64_t)a.hq + a.hk));
+        int64_t want = (int64_t)kGradBlocks * heads / ((int64_t)a.n * ((int64_t)a.hq + a.hk));
         const int64_t most = (units + groups - 1) / groups;
         want = want < 1 ? 1 : (want > most ? most : want);
         per = (uint32_t)(((units + want - 1) / want + groups - 1) / groups * groups);
@@ -833,9 +850,10 @@ extern "C" int widek_qk_norm_rope_fwd(const void* q, const void* k, const void* 
     const size_t esz = dtype_size(dtype);
     if (esz == 0) return set_error(WIDEK_ERR_INVALID, "%s: unknown dtype code %d", what, dtype);
     const int vec = row_vec(a, esz, {qw, kw, yq, yk}, false);
-    rc = row_units(a, what, vec, esz, 1);
+    const int hpt = heads_at_once(a, vec, esz, 1);
+    rc = row_units(a, what, vec, hpt, 1);
     if (rc != WIDEK_OK) return rc;
-    return launch_rows<OUT_DENSE, true>(a, vec, what, dtype, (cudaStream_t)stream);
+    return launch_rows<OUT_DENSE, true>(a, vec, hpt, what, dtype, (cudaStream_t)stream);
 }
 
 extern "C" int widek_qk_norm_rope_write_fwd(const void* q, const void* k, const void* v, const void* qw,
@@ -858,9 +876,10 @@ extern "C" int widek_qk_norm_rope_write_fwd(const void* q, const void* k, const 
     const size_t esz = dtype_size(dtype);
     if (esz == 0) return set_error(WIDEK_ERR_INVALID, "%s: unknown dtype code %d", what, dtype);
     const int vec = row_vec(a, esz, {qw, kw, yq}, !cache_fmt_8bit(fmt));
-    rc = row_units(a, what, vec, esz, 2);
+    const int hpt = heads_at_once(a, vec, esz, 2);
+    rc = row_units(a, what, vec, hpt, 2);
     if (rc != WIDEK_OK) return rc;
-    return launch_rows_fmt<true>(a, vec, what, fmt, dtype, (cudaStream_t)stream);
+    return launch_rows_fmt<true>(a, vec, hpt, what, fmt, dtype, (cudaStream_t)stream);
 }
 
 extern "C" int widek_cache_write_fwd(const void* k, const void* v, const void* positions, void* kc, void* vc,
@@ -879,9 +898,10 @@ extern "C" int widek_cache_write_fwd(const void* k, const void* v, const void* p
     const size_t esz = dtype_size(dtype);
     if (esz == 0) return set_error(WIDEK_ERR_INVALID, "%s: unknown dtype code %d", what, dtype);
     const int vec = row_vec(a, esz, {}, !cache_fmt_8bit(fmt));
-    rc = row_units(a, what, vec, esz, 2);
+    const int hpt = heads_at_once(a, vec, esz, 2);
+    rc = row_units(a, what, vec, hpt, 2);
     if (rc != WIDEK_OK) return rc;
-    return launch_rows_fmt<false>(a, vec, what, fmt, dtype, (cudaStream_t)stream);
+    return launch_rows_fmt<false>(a, vec, hpt, what, fmt, dtype, (cudaStream_t)stream);
 }
 
 extern "C" int widek_cache_read_fwd(const void* kc, const void* vc, const float* ks, const float* vs,
@@ -901,18 +921,19 @@ extern "C" int widek_cache_read_fwd(const void* kc, const void* vc, const float*
     const size_t esz = dtype_size(dtype);
     if (esz == 0) return set_error(WIDEK_ERR_INVALID, "%s: unknown dtype code %d", what, dtype);
     const int vec = row_vec(a, esz, {k, v}, !cache_fmt_8bit(fmt));
-    rc = row_units(a, what, vec, esz, 2);
+    const int hpt = heads_at_once(a, vec, esz, 2);
+    rc = row_units(a, what, vec, hpt, 2);
     if (rc != WIDEK_OK) return rc;
     cudaStream_t st = (cudaStream_t)stream;
     if (fmt == WIDEK_I8) {
-        ReadLaunch<OUT_I8> L{a, vec, st};
+        ReadLaunch<OUT_I8> L{a, vec, hpt, st};
         return dispatch_dtype(dtype, L);
     }
     if (fmt == WIDEK_E4M3) {
-        ReadLaunch<OUT_E4M3> L{a, vec, st};
+        ReadLaunch<OUT_E4M3> L{a, vec, hpt, st};
         return dispatch_dtype(dtype, L);
     }
-    ReadLaunch<OUT_SAME> L{a, vec, st};
+    ReadLaunch<OUT_SAME> L{a, vec, hpt, st};
     return dispatch_dtype(dtype, L);
 }
 
@@ -957,7 +978,7 @@ extern "C" int widek_qk_norm_rope_bwd(const void* q, const void* k, const void* 
     if (esz == 0) return set_error(WIDEK_ERR_INVALID, "%s: unknown dtype code %d", what, dtype);
     const int vec = row_vec(a, esz, {qw, kw, dyq, dyk, dq, dk}, false);
     const int hpt = grad_heads(vec, esz);
-    rc = row_units(a, what, 1, esz, 1);          // the narrowest: units of one head, for the size check
+    rc = row_units(a, what, 1, 1, 1);            // the narrowest: units of one head, for the size check
     if (rc != WIDEK_OK) return rc;
     grad_chunks(a, vec, hpt, g.cq, g.ck, g.per_q, g.per_k);
     a.lanes_log2 = lanes_log2(a.d, vec);
