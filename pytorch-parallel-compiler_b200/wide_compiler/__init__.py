@@ -21,7 +21,7 @@ from .core.ensemble_util import pack_inputs, unpack_outputs
 from .core.paged_cache import WidePagedCache
 from .core.primitives import (WideLinear, WideConv1d, WideConv2d, WideConv3d, WideBatchNorm1d, WideBatchNorm2d,
                               WideLayerNorm, WideGroupNorm, WideInstanceNorm1d, WideInstanceNorm2d, WideEmbedding,
-                              WideAttention, WideGRU, WideLSTM)
+                              WideAttention, WideDecoderAttention, WideGRU, WideLSTM)
 
 _HAS_BENCHMARK = False
 benchmark_primitive = None
@@ -41,7 +41,8 @@ __all__ = [
     'TracedWideModel', 'FunctionalOp', 'BinaryOp', 'print_trace', 'pack_inputs', 'unpack_outputs',
     'WideLinear', 'WideConv1d', 'WideConv2d', 'WideConv3d', 'WideBatchNorm1d', 'WideBatchNorm2d',
     'WideLayerNorm', 'WideGroupNorm', 'WideInstanceNorm1d', 'WideInstanceNorm2d', 'WideEmbedding',
-    'WideAttention', 'WideGRU', 'WideLSTM', 'WidePagedCache',
+    'WideAttention', 'WideGRU', 'WideLSTM',
+    'WideDecoderAttention', 'WidePagedCache',
     'benchmark_primitive', 'benchmark_multi', 'benchmark_all', 'benchmark_custom', 'list_benchmark_primitives',
     'BenchmarkResult', 'SweepParams',
 ]

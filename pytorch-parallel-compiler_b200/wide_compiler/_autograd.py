@@ -286,6 +286,33 @@ def attention_t(query: Tensor, key: Tensor, value: Tensor, attn_mask, is_causal:
     return linear_t(o, out_weight, out_bias)
 
 
+def causal_attention_t(q: Tensor, k: Tensor, v: Tensor) -> Tensor:
+    n, b, t, hq, d = q.shape
+    split = lambda x: x.repeat_interleave(hq // x.shape[3], dim=3).reshape(n * b, t, hq, d).transpose(1, 2)
+    o = F.scaled_dot_product_attention(split(q), split(k), split(v), is_causal=True, scale=1.0 / math.sqrt(d))
+    return o.transpose(1, 2).reshape(n, b, t, hq, d)
+
+
+def _norm_rope_t(x: Tensor, weight: Tensor, cos: Tensor, sin: Tensor, positions: Tensor, eps: float,
+                 interleaved: bool) -> Tensor:
+    xf = x.float()
+    u = xf * torch.rsqrt((xf * xf).mean(-1, keepdim=True) + eps) * weight.float()[:, None, None, None]
+    pos = positions.long()
+    c, s = cos[pos.clamp(min=0)].unsqueeze(-2), sin[pos.clamp(min=0)].unsqueeze(-2)
+    r = 2 * cos.shape[1]
+    a, b = (u[..., 0:r:2], u[..., 1:r:2]) if interleaved else (u[..., :r // 2], u[..., r // 2:r])
+    a, b = a * c - b * s, b * c + a * s
+    turned = torch.stack((a, b), -1).flatten(-2) if interleaved else torch.cat((a, b), -1)
+    y = torch.cat((turned, u[..., r:]), -1)
+    return torch.where((pos >= 0)[..., None, None], y, torch.zeros_like(y)).to(x.dtype)
+
+
+def qk_norm_rope_t(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, cos: Tensor, sin: Tensor,
+                   positions: Tensor, eps: float, interleaved: bool):
+    return (_norm_rope_t(q, q_weight, cos, sin, positions, eps, interleaved),
+            _norm_rope_t(k, k_weight, cos, sin, positions, eps, interleaved))
+
+
 # ---------------------------------------------------------------------------
 # Kernel-backed gradients
 #

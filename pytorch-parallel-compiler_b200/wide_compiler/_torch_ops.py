@@ -266,7 +266,85 @@ def _(a, b, op):
 _register_autograd(binary, _AG.binary_t)
 
 
+def _cache(k_pages, v_pages, table, k_scale, v_scale):
+    from .core.paged_cache import WidePagedCache
+    return WidePagedCache(k_pages, v_pages, table, k_scale, v_scale)
+
+
+@torch.library.custom_op("widek::qk_norm_rope", mutates_args=())
+def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, cos: Tensor, sin: Tensor,
+                 positions: Tensor, eps: float, interleaved: bool) -> Tuple[Tensor, Tensor]:
+    """Norm and rotation of query and key heads (ops.qk_norm_rope)."""
+    with torch.no_grad():
+        return ops.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+
+
+@qk_norm_rope.register_fake
+def _(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+_register_autograd(qk_norm_rope, _AG.qk_norm_rope_t)
+
+
+@torch.library.custom_op("widek::qk_norm_rope_write", mutates_args=("k_pages", "v_pages", "k_scale", "v_scale"))
+def qk_norm_rope_write(q: Tensor, k: Tensor, v: Tensor, q_weight: Tensor, k_weight: Tensor, cos: Tensor, sin: Tensor,
+                       positions: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor,
+                       k_scale: Optional[Tensor], v_scale: Optional[Tensor], eps: float, interleaved: bool) -> Tensor:
+    """The same with the keys and values written to the cache (ops.qk_norm_rope_write)."""
+    with torch.no_grad():
+        return ops.qk_norm_rope_write(q, k, v, q_weight, k_weight, cos, sin, positions,
+                                      _cache(k_pages, v_pages, table, k_scale, v_scale), eps, interleaved)
+
+
+@qk_norm_rope_write.register_fake
+def _(q, k, v, q_weight, k_weight, cos, sin, positions, k_pages, v_pages, table, k_scale, v_scale, eps, interleaved):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("widek::cache_write", mutates_args=("k_pages", "v_pages", "k_scale", "v_scale"))
+def cache_write(k_pages: Tensor, v_pages: Tensor, table: Tensor, k_scale: Optional[Tensor],
+                v_scale: Optional[Tensor], k: Tensor, v: Tensor, positions: Tensor) -> None:
+    """Keys and values into the paged cache (ops.cache_write)."""
+    with torch.no_grad():
+        ops.cache_write(_cache(k_pages, v_pages, table, k_scale, v_scale), k, v, positions)
+
+
+@cache_write.register_fake
+def _(k_pages, v_pages, table, k_scale, v_scale, k, v, positions):
+    return None
+
+
+@torch.library.custom_op("widek::cache_read", mutates_args=())
+def cache_read(k_pages: Tensor, v_pages: Tensor, table: Tensor, k_scale: Optional[Tensor],
+               v_scale: Optional[Tensor], positions: Tensor, dtype: Optional[torch.dtype]) -> Tuple[Tensor, Tensor]:
+    """Cached keys and values of the tokens at ``positions`` (ops.cache_read)."""
+    return ops.cache_read(_cache(k_pages, v_pages, table, k_scale, v_scale), positions, dtype)
+
+
+@cache_read.register_fake
+def _(k_pages, v_pages, table, k_scale, v_scale, positions, dtype):
+    if dtype is None:
+        dtype = torch.bfloat16 if k_scale is not None else k_pages.dtype
+    shape = (k_pages.shape[0], table.shape[-2], positions.shape[-1], k_pages.shape[2], k_pages.shape[4])
+    return k_pages.new_empty(shape, dtype=dtype), k_pages.new_empty(shape, dtype=dtype)
+
+
+@torch.library.custom_op("widek::decode_attention", mutates_args=())
+def decode_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, k_scale: Optional[Tensor],
+                     v_scale: Optional[Tensor], lengths: Tensor, scale: float, window: int) -> Tensor:
+    """Attention of one new token over the paged cache (ops.decode_attention)."""
+    with torch.no_grad():
+        return ops.decode_attention(q, _cache(k_pages, v_pages, table, k_scale, v_scale), lengths, scale, window)
+
+
+@decode_attention.register_fake
+def _(q, k_pages, v_pages, table, k_scale, v_scale, lengths, scale, window):
+    return q.new_empty(q.shape)
+
+
 OPERATORS = ('linear', 'layernorm', 'batchnorm', 'groupnorm', 'embedding', 'conv', 'gru', 'lstm', 'attention',
-             'swap01', 'unary', 'binary')
+             'swap01', 'unary', 'binary', 'qk_norm_rope', 'qk_norm_rope_write', 'cache_write', 'cache_read',
+             'decode_attention')
 
 __all__ = ['OPERATORS']

@@ -12,6 +12,7 @@ from .wide_groupnorm import WideGroupNorm, GroupNormStrategy
 from .wide_instancenorm import WideInstanceNorm1d, WideInstanceNorm2d, InstanceNormStrategy
 from .wide_embedding import WideEmbedding, EmbeddingStrategy
 from .wide_attention import WideAttention, AttentionStrategy
+from .wide_decoder_attention import WideDecoderAttention
 from .wide_gru import WideGRU, GRUStrategy
 from .wide_lstm import WideLSTM, LSTMStrategy
 
@@ -43,6 +44,7 @@ __all__ = [
     'WideInstanceNorm1d', 'WideInstanceNorm2d', 'InstanceNormStrategy',
     'WideEmbedding', 'EmbeddingStrategy',
     'WideAttention', 'AttentionStrategy',
+    'WideDecoderAttention',
     'WideGRU', 'GRUStrategy',
     'WideLSTM', 'LSTMStrategy',
     'BUILTIN_PRIMITIVES',

@@ -1186,6 +1186,29 @@ def cache_read(cache, positions: Tensor, dtype: Optional[torch.dtype] = None):
     return k, v
 
 
+def causal_attention(q: Tensor, k: Tensor, v: Tensor) -> Tensor:
+    """Causal attention over whole sequences with grouped key heads: q
+    [N, B, T, Hq, D], k and v [N, B, T, Hk, D] -> [N, B, T, Hq, D] (the core of
+    WideAttention, widek_attention_fwd, on one key head for each query head;
+    differentiable: the backward re-runs the torch formulation)."""
+    if _AG.needs_grad(q, k, v):
+        return _AG.run(causal_attention, _AG.causal_attention_t, q, k, v)
+    what = "causal_attention"
+    dev = N.require_cuda(q, k, v, what=what)
+    _same_dtype(what, q, k, v)
+    n, b, t, hq, d = q.shape
+    hk = k.shape[3]
+    if v.shape != k.shape or k.shape[:3] != q.shape[:3] or k.shape[4] != d or hk < 1 or hq % hk != 0:
+        raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
+    if hk != hq:
+        k, v = (x.repeat_interleave(hq // hk, dim=3) for x in (k, v))
+    q, k, v = _dense(q), _dense(k), _dense(v)
+    out = torch.empty(q.shape, device=dev, dtype=q.dtype)
+    if out.numel():
+        attention_core(q, k, v, n * b, hq, t, t, d, hq * d, hq * d, hq * d, out, True, None)
+    return out
+
+
 def decode_attention(q: Tensor, cache, lengths: Tensor, scale: Optional[float] = None, window: int = 0) -> Tensor:
     """Attention of one new token of every sequence over its cached tokens
     (widek_decode_attention_fwd).
