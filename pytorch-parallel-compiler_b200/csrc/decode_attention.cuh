@@ -50,7 +50,8 @@
 // queries stay exact, which bf16 would not give f16 ones). The scale of a key
 // row multiplies its score; that of a value row goes into its weight, whose
 // product p vs has no fixed range: V and the weights meet in bf16, which has
-// fp32's.
+// fp32's, in three pieces where the result is fp32. The tensor core's sums
+// round towards zero: fp32 results take them in short chains, added in fp32.
 #pragma once
 
 #include "paged_cache.cuh"
@@ -660,14 +661,19 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
                         for (int w = 0; w < S::KW; ++w) r0[w] = kr[0][w], r1[w] = kr[1][w];
                     }
 #pragma unroll
-                    for (int e = 0; e < S::KR; e += 2)
+                    for (int t = 0; t < NT; ++t) {
+                        float part[4] = {0.f, 0.f, 0.f, 0.f};
+                        float(&o)[4] = SPLITQ ? part : s[t][mt];
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) {
+                        for (int e = 0; e < S::KR; e += 2) {
                             const int j = p * S::KR + e;
                             if constexpr (SPLITQ)
-                                mma<KIND>(s[t][mt], r0[e], r1[e], r0[e + 1], r1[e + 1], ql[t][j], ql[t][j + 1]);
-                            mma<KIND>(s[t][mt], r0[e], r1[e], r0[e + 1], r1[e + 1], q[t][j], q[t][j + 1]);
+                                mma<KIND>(o, r0[e], r1[e], r0[e + 1], r1[e + 1], ql[t][j], ql[t][j + 1]);
+                            mma<KIND>(o, r0[e], r1[e], r0[e + 1], r1[e + 1], q[t][j], q[t][j + 1]);
                         }
+#pragma unroll
+                        for (int e = 0; e < (SPLITQ ? 4 : 0); ++e) s[t][mt][e] += part[e];
+                    }
                 }
             }
         }
@@ -730,8 +736,9 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
                     for (int e = 0; e < 4; ++e) acc[t][j][e] *= f[t][e & 1];
         }
     };
-    // Weights as B operands: hi and lo pieces of tokens (k) by heads (n)
-    uint32_t ph[NT][MT][K::f32 ? 4 : 2], pl[NT][MT][K::f32 ? 4 : 2];
+    // Weights as B operands: hi and lo pieces of tokens (k) by heads (n), and
+    // a third where the result is fp32
+    uint32_t ph[NT][MT][K::f32 ? 4 : 2], pl[NT][MT][K::f32 ? 4 : 2], pr[SPLITQ ? NT : 1][SPLITQ ? MT : 1][2];
     auto turn_weights = [&]() {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -753,6 +760,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
                         const uint32_t lo = pack2<K::values>(rx, ry, rx, ry);
                         ph[t][mt][hf] = transpose8x8(hi);
                         pl[t][mt][hf] = transpose8x8(lo);
+                        if constexpr (SPLITQ) pr[t][mt][hf] = transpose8x8(pack2<K::values>(rx, ry, rx, ry));
                     }
                 }
             }
@@ -839,9 +847,14 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
                     for (int w = 0; w < S::VD / 2; ++w)
 #pragma unroll
                         for (int t = 0; t < NT; ++t) {
-                            float(&o)[4] = acc[t][p * S::VD / 2 + w];
+                            float part[4] = {0.f, 0.f, 0.f, 0.f};
+                            float(&o)[4] = SPLITQ ? part : acc[t][p * S::VD / 2 + w];
+                            if constexpr (SPLITQ)
+                                mma<K::values>(o, av[w][0], av[w][1], av[w][2], av[w][3], pr[t][mt][0], pr[t][mt][1]);
                             mma<K::values>(o, av[w][0], av[w][1], av[w][2], av[w][3], pl[t][mt][0], pl[t][mt][1]);
                             mma<K::values>(o, av[w][0], av[w][1], av[w][2], av[w][3], ph[t][mt][0], ph[t][mt][1]);
+#pragma unroll
+                            for (int e = 0; e < (SPLITQ ? 4 : 0); ++e) acc[t][p * S::VD / 2 + w][e] += part[e];
                         }
                 }
             }
