@@ -10,19 +10,23 @@ namespace {
 
 constexpr int kJoinThreads = 256;
 constexpr int kMostBlocks = 1024;
+constexpr int kWideThreads = kMostBlocks;       // one for each block's maximum and sum
 // Sequences whose steps every block adds up to find its place in line (32 for
 // each thread).
 constexpr int kMostInLine = 4096;
 
 // out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c over the blocks c that a
 // segment lies in, in a fixed order. WIDE: a block for 32 channels of a query
-// head, its 8 warps taking every 8th c; else a warp for each head. Segments
-// that lie in one block were finished by the attention itself.
+// head, its 32 warps taking every 32nd c, with the first outputs on their way
+// while the factors are found; else a warp for each head. Segments that lie in
+// one block were finished by the attention itself.
 template <bool WIDE>
-__global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_constant__ DecodeArgs a) {
-    constexpr int kWarps = kJoinThreads / 32;
+__global__ void __launch_bounds__(WIDE ? kWideThreads : kJoinThreads)
+    decode_join_kernel(const __grid_constant__ DecodeArgs a) {
+    constexpr int kWarps = (WIDE ? kWideThreads : kJoinThreads) / 32;
     __shared__ float factor[WIDE ? kMostBlocks : 1];
     __shared__ float red[WIDE ? kWarps : 1][33];
+    __shared__ float2 red_ml[WIDE ? kWarps : 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t last = (int64_t)a.n * a.b * a.hq - 1;
     const int64_t row = WIDE ? blockIdx.x : min((int64_t)blockIdx.x * kWarps + warp, last);
@@ -53,34 +57,50 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
         return ((int64_t)c * 2 + (c == c0 ? late : 0)) * 8 * a.nt + in_group % (8 * a.nt);
     };
     float top = -INFINITY, total = 0.f;
-    for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, a.part_ml[place(c)].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float ref = top == -INFINITY ? 0.f : top;
     if constexpr (WIDE) {
-        for (int c = c0 + lane; c <= c1; c += 32) {
-            const float2 x = a.part_ml[place(c)];
-            const float f = ex2(x.x - ref);
-            total += f * x.y;
-            if (warp == 0) factor[c - c0] = f;
+        constexpr int kAhead = 8;
+        const int ch = blockIdx.y * 32 + lane, count = c1 - c0 + 1;
+        const bool mine = (int)threadIdx.x < count;
+        const float2 x = mine ? a.part_ml[place(c0 + threadIdx.x)] : make_float2(-INFINITY, 0.f);
+        float ahead[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int c = warp + kWarps * i;
+            ahead[i] = c < count && ch < a.d ? a.part_o[place(c0 + c) * a.d + ch] : 0.f;
         }
-        total = warp_sum(total);
+        top = x.x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (lane == 0) red_ml[warp].x = top;
         __syncthreads();
-        const int ch = blockIdx.y * 32 + lane;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, red_ml[w].x);
+        const float f = mine ? ex2(x.x - (top == -INFINITY ? 0.f : top)) : 0.f;
+        factor[threadIdx.x] = f;
+        total = warp_sum(f * x.y);
+        if (lane == 0) red_ml[warp].y = total;
+        __syncthreads();
         float o = 0.f;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (warp + kWarps * i < count) o += factor[warp + kWarps * i] * ahead[i];
         if (ch < a.d) {
 #pragma unroll 8
-            for (int c = c0 + warp; c <= c1; c += kWarps) o += factor[c - c0] * a.part_o[place(c) * a.d + ch];
+            for (int c = warp + kWarps * kAhead; c < count; c += kWarps) o += factor[c] * a.part_o[place(c0 + c) * a.d + ch];
         }
         red[warp][lane] = o;
         __syncthreads();
         if (warp == 0 && ch < a.d) {
-            o = 0.f;
+            o = total = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) o += red[w][lane];
+            for (int w = 0; w < kWarps; ++w) o += red[w][lane], total += red_ml[w].y;
             store_out(a.out, row * a.d + ch, total == 0.f ? 0.f : o / total, a.dtype);
         }
     } else {
+        for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, a.part_ml[place(c)].x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float ref = top == -INFINITY ? 0.f : top;
         float acc[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[j] = 0.f;
@@ -197,7 +217,7 @@ extern "C" int widek_decode_attention_fwd(const void* q, const void* kc, const v
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = wide ? dim3((unsigned)heads, (unsigned)((a.d + 31) / 32))
                        : dim3((unsigned)((heads + kJoinThreads / 32 - 1) / (kJoinThreads / 32)));
-    cfg.blockDim = dim3(kJoinThreads);
+    cfg.blockDim = dim3(wide ? kWideThreads : kJoinThreads);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

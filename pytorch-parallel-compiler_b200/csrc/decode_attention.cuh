@@ -241,42 +241,71 @@ __device__ __forceinline__ uint32_t code_word(uint32_t w) {
     return KIND == DK_I8 ? w ^ 0x80808080u : w;
 }
 
-// How cached rows lie: of any size and place, of multiples of 16 bytes, or
-// those with exactly the channels of the tiles.
-enum RowsAre : int { ROWS_ANY, ROWS_16, ROWS_FULL };
+// How cached rows lie: of any size and place, as bytes that start inside words
+// (see copy_place), of multiples of 16 bytes, or those with exactly the
+// channels of the tiles.
+enum RowsAre : int { ROWS_ANY, ROWS_BYTES, ROWS_16, ROWS_FULL };
 
 // Copies 16 bytes at byte `off` of a cached row (of `bytes`) to shared memory
 // without waiting; zeros past the row, or all of them unless `live`. Rows of
-// 16 bytes' multiples have the place inside or outside; others come as words
-// (cp.async of 4 bytes) or, where even these are not aligned, as elements.
-template <int SIZE, int ROWS>
-__device__ __forceinline__ void copy_place(uint32_t dst, const uint8_t* row, int off, int bytes, bool words,
+// 16 bytes' multiples have the place inside or outside; others come 8 or 4
+// bytes at a time (cp.async's other sizes), as `grain`, the alignment of all
+// rows, allows (below 4 bytes: copy_elements). ROWS_BYTES are rows of such
+// sizes in a pool that starts on a word: they come as the words that they lie
+// in, so that channel 0 is up to 3 bytes into the first place (`off` then
+// counts from there), and the reader shifts. A 265 MB e4m3 cache with rows of
+// 138 bytes takes 221 us so, 1150 us by elements; rows of 136 bytes take 170
+// us, of 128 bytes 63.
+template <int ROWS>
+__device__ __forceinline__ void copy_place(uint32_t dst, const uint8_t* row, int off, int bytes, int grain,
                                            bool live) {
-    if constexpr (ROWS != ROWS_ANY) {
+    if constexpr (ROWS == ROWS_16 || ROWS == ROWS_FULL) {
         const int n = live && (ROWS == ROWS_FULL || off < bytes) ? 16 : 0;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(row + off), "r"(n) : "memory");
         return;
     }
-    if (words) {
+    if constexpr (ROWS == ROWS_BYTES) {
+        const int into = (int)(reinterpret_cast<uintptr_t>(row) & 3);
+        const uint8_t* first = row - into;               // of the pool: the pool's own start is on a word
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const int n = live ? max(0, min(4, into + bytes - off - 4 * w)) : 0;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + 4 * w),
+                         "l"(first + (n ? off + 4 * w : 0)), "r"(n) : "memory");
+        }
+        return;
+    }
+    if (grain >= 8) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            const int n = live && off + 8 * w < bytes ? 8 : 0;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst + 8 * w),
+                         "l"(row + (n ? off + 8 * w : 0)), "r"(n) : "memory");
+        }
+    } else {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const int n = live && off + 4 * w < bytes ? 4 : 0;
             asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + 4 * w),
                          "l"(row + (n ? off + 4 * w : 0)), "r"(n) : "memory");
         }
-    } else {
+    }
+}
+
+// The same by elements, for rows that cp.async cannot take.
+template <int SIZE>
+__device__ __forceinline__ void copy_elements(uint32_t dst, const uint8_t* row, int off, int bytes, bool live) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            uint32_t x = 0;
+    for (int w = 0; w < 4; ++w) {
+        uint32_t x = 0;
 #pragma unroll
-            for (int e = 0; e < 4 / SIZE; ++e) {
-                const int o = off + 4 * w + e * SIZE;
-                if (live && o < bytes)
-                    x |= (uint32_t)(SIZE == 1 ? __ldg(row + o) : __ldg(reinterpret_cast<const uint16_t*>(row + o)))
-                         << (8 * SIZE * e);
-            }
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + 4 * w), "r"(x) : "memory");
+        for (int e = 0; e < 4 / SIZE; ++e) {
+            const int o = off + 4 * w + e * SIZE;
+            if (live && o < bytes)
+                x |= (uint32_t)(SIZE == 1 ? __ldg(row + o) : __ldg(reinterpret_cast<const uint16_t*>(row + o)))
+                     << (8 * SIZE * e);
         }
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + 4 * w), "r"(x) : "memory");
     }
 }
 
@@ -287,6 +316,18 @@ __device__ __forceinline__ void read_piece(uint32_t (&r)[W], uint32_t src) {
                      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(src) : "memory");
     else
         asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(src) : "memory");
+}
+
+// A piece that starts `bits` into its first word; the word after the piece is
+// at `next`, or zero if negative.
+template <int W>
+__device__ __forceinline__ void read_piece(uint32_t (&r)[W], uint32_t src, int next, uint32_t bits) {
+    uint32_t last;
+    read_piece(r, src);
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(last) : "r"(next < 0 ? src : (uint32_t)next) : "memory");
+    if (next < 0) last = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) r[w] = __funnelshift_r(r[w], w + 1 < W ? r[w + 1] : last, bits);
 }
 
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -354,6 +395,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
     __shared__ float sm_o[kDecodeWarps][8 * NT][16 * S::JC + 2];
     // scales of the key and value rows of a tile and the next
     __shared__ float sm_s[2][kDecodeWarps][2][K::code ? TOK : 1];
+    __shared__ int sm_into[2][kDecodeWarps][ROWS == ROWS_BYTES ? TOK : 1];       // bytes from a word to a row's start
     __shared__ long long sm_sum[kDecodeWarps];
     __shared__ int sm_at[3];
 
@@ -362,7 +404,11 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
     constexpr int STEP = kDecodeWarps * TOK;
     const int bytes = a.d * S::size;
     const int64_t pool_rows = (int64_t)a.c.pages * a.hk * a.c.page;      // rows of one model's pool
-    const bool words = ((bytes | reinterpret_cast<uintptr_t>(a.c.k) | reinterpret_cast<uintptr_t>(a.c.v)) & 3) == 0;
+    const int lowest = (bytes | (int)reinterpret_cast<uintptr_t>(a.c.k) | (int)reinterpret_cast<uintptr_t>(a.c.v)) & 7;
+    const int grain = lowest == 0 ? 8 : (lowest == 4 ? 4 : 1);           // alignment of every row
+    // ROWS_ANY, ROWS_BYTES: the places that rows reach into; 65536 / live_places, rounded up
+    const int live_places = (bytes + (ROWS == ROWS_BYTES ? (bytes % 2 ? 3 : 2) : 0) + 15) / 16;
+    const int per_place = (65535 + live_places) / live_places;
     const int sequences = a.n * a.b, per_seq = a.hk * a.tiles;           // per_seq: segments of a sequence
     if (!a.in_turn) sm100::grid_dep_launch_dependents();                 // the join waits for this grid's end by itself
 
@@ -476,12 +522,36 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
     auto copy_rows = [&](int place, const void* pages, const Slots& x) {
         const uint8_t* base = static_cast<const uint8_t*>(pages) + x.model * pool_rows * bytes;
         const uint32_t dst = mine + place * S::unit;
-        if (x.run) {
+        if constexpr (ROWS < ROWS_16) {
+            auto one = [&](int n, auto copy) {
+                const int row = n * per_place >> 16, p = n - row * live_places;
+                int r = __shfl_sync(0xffffffffu, x.row[0], row & 31);
+                if constexpr (S::NR > 1) {
+                    const int r1 = __shfl_sync(0xffffffffu, x.row[1], row & 31);
+                    if (row >= 32) r = r1;
+                }
+                if (row < TOK) copy(dst + S::at(row, p), base + (int64_t)max(r, 0) * bytes, p * 16, r >= 0);
+            };
+            // loops, as their unrolled code was more than the instruction cache holds
+            if (ROWS == ROWS_ANY && S::size < 4 && grain < 4) {
+#pragma unroll 1
+                for (int n = lane; n < TOK * live_places + lane; n += 32)
+                    one(n, [&](uint32_t to, const uint8_t* row, int off, bool live) {
+                        if constexpr (S::size < 4) copy_elements<S::size>(to, row, off, bytes, live);
+                    });
+            } else {
+#pragma unroll 4
+                for (int n = lane; n < TOK * live_places + lane; n += 32)
+                    one(n, [&](uint32_t to, const uint8_t* row, int off, bool live) {
+                        copy_place<ROWS>(to, row, off, bytes, grain, live);
+                    });
+            }
+        } else if (x.run) {
             const uint8_t* from = base + (int64_t)__shfl_sync(0xffffffffu, x.row[0], 0) * bytes;
 #pragma unroll
             for (int j = 0; j < S::copies; ++j) {
                 const int n = j * 32 + lane, row = n / S::places, p = n % S::places;
-                copy_place<S::size, ROWS>(dst + S::at(row, p), from + row * bytes, p * 16, bytes, words, true);
+                copy_place<ROWS>(dst + S::at(row, p), from + row * bytes, p * 16, bytes, grain, true);
             }
         } else {
 #pragma unroll
@@ -489,7 +559,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
                 const int n = j * 32 + lane, row = n / S::places, p = n % S::places;
                 // the register that holds the row's slot is known at compile time, its lane is not
                 const int r = __shfl_sync(0xffffffffu, x.row[S::NR == 1 ? 0 : (j * 32 / S::places) >> 5], row & 31);
-                copy_place<S::size, ROWS>(dst + S::at(row, p), base + (int64_t)max(r, 0) * bytes, p * 16, bytes, words,
+                copy_place<ROWS>(dst + S::at(row, p), base + (int64_t)max(r, 0) * bytes, p * 16, bytes, grain,
                                           r >= 0);
             }
         }
@@ -506,6 +576,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
             seen[r] = __ballot_sync(0xffffffffu, x.row[r] >= 0);
             run = run && x.row[r] == first + t;
             if (x.row[r] == -2) raise_device_error(a.err, DEV_ERR_INDEX);
+            if constexpr (ROWS == ROWS_BYTES)
+                sm_into[turn][warp][t] = (int)(((uint32_t)pool + (uint32_t)max(x.row[r], 0)) * (uint32_t)bytes & 3);
             if constexpr (K::code) {
                 const int64_t at = pool + (x.row[r] < 0 ? 0 : x.row[r]);
                 const int n = x.row[r] >= 0 ? 4 : 0;
@@ -521,6 +593,15 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
         copy_rows(place, a.c.k, x);
     };
     auto copy_v = [&](int place, const Slots& x) { copy_rows(place, a.c.v, x); };
+
+    if constexpr (ROWS < ROWS_16) {          // zeros in the places that no row reaches
+#pragma unroll 1
+        for (int u = 0; u < S::units; ++u)
+#pragma unroll 1
+            for (int o = 16 * lane; o < S::unit / kDecodeWarps; o += 512)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(mine + u * S::unit + o), "r"(0) : "memory");
+        __syncwarp();
+    }
 
     Slots x1, x2;                            // slots of the next step and of the one after it
     uint32_t seen[2][S::NR];                 // tokens that are there, of the current step and the next
@@ -557,7 +638,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
             const int ch = (p * 4 + c) * S::KD;
 #pragma unroll
             for (int e = 0; e < S::KD; ++e) x[p][e] = 0.f;
-            if (ROWS != ROWS_ANY && a.q_vec) {
+            if (ROWS >= ROWS_16 && a.q_vec) {
                 if (h < heads && ch < a.d) load_in16<S::KD>(a.q, at + ch, a.dtype, x[p]);
             } else {
 #pragma unroll
@@ -599,6 +680,9 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
     float acc[NT][DP / 16][4];
     float m[NT][2], l[NT][2];
 
+    // ROWS_BYTES: bytes into a word at which the lane's rows of K and V start, 2 bits each
+    uint32_t k_into = 0, v_into = 0;
+
     // S^T += K q^T over the pieces in registers
     float s[NT][MT][4];
     auto scores = [&](int place) {
@@ -611,7 +695,14 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
 #pragma unroll
             for (int p = 0; p < S::KB; ++p)
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) read_piece(batch[mt][p][hf], from + S::at(16 * mt + 8 * hf + g, (p0 + p) * 4 + c));
+                for (int hf = 0; hf < 2; ++hf) {
+                    const int row = 16 * mt + 8 * hf + g, at = (p0 + p) * 4 + c;
+                    if constexpr (ROWS == ROWS_BYTES)
+                        read_piece(batch[mt][p][hf], from + S::at(row, at),
+                                   at + 1 < S::places ? (int)(from + S::at(row, at + 1)) : -1,
+                                   8 * (k_into >> 2 * (2 * mt + hf) & 3));
+                    else read_piece(batch[mt][p][hf], from + S::at(row, at));
+                }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -779,8 +870,16 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
                 for (int t = 0; t < 4; ++t) {
                     // the k index of lane c: tokens 2c, 2c + 1, 2c + 8, 2c + 9; tf32 c, c + 4, c + 8, c + 12
                     const int row = 16 * mt + (K::f32 ? c + 4 * t : 2 * c + (t & 1) + 8 * (t >> 1));
-                    if constexpr (S::VW == 4) read_piece(batch[mt][p][t], from + S::at(row, (p0 + p) * 8 + g));
-                    else read_piece(batch[mt][p][t], from + S::at(row, (p0 + p) * 4 + g / 2) + g % 2 * 8);
+                    // the 16-byte place, and the half in it
+                    const int at = S::VW == 4 ? (p0 + p) * 8 + g : (p0 + p) * 4 + g / 2, half = S::VW == 4 ? 0 : g % 2 * 8;
+                    const uint32_t src = from + S::at(row, at) + half;
+                    if constexpr (ROWS == ROWS_BYTES)
+                        read_piece(batch[mt][p][t], src,
+                                   S::VW == 2 && half == 0 ? (int)(src + 8)
+                                   : at + 1 < S::places    ? (int)(from + S::at(row, at + 1))
+                                                           : -1,
+                                   8 * (v_into >> 2 * (4 * mt + t) & 3));
+                    else read_piece(batch[mt][p][t], src);
                 }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -959,6 +1058,19 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
                         vt[mt][hf] = sm_s[turn][warp][1][16 * mt + 8 * hf + g];
                     }
             }
+            if constexpr (ROWS == ROWS_BYTES) {
+                k_into = v_into = 0;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf)
+                        k_into |= (uint32_t)sm_into[turn][warp][16 * mt + 8 * hf + g] << 2 * (2 * mt + hf);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+                        v_into |= (uint32_t)sm_into[turn][warp][16 * mt + 2 * c + (t & 1) + 8 * (t >> 1)]
+                                  << 2 * (4 * mt + t);
+                }
+            }
             uint32_t now[S::NR], any = 0;
 #pragma unroll
             for (int r = 0; r < S::NR; ++r) now[r] = seen[0][r], any |= now[r], seen[0][r] = seen[1][r];
@@ -1037,18 +1149,27 @@ inline int decode_places(int d, int fmt, int nt) {
 
 template <int KIND, bool SPLITQ>
 int launch_decode(const DecodeArgs& a, cudaStream_t st) {
-    const bool aligned = (a.d * Kind<KIND>::size) % 16 == 0 && aligned16(a.c.k) && aligned16(a.c.v);
-    #define WIDEK_DECODE(DP, NT)                                                             \
-    return !aligned    ? launch_decode_shape<KIND, DP, NT, ROWS_ANY, SPLITQ>(a, st)      \
-           : a.d == DP ? launch_decode_shape<KIND, DP, NT, ROWS_FULL, SPLITQ>(a, st)     \
-                       : launch_decode_shape<KIND, DP, NT, ROWS_16, SPLITQ>(a, st)
-    if constexpr (KIND != DK_F32) {
-        if (a.nt == 2 && a.d <= 64) WIDEK_DECODE(64, 2);
-        if (a.nt == 2) WIDEK_DECODE(128, 2);
+    const int bytes = a.d * Kind<KIND>::size;
+    const bool aligned = bytes % 16 == 0 && aligned16(a.c.k) && aligned16(a.c.v);
+    // rows that start inside a word, with room for the bytes before them
+    const int most = (a.d <= 64 ? 64 : (a.d <= 128 ? 128 : 256)) * Kind<KIND>::size - (bytes % 2 ? 3 : 2);
+    const bool inside = bytes % 4 != 0 && bytes <= most &&
+                        ((reinterpret_cast<uintptr_t>(a.c.k) | reinterpret_cast<uintptr_t>(a.c.v)) & 3) == 0;
+#define WIDEK_DECODE(DP, NT)                                                                 \
+    {                                                                                        \
+        if constexpr (KIND != DK_F32)                                                        \
+            if (inside) return launch_decode_shape<KIND, DP, NT, ROWS_BYTES, SPLITQ>(a, st); \
+        return !aligned    ? launch_decode_shape<KIND, DP, NT, ROWS_ANY, SPLITQ>(a, st)      \
+               : a.d == DP ? launch_decode_shape<KIND, DP, NT, ROWS_FULL, SPLITQ>(a, st)     \
+                           : launch_decode_shape<KIND, DP, NT, ROWS_16, SPLITQ>(a, st);      \
     }
-    if (a.d <= 64) WIDEK_DECODE(64, 1);
-    if (a.d <= 128) WIDEK_DECODE(128, 1);
-    WIDEK_DECODE(256, 1);
+    if constexpr (KIND != DK_F32) {
+        if (a.nt == 2 && a.d <= 64) WIDEK_DECODE(64, 2)
+        if (a.nt == 2) WIDEK_DECODE(128, 2)
+    }
+    if (a.d <= 64) WIDEK_DECODE(64, 1)
+    if (a.d <= 128) WIDEK_DECODE(128, 1)
+    WIDEK_DECODE(256, 1)
 #undef WIDEK_DECODE
 }
 

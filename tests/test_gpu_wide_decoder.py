@@ -364,6 +364,32 @@ def test_decode_attention(shape, dtype, fmt):
     no_device_error()
 
 
+@pytest.mark.parametrize("off", [0, 1, 2, 4])
+@pytest.mark.parametrize("dtype,fmt,d", [(BF16, I8, 138), (F32, E4M3, 138), (F16, E4M3, 62), (BF16, I8, 61), (BF16, I8, 63),
+                                         (F32, I8, 125), (BF16, E4M3, 127), (BF16, I8, 253), (F16, E4M3, 255), (F16, I8, 100),
+                                         (BF16, E4M3, 24), (BF16, BF16, 31), (F16, F16, 127), (BF16, BF16, 255),
+                                         (BF16, BF16, 68), (F32, F32, 61)])
+def test_decode_rows_of_any_size_and_place(dtype, fmt, d, off):
+    """Rows that start at any byte, in pools that start `off` elements into
+    their storage."""
+    n, b, hq, hk, page, longest = 2, 3, 12, 1, 20, 310
+    gen = torch.Generator().manual_seed(d + off)
+    lengths = torch.randint(1, longest + 1, (n, b), generator=gen, dtype=torch.int32)
+    lengths[1, 1] = longest
+    cache = fill(empty_cache(n, b, hk, d, longest, page, fmt, gen), lengths, gen)
+    moved = []
+    for x in (cache.k, cache.v):
+        flat = torch.empty(x.numel() + 8, device=DEV, dtype=x.dtype)
+        moved.append(flat[off:off + x.numel()].view(x.shape))
+        moved[-1].copy_(x)
+    cache = wc.WidePagedCache(*moved, cache.table, cache.k_scale, cache.v_scale)
+    q = torch.randn(n, b, hq, d, generator=gen).to(dtype).to(DEV)
+    out = ops.decode_attention(q, cache, lengths.to(DEV))
+    want, mag, reach = R.decode(q, cache, lengths)
+    R.assert_within(out, want, R.decode_bound(want, mag, reach, d, dtype))
+    no_device_error()
+
+
 @pytest.mark.parametrize("window", [1, 15, 16, 17, 64, 5000])
 @pytest.mark.parametrize("fmt", [BF16, I8])
 def test_decode_window_and_empty_sequences(window, fmt):
