@@ -26,7 +26,7 @@
 // the weights are folded into the angles' coefficients, fp32 arithmetic runs
 // two to an instruction, and codes and values change form by byte permutes.
 // Measured (B200, floor at the measured copy rate): norm + rotation of 168 M
-// bf16 values 135 us (103), its backward over 84 M 119 us (77), int8 write of
+// bf16 values 137 us (103), its backward over 84 M 118 us (77), int8 write of
 // 268 M 183 us (124), read 127 us (125).
 #include "paged_cache.cuh"
 
