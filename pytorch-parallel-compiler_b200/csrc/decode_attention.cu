@@ -183,6 +183,9 @@ extern "C" int widek_decode_attention_fwd(const void* q, const void* kc, const v
     int rc = decode_args(a, what, geom, cgeom, window, fmt);
     if (rc != WIDEK_OK) return rc;
     if (dtype_size(dtype) == 0) return set_error(WIDEK_ERR_INVALID, "%s: unknown dtype code %d", what, dtype);
+    // their kernels hold more and leave room for two blocks, not three (a third
+    // of the line would come in a second wave)
+    if (dtype == WIDEK_F32 && cache_fmt_8bit(fmt)) a.blocks = std::min(a.blocks, 2 * sm_count(current_device()));
     rc = cache_args(a.c, what, const_cast<void*>(kc), const_cast<void*>(vc), const_cast<float*>(ks),
                     const_cast<float*>(vs), table, cgeom, (int64_t)a.n * a.b, a.hk, a.d, fmt, dtype);
     if (rc != WIDEK_OK) return rc;

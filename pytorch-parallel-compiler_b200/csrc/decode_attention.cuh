@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, c = lane & 3;
     constexpr int STEP = kDecodeWarps * TOK;
-    const int bytes = a.d * S::size;
+    const int bytes = ROWS == ROWS_FULL ? S::row_bytes : a.d * S::size;
     const int64_t pool_rows = (int64_t)a.c.pages * a.hk * a.c.page;      // rows of one model's pool
     const int lowest = (bytes | (int)reinterpret_cast<uintptr_t>(a.c.k) | (int)reinterpret_cast<uintptr_t>(a.c.v)) & 7;
     const int grain = lowest == 0 ? 8 : (lowest == 4 ? 4 : 1);           // alignment of every row
@@ -1148,7 +1148,8 @@ inline int decode_step(int d, int fmt) {
     return kDecodeWarps * 16 * (bytes >= 512 ? 1 : (bytes == 256 ? 2 : 256 / bytes));
 }
 
-// Blocks of an SM, as DecodeShape has them (fp32 queries over codes: 2, not 3).
+// Blocks of an SM, as DecodeShape has them (for fp32 queries over codes the
+// entry takes 2).
 inline int decode_places(int d, int fmt, int nt) {
     const int bytes = (d <= 64 ? 64 : (d <= 128 ? 128 : 256)) * (int)cache_fmt_size(fmt);
     return bytes > 512 ? 1 : (bytes >= 256 || nt == 2 || d > 128 ? 2 : 3);
