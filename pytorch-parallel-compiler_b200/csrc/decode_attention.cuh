@@ -55,9 +55,9 @@
 //
 // Measured (B200; floor at the measured copy rate): 1.6 GB of bf16 pages, 128
 // ragged sequences, 32 over 8 heads of 128: 275 us (245). 411 MB of e4m3 pages,
-// 256 sequences, 16 over 4 heads: 93 us (63); bound by instructions, of which
+// 256 sequences, 16 over 4 heads: 89 us (63); bound by instructions, of which
 // the codes' conversion for the second product is the largest part. One int8
-// sequence of 131007 tokens, 16 over 2 heads: 25 us (10.6), bound by the chain
+// sequence of 131007 tokens, 16 over 2 heads: 24 us (10.6), bound by the chain
 // of loads at a block's start and end. fp32, window 511, heads of 84: 17 us (2).
 #pragma once
 
