@@ -648,10 +648,11 @@ inline bool strides_fit(const Strides& s, int vec) {
     return s.n % vec == 0 && s.b % vec == 0 && s.t % vec == 0 && s.h % vec == 0;
 }
 
-// Widest vector (elements) that every row address allows: 16 bytes, else 2
-// elements, else 1. The halves of a rotation have to start on one too.
+// Widest vector (elements) that every row address allows: 16 bytes, else 4 or 2
+// elements, else 1. The halves of a rotation have to start on one too (bf16
+// heads of 96 with 24 channels turned, 40 M values: 69 us with 4, 192 with 2).
 int row_vec(const RowArgs& a, size_t esz, std::initializer_list<const void*> dense, bool cache_same) {
-    for (int vec : {(int)(16 / esz), 2}) {
+    for (int vec : {(int)(16 / esz), 4, 2}) {
         bool ok = a.d % vec == 0 && (a.rot / 2) % vec == 0;
         ok = ok && (!a.q || (aligned_to(a.q, vec * esz) && strides_fit(a.sq, vec)));
         ok = ok && (!a.k || (aligned_to(a.k, vec * esz) && strides_fit(a.sk, vec)));
@@ -702,10 +703,12 @@ int row_args(RowArgs& a, const char* what, const int64_t* g, int pos64) {
 // took 228, 194 and 193 us where 4 took 145, at 168 M values), one in the
 // narrow paths, whose rows take more registers, and where there are so few
 // rows that one each does not fill the GPU (a decoder step of 6144 rows: 4.8
-// us, not 7.2).
+// us, not 7.2). 2 with vectors of 4 16-bit channels, which rotations of 8 r + 4
+// pairs take.
 constexpr int kHeadsAtOnce = 4;
 
 int heads_at_once(const RowArgs& a, int vec, size_t esz, int sides) {
+    if (vec == 4 && esz == 2) return 2;
     if (vec != (int)(16 / esz)) return 1;
     const double lanes = (double)a.n * a.b * a.t * ((double)a.hq + (double)sides * a.hk) * (1 << lanes_log2(a.d, vec));
     return lanes > 2048.0 * sm_count(current_device()) ? kHeadsAtOnce : 1;
@@ -744,6 +747,7 @@ struct RowLaunch {
         const unsigned blocks = (a.units + per - 1) / per;
         if (vec == W && hpt == H) rows_kernel<T, W, 1, H, OUT, ROPE, INTER><<<blocks, kThreads, 0, st>>>(a);
         else if (vec == W) rows_kernel<T, W, 1, 1, OUT, ROPE, INTER><<<blocks, kThreads, 0, st>>>(a);
+        else if (W > 4 && vec == 4) rows_kernel<T, 4, 1, (W > 4 ? 2 : 1), OUT, ROPE, INTER><<<blocks, kThreads, 0, st>>>(a);
         else if (vec == 2) rows_kernel<T, 2, 2, 1, OUT, ROPE, INTER><<<blocks, kThreads, 0, st>>>(a);
         else rows_kernel<T, 1, 4, 1, OUT, ROPE, INTER><<<blocks, kThreads, 0, st>>>(a);
     }
@@ -771,6 +775,7 @@ struct ReadLaunch {
         const unsigned blocks = (a.units + per - 1) / per;
         if (vec == W && hpt > 1) cache_read_kernel<T, W, 1, kHeadsAtOnce, IN><<<blocks, kThreads, 0, st>>>(a);
         else if (vec == W) cache_read_kernel<T, W, 1, 1, IN><<<blocks, kThreads, 0, st>>>(a);
+        else if (W > 4 && vec == 4) cache_read_kernel<T, 4, 1, (W > 4 ? 2 : 1), IN><<<blocks, kThreads, 0, st>>>(a);
         else if (vec == 2) cache_read_kernel<T, 2, 2, 1, IN><<<blocks, kThreads, 0, st>>>(a);
         else cache_read_kernel<T, 1, 4, 1, IN><<<blocks, kThreads, 0, st>>>(a);
         return check_launch("widek_cache_read_fwd");
@@ -792,7 +797,7 @@ int launch_rows_fmt(const RowArgs& a, int vec, int hpt, const char* what, int fm
 
 constexpr int kGradBlocks = 444;  // of the backward over all models, 3 for each SM: twice as many cost the join what they gave
 constexpr int kGradHeads = 2;     // heads at once in the backward, whose rows take twice the registers
-constexpr int grad_heads(int vec, size_t esz) { return vec == (int)(16 / esz) ? kGradHeads : 1; }
+constexpr int grad_heads(int vec, size_t) { return vec >= 4 ? kGradHeads : 1; }
 
 // Blocks per model of the backward: about three blocks for each SM over all
 // models and both sides, none with fewer units than its groups of lanes.
@@ -819,6 +824,7 @@ struct GradLaunch {
     void go(unsigned blocks) {
         constexpr int W = 16 / sizeof(T);
         if (vec == W) rope_bwd_kernel<T, W, 1, grad_heads(W, sizeof(T)), INTER><<<blocks, kThreads, 0, st>>>(g);
+        else if (W > 4 && vec == 4) rope_bwd_kernel<T, 4, 1, kGradHeads, INTER><<<blocks, kThreads, 0, st>>>(g);
         else if (vec == 2) rope_bwd_kernel<T, 2, 2, 1, INTER><<<blocks, kThreads, 0, st>>>(g);
         else rope_bwd_kernel<T, 1, 4, 1, INTER><<<blocks, kThreads, 0, st>>>(g);
     }
