@@ -161,6 +161,18 @@ int decode_args(DecodeArgs& a, const char* what, const int64_t* g, const int64_t
 
 int64_t part_rows(const DecodeArgs& a) { return a.in_turn ? 0 : (int64_t)a.blocks * 2 * 8 * a.nt; }
 
+// Totals of chains, where the table has room for segments of more than one.
+int64_t done_floats(const DecodeArgs& a, const int64_t* cgeom) {
+    const int dp = a.d <= 64 ? 64 : (a.d <= 128 ? 128 : 256);
+    const bool more = (double)cgeom[1] * (double)cgeom[2] > (double)kChainTokens * kDecodeWarps;
+    return a.fmt != WIDEK_F32 && more ? (int64_t)a.blocks * a.nt * (dp / 4 + 2) * 32 * kDecodeWarps : 0;
+}
+
+int64_t workspace_bytes_of(const DecodeArgs& a, const int64_t* cgeom) {
+    return part_rows(a) * (int64_t)(sizeof(float2) + a.d * sizeof(float)) +
+           done_floats(a, cgeom) * (int64_t)sizeof(float);
+}
+
 }  // namespace
 }  // namespace widek
 
@@ -170,7 +182,7 @@ extern "C" int64_t widek_decode_attention_workspace(const int64_t* geom, const i
                                                     int fmt) {
     DecodeArgs a;
     if (decode_args(a, "widek_decode_attention_workspace", geom, cgeom, window, fmt) != WIDEK_OK) return -1;
-    return part_rows(a) * (int64_t)(sizeof(float2) + a.d * sizeof(float));
+    return workspace_bytes_of(a, cgeom);
 }
 
 extern "C" int widek_decode_attention_fwd(const void* q, const void* kc, const void* vc, const float* ks,
@@ -191,12 +203,13 @@ extern "C" int widek_decode_attention_fwd(const void* q, const void* kc, const v
     if (rc != WIDEK_OK) return rc;
     if (a.n == 0 || a.b == 0 || a.d == 0) return WIDEK_OK;
     if (!q || !lengths || !out) return set_error(WIDEK_ERR_INVALID, "%s: null pointer", what);
-    const int64_t rows = part_rows(a), need = rows * (int64_t)(sizeof(float2) + a.d * sizeof(float));
+    const int64_t rows = part_rows(a), need = workspace_bytes_of(a, cgeom);
     if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 7)))
         return set_error(WIDEK_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed", what,
                          (long long)workspace_bytes, (long long)need);
     a.part_ml = static_cast<float2*>(workspace);
     a.part_o = reinterpret_cast<float*>(a.part_ml + rows);
+    a.done = a.part_o + rows * a.d;
     a.q = q, a.lengths = lengths, a.out = out, a.len64 = len64, a.dtype = dtype;
     a.scale_log2 = (float)(scale * 1.4426950408889634);
     const int64_t in16 = 16 / (int64_t)dtype_size(dtype);

@@ -51,7 +51,12 @@
 // row multiplies its score; that of a value row goes into its weight, whose
 // product p vs has no fixed range: V and the weights meet in bf16, which has
 // fp32's, in three pieces where the result is fp32. The tensor core's sums
-// round towards zero: fp32 results take them in short chains, added in fp32.
+// round towards zero: fp32 results take them in short chains, added in fp32,
+// and 16-bit ones in chains of 1024 tokens a warp, whose totals lie in the
+// workspace meanwhile. (In one chain, 131072 values of one sign lost 1.8e-4 of
+// their sum; 6e-6 so. Short chains for 16-bit results, as the adds and the
+// registers of more products under way, cost 4 to 9 % with 8-bit caches or two
+// head tiles; totals in local memory 4 to 6 % even where no chain was full.)
 //
 // Measured (B200; floor at the measured copy rate): 1.6 GB of bf16 pages, 128
 // ragged sequences, 32 over 8 heads of 128: 275 us (245). 411 MB of e4m3 pages,
@@ -74,6 +79,7 @@ struct DecodeArgs {
     void* out;
     float* part_o;               // [blocks, 2, 8 NT, d] partial outputs (relative to their own maximum)
     float2* part_ml;             // [blocks, 2, 8 NT] maximum and sum
+    float* done;                 // [blocks, NT (channels / 4 + 2), threads] totals of chains that are done
     int64_t q_n, q_b, q_h, len_n, len_b;
     int n, b, hq, hk, d, group, len64, window, dtype, fmt;
     int nt, tiles, step;         // 8 nt query heads of a segment, tiles of a group, tokens of a step
@@ -85,6 +91,7 @@ struct DecodeArgs {
 };
 
 constexpr int kDecodeWarps = 4;
+constexpr int kChainTokens = 1024;           // of a warp in one chain of tensor-core sums of a 16-bit result
 
 // Visible tokens of sequence nb.
 struct DecodeRange {
@@ -388,6 +395,8 @@ struct DecodeShape {
     static constexpr int blocks =                                           // of an SM
         row_bytes > 512 ? 1 : (row_bytes >= 256 || NT == 2 || SPLITQ || DP == 256 ? 2 : 3);
     static constexpr int JC = DP > 64 ? 2 : 1;                              // 16-channel tiles joined at a time
+    static constexpr bool chains = !Kind<KIND>::f32 && !SPLITQ;             // sums in long chains
+    static constexpr int chain = kChainTokens / TOK;                        // and their steps
 };
 
 template <int KIND, int DP, int NT, int ROWS, bool SPLITQ>
@@ -686,6 +695,31 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
 
     float acc[NT][DP / 16][4];
     float m[NT][2], l[NT][2];
+
+    // acc += the totals of the segment's chains before (none if `first`), which
+    // are relative to the maximum they had; `keep`: as the new totals.
+    auto add_done = [&](bool first, bool keep) {
+        constexpr int threads = 32 * kDecodeWarps;
+        float* held = a.done + (int64_t)blockIdx.x * (NT * (DP / 4 + 2) * threads) + threadIdx.x;
+#pragma unroll
+        for (int t = 0; t < NT; ++t, held += (DP / 4 + 2) * threads) {
+            float f[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                f[e] = first ? 0.f : ex2(held[(DP / 4 + e) * threads] - (m[t][e] == -INFINITY ? 0.f : m[t][e]));
+                if (keep) held[(DP / 4 + e) * threads] = m[t][e];
+            }
+#pragma unroll
+            for (int j = 0; j < DP / 16; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float* at = held + (4 * j + e) * threads;
+                    const float x = first ? acc[t][j][e] : fmaf(*at, f[e & 1], acc[t][j][e]);
+                    if (keep) *at = x;
+                    acc[t][j][e] = keep ? 0.f : x;
+                }
+        }
+    };
 
     // ROWS_BYTES: bytes into a word at which the lane's rows of K and V start, 2 bits each
     uint32_t k_into = 0, v_into = 0;
@@ -1052,67 +1086,76 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
             l[t][0] = l[t][1] = 0.f;
         }
         const int entered = at.pos;
-        do {
-            copy_wait<S::units - 1>();
-            __syncwarp();                        // what the other lanes copied
-            float kt[MT][2], vt[MT][2];
-            if constexpr (K::code) {
+        bool first = true, more = false;
+        do {                                     // a chain of sums
+            const int stop = S::chains ? min(at.len, at.pos + S::chain * STEP) : at.len;
+            do {
+                copy_wait<S::units - 1>();
+                __syncwarp();                        // what the other lanes copied
+                float kt[MT][2], vt[MT][2];
+                if constexpr (K::code) {
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                    for (int hf = 0; hf < 2; ++hf) {
-                        kt[mt][hf] = sm_s[turn][warp][0][16 * mt + 8 * hf + g];
-                        vt[mt][hf] = sm_s[turn][warp][1][16 * mt + 8 * hf + g];
-                    }
-            }
-            if constexpr (ROWS == ROWS_BYTES) {
-                k_into = v_into = 0;
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-                    for (int hf = 0; hf < 2; ++hf)
-                        k_into |= (uint32_t)sm_into[turn][warp][16 * mt + 8 * hf + g] << 2 * (2 * mt + hf);
-#pragma unroll
-                    for (int t = 0; t < 4; ++t)
-                        v_into |= (uint32_t)sm_into[turn][warp][16 * mt + 2 * c + (t & 1) + 8 * (t >> 1)]
-                                  << 2 * (4 * mt + t);
+                        for (int hf = 0; hf < 2; ++hf) {
+                            kt[mt][hf] = sm_s[turn][warp][0][16 * mt + 8 * hf + g];
+                            vt[mt][hf] = sm_s[turn][warp][1][16 * mt + 8 * hf + g];
+                        }
                 }
-            }
-            uint32_t now[S::NR], any = 0;
+                if constexpr (ROWS == ROWS_BYTES) {
+                    k_into = v_into = 0;
 #pragma unroll
-            for (int r = 0; r < S::NR; ++r) now[r] = seen[0][r], any |= now[r], seen[0][r] = seen[1][r];
-            const int second = S::units == 3 && place == 2 ? 0 : place + 1;
-            if (any) {
-                clear_scores();
-                scores(place);
-            }
-            __syncwarp();                        // all lanes have read the unit
-            if constexpr (S::units == 3) copy_v(place, x1);
-            else copy_k(place, 0, x1, seen[0]);
-            copy_commit();
-            if (any) {
-                softmax(now, kt, vt);
-                turn_weights();
-            }
-            copy_wait<S::units - 1>();
-            __syncwarp();
-            if (any) values(second);
-            __syncwarp();
-            if constexpr (S::units == 3) {
-                copy_k(second, turn, x2, seen[1]);
+                    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                        for (int hf = 0; hf < 2; ++hf)
+                            k_into |= (uint32_t)sm_into[turn][warp][16 * mt + 8 * hf + g] << 2 * (2 * mt + hf);
+#pragma unroll
+                        for (int t = 0; t < 4; ++t)
+                            v_into |= (uint32_t)sm_into[turn][warp][16 * mt + 2 * c + (t & 1) + 8 * (t >> 1)]
+                                      << 2 * (4 * mt + t);
+                    }
+                }
+                uint32_t now[S::NR], any = 0;
+#pragma unroll
+                for (int r = 0; r < S::NR; ++r) now[r] = seen[0][r], any |= now[r], seen[0][r] = seen[1][r];
+                const int second = S::units == 3 && place == 2 ? 0 : place + 1;
+                if (any) {
+                    clear_scores();
+                    scores(place);
+                }
+                __syncwarp();                        // all lanes have read the unit
+                if constexpr (S::units == 3) copy_v(place, x1);
+                else copy_k(place, 0, x1, seen[0]);
                 copy_commit();
-                x1 = x2;
-                look_up(x2);
-                turn ^= 1;
-                place = place == 0 ? 2 : place - 1;          // (place + 2) % 3
-            } else {
-                copy_v(second, x1);
-                copy_commit();
-                look_up(x1);
+                if (any) {
+                    softmax(now, kt, vt);
+                    turn_weights();
+                }
+                copy_wait<S::units - 1>();
+                __syncwarp();
+                if (any) values(second);
+                __syncwarp();
+                if constexpr (S::units == 3) {
+                    copy_k(second, turn, x2, seen[1]);
+                    copy_commit();
+                    x1 = x2;
+                    look_up(x2);
+                    turn ^= 1;
+                    place = place == 0 ? 2 : place - 1;          // (place + 2) % 3
+                } else {
+                    copy_v(second, x1);
+                    copy_commit();
+                    look_up(x1);
+                }
+                --at.left;
+                at.pos += STEP;
+            } while (at.pos < stop && at.left > 0);
+            if constexpr (S::chains) {
+                more = at.pos < at.len && at.left > 0;
+                if (more || !first) add_done(first, more);
+                first = false;
             }
-            --at.left;
-            at.pos += STEP;
-        } while (at.pos < at.len && at.left > 0);
+        } while (more);
         finish(entered == at.start && at.pos >= at.len, part);
         part = 1;
         if (at.left > 0) next_segment(at);

@@ -187,3 +187,57 @@ def test_whole_segments_in_turn(dtype, fmt, n, b, longest):
     q = torch.randn(n, b, hk * 2, d, device=DEV, generator=gen).to(dtype)
     assert n * b * hk > 3 * 3 * torch.cuda.get_device_properties(0).multi_processor_count
     check(q, cache, lengths)
+
+
+@pytest.mark.parametrize("dtype,fmt", [(F16, F16), (BF16, BF16), (F16, I8), (F16, E4M3), (F32, F32), (F32, I8)])
+def test_long_sums_of_one_sign_are_not_biased(dtype, fmt):
+    """131072 values of one sign summed by one block: sums that round towards
+    zero would all lose the same way. The mean of the signed relative errors
+    keeps that and averages out the results' own rounding (uniform, at most
+    2^-p: 2^-11 or 2^-8 / sqrt(3 * 16384) here, 2.2e-6 or 1.8e-5, and more than
+    three times that allowed); the weights' pieces allow 2^-16 themselves."""
+    n, b, hk, d, page, held, length = 16, 4, 8, 128, 128, 32, 131072
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    base = 1 + torch.rand(n, 1, hk, 1, d, device=DEV, generator=gen)
+    v = base * (0.9 + 0.2 * torch.rand(n, held, hk, page, d, device=DEV, generator=gen))
+    k = 0.3 * torch.randn(n, held, hk, page, d, device=DEV, generator=gen)
+    table = torch.randint(0, held, (n, b, length // page), device=DEV, generator=gen, dtype=torch.int32)
+    (k, ks), (v, vs) = encode(k, fmt), encode(v, fmt)
+    cache = wc.WidePagedCache(k, v, table, ks, vs)
+    q = torch.randn(n, b, hk, d, device=DEV, generator=gen).to(dtype)
+    lengths = torch.full((n, b), length, device=DEV, dtype=torch.int32)
+    assert steps_of_a_block(cache, lengths, 1) > 500
+    out = ops.decode_attention(q, cache, lengths)
+    wide = lambda x, s: x.double() if s is None else x.double() * s.double().unsqueeze(-1)
+    want = torch.empty(q.shape, device=DEV, dtype=torch.float64)
+    for i in range(n):
+        kk, vv = wide(k[i], None if ks is None else ks[i]), wide(v[i], None if vs is None else vs[i])
+        times = torch.stack([torch.bincount(table[i, j].long(), minlength=held) for j in range(b)]).double()
+        w = torch.exp(torch.einsum('bhd,phtd->bhpt', q[i].double(), kk) / math.sqrt(d)) * times[:, None, :, None]
+        want[i] = torch.einsum('bhpt,phtd->bhd', w, vv) / w.sum((2, 3)).unsqueeze(-1)
+    err = (out.double() - want) / want
+    assert abs(float(err.mean())) <= {F32: 2.0 ** -20, F16: 2.0 ** -16, BF16: 2.0 ** -14}[dtype]
+    # the rounding of one result, and what decode_bound allows the weights
+    assert float(err.abs().max()) <= R.store_ulp(dtype) + 2 * (2.0 ** -20 + (2.0 ** -20 if dtype == F32 else 2.0 ** -16)
+                                                               + (d + 8) * R.U * 4)
+
+
+@pytest.mark.parametrize("d,group", [(64, 2), (128, 1), (128, 12), (256, 2)])
+@pytest.mark.parametrize("dtype,fmt", [(BF16, BF16), (F16, F16), (BF16, I8), (F16, E4M3), (F32, F32)])
+def test_totals_of_chains_follow_the_maximum(dtype, fmt, d, group):
+    """Whole sequences of several thousand tokens in one block, whose keys grow
+    (or shrink) towards the end, so that sums of many steps ago are rescaled."""
+    n, b, hk, page, held = 4, 16, 8, 100, 40
+    gen = torch.Generator(device=DEV).manual_seed(d + group)
+    gain = torch.linspace(0.1, 2.5, held, device=DEV).view(1, held, 1, 1, 1)
+    k = gain * torch.randn(n, held, hk, page, d, device=DEV, generator=gen)
+    v = torch.randn(n, held, hk, page, d, device=DEV, generator=gen)
+    (k, ks), (v, vs) = encode(k, fmt), encode(v, fmt)
+    lengths = torch.randint(9000, 14000, (n, b), device=DEV, generator=gen, dtype=torch.int32)
+    cols = 14000 // page
+    table = torch.randint(0, held, (n, b, cols), device=DEV, generator=gen, dtype=torch.int32).sort(-1).values
+    table[:, ::2] = table[:, ::2].flip(-1)
+    cache = wc.WidePagedCache(k, v, table, ks, vs)
+    q = torch.randn(n, b, hk * group, d, device=DEV, generator=gen).to(dtype)
+    assert steps_of_a_block(cache, lengths, group) > 40
+    check(q, cache, lengths)
