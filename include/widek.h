@@ -649,8 +649,10 @@ WIDEK_API int widek_groupnorm_bwd(const void* x, const void* dy, const void* wei
  *     element strides (model, sequence, token, head) of q, of k and of v, and
  *     (model, sequence, token) of the positions.
  *   positions: int32, or int64 with pos64 = 1; a negative one marks a padding
- *     row (zeros out, nothing written, zero gradient). One past the table or
- *     the cache records WIDEK_DEV_ERR_INDEX and is treated the same way.
+ *     row (zeros out, nothing written, zero gradient). One past the table
+ *     records WIDEK_DEV_ERR_INDEX and is treated the same way; one past the
+ *     cache records it, writes nothing and reads as zeros (queries do not go to
+ *     the cache: theirs come out).
  *   cos, sin: [table_rows, rot / 2] fp32.
  *   Cache: kc, vc [n, pages, hk, page, d] dense in `fmt` (the tensors' dtype,
  *     WIDEK_I8 or WIDEK_E4M3), ks, vs [n, pages, hk, page] fp32 for the 8-bit

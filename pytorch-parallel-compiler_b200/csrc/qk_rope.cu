@@ -10,8 +10,8 @@
 //   gradient  du = dy turned back, dw = sum over rows of du x r, g = du w,
 //             dx = r (g - x r^2 mean(g x))
 // A row whose position is negative is padding: zeros out, nothing written,
-// zero gradient. A position outside the table or the cache records an index
-// error and does the same.
+// zero gradient. A position outside the table records an index error and does
+// the same; one outside the cache records it and writes nothing.
 //
 // Mapping: a power of two of lanes share a row and each lane holds both
 // members of its pairs (vector A at u VEC and vector B at u VEC + R/2; one
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ 
 
     bool keep = pos >= 0;
     const bool rope = ROPE && !is_v;
-    if (rope && pos >= a.table_rows) {
+    if (ROPE && pos >= a.table_rows) {            // for the values as well: a slot gets both sides or neither
         keep = false;
         if (lane == 0) raise_device_error(a.err, DEV_ERR_INDEX);
     }

@@ -1,0 +1,61 @@
+"""GPU tests of the decoder-attention operators and their layer at the edges of
+what they take: positions past a table, caches longer than one, gradients of
+gradients, first calls in unusual modes."""
+import pytest
+import torch
+
+import decoder_ref as R
+import wide_compiler as wc
+from gpu_util import FP32_TOL, no_device_error
+from wide_compiler import _native, ops
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda'
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+I8, E4M3 = torch.int8, torch.float8_e4m3fn
+
+
+def heads(n, b, t, hq, hk, d, dtype, seed):
+    gen = torch.Generator().manual_seed(seed)
+    return [torch.randn(n, b, t, h, d, generator=gen).to(dtype).to(DEV) for h in (hq, hk, hk)]
+
+
+@pytest.mark.parametrize("dtype,fmt", [(BF16, BF16), (F32, I8), (F16, E4M3)])
+def test_fused_write_past_the_rotation_table_writes_neither_side(dtype, fmt):
+    """Inside the cache but past cos / sin: as a padding row, for the key, the
+    value and their scales."""
+    q, k, v = heads(1, 2, 3, 2, 1, 64, dtype, 1)
+    w = torch.ones(1, 64, device=DEV, dtype=dtype)
+    cos, sin = (x.to(DEV) for x in R.tables(4, 64))
+    cache = wc.WidePagedCache.allocate(1, 2, 1, 64, 16, 4, fmt, DEV)
+    for x in (cache.k, cache.v, cache.k_scale, cache.v_scale):
+        if x is not None:
+            x.zero_()
+    pos = torch.tensor([[0, 4, 3], [15, 1, 2]], device=DEV)
+    y = ops.qk_norm_rope_write(q, k, v, w, w, cos, sin, pos, cache)
+    assert _native.device_error() == _native.DEV_ERR_INDEX
+    kr, vr = ops.cache_read(cache, pos, dtype=dtype if fmt != dtype else None)
+    no_device_error()
+    past = (pos >= 4)[None]
+    for x in (y, kr, vr):
+        assert float(x[past].float().abs().max()) == 0.0
+        assert float(x[~past].float().abs().amax((-1, -2)).min()) > 0.0
+    for s in (cache.k_scale, cache.v_scale):
+        if s is not None:
+            assert int((s != 0).sum()) == 4
+
+
+def test_fused_write_past_the_cache_leaves_the_queries():
+    """Past the cache but inside cos / sin: nothing is written, and the
+    queries, which do not go there, come out as elsewhere."""
+    q, k, v = heads(1, 1, 2, 2, 1, 64, BF16, 2)
+    w = torch.ones(1, 64, device=DEV, dtype=BF16)
+    cos, sin = (x.to(DEV) for x in R.tables(32, 64))
+    cache = wc.WidePagedCache.allocate(1, 1, 1, 64, 8, 4, BF16, DEV)
+    cache.k.zero_(), cache.v.zero_()
+    pos = torch.tensor([9, 31], device=DEV)
+    y = ops.qk_norm_rope_write(q, k, v, w, w, cos, sin, pos, cache)
+    assert _native.device_error() == _native.DEV_ERR_INDEX
+    assert torch.equal(y, ops.qk_norm_rope(q, k, w, w, cos, sin, pos)[0])
+    assert float(cache.k.abs().max()) == 0.0 and float(cache.v.abs().max()) == 0.0
+    no_device_error()
