@@ -295,16 +295,23 @@ def causal_attention_t(q: Tensor, k: Tensor, v: Tensor) -> Tensor:
 
 def _norm_rope_t(x: Tensor, weight: Tensor, cos: Tensor, sin: Tensor, positions: Tensor, eps: float,
                  interleaved: bool) -> Tensor:
-    xf = x.float()
-    u = xf * torch.rsqrt((xf * xf).mean(-1, keepdim=True) + eps) * weight.float()[:, None, None, None]
+    # Padding, and positions past the table (which the kernel records as index
+    # errors), read nothing of the table or the row: zeros, also in the gradient.
     pos = positions.long()
-    c, s = cos[pos.clamp(min=0)].unsqueeze(-2), sin[pos.clamp(min=0)].unsqueeze(-2)
+    keep = (pos >= 0) & (pos < cos.shape[0])
+    if cos.shape[0] == 0:
+        cos, sin = cos.new_zeros(1, cos.shape[1]), sin.new_zeros(1, sin.shape[1])
+    at = torch.where(keep, pos, torch.zeros_like(pos))
+    c, s = cos[at].unsqueeze(-2), sin[at].unsqueeze(-2)
+    keep = keep[..., None, None]
+    xf = torch.where(keep, x.float(), torch.ones((), device=x.device))
+    u = xf * torch.rsqrt((xf * xf).mean(-1, keepdim=True) + eps) * weight.float()[:, None, None, None]
     r = 2 * cos.shape[1]
     a, b = (u[..., 0:r:2], u[..., 1:r:2]) if interleaved else (u[..., :r // 2], u[..., r // 2:r])
     a, b = a * c - b * s, b * c + a * s
     turned = torch.stack((a, b), -1).flatten(-2) if interleaved else torch.cat((a, b), -1)
     y = torch.cat((turned, u[..., r:]), -1)
-    return torch.where((pos >= 0)[..., None, None], y, torch.zeros_like(y)).to(x.dtype)
+    return torch.where(keep, y, torch.zeros_like(y)).to(x.dtype)
 
 
 def qk_norm_rope_t(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, cos: Tensor, sin: Tensor,
