@@ -24,12 +24,14 @@ The torch formulations restate, per op, the reference's forward:
 """
 from __future__ import annotations
 
+import contextlib
 import math
 from typing import Any, Callable, List, Optional, Sequence
 
 import torch
 import torch.nn.functional as F
 from torch import Tensor
+from torch.nn.attention import SDPBackend, sdpa_kernel
 
 
 def needs_grad(*objs: Any) -> bool:
@@ -82,6 +84,27 @@ def _rebuild(spec, tensors: Sequence[Tensor]):
     return out
 
 
+def torch_grads(torch_fn: Callable, args: Sequence[Any], needs: Sequence[bool], grads: Sequence[Optional[Tensor]]):
+    """Gradients of ``torch_fn(*args)`` with respect to the floating-point
+    tensors among ``args`` that ``needs`` marks (None for the others). Where a
+    gradient of these is asked for (create_graph: a backward then runs with grad
+    mode on) they carry a graph, by way of aliases, as one argument may have
+    been computed from another, and attention takes the form that has one."""
+    again = torch.is_grad_enabled()
+    with torch.enable_grad(), (sdpa_kernel(SDPBackend.MATH) if again else contextlib.nullcontext()):
+        ins = [a if not isinstance(a, Tensor) else
+               (a.view_as(a) if again else a.detach().requires_grad_(True)) if need and a.is_floating_point() else
+               a.detach() for a, need in zip(args, needs)]
+        out = torch_fn(*ins)
+        outs = out if isinstance(out, tuple) else (out,)
+        pairs = [(o, g) for o, g in zip(outs, grads) if g is not None and o.requires_grad]
+        wanted = [a for a in ins if isinstance(a, Tensor) and a.requires_grad]
+        got = (torch.autograd.grad([o for o, _ in pairs], wanted, [g for _, g in pairs], create_graph=again,
+                                   allow_unused=True) if pairs and wanted else [None] * len(wanted))
+    it = iter(got)
+    return tuple(next(it) if isinstance(a, Tensor) and a.requires_grad else None for a in ins)
+
+
 class Recompute(torch.autograd.Function):
     """forward: ``kernel_fn(*args)``; backward: gradients of
     ``torch_fn(*args)`` with respect to the tensor arguments. Both functions
@@ -100,18 +123,9 @@ class Recompute(torch.autograd.Function):
     @staticmethod
     def backward(ctx, *grads):
         saved = ctx.saved_tensors
-        with torch.enable_grad():
-            inputs = [t.detach().requires_grad_(t.requires_grad and t.is_floating_point()) for t in saved]
-            out = ctx.torch_fn(*_rebuild(ctx.spec, inputs))
-            outs = out if isinstance(out, tuple) else (out,)
-            pairs = [(o, g) for o, g in zip(outs, grads) if g is not None and o.requires_grad]
-            wanted = [t for t in inputs if t.requires_grad]
-            got = torch.autograd.grad([o for o, _ in pairs], wanted, [g for _, g in pairs],
-                                      allow_unused=True) if pairs and wanted else [None] * len(wanted)
-        res, it = [], iter(got)
-        for t in inputs:
-            res.append(next(it) if t.requires_grad else None)
-        return (None, None, None, *res)
+        got = torch_grads(lambda *ts: ctx.torch_fn(*_rebuild(ctx.spec, ts)), saved, [t.requires_grad for t in saved],
+                          grads)
+        return (None, None, None, *got)
 
 
 def run(kernel_fn: Callable, torch_fn: Callable, *args):
@@ -404,6 +418,9 @@ class QkNormRopeFn(torch.autograd.Function):
         from . import ops
         q, k, qw, kw, cos, sin, positions = ctx.saved_tensors
         need = ctx.needs_input_grad
+        if torch.is_grad_enabled():          # a gradient of these gradients is asked for: the kernel's have no graph
+            return torch_grads(qk_norm_rope_t, (q, k, qw, kw, cos, sin, positions, ctx.eps, ctx.interleaved),
+                               (*need[:4], *(False,) * 5), (dyq, dyk))
         grads = ops.qk_norm_rope_bwd(q, k, qw, kw, cos, sin, positions, dyq, dyk, ctx.eps, ctx.interleaved,
                                      need_dw=need[2] or need[3])
         return (*(g if want else None for g, want in zip(grads, need[:4])), None, None, None, None, None)

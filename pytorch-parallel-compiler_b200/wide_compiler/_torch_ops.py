@@ -40,17 +40,7 @@ def _register_autograd(op, torch_fn) -> None:
     def backward(ctx, *grads):
         saved = iter(ctx.saved_tensors)
         args = [next(saved) if k else c for k, c in zip(ctx.kinds, ctx.consts)]
-        with torch.enable_grad():
-            det = [a.detach().requires_grad_(bool(need) and a.is_floating_point()) if isinstance(a, Tensor) else a
-                   for a, need in zip(args, ctx.needs_input_grad)]
-            out = torch_fn(*det)
-            outs = out if isinstance(out, tuple) else (out,)
-            pairs = [(o, g) for o, g in zip(outs, grads) if g is not None and o.requires_grad]
-            wanted = [a for a in det if isinstance(a, Tensor) and a.requires_grad]
-            got = (torch.autograd.grad([o for o, _ in pairs], wanted, [g for _, g in pairs], allow_unused=True)
-                   if pairs and wanted else [None] * len(wanted))
-        it = iter(got)
-        return tuple(next(it) if isinstance(a, Tensor) and a.requires_grad else None for a in det)
+        return _AG.torch_grads(torch_fn, args, ctx.needs_input_grad, grads)
 
     op.register_autograd(backward, setup_context=setup_context)
 

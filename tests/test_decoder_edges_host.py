@@ -2,6 +2,7 @@
 at the edges of what they take."""
 import pytest
 import torch
+from torch.nn.attention import SDPBackend, sdpa_kernel
 
 import decoder_ref as R
 import wide_compiler as wc
@@ -44,3 +45,67 @@ def test_torch_formulation_gradient_of_padding_that_holds_nan():
     dx, dw, dx_amp, dw_amp = R.rope_grad(x.detach(), w.detach(), cos, sin, pos, 1e-6, False, dy)
     R.assert_within(gx, dx, 48 * R.U * dx_amp)
     R.assert_within(gw, dw, (24 + b * t * 2) * R.U * dw_amp)
+
+
+def plain_kernels(monkeypatch):
+    """Stands the launches of norm + rotation in with graph-free formulas."""
+    from wide_compiler import ops
+
+    def forward(*args):
+        with torch.no_grad():
+            return AG.qk_norm_rope_t(*args)
+
+    def backward(q, k, qw, kw, cos, sin, pos, dyq, dyk, eps=1e-6, interleaved=False, need_dw=True):
+        with torch.enable_grad():
+            ins = [x.detach().requires_grad_(True) for x in (q, k, qw, kw)]
+            y = AG.qk_norm_rope_t(*ins, cos, sin, pos, eps, interleaved)
+            return torch.autograd.grad(y, ins, [dyq.detach(), dyk.detach()])
+
+    monkeypatch.setattr(ops, "_qk_norm_rope", forward)
+    monkeypatch.setattr(ops, "qk_norm_rope_bwd", backward)
+    return ops
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_gradient_penalty_through_norm_and_rotation(monkeypatch, shared):
+    """A gradient of a gradient: also where k is computed from q, and where
+    only one output is used."""
+    ops = plain_kernels(monkeypatch)
+    gen = torch.Generator().manual_seed(4)
+    x = torch.randn(2, 2, 3, 2, 8, generator=gen).requires_grad_(True)
+    w = (1 + 0.2 * torch.randn(2, 8, generator=gen)).requires_grad_(True)
+    cos, sin = R.tables(4, 4)
+    pos = torch.tensor([0, -1, 3])
+
+    def penalty(f):
+        q = x * 1.5
+        k = q.tanh() if shared else x[..., :1, :]
+        yq, yk = f(q, k, w, w * 0.5, cos, sin, pos, 1e-6, True)
+        out = (yq ** 3).sum() + ((yk ** 2).sum() if shared else 0)
+        g, = torch.autograd.grad(out, x, create_graph=True)
+        return torch.autograd.grad((g ** 2).sum(), (x, w))
+
+    for got, want in zip(penalty(ops.qk_norm_rope), penalty(AG.qk_norm_rope_t)):
+        torch.testing.assert_close(got, want, rtol=1e-4, atol=1e-5)
+
+
+def test_gradient_penalty_through_the_recomputed_attention(monkeypatch):
+    """ops.causal_attention's backward is the torch formulation's: with a graph
+    where one is asked for."""
+    gen = torch.Generator().manual_seed(5)
+    q, k, v = (torch.randn(1, 2, 5, h, 8, generator=gen).requires_grad_(True) for h in (4, 2, 2))
+
+    def forward(q, k, v):
+        with torch.no_grad():
+            return AG.causal_attention_t(q, k, v)
+
+    def penalty(f):
+        out = f(q, k, v)
+        g = torch.autograd.grad((out ** 2).sum(), (q, k, v), create_graph=True)
+        return torch.autograd.grad(sum((x ** 2).sum() for x in g), (q, k, v))
+
+    got = penalty(lambda *a: AG.run(forward, AG.causal_attention_t, *a))
+    with sdpa_kernel(SDPBackend.MATH):                       # torch's other forms have no second gradient
+        plain = penalty(AG.causal_attention_t)
+    for got, want in zip(got, plain):
+        torch.testing.assert_close(got, want, rtol=1e-4, atol=1e-5)

@@ -59,3 +59,29 @@ def test_fused_write_past_the_cache_leaves_the_queries():
     assert torch.equal(y, ops.qk_norm_rope(q, k, w, w, cos, sin, pos)[0])
     assert float(cache.k.abs().max()) == 0.0 and float(cache.v.abs().max()) == 0.0
     no_device_error()
+
+
+@pytest.mark.grad
+@pytest.mark.parametrize("compiled", [False, True])
+def test_gradient_penalty_through_norm_and_rotation(compiled):
+    """The kernels' outputs, and gradients of gradients as the torch
+    formulation's; first gradients stay the kernel's."""
+    from wide_compiler import _autograd as AG
+    gen = torch.Generator().manual_seed(3)
+    x = torch.randn(2, 2, 5, 3, 64, generator=gen).to(DEV).requires_grad_(True)
+    w = (1 + 0.2 * torch.randn(2, 64, generator=gen)).to(DEV).requires_grad_(True)
+    cos, sin = (t.to(DEV) for t in R.tables(8, 32))
+    pos = torch.tensor([0, 3, -1, 7, 2], device=DEV)
+    call = lambda q, k, w: ops.qk_norm_rope(q, k, w, w * 0.5, cos, sin, pos, 1e-6, True)
+    if compiled:
+        call = torch.compile(call, fullgraph=True, backend="eager")
+    plain = lambda q, k, w: AG.qk_norm_rope_t(q, k, w, w * 0.5, cos, sin, pos, 1e-6, True)
+
+    def penalty(f):
+        yq, yk = f(x * 1.5, x[..., :1, :], w)
+        g, = torch.autograd.grad((yq ** 3).sum() + (yk ** 2).sum(), x, create_graph=True)
+        return torch.autograd.grad((g ** 2).sum(), (x, w))
+
+    for got, want in zip(penalty(call), penalty(plain)):
+        torch.testing.assert_close(got, want, rtol=1e-3, atol=1e-3 * float(want.abs().max()))
+    no_device_error()
