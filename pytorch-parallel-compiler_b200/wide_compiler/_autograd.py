@@ -31,6 +31,7 @@ from typing import Any, Callable, List, Optional, Sequence
 import torch
 import torch.nn.functional as F
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 from torch.nn.attention import SDPBackend, sdpa_kernel
 
 
@@ -341,6 +342,9 @@ def qk_norm_rope_t(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, cos
 # have backward kernels (csrc/backward.cu): their forward runs once, on the
 # kernels, and the backward launches the gradient kernels on the saved
 # tensors instead of re-running a torch formulation.
+# Those gradients have no graph. Where a gradient of them is asked for (grad
+# mode is on in a backward) the torch formulation is differentiated instead, and
+# the batch and group norms refuse.
 # ---------------------------------------------------------------------------
 _KERNEL_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -361,13 +365,15 @@ class LinearFn(torch.autograd.Function):
                 y = ops.linear(x, weight, bias, act)
                 saved = y if act == 1 else None
         ctx.act, ctx.has_bias = act, bias is not None
-        ctx.save_for_backward(x, weight, saved)
+        ctx.save_for_backward(x, weight, bias, saved)
         return y
 
     @staticmethod
     def backward(ctx, dy):
         from . import ops
-        x, weight, saved = ctx.saved_tensors
+        x, weight, bias, saved = ctx.saved_tensors
+        if torch.is_grad_enabled():
+            return torch_grads(linear_t, (x, weight, bias, ctx.act), ctx.needs_input_grad, (dy,))
         dy = dy.to(weight.dtype).contiguous()
         if ctx.act:
             dy = ops.act_bwd(dy, saved, ctx.act)
@@ -394,6 +400,9 @@ class LayerNormFn(torch.autograd.Function):
     def backward(ctx, dy):
         from . import ops
         x, weight = ctx.saved_tensors
+        if torch.is_grad_enabled():          # no gradient depends on the bias
+            return torch_grads(layernorm_t, (x, weight, weight.new_zeros(ctx.bias_shape), ctx.n, ctx.d, ctx.eps),
+                               ctx.needs_input_grad, (dy,))
         dx, dw, db = ops.layernorm_bwd(x, weight, dy.to(x.dtype).contiguous(), ctx.n, ctx.d, ctx.eps,
                                        ctx.needs_input_grad[1], ctx.needs_input_grad[2])
         dw = None if dw is None else dw.view(weight.shape)
@@ -458,6 +467,8 @@ class ActFn(torch.autograd.Function):
     def backward(ctx, dy):
         from . import ops
         saved, = ctx.saved_tensors
+        if torch.is_grad_enabled():          # ReLU of its output has the input's gradient
+            return torch_grads(act_t, (saved, ctx.act), (True, False), (dy,))
         return ops.act_bwd(dy.to(saved.dtype).contiguous(), saved, ctx.act).view(saved.shape), None
 
 
@@ -507,6 +518,7 @@ class BatchNormFn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         from . import ops
         x, weight, rm, rv = ctx.saved_tensors
@@ -531,6 +543,7 @@ class GroupNormFn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         from . import ops
         x, weight = ctx.saved_tensors

@@ -85,3 +85,52 @@ def test_gradient_penalty_through_norm_and_rotation(compiled):
     for got, want in zip(penalty(call), penalty(plain)):
         torch.testing.assert_close(got, want, rtol=1e-3, atol=1e-3 * float(want.abs().max()))
     no_device_error()
+
+
+@pytest.mark.grad
+@pytest.mark.parametrize("act", ['none', 'relu', 'gelu'])
+def test_gradient_penalty_through_a_decoder_layer(act):
+    """Projections, norm + rotation and attention of WideDecoderAttention, and
+    the norm and activation beside it, against their torch formulations."""
+    from wide_compiler import _autograd as AG
+    torch.manual_seed(5)
+    n, b, t, d = 2, 2, 5, 32
+    layer = wc.WideDecoderAttention(n, d, 4, 2, max_positions=8, bias=True).to(DEV)
+    norm = wc.WideLayerNorm(n, d).to(DEV)
+    up = wc.WideLinear(n, d, d).to(DEV)
+    x = torch.randn(n, b, t, d, device=DEV, requires_grad=True)
+    params = [*layer.parameters(), *norm.parameters(), *up.parameters()]
+
+    def ours(x):
+        y = ops.linear(layer(norm(x)), up.weight, up.bias, {'none': 0, 'relu': 1, 'gelu': 2}[act])
+        return y if act == 'none' else ops.unary(y, act)
+
+    def plain(x):
+        h = AG.layernorm_t(x, norm.weight, norm.bias, n, d, norm.eps)
+        qkv = AG.linear_t(h, layer.qkv_weight, layer.qkv_bias)
+        cut = lambda a, c: qkv[..., a * 8:(a + c) * 8].unflatten(-1, (c, 8))
+        q, k = AG.qk_norm_rope_t(cut(0, 4), cut(4, 2), layer.q_norm, layer.k_norm, *layer.rotation(x.device),
+                                 torch.arange(t, device=DEV), layer.eps, False)
+        with torch.nn.attention.sdpa_kernel(torch.nn.attention.SDPBackend.MATH):
+            h = AG.linear_t(AG.causal_attention_t(q, k, cut(6, 2)).flatten(-2), layer.out_weight, layer.out_bias)
+        y = AG.linear_t(h, up.weight, up.bias, {'none': 0, 'relu': 1, 'gelu': 2}[act])
+        return y if act == 'none' else AG.act_t(y, {'relu': 1, 'gelu': 2}[act])
+
+    def penalty(f):
+        g, = torch.autograd.grad((f(x) ** 2).sum(), x, create_graph=True)
+        return torch.autograd.grad((g ** 2).sum(), [x, *params], allow_unused=True)
+
+    for got, want in zip(penalty(ours), penalty(plain)):
+        assert (got is None) == (want is None)
+        if got is not None:
+            torch.testing.assert_close(got, want, rtol=5e-3, atol=2e-3 * float(want.abs().max()) + 1e-6)
+
+
+@pytest.mark.grad
+def test_gradient_penalty_through_batch_and_group_norm_is_refused():
+    for f in (lambda x: ops.groupnorm(x, 2, 2, None, None, 1e-5),
+              lambda x: ops.batchnorm(x, 2, 4, None, None, None, None, True, False, 0.1, 1e-5)):
+        x = torch.randn(2, 3, 4, 5, device=DEV, requires_grad=True)
+        g, = torch.autograd.grad((f(x) ** 3).sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad((g ** 2).sum(), x)
