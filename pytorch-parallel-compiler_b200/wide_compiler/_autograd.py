@@ -31,13 +31,20 @@ from typing import Any, Callable, List, Optional, Sequence
 import torch
 import torch.nn.functional as F
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.nn.attention import SDPBackend, sdpa_kernel
 
 
 def needs_grad(*objs: Any) -> bool:
     """Grad mode is on and some tensor argument (also inside a list/tuple)
-    requires grad."""
+    requires grad. Forward-mode tangents, which no kernel carries on, are
+    refused."""
+    if forward_ad._current_level >= 0:
+        for o in objs:
+            for t in o if isinstance(o, (list, tuple)) else (o,):
+                if isinstance(t, Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                    raise RuntimeError("the wide operators have no forward-mode gradients")
     if not torch.is_grad_enabled():
         return False
     for o in objs:

@@ -109,3 +109,20 @@ def test_gradient_penalty_through_the_recomputed_attention(monkeypatch):
         plain = penalty(AG.causal_attention_t)
     for got, want in zip(got, plain):
         torch.testing.assert_close(got, want, rtol=1e-4, atol=1e-5)
+
+
+def test_forward_mode_tangents_are_refused(monkeypatch):
+    """The kernels have no forward-mode gradients: a tangent was dropped."""
+    import torch.autograd.forward_ad as fwd
+    ops = plain_kernels(monkeypatch)
+    x, w = torch.randn(1, 1, 2, 1, 8), torch.ones(1, 8)
+    cos, sin = R.tables(4, 4)
+    pos = torch.arange(2)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for grad in (False, True):
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                ops.qk_norm_rope(dual, x, w, w, cos, sin, pos)
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                ops.decode_attention(dual[:, :, 0], None, pos[:1])
+        ops.qk_norm_rope(x, x, w, w, cos, sin, pos)
