@@ -54,13 +54,19 @@ class WideDecoderAttention(nn.Module):
             nn.init.xavier_uniform_(self.out_weight[i])
         self._tables = {}                # fp32 whatever the module's type, so not buffers
 
-    def rotation(self, device: torch.device):
-        """cos / sin [max_positions, rotary_dim / 2] in fp32, angles in 64 bits."""
-        if device not in self._tables:
-            i = torch.arange(0, self.rotary_dim, 2, dtype=torch.float64) / max(self.rotary_dim, 1)
-            ang = torch.arange(self.max_positions, dtype=torch.float64)[:, None] * self.theta ** -i[None]
-            self._tables[device] = (torch.cos(ang).float().to(device), torch.sin(ang).float().to(device))
-        return self._tables[device]
+    def rotation(self, device: torch.device, rows: Optional[int] = None):
+        """cos / sin [rows, rotary_dim / 2] in fp32 (rows: max_positions unless
+        given), angles in 64 bits; made once for each use they serve."""
+        key = (device, self.max_positions if rows is None else rows, self.rotary_dim, self.theta)
+        if key not in self._tables:
+            if device.type == 'cuda' and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("WideDecoderAttention: the rotation tables cannot be made while a CUDA graph is "
+                                   "captured: run the layer once before")
+            with torch.inference_mode(False):            # they serve training as well
+                i = torch.arange(0, self.rotary_dim, 2, dtype=torch.float64) / max(self.rotary_dim, 1)
+                ang = torch.arange(key[1], dtype=torch.float64)[:, None] * self.theta ** -i[None]
+                self._tables[key] = (torch.cos(ang).float().to(device), torch.sin(ang).float().to(device))
+        return self._tables[key]
 
     def _project(self, x: Tensor):
         if x.dim() != 4 or x.shape[0] != self.n or x.shape[3] != self.d_model:

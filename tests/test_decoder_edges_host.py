@@ -126,3 +126,30 @@ def test_forward_mode_tangents_are_refused(monkeypatch):
             with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
                 ops.decode_attention(dual[:, :, 0], None, pos[:1])
         ops.qk_norm_rope(x, x, w, w, cos, sin, pos)
+
+
+def test_rotation_tables_follow_what_they_are_made_from():
+    layer = wc.WideDecoderAttention(1, 32, 4, max_positions=20)
+    cpu = torch.device('cpu')
+    assert layer.rotation(cpu)[0].shape == (20, 4) and layer.rotation(cpu)[0] is layer.rotation(cpu)[0]
+    cos = layer.rotation(cpu, 32)[0]
+    assert cos.shape == (32, 4) and torch.equal(cos[:20], layer.rotation(cpu)[0])
+    layer.theta = 100.0
+    assert not torch.equal(layer.rotation(cpu)[0], cos[:20])
+    layer.rotary_dim, layer.max_positions = 4, 7
+    assert layer.rotation(cpu)[0].shape == (7, 2)
+
+
+def test_rotation_tables_first_made_under_inference_mode_can_train():
+    layer = wc.WideDecoderAttention(1, 32, 4, max_positions=20)
+    with torch.inference_mode():
+        cos, sin = layer.rotation(torch.device('cpu'))
+    assert not cos.is_inference() and not sin.is_inference()
+
+
+def test_rotation_tables_are_not_made_during_a_graph_capture(monkeypatch):
+    """Their copy to the device cannot be recorded; made before, they serve."""
+    layer = wc.WideDecoderAttention(1, 32, 4, max_positions=20)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="captur"):
+        layer.rotation(torch.device('cuda', 0))

@@ -134,3 +134,33 @@ def test_gradient_penalty_through_batch_and_group_norm_is_refused():
         g, = torch.autograd.grad((f(x) ** 3).sum(), x, create_graph=True)
         with pytest.raises(RuntimeError):
             torch.autograd.grad((g ** 2).sum(), x)
+
+
+@pytest.mark.grad
+def test_training_after_a_first_use_under_inference_mode():
+    torch.manual_seed(7)
+    layer = wc.WideDecoderAttention(2, 64, 4, 2, max_positions=16).to(DEV)
+    x = torch.randn(2, 2, 5, 64, device=DEV)
+    with torch.inference_mode():
+        cache = layer.new_cache(2, 16, page_size=4)
+        layer.prefill(x, cache)
+        layer.step(x[:, :, :1], cache, torch.full((2,), 6, device=DEV, dtype=torch.int32))
+        want = layer(x)
+    y = layer(x)
+    assert torch.equal(y, want)
+    y.sum().backward()
+    assert all(torch.isfinite(p.grad).all() for p in layer.parameters())
+
+
+@pytest.mark.grad
+def test_layer_under_torch_compile():
+    torch.manual_seed(8)
+    layer = wc.WideDecoderAttention(2, 64, 4, 2, max_positions=16).to(DEV)
+    x = torch.randn(2, 2, 5, 64, device=DEV, requires_grad=True)
+    want = layer(x)
+    got = torch.compile(layer, backend="eager")(x)
+    torch.testing.assert_close(got, want, **FP32_TOL)
+    dy = torch.randn_like(want)
+    for a, b in zip(torch.autograd.grad(got, [x, *layer.parameters()], dy),
+                    torch.autograd.grad(want, [x, *layer.parameters()], dy)):
+        torch.testing.assert_close(a, b, **FP32_TOL)
