@@ -68,10 +68,26 @@ class WideDecoderAttention(nn.Module):
                 self._tables[key] = (torch.cos(ang).float().to(device), torch.sin(ang).float().to(device))
         return self._tables[key]
 
-    def _project(self, x: Tensor):
+    def _cache_rotation(self, x: Tensor, cache: WidePagedCache):
+        """Tables that reach as far as the cache (whole pages, or one that the
+        caller made): every key that a step's attention sees was written."""
+        return self.rotation(x.device, max(self.max_positions, cache.max_len))
+
+    def _positions(self, x: Tensor, positions: Optional[Tensor], most: int) -> Tensor:
+        """Positions of x's tokens: those given, or 0, 1, .. below ``most``."""
+        if positions is not None:
+            return positions
+        if x.shape[2] > most:
+            raise ValueError(f"WideDecoderAttention: {x.shape[2]} tokens where there are positions for {most}")
+        return torch.arange(x.shape[2], device=x.device)
+
+    def _check(self, x: Tensor) -> None:
         if x.dim() != 4 or x.shape[0] != self.n or x.shape[3] != self.d_model:
             raise ValueError(f"WideDecoderAttention: input must be [N={self.n}, B, T, D={self.d_model}], got "
                              f"{tuple(x.shape)}")
+
+    def _project(self, x: Tensor):
+        self._check(x)
         qkv = ops.linear(x, self.qkv_weight, self.qkv_bias)
         d, hq, hk = self.head_dim, self.n_heads, self.n_kv_heads
         cut = lambda a, h: qkv[..., a * d:(a + h) * d].unflatten(-1, (h, d))
@@ -83,14 +99,18 @@ class WideDecoderAttention(nn.Module):
     def new_cache(self, batch: int, max_len: int, page_size: int = 64, dtype: Optional[torch.dtype] = None
                   ) -> WidePagedCache:
         """A cache for this layer; ``dtype`` int8 or float8_e4m3fn quantises it."""
+        if max_len > self.max_positions:
+            raise ValueError(f"WideDecoderAttention: a cache of {max_len} tokens goes past max_positions = "
+                             f"{self.max_positions}")
         return WidePagedCache.allocate(self.n, batch, self.n_kv_heads, self.head_dim, max_len, page_size,
                                        self.qkv_weight.dtype if dtype is None else dtype, self.qkv_weight.device)
 
     def forward(self, x: Tensor, positions: Optional[Tensor] = None) -> Tensor:
-        """x [N, B, T, d_model] -> the same shape, causal over the T tokens."""
+        """x [N, B, T, d_model] -> the same shape, causal over the T tokens
+        (padding, whose ``positions`` are negative, at their end)."""
+        self._check(x)
+        positions = self._positions(x, positions, self.max_positions)
         q, k, v = self._project(x)
-        if positions is None:
-            positions = torch.arange(x.shape[2], device=x.device)
         q, k = ops.qk_norm_rope(q, k, self.q_norm, self.k_norm, *self.rotation(x.device), positions, self.eps,
                                 self.interleaved)
         return self._output(ops.causal_attention(q, k, v))
@@ -100,10 +120,10 @@ class WideDecoderAttention(nn.Module):
         """``forward`` on prompts from position 0, padded at the end where
         ``positions`` ([B, T] or [N, B, T]) is negative, with the keys and
         values written to the cache."""
+        self._check(x)
+        positions = self._positions(x, positions, min(self.max_positions, cache.max_len))
         q, k, v = self._project(x)
-        if positions is None:
-            positions = torch.arange(x.shape[2], device=x.device)
-        q, k = ops.qk_norm_rope(q, k, self.q_norm, self.k_norm, *self.rotation(x.device), positions, self.eps,
+        q, k = ops.qk_norm_rope(q, k, self.q_norm, self.k_norm, *self._cache_rotation(x, cache), positions, self.eps,
                                 self.interleaved)
         ops.cache_write(cache, k, v, positions)
         return self._output(ops.causal_attention(q, k, v))
@@ -114,7 +134,7 @@ class WideDecoderAttention(nn.Module):
         the tokens of each sequence with the new one, whose position is
         length - 1 (a length of 0 leaves the sequence out: zeros attend)."""
         q, k, v = self._project(x)
-        q = ops.qk_norm_rope_write(q, k, v, self.q_norm, self.k_norm, *self.rotation(x.device),
+        q = ops.qk_norm_rope_write(q, k, v, self.q_norm, self.k_norm, *self._cache_rotation(x, cache),
                                    (lengths - 1).unsqueeze(-1), cache, self.eps, self.interleaved)
         o = ops.decode_attention(q.squeeze(2), cache, lengths, window=window)
         return self._output(o.unsqueeze(2))

@@ -128,6 +128,23 @@ def test_forward_mode_tangents_are_refused(monkeypatch):
         ops.qk_norm_rope(x, x, w, w, cos, sin, pos)
 
 
+def test_layer_refuses_what_its_positions_do_not_reach():
+    """Both lengths are known on the host: past the rotation table keys were
+    left out of the cache and then attended over."""
+    layer = wc.WideDecoderAttention(1, 32, 4, 2, max_positions=20)
+    with pytest.raises(ValueError, match="max_positions"):
+        layer.new_cache(2, 21)
+    cache = layer.new_cache(2, 20, page_size=16)                 # room for 32 in whole pages
+    with pytest.raises(ValueError, match="21 tokens"):
+        layer(torch.zeros(1, 2, 21, 32))
+    with pytest.raises(ValueError, match="21 tokens"):
+        layer.prefill(torch.zeros(1, 2, 21, 32), layer.new_cache(2, 12, page_size=4))
+    with pytest.raises(ValueError, match="13 tokens"):
+        layer.prefill(torch.zeros(1, 2, 13, 32), layer.new_cache(2, 12, page_size=4))
+    with pytest.raises(RuntimeError, match="CUDA"):              # this one fits: only the device is missing
+        layer.prefill(torch.zeros(1, 2, 20, 32), cache)
+
+
 def test_rotation_tables_follow_what_they_are_made_from():
     layer = wc.WideDecoderAttention(1, 32, 4, max_positions=20)
     cpu = torch.device('cpu')

@@ -136,6 +136,27 @@ def test_gradient_penalty_through_batch_and_group_norm_is_refused():
             torch.autograd.grad((g ** 2).sum(), x)
 
 
+def test_steps_into_the_last_page_past_max_positions():
+    """A cache's pages may reach past max_positions: steps there give what a
+    layer with a longer table gives, and read no key that was not written."""
+    torch.manual_seed(6)
+    n, b, d, page = 2, 2, 64, 16
+    short = wc.WideDecoderAttention(n, d, 4, 2, max_positions=17).to(DEV)
+    long = wc.WideDecoderAttention(n, d, 4, 2, max_positions=64).to(DEV)
+    long.load_state_dict(short.state_dict())
+    x = torch.randn(n, b, 20, d, device=DEV)
+    caches = [m.new_cache(b, 17, page_size=page) for m in (short, long)]
+    for c in caches:
+        c.k.fill_(float('nan'))
+    for m, c in zip((short, long), caches):
+        m.prefill(x[:, :, :16], c)
+    for i in range(16, 20):
+        ln = torch.full((b,), i + 1, device=DEV, dtype=torch.int32)
+        got, want = (m.step(x[:, :, i:i + 1], c, ln) for m, c in zip((short, long), caches))
+        assert torch.isfinite(got).all() and torch.equal(got, want)
+    no_device_error()
+
+
 @pytest.mark.grad
 def test_training_after_a_first_use_under_inference_mode():
     torch.manual_seed(7)
