@@ -68,13 +68,16 @@ class WideDecoder(nn.Module):
     @torch.no_grad()
     def generate(self, prompts: Tensor, prompt_lengths: Tensor, new: int, cache_dtype=None):
         """prompts [N, B, T] (padded at the end), prompt_lengths [N, B]. Returns
-        the new tokens [N, B, new] and the logits they were taken from."""
+        the new tokens [N, B, new] and the logits they were taken from. (A
+        prompt of no tokens goes on from its first padded one.)"""
         n, b, t = prompts.shape
+        if t + new - 1 > self.max_len:
+            raise ValueError(f"prompts of {t} tokens and {new} more go past max_len = {self.max_len}")
         caches = self.caches(b, dtype=cache_dtype)
         pos = torch.arange(t, device=prompts.device).expand(n, b, t)
         pos = torch.where(pos < prompt_lengths[..., None], pos, torch.full_like(pos, -1))
         logits = self.prefill(prompts, caches, pos)
-        last = (prompt_lengths - 1).long()[..., None, None].expand(n, b, 1, self.vocab)
+        last = (prompt_lengths - 1).clamp(min=0).long()[..., None, None].expand(n, b, 1, self.vocab)
         logits = logits.gather(2, last)
         out, lengths, kept = [], prompt_lengths.clone(), []
         for i in range(new):

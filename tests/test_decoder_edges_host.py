@@ -1,11 +1,14 @@
 """Host-side checks (no GPU) of the decoder-attention operators and their layer
 at the edges of what they take."""
+import os
+
 import pytest
 import torch
 from torch.nn.attention import SDPBackend, sdpa_kernel
 
 import decoder_ref as R
 import wide_compiler as wc
+from conftest import ROOT
 from wide_compiler import _autograd as AG
 
 
@@ -170,3 +173,17 @@ def test_rotation_tables_are_not_made_during_a_graph_capture(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(RuntimeError, match="captur"):
         layer.rotation(torch.device('cuda', 0))
+
+
+def test_example_takes_prompts_of_no_tokens(monkeypatch):
+    """Their row of logits was row -1: on a GPU an index out of range."""
+    monkeypatch.syspath_prepend(os.path.join(ROOT, "examples"))
+    from wide_decoder import WideDecoder
+    model = WideDecoder(2, 10, 16, 1, 2, 1, 8)
+    monkeypatch.setattr(model, "prefill", lambda tokens, caches, pos: torch.randn(2, 3, tokens.shape[2], 10))
+    monkeypatch.setattr(model, "step", lambda tokens, caches, lengths: torch.randn(2, 3, 1, 10))
+    lengths = torch.tensor([[0, 1, 4], [4, 0, 2]], dtype=torch.int32)
+    tokens, logits = model.generate(torch.zeros(2, 3, 4, dtype=torch.long), lengths, 5)
+    assert tokens.shape == (2, 3, 5) and logits.shape == (2, 3, 5, 10)
+    with pytest.raises(ValueError, match="max_len"):
+        model.generate(torch.zeros(2, 3, 4, dtype=torch.long), lengths, 6)
