@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
     extern __shared__ __align__(16) uint8_t decode_ring[];
     __shared__ float sm_m[kDecodeWarps][8 * NT], sm_l[kDecodeWarps][8 * NT];
     __shared__ float2 sm_t[8 * NT];
-    __shared__ float sm_o[kDecodeWarps][8 * NT][16 * S::JC + 2];
+    __shared__ float2 sm_o[kDecodeWarps][8 * NT][8 * S::JC + 1];      // channels in pairs
     // scales of the key and value rows of a tile and the next
     __shared__ float sm_s[2][kDecodeWarps][2][K::code ? TOK : 1];
     __shared__ int sm_into[2][kDecodeWarps][ROWS == ROWS_BYTES ? TOK : 1];       // bytes from a word to a row's start
@@ -1055,7 +1055,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
                 for (int jj = 0; jj < S::JC; ++jj)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
-                        *reinterpret_cast<float2*>(&sm_o[warp][t * 8 + 2 * c + e][jj * 16 + 2 * g]) =
+                        sm_o[warp][t * 8 + 2 * c + e][jj * 8 + g] =
                             make_float2(acc[t][j0 + jj][e] * f[t][e], acc[t][j0 + jj][e + 2] * f[t][e]);
             __syncthreads();
             for (int e = threadIdx.x; e < heads * 16 * S::JC; e += 32 * kDecodeWarps) {
@@ -1064,7 +1064,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
                 if (ROWS != ROWS_FULL && ch >= a.d) continue;
                 float o = 0.f;
 #pragma unroll
-                for (int w = 0; w < kDecodeWarps; ++w) o += sm_o[w][h][x];
+                for (int w = 0; w < kDecodeWarps; ++w) o += reinterpret_cast<const float*>(sm_o[w][h])[x];
                 const float total = sm_t[h].y;
                 if (whole) store_out(a.out, (row0 + h) * a.d + ch, total == 0.f ? 0.f : o / total, a.dtype);
                 else a.part_o[(part0 + h) * a.d + ch] = o;
