@@ -971,23 +971,28 @@ def _device(what: str, ref: Tensor, *others: Optional[Tensor]) -> int:
     return idx
 
 
-def _launch(idx: int, name: str, *args) -> None:
-    """Calls the entry point on device ``idx`` (its stream is torch's current one)."""
+def _call(idx: int, name: str, *args) -> int:
+    """The library's function with device ``idx`` current."""
     fn = getattr(N.lib(), name)
     if idx == _current_device():
-        rc = fn(*args, N.raw_stream(idx))
-    else:
-        with torch.cuda.device(idx):
-            rc = fn(*args, N.raw_stream(idx))
+        return fn(*args)
+    with torch.cuda.device(idx):
+        return fn(*args)
+
+
+def _launch(idx: int, name: str, *args) -> None:
+    """Calls the entry point on device ``idx`` (its stream is torch's current one)."""
+    rc = _call(idx, name, *args, N.raw_stream(idx))
     if rc:
         N.check(rc, name)
 
 
-def _workspace(name: str, key, *args) -> int:
-    """Workspace bytes by the library's own query, remembered by its arguments."""
+def _workspace(name: str, idx: int, key, *args) -> int:
+    """Workspace bytes by the library's own query on device ``idx`` (they depend
+    on its SM count), remembered by ``key``: its arguments and the device."""
     size = _WS_BYTES.get(key)
     if size is None:
-        size = int(getattr(N.lib(), name)(*args))
+        size = int(_call(idx, name, *args))
         if size < 0:
             raise ValueError(f"{name}: {N.last_error()}")
         if len(_WS_BYTES) > 4096:
@@ -1098,7 +1103,7 @@ def qk_norm_rope_bwd(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, c
     if k.numel() == 0 or q.numel() == 0:
         return dq, dk, *((torch.zeros_like(qw), torch.zeros_like(kw)) if need_dw else (None, None))
     dqw, dkw = (torch.empty_like(qw), torch.empty_like(kw)) if need_dw else (None, None)
-    ws_bytes = _workspace("widek_qk_norm_rope_bwd_workspace", geom, geom)
+    ws_bytes = _workspace("widek_qk_norm_rope_bwd_workspace", idx, (geom, idx), geom)
     ws = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8)
     _launch(idx, "widek_qk_norm_rope_bwd", q.data_ptr(), k.data_ptr(), qw.data_ptr(), kw.data_ptr(), co.data_ptr(),
             si.data_ptr(), positions.data_ptr(), dyq.data_ptr(), dyk.data_ptr(), dq.data_ptr(), dk.data_ptr(),
@@ -1234,7 +1239,7 @@ def decode_attention(q: Tensor, cache, lengths: Tensor, scale: Optional[float] =
     if hk < 1 or hq % hk != 0:
         raise ValueError(f"{what}: {hq} query heads over {hk} key heads")
     geom = _pack_decode(n, b, hq, hk, d, *_head_strides(q, what), *_index_strides(lengths, (n, b), what, "lengths"))
-    ws_bytes = _workspace("widek_decode_attention_workspace", (geom, cache.geom, window, cache.fmt, idx), geom,
+    ws_bytes = _workspace("widek_decode_attention_workspace", idx, (geom, cache.geom, window, cache.fmt, idx), geom,
                           cache.geom, window, cache.fmt)
     ws = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8) if ws_bytes else None
     out = q.new_empty(qs)

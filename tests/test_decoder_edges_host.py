@@ -187,3 +187,35 @@ def test_example_takes_prompts_of_no_tokens(monkeypatch):
     assert tokens.shape == (2, 3, 5) and logits.shape == (2, 3, 5, 10)
     with pytest.raises(ValueError, match="max_len"):
         model.generate(torch.zeros(2, 3, 4, dtype=torch.long), lengths, 6)
+
+
+def test_workspace_is_asked_for_on_the_tensors_device(monkeypatch):
+    """It depends on that GPU's SM count; asked for on the current device, a
+    size that another one needs was refused, and remembered."""
+    from wide_compiler import _native as N
+    from wide_compiler import ops
+    at = [0]
+
+    class Device:
+        def __init__(self, idx):
+            self.idx = idx
+
+        def __enter__(self):
+            self.was, at[0] = at[0], self.idx
+
+        def __exit__(self, *_):
+            at[0] = self.was
+
+    class Lib:
+        @staticmethod
+        def query(*args):
+            return 100 + at[0]
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(ops, "_current_device", lambda: at[0])
+    monkeypatch.setattr(N, "lib", lambda: Lib)
+    monkeypatch.setattr(ops, "_WS_BYTES", {})
+    for _ in range(2):
+        assert ops._workspace("query", 0, ("a", 0), 1) == 100
+        assert ops._workspace("query", 3, ("a", 3), 1) == 103
+    assert at[0] == 0
