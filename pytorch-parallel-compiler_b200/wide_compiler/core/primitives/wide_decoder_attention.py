@@ -58,15 +58,22 @@ class WideDecoderAttention(nn.Module):
         """cos / sin [rows, rotary_dim / 2] in fp32 (rows: max_positions unless
         given), angles in 64 bits; made once for each use they serve."""
         key = (device, self.max_positions if rows is None else rows, self.rotary_dim, self.theta)
-        if key not in self._tables:
+        if torch.compiler.is_compiling():                # the traced graph makes them
+            if key not in self._tables:
+                self._tables[key] = self._make_rotation(device, key[1])
+            return self._tables[key]
+        if key not in self._tables or self._tables[key][0].is_inference():
             if device.type == 'cuda' and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("WideDecoderAttention: the rotation tables cannot be made while a CUDA graph is "
                                    "captured: run the layer once before")
             with torch.inference_mode(False):            # they serve training as well
-                i = torch.arange(0, self.rotary_dim, 2, dtype=torch.float64) / max(self.rotary_dim, 1)
-                ang = torch.arange(key[1], dtype=torch.float64)[:, None] * self.theta ** -i[None]
-                self._tables[key] = (torch.cos(ang).float().to(device), torch.sin(ang).float().to(device))
+                self._tables[key] = self._make_rotation(device, key[1])
         return self._tables[key]
+
+    def _make_rotation(self, device: torch.device, rows: int):
+        i = torch.arange(0, self.rotary_dim, 2, dtype=torch.float64) / max(self.rotary_dim, 1)
+        ang = torch.arange(rows, dtype=torch.float64)[:, None] * self.theta ** -i[None]
+        return torch.cos(ang).float().to(device), torch.sin(ang).float().to(device)
 
     def _cache_rotation(self, x: Tensor, cache: WidePagedCache):
         """Tables that reach as far as the cache (whole pages, or one that the

@@ -185,3 +185,13 @@ def test_layer_under_torch_compile():
     for a, b in zip(torch.autograd.grad(got, [x, *layer.parameters()], dy),
                     torch.autograd.grad(want, [x, *layer.parameters()], dy)):
         torch.testing.assert_close(a, b, **FP32_TOL)
+
+
+def test_step_first_traced_in_one_graph():
+    torch.manual_seed(10)
+    layer, ref = (wc.WideDecoderAttention(2, 64, 4, 2, max_positions=16).to(DEV) for _ in range(2))
+    ref.load_state_dict(layer.state_dict())
+    x, ln = torch.randn(2, 2, 1, 64, device=DEV), torch.ones(2, device=DEV, dtype=torch.int32)
+    caches = [m.new_cache(2, 8, page_size=4) for m in (layer, ref)]
+    step = torch.compile(layer.step, fullgraph=True, backend="eager")
+    assert torch.equal(step(x, caches[0], ln), ref.step(x, caches[1], ln))
