@@ -320,6 +320,21 @@ def _(k_pages, v_pages, table, k_scale, v_scale, positions, dtype):
     return k_pages.new_empty(shape, dtype=dtype), k_pages.new_empty(shape, dtype=dtype)
 
 
+@torch.library.custom_op("widek::causal_attention", mutates_args=())
+def causal_attention(q: Tensor, k: Tensor, v: Tensor) -> Tensor:
+    """Causal attention over whole sequences, grouped key heads (ops.causal_attention)."""
+    with torch.no_grad():
+        return ops.causal_attention(q, k, v)
+
+
+@causal_attention.register_fake
+def _(q, k, v):
+    return q.new_empty(q.shape)
+
+
+_register_autograd(causal_attention, _AG.causal_attention_t)
+
+
 @torch.library.custom_op("widek::decode_attention", mutates_args=())
 def decode_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, k_scale: Optional[Tensor],
                      v_scale: Optional[Tensor], lengths: Tensor, scale: float, window: int) -> Tensor:
@@ -335,6 +350,6 @@ def _(q, k_pages, v_pages, table, k_scale, v_scale, lengths, scale, window):
 
 OPERATORS = ('linear', 'layernorm', 'batchnorm', 'groupnorm', 'embedding', 'conv', 'gru', 'lstm', 'attention',
              'swap01', 'unary', 'binary', 'qk_norm_rope', 'qk_norm_rope_write', 'cache_write', 'cache_read',
-             'decode_attention')
+             'causal_attention', 'decode_attention')
 
 __all__ = ['OPERATORS']

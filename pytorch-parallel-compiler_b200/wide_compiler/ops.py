@@ -1196,6 +1196,8 @@ def causal_attention(q: Tensor, k: Tensor, v: Tensor) -> Tensor:
     [N, B, T, Hq, D], k and v [N, B, T, Hk, D] -> [N, B, T, Hq, D] (the core of
     WideAttention, widek_attention_fwd, on one key head for each query head;
     differentiable: the backward re-runs the torch formulation)."""
+    if _compiling():
+        return torch.ops.widek.causal_attention(q, k, v)
     if _AG.needs_grad(q, k, v):
         return _AG.run(causal_attention, _AG.causal_attention_t, q, k, v)
     what = "causal_attention"

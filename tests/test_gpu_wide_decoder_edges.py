@@ -187,6 +187,34 @@ def test_layer_under_torch_compile():
         torch.testing.assert_close(a, b, **FP32_TOL)
 
 
+@pytest.mark.grad
+@pytest.mark.parametrize("first", ["traced", "eager"])
+def test_layer_is_one_graph_under_torch_compile(first):
+    """forward with gradients, prefill and step, without a break; the rotation
+    tables made in the traced call or before it."""
+    torch.manual_seed(9)
+    n, b, t, d = 2, 2, 5, 64
+    layer, ref = (wc.WideDecoderAttention(n, d, 4, 2, max_positions=16).to(DEV) for _ in range(2))
+    ref.load_state_dict(layer.state_dict())
+    x = torch.randn(n, b, t + 1, d, device=DEV, requires_grad=True)
+    if first == "eager":
+        layer(x)
+    one = lambda f: torch.compile(f, fullgraph=True, backend="eager")
+    got, want = one(layer)(x), ref(x)
+    torch.testing.assert_close(got, want, **FP32_TOL)
+    dy = torch.randn_like(want)
+    for g, w in zip(torch.autograd.grad(got, [x, *layer.parameters()], dy),
+                    torch.autograd.grad(want, [x, *ref.parameters()], dy)):
+        torch.testing.assert_close(g, w, **FP32_TOL)
+    caches = [m.new_cache(b, 8, page_size=4) for m in (layer, ref)]
+    y = x.detach()
+    assert torch.equal(one(layer.prefill)(y[:, :, :t], caches[0]), ref.prefill(y[:, :, :t], caches[1]))
+    ln = torch.full((b,), t + 1, device=DEV, dtype=torch.int32)
+    assert torch.equal(one(layer.step)(y[:, :, t:], caches[0], ln), ref.step(y[:, :, t:], caches[1], ln))
+    assert torch.equal(layer(x), want)
+    no_device_error()
+
+
 def test_step_first_traced_in_one_graph():
     torch.manual_seed(10)
     layer, ref = (wc.WideDecoderAttention(2, 64, 4, 2, max_positions=16).to(DEV) for _ in range(2))
