@@ -46,9 +46,10 @@
 // more; one piece alone would show in a bf16 result). fp32 caches split both
 // operands in two tf32 pieces and drop the product of the low ones (2^-22).
 // 8-bit codes are exact in f16 and in bf16. Against K, q is scaled by a power
-// of two per head into f16's range, in two pieces when it is fp32 (16-bit
-// queries stay exact, which bf16 would not give f16 ones). The scale of a key
-// row multiplies its score; that of a value row goes into its weight, whose
+// of two per head to the top of f16's range, in two pieces when it is fp32. A
+// 16-bit query stays exact in channels above 2^-31 of the head's largest and is
+// off by 2^-39 of it at most below (bf16 would round every f16 query). The scale
+// of a key row multiplies its score; that of a value row goes into its weight, whose
 // product p vs has no fixed range: V and the weights meet in bf16, which has
 // fp32's, in three pieces where the result is fp32. The tensor core's sums
 // round towards zero: fp32 results take them in short chains, added in fp32,
@@ -644,53 +645,52 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
         const int heads = min(8 * NT, a.group - h0);
         const int64_t base = i * a.q_n + (at.nb - i * a.b) * a.q_b + (int64_t)(kh * a.group + h0) * a.q_h;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int h = t * 8 + g;
-        const int64_t at = base + (h < heads ? h : 0) * a.q_h;
-        float x[S::KP][S::KD];
-        float top = 0.f;
+        for (int t = 0; t < NT; ++t) {
+            const int h = t * 8 + g;
+            const int64_t at = base + (h < heads ? h : 0) * a.q_h;
+            float x[S::KP][S::KD];
+            float top = 0.f;
 #pragma unroll
-        for (int p = 0; p < S::KP; ++p) {
-            const int ch = (p * 4 + c) * S::KD;
+            for (int p = 0; p < S::KP; ++p) {
+                const int ch = (p * 4 + c) * S::KD;
 #pragma unroll
-            for (int e = 0; e < S::KD; ++e) x[p][e] = 0.f;
-            if (ROWS >= ROWS_16 && a.q_vec) {
-                if (h < heads && ch < a.d) load_in16<S::KD>(a.q, at + ch, a.dtype, x[p]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < S::KD; ++e)
-                    if (h < heads && ch + e < a.d) x[p][e] = load_in(a.q, at + ch + e, a.dtype);
-            }
-#pragma unroll
-            for (int e = 0; e < S::KD; ++e) top = fmaxf(top, fabsf(x[p][e]));
-        }
-        zs[t][0] = zs[t][1] = a.scale_log2;
-        float up = 1.f;
-        if constexpr (K::code) {
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // 2^(14 - exponent): the largest magnitude lands in [2^14, 2^15)
-            const int ex = (int)(__float_as_uint(top) >> 23);
-            const bool sized = ex >= 16 && ex < 255;
-            up = sized ? __uint_as_float((uint32_t)(268 - ex) << 23) : 1.f;
-            const float down = sized ? __uint_as_float((uint32_t)(ex - 14) << 23) : 1.f;
-            zs[t][0] *= __shfl_sync(0xffffffffu, down, 8 * c);
-            zs[t][1] *= __shfl_sync(0xffffffffu, down, 8 * c + 4);
-        }
-#pragma unroll
-        for (int p = 0; p < S::KP; ++p)
-#pragma unroll
-            for (int e = 0; e < S::KR; ++e) {
-                if constexpr (K::f32) {
-                    q[t][p * S::KR + e] = __float_as_uint(x[p][e]);
+                for (int e = 0; e < S::KD; ++e) x[p][e] = 0.f;
+                if (ROWS >= ROWS_16 && a.q_vec) {
+                    if (h < heads && ch < a.d) load_in16<S::KD>(a.q, at + ch, a.dtype, x[p]);
                 } else {
-                    float rx, ry;
-                    q[t][p * S::KR + e] = pack2<KIND>(x[p][2 * e] * up, x[p][2 * e + 1] * up, rx, ry);
-                    if constexpr (SPLITQ) ql[t][p * S::KR + e] = pack2<KIND>(rx, ry, rx, ry);
+#pragma unroll
+                    for (int e = 0; e < S::KD; ++e)
+                        if (h < heads && ch + e < a.d) x[p][e] = load_in(a.q, at + ch + e, a.dtype);
                 }
+#pragma unroll
+                for (int e = 0; e < S::KD; ++e) top = fmaxf(top, fabsf(x[p][e]));
             }
-    }
-
+            zs[t][0] = zs[t][1] = a.scale_log2;
+            float up = 1.f;
+            if constexpr (K::code) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                // 2^(14 - exponent): the largest magnitude lands in [2^14, 2^15)
+                const int ex = (int)(__float_as_uint(top) >> 23);
+                const bool sized = ex >= 16 && ex < 255;
+                up = sized ? __uint_as_float((uint32_t)(268 - ex) << 23) : 1.f;
+                const float down = sized ? __uint_as_float((uint32_t)(ex - 14) << 23) : 1.f;
+                zs[t][0] *= __shfl_sync(0xffffffffu, down, 8 * c);
+                zs[t][1] *= __shfl_sync(0xffffffffu, down, 8 * c + 4);
+            }
+#pragma unroll
+            for (int p = 0; p < S::KP; ++p)
+#pragma unroll
+                for (int e = 0; e < S::KR; ++e) {
+                    if constexpr (K::f32) {
+                        q[t][p * S::KR + e] = __float_as_uint(x[p][e]);
+                    } else {
+                        float rx, ry;
+                        q[t][p * S::KR + e] = pack2<KIND>(x[p][2 * e] * up, x[p][2 * e + 1] * up, rx, ry);
+                        if constexpr (SPLITQ) ql[t][p * S::KR + e] = pack2<KIND>(rx, ry, rx, ry);
+                    }
+                }
+        }
     };
 
     float acc[NT][DP / 16][4];
@@ -732,82 +732,82 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
 #pragma unroll
         for (int p0 = 0; p0 < S::KP; p0 += S::KB) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int p = 0; p < S::KB; ++p)
+                for (int p = 0; p < S::KB; ++p)
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const int row = 16 * mt + 8 * hf + g, at = (p0 + p) * 4 + c;
-                    if constexpr (ROWS == ROWS_BYTES)
-                        read_piece(batch[mt][p][hf], from + S::at(row, at),
-                                   at + 1 < S::places ? (int)(from + S::at(row, at + 1)) : -1,
-                                   8 * (k_into >> 2 * (2 * mt + hf) & 3));
-                    else read_piece(batch[mt][p][hf], from + S::at(row, at));
-                }
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int p = p0; p < p0 + S::KB; ++p) {
-                const uint32_t(&kr)[2][S::KW] = batch[mt][p - p0];
-                if constexpr (K::f32) {
-                    // the tensor core's sums round towards zero: chains of 6, added up in fp32
-                    float part[NT][4];
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) part[t][j] = 0.f;
-#pragma unroll
-                    for (int e = 0; e < S::KR; e += 2) {
-                        uint32_t hi[4], lo[4];
-                        split_tf32(kr[0][e], hi[0], lo[0]);
-                        split_tf32(kr[1][e], hi[1], lo[1]);
-                        split_tf32(kr[0][e + 1], hi[2], lo[2]);
-                        split_tf32(kr[1][e + 1], hi[3], lo[3]);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            uint32_t qh0, ql0, qh1, ql1;
-                            split_tf32(q[t][p * S::KR + e], qh0, ql0);
-                            split_tf32(q[t][p * S::KR + e + 1], qh1, ql1);
-                            mma<KIND>(part[t], lo[0], lo[1], lo[2], lo[3], qh0, qh1);
-                            mma<KIND>(part[t], hi[0], hi[1], hi[2], hi[3], ql0, ql1);
-                            mma<KIND>(part[t], hi[0], hi[1], hi[2], hi[3], qh0, qh1);
-                        }
+                    for (int hf = 0; hf < 2; ++hf) {
+                        const int row = 16 * mt + 8 * hf + g, at = (p0 + p) * 4 + c;
+                        if constexpr (ROWS == ROWS_BYTES)
+                            read_piece(batch[mt][p][hf], from + S::at(row, at),
+                                       at + 1 < S::places ? (int)(from + S::at(row, at + 1)) : -1,
+                                       8 * (k_into >> 2 * (2 * mt + hf) & 3));
+                        else read_piece(batch[mt][p][hf], from + S::at(row, at));
                     }
 #pragma unroll
-                    for (int t = 0; t < NT; ++t)
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) s[t][mt][j] += part[t][j];
-                } else {
-                    uint32_t r0[S::KR], r1[S::KR];
-                    if constexpr (K::code) {
+                for (int p = p0; p < p0 + S::KB; ++p) {
+                    const uint32_t(&kr)[2][S::KW] = batch[mt][p - p0];
+                    if constexpr (K::f32) {
+                        // the tensor core's sums round towards zero: chains of 6, added up in fp32
+                        float part[NT][4];
 #pragma unroll
-                        for (int w = 0; w < S::KW; ++w) {
-                            const uint32_t x0 = code_word<KIND>(kr[0][w]), x1 = code_word<KIND>(kr[1][w]);
-                            r0[2 * w] = code_pair<KIND, 0>(x0);
-                            r0[2 * w + 1] = code_pair<KIND, 1>(x0);
-                            r1[2 * w] = code_pair<KIND, 0>(x1);
-                            r1[2 * w + 1] = code_pair<KIND, 1>(x1);
-                        }
-                    } else {
+                        for (int t = 0; t < NT; ++t)
 #pragma unroll
-                        for (int w = 0; w < S::KW; ++w) r0[w] = kr[0][w], r1[w] = kr[1][w];
-                    }
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        float part[4] = {0.f, 0.f, 0.f, 0.f};
-                        float(&o)[4] = SPLITQ ? part : s[t][mt];
+                            for (int j = 0; j < 4; ++j) part[t][j] = 0.f;
 #pragma unroll
                         for (int e = 0; e < S::KR; e += 2) {
-                            const int j = p * S::KR + e;
-                            if constexpr (SPLITQ)
-                                mma<KIND>(o, r0[e], r1[e], r0[e + 1], r1[e + 1], ql[t][j], ql[t][j + 1]);
-                            mma<KIND>(o, r0[e], r1[e], r0[e + 1], r1[e + 1], q[t][j], q[t][j + 1]);
+                            uint32_t hi[4], lo[4];
+                            split_tf32(kr[0][e], hi[0], lo[0]);
+                            split_tf32(kr[1][e], hi[1], lo[1]);
+                            split_tf32(kr[0][e + 1], hi[2], lo[2]);
+                            split_tf32(kr[1][e + 1], hi[3], lo[3]);
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) {
+                                uint32_t qh0, ql0, qh1, ql1;
+                                split_tf32(q[t][p * S::KR + e], qh0, ql0);
+                                split_tf32(q[t][p * S::KR + e + 1], qh1, ql1);
+                                mma<KIND>(part[t], lo[0], lo[1], lo[2], lo[3], qh0, qh1);
+                                mma<KIND>(part[t], hi[0], hi[1], hi[2], hi[3], ql0, ql1);
+                                mma<KIND>(part[t], hi[0], hi[1], hi[2], hi[3], qh0, qh1);
+                            }
                         }
 #pragma unroll
-                        for (int e = 0; e < (SPLITQ ? 4 : 0); ++e) s[t][mt][e] += part[e];
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) s[t][mt][j] += part[t][j];
+                    } else {
+                        uint32_t r0[S::KR], r1[S::KR];
+                        if constexpr (K::code) {
+#pragma unroll
+                            for (int w = 0; w < S::KW; ++w) {
+                                const uint32_t x0 = code_word<KIND>(kr[0][w]), x1 = code_word<KIND>(kr[1][w]);
+                                r0[2 * w] = code_pair<KIND, 0>(x0);
+                                r0[2 * w + 1] = code_pair<KIND, 1>(x0);
+                                r1[2 * w] = code_pair<KIND, 0>(x1);
+                                r1[2 * w + 1] = code_pair<KIND, 1>(x1);
+                            }
+                        } else {
+#pragma unroll
+                            for (int w = 0; w < S::KW; ++w) r0[w] = kr[0][w], r1[w] = kr[1][w];
+                        }
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            float part[4] = {0.f, 0.f, 0.f, 0.f};
+                            float(&o)[4] = SPLITQ ? part : s[t][mt];
+#pragma unroll
+                            for (int e = 0; e < S::KR; e += 2) {
+                                const int j = p * S::KR + e;
+                                if constexpr (SPLITQ)
+                                    mma<KIND>(o, r0[e], r1[e], r0[e + 1], r1[e + 1], ql[t][j], ql[t][j + 1]);
+                                mma<KIND>(o, r0[e], r1[e], r0[e + 1], r1[e + 1], q[t][j], q[t][j + 1]);
+                            }
+#pragma unroll
+                            for (int e = 0; e < (SPLITQ ? 4 : 0); ++e) s[t][mt][e] += part[e];
+                        }
                     }
                 }
-            }
         }
     };
     // Running maxima and sums; s becomes the weights that meet V.
@@ -904,100 +904,102 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<KIND, DP, NT, R
 #pragma unroll
         for (int p0 = 0; p0 < S::VP; p0 += S::VB) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int p = 0; p < S::VB; ++p)
+                for (int p = 0; p < S::VB; ++p)
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    // the k index of lane c: tokens 2c, 2c + 1, 2c + 8, 2c + 9; tf32 c, c + 4, c + 8, c + 12
-                    const int row = 16 * mt + (K::f32 ? c + 4 * t : 2 * c + (t & 1) + 8 * (t >> 1));
-                    // the 16-byte place, and the half in it
-                    const int at = S::VW == 4 ? (p0 + p) * 8 + g : (p0 + p) * 4 + g / 2, half = S::VW == 4 ? 0 : g % 2 * 8;
-                    const uint32_t src = from + S::at(row, at) + half;
-                    if constexpr (ROWS == ROWS_BYTES)
-                        read_piece(batch[mt][p][t], src,
-                                   S::VW == 2 && half == 0 ? (int)(src + 8)
-                                   : at + 1 < S::places    ? (int)(from + S::at(row, at + 1))
-                                                           : -1,
-                                   8 * (v_into >> 2 * (4 * mt + t) & 3));
-                    else read_piece(batch[mt][p][t], src);
-                }
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int p = p0; p < p0 + S::VB; ++p) {
-                const uint32_t(&vr)[4][S::VW] = batch[mt][p - p0];
-                if constexpr (K::f32) {
-#pragma unroll
-                    for (int e = 0; e < S::VD; e += 2) {
-                        float part[NT][4];
-#pragma unroll
-                        for (int t = 0; t < NT; ++t)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) part[t][j] = 0.f;
-#pragma unroll
-                        for (int k8 = 0; k8 < 2; ++k8) {
-                            uint32_t hi[4], lo[4];
-                            split_tf32(vr[2 * k8][e], hi[0], lo[0]);
-                            split_tf32(vr[2 * k8][e + 1], hi[1], lo[1]);
-                            split_tf32(vr[2 * k8 + 1][e], hi[2], lo[2]);
-                            split_tf32(vr[2 * k8 + 1][e + 1], hi[3], lo[3]);
-#pragma unroll
-                            for (int t = 0; t < NT; ++t) {
-                                const uint32_t* bh = &ph[t][mt][2 * k8];
-                                const uint32_t* bl = &pl[t][mt][2 * k8];
-                                mma<KIND>(part[t], lo[0], lo[1], lo[2], lo[3], bh[0], bh[1]);
-                                mma<KIND>(part[t], hi[0], hi[1], hi[2], hi[3], bl[0], bl[1]);
-                                mma<KIND>(part[t], hi[0], hi[1], hi[2], hi[3], bh[0], bh[1]);
-                            }
-                        }
-#pragma unroll
-                        for (int t = 0; t < NT; ++t)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) acc[t][(p * S::VD + e) / 2][j] += part[t][j];
+                    for (int t = 0; t < 4; ++t) {
+                        // the k index of lane c: tokens 2c, 2c + 1, 2c + 8, 2c + 9; tf32 c, c + 4, c + 8, c + 12
+                        const int row = 16 * mt + (K::f32 ? c + 4 * t : 2 * c + (t & 1) + 8 * (t >> 1));
+                        // the 16-byte place, and the half in it
+                        const int at = S::VW == 4 ? (p0 + p) * 8 + g : (p0 + p) * 4 + g / 2;
+                        const int half = S::VW == 4 ? 0 : g % 2 * 8;
+                        const uint32_t src = from + S::at(row, at) + half;
+                        if constexpr (ROWS == ROWS_BYTES)
+                            read_piece(batch[mt][p][t], src,
+                                       S::VW == 2 && half == 0 ? (int)(src + 8)
+                                       : at + 1 < S::places    ? (int)(from + S::at(row, at + 1))
+                                                               : -1,
+                                       8 * (v_into >> 2 * (4 * mt + t) & 3));
+                        else read_piece(batch[mt][p][t], src);
                     }
-                } else {
-                    uint32_t av[S::VD / 2][4];
-                    if constexpr (K::code) {
 #pragma unroll
-                        for (int w = 0; w < S::VW; ++w) {
-                            uint32_t x[4];
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                            for (int t = 0; t < 4; ++t) x[t] = vr[t][w];
+                for (int p = p0; p < p0 + S::VB; ++p) {
+                    const uint32_t(&vr)[4][S::VW] = batch[mt][p - p0];
+                    if constexpr (K::f32) {
 #pragma unroll
-                            for (int k = 0; k < 2; ++k) {            // token pairs
-                                const uint32_t x01 = prmt(x[2 * k], x[2 * k + 1], 0x5140);
-                                const uint32_t x23 = prmt(x[2 * k], x[2 * k + 1], 0x7362);
-                                av[2 * w][2 * k] = code_pair_bf16<KIND, 0>(x01);
-                                av[2 * w][2 * k + 1] = code_pair_bf16<KIND, 1>(x01);
-                                av[2 * w + 1][2 * k] = code_pair_bf16<KIND, 0>(x23);
-                                av[2 * w + 1][2 * k + 1] = code_pair_bf16<KIND, 1>(x23);
+                        for (int e = 0; e < S::VD; e += 2) {
+                            float part[NT][4];
+#pragma unroll
+                            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) part[t][j] = 0.f;
+#pragma unroll
+                            for (int k8 = 0; k8 < 2; ++k8) {
+                                uint32_t hi[4], lo[4];
+                                split_tf32(vr[2 * k8][e], hi[0], lo[0]);
+                                split_tf32(vr[2 * k8][e + 1], hi[1], lo[1]);
+                                split_tf32(vr[2 * k8 + 1][e], hi[2], lo[2]);
+                                split_tf32(vr[2 * k8 + 1][e + 1], hi[3], lo[3]);
+#pragma unroll
+                                for (int t = 0; t < NT; ++t) {
+                                    const uint32_t* bh = &ph[t][mt][2 * k8];
+                                    const uint32_t* bl = &pl[t][mt][2 * k8];
+                                    mma<KIND>(part[t], lo[0], lo[1], lo[2], lo[3], bh[0], bh[1]);
+                                    mma<KIND>(part[t], hi[0], hi[1], hi[2], hi[3], bl[0], bl[1]);
+                                    mma<KIND>(part[t], hi[0], hi[1], hi[2], hi[3], bh[0], bh[1]);
+                                }
                             }
+#pragma unroll
+                            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) acc[t][(p * S::VD + e) / 2][j] += part[t][j];
                         }
                     } else {
+                        uint32_t av[S::VD / 2][4];
+                        if constexpr (K::code) {
 #pragma unroll
-                        for (int w = 0; w < S::VW; ++w) {
-                            av[w][0] = prmt(vr[0][w], vr[1][w], 0x5410);
-                            av[w][1] = prmt(vr[0][w], vr[1][w], 0x7632);
-                            av[w][2] = prmt(vr[2][w], vr[3][w], 0x5410);
-                            av[w][3] = prmt(vr[2][w], vr[3][w], 0x7632);
+                            for (int w = 0; w < S::VW; ++w) {
+                                uint32_t x[4];
+#pragma unroll
+                                for (int t = 0; t < 4; ++t) x[t] = vr[t][w];
+#pragma unroll
+                                for (int k = 0; k < 2; ++k) {            // token pairs
+                                    const uint32_t x01 = prmt(x[2 * k], x[2 * k + 1], 0x5140);
+                                    const uint32_t x23 = prmt(x[2 * k], x[2 * k + 1], 0x7362);
+                                    av[2 * w][2 * k] = code_pair_bf16<KIND, 0>(x01);
+                                    av[2 * w][2 * k + 1] = code_pair_bf16<KIND, 1>(x01);
+                                    av[2 * w + 1][2 * k] = code_pair_bf16<KIND, 0>(x23);
+                                    av[2 * w + 1][2 * k + 1] = code_pair_bf16<KIND, 1>(x23);
+                                }
+                            }
+                        } else {
+#pragma unroll
+                            for (int w = 0; w < S::VW; ++w) {
+                                av[w][0] = prmt(vr[0][w], vr[1][w], 0x5410);
+                                av[w][1] = prmt(vr[0][w], vr[1][w], 0x7632);
+                                av[w][2] = prmt(vr[2][w], vr[3][w], 0x5410);
+                                av[w][3] = prmt(vr[2][w], vr[3][w], 0x7632);
+                            }
                         }
+#pragma unroll
+                        for (int w = 0; w < S::VD / 2; ++w)
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) {
+                                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                                float(&o)[4] = SPLITQ ? part : acc[t][p * S::VD / 2 + w];
+                                if constexpr (SPLITQ)
+                                    mma<K::values>(o, av[w][0], av[w][1], av[w][2], av[w][3], pr[t][mt][0],
+                                                   pr[t][mt][1]);
+                                mma<K::values>(o, av[w][0], av[w][1], av[w][2], av[w][3], pl[t][mt][0], pl[t][mt][1]);
+                                mma<K::values>(o, av[w][0], av[w][1], av[w][2], av[w][3], ph[t][mt][0], ph[t][mt][1]);
+#pragma unroll
+                                for (int e = 0; e < (SPLITQ ? 4 : 0); ++e) acc[t][p * S::VD / 2 + w][e] += part[e];
+                            }
                     }
-#pragma unroll
-                    for (int w = 0; w < S::VD / 2; ++w)
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            float part[4] = {0.f, 0.f, 0.f, 0.f};
-                            float(&o)[4] = SPLITQ ? part : acc[t][p * S::VD / 2 + w];
-                            if constexpr (SPLITQ)
-                                mma<K::values>(o, av[w][0], av[w][1], av[w][2], av[w][3], pr[t][mt][0], pr[t][mt][1]);
-                            mma<K::values>(o, av[w][0], av[w][1], av[w][2], av[w][3], pl[t][mt][0], pl[t][mt][1]);
-                            mma<K::values>(o, av[w][0], av[w][1], av[w][2], av[w][3], ph[t][mt][0], ph[t][mt][1]);
-#pragma unroll
-                            for (int e = 0; e < (SPLITQ ? 4 : 0); ++e) acc[t][p * S::VD / 2 + w][e] += part[e];
-                        }
                 }
-            }
         }
     };
     auto clear_scores = [&]() {

@@ -241,3 +241,16 @@ def test_totals_of_chains_follow_the_maximum(dtype, fmt, d, group):
     q = torch.randn(n, b, hk * group, d, device=DEV, generator=gen).to(dtype)
     assert steps_of_a_block(cache, lengths, group) > 40
     check(q, cache, lengths)
+
+
+@pytest.mark.parametrize("dtype,fmt", [(BF16, BF16), (F16, E4M3), (F32, I8)])
+def test_long_segments_in_turn(dtype, fmt):
+    """More than 4096 sequences, some of them longer than one chain of sums."""
+    n, b, hk, d, page, held, longest = 3, 1500, 1, 64, 100, 64, 6000
+    gen = torch.Generator(device=DEV).manual_seed(13)
+    (k, ks), (v, vs) = (encode(torch.randn(n, held, hk, page, d, device=DEV, generator=gen), fmt) for _ in range(2))
+    table = torch.randint(0, held, (n, b, longest // page), device=DEV, generator=gen, dtype=torch.int32)
+    lengths = torch.randint(0, longest + 1, (n, b), device=DEV, generator=gen, dtype=torch.int32)
+    cache = wc.WidePagedCache(k, v, table, ks, vs)
+    q = torch.randn(n, b, hk * 2, d, device=DEV, generator=gen).to(dtype)
+    check(q, cache, lengths)
