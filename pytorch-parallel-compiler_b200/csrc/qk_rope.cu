@@ -992,7 +992,7 @@ extern "C" int widek_qk_norm_rope_bwd(const void* q, const void* k, const void* 
     if (no_rows(a, a.hq)) return WIDEK_OK;
     if (!dk || !dyq || !dyk) return set_error(WIDEK_ERR_INVALID, "%s: null pointer", what);
     const int64_t need = widek_qk_norm_rope_bwd_workspace(geom);
-    if (!workspace || workspace_bytes < need)
+    if (!workspace || workspace_bytes < need || !aligned_to(workspace, sizeof(float)))
         return set_error(WIDEK_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed", what,
                          (long long)workspace_bytes, (long long)need);
     g.dyq = dyq, g.dyk = dyk, g.dqw = dqw, g.dkw = dkw, g.part = static_cast<float*>(workspace);

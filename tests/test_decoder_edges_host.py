@@ -219,3 +219,19 @@ def test_workspace_is_asked_for_on_the_tensors_device(monkeypatch):
         assert ops._workspace("query", 0, ("a", 0), 1) == 100
         assert ops._workspace("query", 3, ("a", 3), 1) == 103
     assert at[0] == 0
+
+
+def test_gradient_entry_refuses_a_workspace_that_floats_cannot_lie_in():
+    import struct
+
+    from wide_compiler import _native as N
+    lib = N.load()
+    n, b, t, hq, hk, d = 2, 2, 3, 4, 2, 64
+    geom = [n, b, t, hq, hk, d, d, 8]
+    for h in (hq, hk, hk):
+        geom += [b * t * h * d, t * h * d, h * d, d]
+    geom = struct.pack('=23q', *geom, 0, t, 1)
+    size = lib.widek_qk_norm_rope_bwd_workspace(geom)
+    P = 16                               # stand-in pointers: never dereferenced on this path
+    rc = lib.widek_qk_norm_rope_bwd(*[P] * 13, geom, 1e-6, 0, 0, N.BF16, P + 2, size, None)
+    assert rc == N.WIDEK_ERR_INVALID and "workspace" in N.last_error()
