@@ -686,7 +686,8 @@ WIDEK_API int widek_qk_norm_rope_write_fwd(const void* q, const void* k, const v
 WIDEK_API int64_t widek_qk_norm_rope_bwd_workspace(const int64_t* geom);
 
 /* Gradients of widek_qk_norm_rope_fwd: dyq, dyk, dq, dk dense; dqw, dkw
- * [n, d], nullable. The weight gradients are summed in a fixed order. */
+ * [n, d], nullable (zeros when there are no rows). The weight gradients are
+ * summed in a fixed order. */
 WIDEK_API int widek_qk_norm_rope_bwd(const void* q, const void* k, const void* qw, const void* kw,
                                      const float* cos, const float* sin, const void* positions,
                                      const void* dyq, const void* dyk, void* dq, void* dk,

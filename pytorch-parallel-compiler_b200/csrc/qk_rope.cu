@@ -989,15 +989,21 @@ extern "C" int widek_qk_norm_rope_bwd(const void* q, const void* k, const void* 
     a.eps = (float)eps, a.inter = interleaved;
     rc = rope_pointers(a, what);
     if (rc != WIDEK_OK) return rc;
-    if (no_rows(a, a.hq)) return WIDEK_OK;
+    const size_t esz = dtype_size(dtype);
+    if (esz == 0) return set_error(WIDEK_ERR_INVALID, "%s: unknown dtype code %d", what, dtype);
+    if (no_rows(a, a.hq)) {                      // sums over nothing
+        for (void* dw : {dqw, dkw})
+            if (dw && a.n > 0 && a.d > 0 &&
+                cudaMemsetAsync(dw, 0, (size_t)a.n * a.d * esz, (cudaStream_t)stream) != cudaSuccess)
+                return check_launch(what);
+        return WIDEK_OK;
+    }
     if (!dk || !dyq || !dyk) return set_error(WIDEK_ERR_INVALID, "%s: null pointer", what);
     const int64_t need = widek_qk_norm_rope_bwd_workspace(geom);
     if (!workspace || workspace_bytes < need || !aligned_to(workspace, sizeof(float)))
         return set_error(WIDEK_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed", what,
                          (long long)workspace_bytes, (long long)need);
     g.dyq = dyq, g.dyk = dyk, g.dqw = dqw, g.dkw = dkw, g.part = static_cast<float*>(workspace);
-    const size_t esz = dtype_size(dtype);
-    if (esz == 0) return set_error(WIDEK_ERR_INVALID, "%s: unknown dtype code %d", what, dtype);
     const int vec = row_vec(a, esz, {qw, kw, dyq, dyk, dq, dk}, false);
     const int hpt = grad_heads(vec, esz);
     rc = row_units(a, what, 1, 1, 1);            // the narrowest: units of one head, for the size check

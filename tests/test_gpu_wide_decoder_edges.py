@@ -223,3 +223,19 @@ def test_step_first_traced_in_one_graph():
     caches = [m.new_cache(2, 8, page_size=4) for m in (layer, ref)]
     step = torch.compile(layer.step, fullgraph=True, backend="eager")
     assert torch.equal(step(x, caches[0], ln), ref.step(x, caches[1], ln))
+
+
+def test_gradient_entry_without_rows_gives_weight_gradients_of_zero():
+    """The C entry, for callers other than ops.qk_norm_rope_bwd."""
+    import struct
+    n, b, t, hq, hk, d = 2, 3, 0, 4, 2, 64
+    geom = struct.pack('=23q', n, b, t, hq, hk, d, d, 8, *[d] * 12, 0, t, 1)
+    lib = _native.lib()
+    for dtype, code in ((F32, _native.F32), (BF16, _native.BF16)):
+        dqw, dkw = (torch.full((n, d), float('nan'), device=DEV, dtype=dtype) for _ in range(2))
+        rc = lib.widek_qk_norm_rope_bwd(*[None] * 11, dqw.data_ptr(), dkw.data_ptr(), geom, 1e-6, 0, 0, code, None, 0,
+                                        torch.cuda.current_stream().cuda_stream)
+        assert rc == _native.WIDEK_OK
+        assert float(dqw.abs().max()) == 0.0 and float(dkw.abs().max()) == 0.0
+        rc = lib.widek_qk_norm_rope_bwd(*[None] * 13, geom, 1e-6, 0, 0, code, None, 0, None)
+        assert rc == _native.WIDEK_OK
