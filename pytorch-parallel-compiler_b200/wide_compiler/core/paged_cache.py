@@ -74,6 +74,8 @@ class WidePagedCache:
                  dtype: torch.dtype = torch.bfloat16, device='cuda') -> 'WidePagedCache':
         """A cache with room for ``max_len`` tokens of every sequence, its
         pages handed out in order (one table for all models)."""
+        if page_size < 1 or max_len < 0:
+            raise ValueError(f"WidePagedCache: pages of {page_size} tokens for {max_len}")
         cols = -(-max_len // page_size)
         shape = (n, batch * cols, kv_heads, page_size, head_dim)
         k, v = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)

@@ -1131,7 +1131,8 @@ def qk_norm_rope_write(q: Tensor, k: Tensor, v: Tensor, q_weight: Tensor, k_weig
     """``qk_norm_rope`` whose keys go, with the values, straight into the
     cache at their positions: one launch for a decoder step
     (widek_qk_norm_rope_write_fwd). An 8-bit cache is quantised from the fp32
-    keys. Padding rows (negative positions) write nothing. Returns q'."""
+    keys. Padding rows (negative positions) write nothing; the slots of the
+    others must differ. Returns q'."""
     what = "qk_norm_rope_write"
     _no_grad(what, q, k, v, q_weight, k_weight)
     if _compiling():
@@ -1151,7 +1152,8 @@ def qk_norm_rope_write(q: Tensor, k: Tensor, v: Tensor, q_weight: Tensor, k_weig
 def cache_write(cache, k: Tensor, v: Tensor, positions: Tensor) -> None:
     """Writes k, v [N, B, T, Hk, D] to the cache at ``positions`` ([T],
     [B, T] or [N, B, T]; negative: not written), quantising each (token, head)
-    row for an 8-bit cache (widek_cache_write_fwd)."""
+    row for an 8-bit cache (widek_cache_write_fwd). The slots of one call must
+    differ: two rows written to one may mix."""
     what = "cache_write"
     _no_grad(what, k, v)
     if _compiling():
@@ -1224,7 +1226,8 @@ def decode_attention(q: Tensor, cache, lengths: Tensor, scale: Optional[float] =
     head h // (Hq / Hk)); lengths int32/int64 [B] or [N, B]: tokens visible,
     the new one included; scale defaults to 1/sqrt(D); window > 0: only the
     last ``window`` of them. Returns [N, B, Hq, D]; zeros for a sequence
-    without tokens."""
+    without tokens. Slots that no sequence sees may hold anything; an infinity
+    in a visible row may come out as NaN (rows are split into pieces)."""
     what = "decode_attention"
     _no_grad(what, q)
     if scale is None:

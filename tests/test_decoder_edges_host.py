@@ -235,3 +235,10 @@ def test_gradient_entry_refuses_a_workspace_that_floats_cannot_lie_in():
     P = 16                               # stand-in pointers: never dereferenced on this path
     rc = lib.widek_qk_norm_rope_bwd(*[P] * 13, geom, 1e-6, 0, 0, N.BF16, P + 2, size, None)
     assert rc == N.WIDEK_ERR_INVALID and "workspace" in N.last_error()
+
+
+def test_cache_sizes_that_make_no_pages_are_refused():
+    for kw in (dict(max_len=8, page_size=0), dict(max_len=8, page_size=-4), dict(max_len=-1, page_size=4)):
+        with pytest.raises(ValueError, match="page"):
+            wc.WidePagedCache.allocate(1, 2, 1, 8, device='cpu', **kw)
+    assert wc.WidePagedCache.allocate(1, 2, 1, 8, max_len=0, page_size=4, device='cpu').max_len == 0
