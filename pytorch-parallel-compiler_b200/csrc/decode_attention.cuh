@@ -269,9 +269,9 @@ enum RowsAre : int { ROWS_ANY, ROWS_BYTES, ROWS_16, ROWS_FULL };
 // rows, allows (below 4 bytes: copy_elements). ROWS_BYTES are rows of such
 // sizes in a pool that starts on a word: they come as the words that they lie
 // in, so that channel 0 is up to 3 bytes into the first place (`off` then
-// counts from there), and the reader shifts. A 265 MB e4m3 cache with rows of
-// 138 bytes takes 221 us so, 1150 us by elements; rows of 136 bytes take 170
-// us, of 128 bytes 63.
+// counts from there), and the reader shifts. A 223 MB e4m3 cache with rows of
+// 138 bytes takes 210 us so (a 265 MB one 221 us, 1150 us by elements); rows of
+// 136 bytes take 163 us, of 128 bytes 57.
 template <int ROWS>
 __device__ __forceinline__ void copy_place(uint32_t dst, const uint8_t* row, int off, int bytes, int grain,
                                            bool live) {

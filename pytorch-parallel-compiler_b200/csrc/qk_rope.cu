@@ -20,11 +20,12 @@
 // and the norm one reduction. Every channel is read once and written once,
 // in 16-byte vectors where sizes and strides allow it.
 //
-// Bound by memory (2 D bytes in and out per row of a 16-bit type) but near the
-// instructions' bound: at the copy rate there is time for about 7 of them a
-// channel. So four heads of a token share its angles, weights and addresses,
-// the weights are folded into the angles' coefficients, fp32 arithmetic runs
-// two to an instruction, and codes and values change form by byte permutes.
+// Bound by memory (2 D bytes in and out per row of a 16-bit type), not far from
+// the instructions' bound: at the copy rate there is time for about 22 of them
+// a channel, and norm + rotation takes 15. So four heads of a token share its
+// angles, weights and addresses, the weights are folded into the angles'
+// coefficients, fp32 arithmetic runs two to an instruction, and codes and values
+// change form by byte permutes.
 // Measured (B200, floor at the measured copy rate): norm + rotation of 168 M
 // bf16 values 137 us (103), its backward over 84 M 113 us (77), int8 write of
 // 268 M 183 us (124), read 127 us (125).
@@ -795,7 +796,9 @@ int launch_rows_fmt(const RowArgs& a, int vec, int hpt, const char* what, int fm
     return launch_rows<OUT_SAME, ROPE>(a, vec, hpt, what, dtype, st);
 }
 
-constexpr int kGradBlocks = 444;  // of the backward over all models, 3 for each SM: twice as many cost the join what they gave
+// Blocks of the backward over all models, 3 for each SM of a B200: twice as many
+// cost the join what they gave.
+constexpr int kGradBlocks = 3 * 148;
 constexpr int kGradHeads = 2;     // heads at once in the backward, whose rows take twice the registers
 constexpr int grad_heads(int vec, size_t) { return vec >= 4 ? kGradHeads : 1; }
 
