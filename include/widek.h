@@ -728,6 +728,61 @@ WIDEK_API int widek_decode_attention_fwd(const void* q, const void* kc, const vo
                                          int len64, int fmt, int dtype, void* workspace,
                                          int64_t workspace_bytes, void* stream);
 
+/* ---- Block boundaries: the residual stream and its norms, rows as codes ---
+ *
+ * No counterpart in the reference (its norms and additions are separate
+ * torch calls, wide_compiler/core/primitives/wide_layernorm.py:62-65 and
+ * wide_compiler/core/traced_wide.py:189-211).
+ *
+ * Common arguments:
+ *   x, y, h, z [n, rows, d] dense; w, wb (norm of h), pw, pb (norm of y) [n, d],
+ *     all but w nullable: no pw, no norm of y; y itself NULL: h = x.
+ *   gate: dense rows of d channels, one for every gate_rows rows (gate_rows
+ *     divides rows: `rows` for one a model, 1 for one a row), or NULL with -1.
+ *   center: 1 LayerNorm, 0 RMS norm (which takes no wb and pb).
+ *   d <= 8192. */
+
+/* h = x + scale * gate * u with u = norm(y; pw, pb), or y; z = norm(h; w, b),
+ * of the unrounded h. stats (nullable, what widek_residual_norm_bwd needs):
+ * [n * rows][4] floats on a 16-byte border. h is not written without y. */
+WIDEK_API int widek_residual_norm_fwd(const void* x, const void* y, const void* w, const void* wb,
+                                      const void* pw, const void* pb, const void* gate, void* h,
+                                      void* z, float* stats, int64_t n, int64_t rows, int64_t d,
+                                      int64_t gate_rows, double scale, double eps, int center,
+                                      int dtype, void* stream);
+
+/* The same with z as int8 codes, rows `ld` bytes apart (ld >= d, a multiple of
+ * 16; bytes past d are left as they were), and one scale a row: scale =
+ * max(max|z|, 2^-40) / 127 in fp32, code = z / scale rounded half to even. A
+ * row that holds an infinity or a NaN gets such a scale and codes of 0. */
+WIDEK_API int widek_residual_norm_quantize_fwd(const void* x, const void* y, const void* w,
+                                               const void* wb, const void* pw, const void* pb,
+                                               const void* gate, void* h, void* codes, float* scales,
+                                               int64_t ld, int64_t n, int64_t rows, int64_t d,
+                                               int64_t gate_rows, double scale, double eps, int center,
+                                               int dtype, void* stream);
+
+/* Such codes of the rows of x [rows, d], x_ld elements apart (any d). */
+WIDEK_API int widek_quantize_rows_fwd(const void* x, void* codes, float* scales, int64_t rows,
+                                      int64_t d, int64_t x_ld, int64_t ld, int dtype, void* stream);
+
+/* Workspace bytes widek_residual_norm_bwd needs (-1 for bad arguments);
+ * gate_rows as there, has_post: with pw. */
+WIDEK_API int64_t widek_residual_norm_bwd_workspace(int64_t n, int64_t rows, int64_t d,
+                                                    int64_t gate_rows, int has_post, int center);
+
+/* Gradients of widek_residual_norm_fwd from its inputs and stats: dh, dz
+ * (nullable: zeros) [n, rows, d] dense; dx, dy like x, dw, dwb, dpw, dpb [n, d],
+ * dgate like gate, each nullable. With rows = 0 nothing is written. Sums over
+ * rows are taken in a fixed order. n <= 65535. */
+WIDEK_API int widek_residual_norm_bwd(const void* x, const void* y, const void* w, const void* wb,
+                                      const void* pw, const void* pb, const void* gate,
+                                      const float* stats, const void* dh, const void* dz, void* dx,
+                                      void* dy, void* dw, void* dwb, void* dpw, void* dpb, void* dgate,
+                                      int64_t n, int64_t rows, int64_t d, int64_t gate_rows,
+                                      double scale, double eps, int center, int dtype,
+                                      void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

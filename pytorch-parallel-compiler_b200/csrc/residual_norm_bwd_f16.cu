@@ -1,0 +1,5 @@
+// Gradients of the residual norm for f16 tensors.
+#define WIDEK_RNORM_BWD_BODY
+#include "residual_norm_bwd.cuh"
+
+template int widek::rnorm::BwdLaunch::run<__half>();

@@ -336,6 +336,29 @@ def _norm_rope_t(x: Tensor, weight: Tensor, cos: Tensor, sin: Tensor, positions:
     return torch.where(keep, y, torch.zeros_like(y)).to(x.dtype)
 
 
+def _norm_t(v: Tensor, weight: Tensor, bias: Optional[Tensor], eps: float, center: bool) -> Tensor:
+    shape = (v.shape[0],) + (1,) * (v.dim() - 2) + (v.shape[-1],)
+    v = v - v.mean(-1, keepdim=True) if center else v
+    v = v * torch.rsqrt((v * v).mean(-1, keepdim=True) + eps) * weight.float().view(shape)
+    return v if bias is None else v + bias.float().view(shape)
+
+
+def residual_norm_t(x, y, weight, bias, post_weight, post_bias, gate, scale, eps, center):
+    """(h, z) of ops.residual_norm in fp32, each rounded once."""
+    u = y.float()
+    if post_weight is not None:
+        u = _norm_t(u, post_weight, post_bias, eps, center)
+    if gate is not None:
+        u = u * gate.float().view(gate.shape[:-1] + (1,) * (x.dim() - gate.dim()) + gate.shape[-1:])
+    h = x.float() + scale * u
+    return h.to(x.dtype), _norm_t(h, weight, bias, eps, center).to(x.dtype)
+
+
+def row_norm_t(x, y, weight, bias, post_weight, post_bias, gate, scale, eps, center):
+    """z of ops.residual_norm without y."""
+    return _norm_t(x.float(), weight, bias, eps, center).to(x.dtype)
+
+
 def qk_norm_rope_t(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, cos: Tensor, sin: Tensor,
                    positions: Tensor, eps: float, interleaved: bool):
     return (_norm_rope_t(q, q_weight, cos, sin, positions, eps, interleaved),
@@ -440,6 +463,34 @@ class QkNormRopeFn(torch.autograd.Function):
         grads = ops.qk_norm_rope_bwd(q, k, qw, kw, cos, sin, positions, dyq, dyk, ctx.eps, ctx.interleaved,
                                      need_dw=need[2] or need[3])
         return (*(g if want else None for g, want in zip(grads, need[:4])), None, None, None, None, None)
+
+
+class ResidualNormFn(torch.autograd.Function):
+    """Residual sum, gate and norms of a block boundary (z alone where y is
+    None); backward: widek_residual_norm_bwd on the inputs and the rows'
+    statistics."""
+
+    @staticmethod
+    def forward(ctx, x, y, weight, bias, post_weight, post_bias, gate, scale, eps, center):
+        from . import ops
+        h, z, stats = ops._residual_norm(x, y, weight, bias, post_weight, post_bias, gate, scale, eps, center, True)
+        ctx.scale, ctx.eps, ctx.center, ctx.has_y = scale, eps, center, y is not None
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, y, weight, bias, post_weight, post_bias, gate, stats)
+        return (h, z) if ctx.has_y else z
+
+    @staticmethod
+    def backward(ctx, *grads):
+        from . import ops
+        *tensors, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad[:7]
+        dh, dz = grads if ctx.has_y else (None, grads[0])
+        if dh is None and dz is None:
+            return (None,) * 10
+        if torch.is_grad_enabled():          # a gradient of these gradients is asked for: the kernel's have no graph
+            return torch_grads(residual_norm_t if ctx.has_y else row_norm_t,
+                               (*tensors, ctx.scale, ctx.eps, ctx.center), (*need, False, False, False), grads)
+        return (*ops.residual_norm_bwd(*tensors, stats, dh, dz, ctx.scale, ctx.eps, ctx.center, need), None, None, None)
 
 
 class Swap01Fn(torch.autograd.Function):

@@ -115,12 +115,18 @@ SIGNATURES = {
     "widek_decode_attention_workspace": [_geom, _geom, _i64, _int],
     "widek_decode_attention_fwd": [_c_void_p] * 8 + [_geom, _geom, _dbl, _i64, _int, _int, _int, _c_void_p, _i64,
                                                      _c_void_p],
+    "widek_residual_norm_fwd": [_c_void_p] * 10 + [_i64] * 4 + [_dbl, _dbl, _int, _int, _c_void_p],
+    "widek_residual_norm_quantize_fwd": [_c_void_p] * 10 + [_i64] * 5 + [_dbl, _dbl, _int, _int, _c_void_p],
+    "widek_quantize_rows_fwd": [_c_void_p] * 3 + [_i64] * 4 + [_int, _c_void_p],
+    "widek_residual_norm_bwd_workspace": [_i64] * 4 + [_int, _int],
+    "widek_residual_norm_bwd": [_c_void_p] * 17 + [_i64] * 4 + [_dbl, _dbl, _int, _int, _c_void_p, _i64, _c_void_p],
 }
 RESTYPES = {"widek_batchnorm_train_workspace": ctypes.c_size_t, "widek_conv_workspace": ctypes.c_size_t,
             "widek_rnn_workspace": ctypes.c_size_t, "widek_conv_packed_weight_elems": _i64,
             "widek_launch_count": ctypes.c_longlong, "widek_linear_bwd_workspace": _i64,
             "widek_layernorm_bwd_workspace": _i64, "widek_groupnorm_bwd_workspace": _i64,
-            "widek_qk_norm_rope_bwd_workspace": _i64, "widek_decode_attention_workspace": _i64}
+            "widek_qk_norm_rope_bwd_workspace": _i64, "widek_decode_attention_workspace": _i64,
+            "widek_residual_norm_bwd_workspace": _i64}
 
 
 class WideKernelError(RuntimeError):

@@ -1255,6 +1255,153 @@ def decode_attention(q: Tensor, cache, lengths: Tensor, scale: Optional[float] =
 
 
 # ---------------------------------------------------------------------------
+# Block boundaries: the residual stream and its norms, rows as 8-bit codes
+# ---------------------------------------------------------------------------
+
+def _block_args(what: str, x: Tensor, y: Optional[Tensor], weight: Tensor, bias: Optional[Tensor],
+                post_weight: Optional[Tensor], post_bias: Optional[Tensor], gate: Optional[Tensor]):
+    """Checks the tensors of a residual norm; returns the device's index, the
+    dense tensors and (n, rows, d, gate_rows)."""
+    idx = _device(what, x, y, weight, bias, post_weight, post_bias, gate)
+    _same_dtype(what, x, y, weight, bias, post_weight, post_bias, gate)
+    shape = x.shape
+    if len(shape) < 2:
+        raise ValueError(f"{what}: x must be [N, ..., D], got {tuple(shape)}")
+    if y is not None and y.shape != shape:
+        raise ValueError(f"{what}: y {tuple(y.shape)} does not match x {tuple(shape)}")
+    n, d = shape[0], shape[-1]
+    for name, p in (("weight", weight), ("bias", bias), ("post_weight", post_weight), ("post_bias", post_bias)):
+        if p is not None and p.shape != (n, d):
+            raise ValueError(f"{what}: {name} must be [N, D] = [{n}, {d}], got {tuple(p.shape)}")
+    rows, gate_rows = math.prod(shape[1:-1]), -1
+    if gate is not None:
+        lead = gate.dim() - 1
+        if lead < 1 or lead >= len(shape) or gate.shape[:-1] != shape[:lead] or gate.shape[-1] != d:
+            raise ValueError(f"{what}: gate {tuple(gate.shape)} is not [N, D], or leading dims of x {tuple(shape)} and D")
+        gate_rows = math.prod(shape[lead:-1])
+    dense = [t if t is None or t.is_contiguous() else t.contiguous()
+             for t in (x, y, weight, bias, post_weight, post_bias, gate)]
+    return idx, dense, (n, rows, d, gate_rows)
+
+
+def residual_norm(x: Tensor, y: Optional[Tensor], weight: Tensor, bias: Optional[Tensor] = None,
+                  post_weight: Optional[Tensor] = None, post_bias: Optional[Tensor] = None,
+                  gate: Optional[Tensor] = None, scale: float = 1.0, eps: float = 1e-6, center: bool = False):
+    """The residual stream after a block and the norm before the next one, in
+    one pass (widek_residual_norm_fwd; differentiable):
+
+        u = norm(y; post_weight, post_bias), or y without ``post_weight``
+        h = x + scale * gate * u
+        z = norm(h; weight, bias)
+
+    x, y [N, ..., D] (D <= 8192), weights and biases [N, D]; RMS norms, or
+    LayerNorm (``center``), which alone has biases. ``gate``: [N, D] (one for
+    each model) or x's leading dims and D ([N, B, D] for each sequence,
+    [N, B, T, D] for each token). z is taken from the unrounded h. y None: h is
+    x itself. Returns (h, z)."""
+    if _compiling():
+        if y is None:
+            return x, torch.ops.widek.row_norm(x, weight, bias, eps, center)
+        return torch.ops.widek.residual_norm(x, y, weight, bias, post_weight, post_bias, gate, scale, eps, center)
+    if _AG.needs_grad(x, y, weight, bias, post_weight, post_bias, gate):
+        out = _AG.ResidualNormFn.apply(x, y, weight, bias, post_weight, post_bias, gate, scale, eps, center)
+        return (x, out) if y is None else out
+    return _residual_norm(x, y, weight, bias, post_weight, post_bias, gate, scale, eps, center, False)[:2]
+
+
+def _residual_norm(x, y, weight, bias, post_weight, post_bias, gate, scale, eps, center, need_stats: bool):
+    idx, dense, sizes = _block_args("residual_norm", x, y, weight, bias, post_weight, post_bias, gate)
+    h = x if y is None else x.new_empty(x.shape)
+    z = x.new_empty(x.shape)
+    stats = torch.empty((sizes[0], sizes[1], 4), device=x.device, dtype=torch.float32) if need_stats else None
+    _launch(idx, "widek_residual_norm_fwd", *map(N.ptr, dense), N.ptr(h), z.data_ptr(), N.ptr(stats), *sizes, scale, eps,
+            center, N.dtype_code(x))
+    return h, z, stats
+
+
+def residual_norm_bwd(x: Tensor, y: Optional[Tensor], weight: Tensor, bias: Optional[Tensor],
+                      post_weight: Optional[Tensor], post_bias: Optional[Tensor], gate: Optional[Tensor], stats: Tensor,
+                      dh: Optional[Tensor], dz: Optional[Tensor], scale: float = 1.0, eps: float = 1e-6,
+                      center: bool = False, need: Sequence[bool] = (True,) * 7):
+    """Gradients of ``residual_norm`` for its seven tensors, None for those that
+    are None or that ``need`` leaves out (widek_residual_norm_bwd). ``stats``: the
+    forward's [N, rows, 4]; dh, dz None: zeros."""
+    what = "residual_norm backward"
+    idx, dense, sizes = _block_args(what, x, y, weight, bias, post_weight, post_bias, gate)
+    _device(what, x, stats, dh, dz)
+    for g in (dh, dz):
+        if g is not None and g.shape != x.shape:
+            raise ValueError(f"{what}: a gradient {tuple(g.shape)} for {tuple(x.shape)}")
+    _same_dtype(what, x, dh, dz)
+    if stats.shape != (sizes[0], sizes[1], 4) or stats.dtype != torch.float32 or not stats.is_contiguous():
+        raise ValueError(f"{what}: stats must be dense float32 [N, rows, 4]")
+    if x.numel() == 0:
+        return [torch.zeros_like(t) if t is not None and k else None for t, k in zip(dense, need)]
+    grads = [torch.empty_like(t) if t is not None and k else None for t, k in zip(dense, need)]
+    has_post = post_weight is not None
+    ws_bytes = _workspace("widek_residual_norm_bwd_workspace", idx, ("residual_norm_bwd", *sizes, has_post, center, idx),
+                          *sizes, has_post, center)
+    ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8)
+    dh, dz = (g if g is None or g.is_contiguous() else g.contiguous() for g in (dh, dz))
+    _launch(idx, "widek_residual_norm_bwd", *map(N.ptr, dense), stats.data_ptr(), N.ptr(dh), N.ptr(dz),
+            *map(N.ptr, grads), *sizes, scale, eps, center, N.dtype_code(x), ws.data_ptr(), ws_bytes)
+    return grads
+
+
+def _code_rows(x: Tensor) -> Tensor:
+    """Room for the codes of x's rows, which start 16 bytes (or a multiple) apart."""
+    d = x.shape[-1]
+    if d % 16 == 0:
+        return torch.empty(x.shape, device=x.device, dtype=torch.int8)
+    return torch.empty((*x.shape[:-1], -(-d // 16) * 16), device=x.device, dtype=torch.int8)[..., :d]
+
+
+def residual_norm_quantize(x: Tensor, y: Optional[Tensor], weight: Tensor, bias: Optional[Tensor] = None,
+                           post_weight: Optional[Tensor] = None, post_bias: Optional[Tensor] = None,
+                           gate: Optional[Tensor] = None, scale: float = 1.0, eps: float = 1e-6, center: bool = False):
+    """``residual_norm`` with z as the codes that ``linear_int8`` takes
+    (widek_residual_norm_quantize_fwd): returns (h, codes, scales), codes int8
+    like x and scales float32 like x without its last dim, quantised from the
+    fp32 z (see ``quantize_rows``). No gradient."""
+    what = "residual_norm_quantize"
+    _no_grad(what, x, y, weight, bias, post_weight, post_bias, gate)
+    if _compiling():
+        if y is None:
+            return x, *torch.ops.widek.row_norm_quantize(x, weight, bias, eps, center)
+        return torch.ops.widek.residual_norm_quantize(x, y, weight, bias, post_weight, post_bias, gate, scale, eps,
+                                                      center)
+    idx, dense, sizes = _block_args(what, x, y, weight, bias, post_weight, post_bias, gate)
+    h = x if y is None else x.new_empty(x.shape)
+    codes = _code_rows(x)
+    scales = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    _launch(idx, "widek_residual_norm_quantize_fwd", *map(N.ptr, dense), N.ptr(h), codes.data_ptr(), scales.data_ptr(),
+            -(-sizes[2] // 16) * 16, *sizes, scale, eps, center, N.dtype_code(x))
+    return h, codes, scales
+
+
+def quantize_rows(x: Tensor):
+    """Rows x [..., K] as int8 codes with one float32 scale each: (codes, scales)
+    with x ~ codes * scales[..., None], scale = max(max|x|, 2^-40) / 127, code =
+    x / scale rounded half to even (widek_quantize_rows_fwd). Activations and
+    weights for ``linear_int8``. A row that holds an infinity or a NaN gets such
+    a scale. Rows of codes start a multiple of 16 bytes apart. No gradient."""
+    what = "quantize_rows"
+    _no_grad(what, x)
+    if _compiling():
+        return torch.ops.widek.quantize_rows(x)
+    idx = _device(what, x)
+    if x.dim() < 1:
+        raise ValueError(f"{what}: x must be [..., K], got a number")
+    k = x.shape[-1]
+    xd = x if x.is_contiguous() else x.contiguous()
+    codes = _code_rows(x)
+    scales = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    _launch(idx, "widek_quantize_rows_fwd", xd.data_ptr(), codes.data_ptr(), scales.data_ptr(), scales.numel(), k, k,
+            -(-k // 16) * 16, N.dtype_code(x))
+    return codes, scales
+
+
+# ---------------------------------------------------------------------------
 # Convolutions
 # ---------------------------------------------------------------------------
 

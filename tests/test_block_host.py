@@ -1,0 +1,103 @@
+"""Refusals of the block-boundary operators: arguments are checked before any
+device call, so no GPU is needed."""
+import pytest
+import torch
+
+from wide_compiler import _native as N
+from wide_compiler import ops
+
+P = 1024                                 # a stand-in pointer: never dereferenced on these paths
+
+
+def rnorm(x=P, y=P, w=P, wb=None, pw=None, pb=None, gate=None, h=P, z=P, stats=None, n=2, rows=6, d=64, gate_rows=-1,
+          scale=1.0, eps=1e-6, center=0, dtype=N.BF16):
+    return N.lib().widek_residual_norm_fwd(x, y, w, wb, pw, pb, gate, h, z, stats, n, rows, d, gate_rows, scale, eps,
+                                           center, dtype, None)
+
+
+@pytest.mark.parametrize("bad, word", [
+    (dict(n=-1), "sizes"), (dict(rows=-1), "sizes"), (dict(d=0), "sizes"), (dict(d=8193), "8192"),
+    (dict(dtype=9), "dtype"), (dict(n=3, rows=0x40000000), "2^31"), (dict(gate=P, gate_rows=4), "gate"),
+    (dict(gate=P), "gate"), (dict(gate_rows=6), "gate"), (dict(y=None, pw=P), "no y"),
+    (dict(y=None, gate=P, gate_rows=6), "no y"), (dict(pb=P, center=1), "without its weight"), (dict(wb=P), "LayerNorm"),
+    (dict(pw=P, pb=P), "LayerNorm"), (dict(x=None), "null"), (dict(w=None), "null"), (dict(z=None), "null"),
+    (dict(h=None), "null"), (dict(stats=P + 4), "border")])
+def test_forward_refuses(bad, word):
+    assert rnorm(**bad) == N.WIDEK_ERR_INVALID
+    assert word in N.last_error()
+
+
+def test_no_rows_is_no_call():
+    assert rnorm(x=None, y=None, w=None, h=None, z=None, n=0) == 0
+    assert rnorm(x=None, y=None, w=None, h=None, z=None, rows=0) == 0
+    assert N.lib().widek_quantize_rows_fwd(None, None, None, 0, 7, 7, 16, N.F32, None) == 0
+
+
+def test_codes_refuse():
+    lib = N.lib()
+    call = lambda ld, codes=P, d=64: lib.widek_residual_norm_quantize_fwd(
+        P, P, P, None, None, None, None, P, codes, P, ld, 2, 6, d, -1, 1.0, 1e-6, 0, N.BF16, None)
+    for args in ((60,), (72,), (64, P + 8)):
+        assert call(*args) == N.WIDEK_ERR_INVALID
+        assert "16 bytes" in N.last_error()
+    quant = lambda rows=3, d=64, x_ld=64, ld=64, x=P, scales=P, dtype=N.F32: lib.widek_quantize_rows_fwd(
+        x, P, scales, rows, d, x_ld, ld, dtype, None)
+    for bad in (dict(rows=-1), dict(d=-1), dict(ld=63), dict(ld=72), dict(x=None), dict(scales=None), dict(dtype=7)):
+        assert quant(**bad) == N.WIDEK_ERR_INVALID
+
+
+def test_backward_refuses(monkeypatch):
+    lib = N.lib()
+    assert lib.widek_residual_norm_bwd_workspace(2, 6, 0, -1, 0, 0) == -1
+    assert lib.widek_residual_norm_bwd_workspace(2, 6, 9000, -1, 0, 0) == -1
+
+    def bwd(y=P, pw=None, gate=None, stats=P, dy=None, dwb=None, dpw=None, dpb=None, dgate=None, n=2, rows=6, d=64,
+            gate_rows=-1, center=0, ws=P, ws_bytes=1 << 30):
+        return lib.widek_residual_norm_bwd(P, y, P, None, pw, None, gate, stats, P, P, P, dy, P, dwb, dpw, dpb, dgate, n,
+                                           rows, d, gate_rows, 1.0, 1e-6, center, N.BF16, ws, ws_bytes, None)
+
+    for bad, word in ((dict(y=None, dy=P), "not there"), (dict(dpw=P), "not there"), (dict(dgate=P), "not there"),
+                      (dict(dwb=P), "not there"), (dict(ws=None), "workspace"), (dict(ws_bytes=8), "workspace"),
+                      (dict(ws=P + 2), "workspace"), (dict(stats=None), "statistics"), (dict(stats=P + 8), "statistics")):
+        assert bwd(**bad) == N.WIDEK_ERR_INVALID
+        assert word in N.last_error(), bad
+    assert bwd(n=70000, rows=1) == N.WIDEK_ERR_UNSUPPORTED
+    assert bwd(rows=0) == 0
+
+
+def test_operators_refuse_cpu_tensors():
+    x, w = torch.zeros(2, 3, 8), torch.ones(2, 8)
+    for call in (lambda: ops.residual_norm(x, x, w), lambda: ops.residual_norm_quantize(x, x, w),
+                 lambda: ops.quantize_rows(x)):
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+            call()
+
+
+def test_operators_refuse_gradients_they_do_not_have():
+    x, w = torch.zeros(2, 3, 8, requires_grad=True), torch.ones(2, 8)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.residual_norm_quantize(x, x, w)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.quantize_rows(x)
+
+
+@pytest.mark.parametrize("change, error, word", [
+    (dict(y=(2, 3, 9)), ValueError, "does not match"), (dict(weight=(8,)), ValueError, "weight"),
+    (dict(weight=(3, 8)), ValueError, "weight"), (dict(post_weight=(2, 7)), ValueError, "post_weight"),
+    (dict(gate=(8,)), ValueError, "gate"), (dict(gate=(2, 2, 8)), ValueError, "gate"),
+    (dict(gate=(2, 3, 1, 8)), ValueError, "gate"), (dict(gate=(2, 3, 1)), ValueError, "gate"),
+    (dict(x=(8,), y=(8,)), ValueError, "x must be")])
+def test_shapes_are_checked(change, error, word, monkeypatch):
+    monkeypatch.setattr(ops, "_device", lambda what, ref, *others: 0)
+    shapes = dict(dict(x=(2, 3, 8), y=(2, 3, 8), weight=(2, 8)), **change)
+    with torch.no_grad(), pytest.raises(error, match=word):
+        ops.residual_norm(**{k: torch.zeros(s) for k, s in shapes.items()})
+
+
+def test_types_are_checked(monkeypatch):
+    monkeypatch.setattr(ops, "_device", lambda what, ref, *others: 0)
+    x, w = torch.zeros(2, 3, 8), torch.ones(2, 8)
+    with torch.no_grad(), pytest.raises(TypeError, match="mismatch"):
+        ops.residual_norm(x, x, w.half())
+    with torch.no_grad(), pytest.raises(TypeError, match="support"):
+        ops.quantize_rows(torch.zeros(2, 8, dtype=torch.int32))
