@@ -783,6 +783,21 @@ WIDEK_API int widek_residual_norm_bwd(const void* x, const void* y, const void* 
                                       double scale, double eps, int center, int dtype,
                                       void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- Linear layers on 8-bit codes ----------------------------------------
+ * y[i] = act((sum_k a[i, m, k] w[i, o, k]) a_scale[i, m] w_scale[i, o] +
+ * bias[i, o]): codes of widek_quantize_rows_fwd, the sum exact in int32, the
+ * rest in fp32, rounded once to y's dtype (which bias, nullable, has too).
+ *   a [n, m, k] rows a_ld bytes apart, models a_ms; w [n, o, k] likewise: 16-byte
+ *   borders and multiples, models behind one another, what lies between rows is
+ *   not used. a_scale [n, m],
+ *   w_scale [n, o], y [n, m, o] dense. 1 <= k <= 131071.
+ * No counterpart in the reference (its linear layers,
+ * wide_compiler/core/primitives/wide_linear.py:162-171, have no 8-bit form). */
+WIDEK_API int widek_linear_int8_fwd(const void* a, const float* a_scale, const void* w,
+                                    const float* w_scale, const void* bias, void* y, int64_t n,
+                                    int64_t m, int64_t k, int64_t o, int64_t a_ld, int64_t a_ms,
+                                    int64_t w_ld, int64_t w_ms, int act, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,583 @@
+// Linear layers of n models on 8-bit codes, on the tensor cores (tcgen05 kind::i8):
+//
+//   y[i, m, o] = act((sum_k a[i, m, k] w[i, o, k]) sa[i, m] sw[i, o] + bias[i, o])
+//
+// The sum is exact in int32 (K <= 131071 keeps it below 2^31); the scales, the
+// bias and the activation are fp32, rounded once to y's type.
+//
+// Two kernels. Both stream 128-code (one swizzle row) blocks of K by TMA into a
+// ring, one thread issuing the MMAs into TMEM:
+//   wide    many rows: a cluster of two CTAs holds a 256 x 256 tile (cta_group::2),
+//           each SM half of both operands; persistent, the epilogue of one tile
+//           under the products of the next. A single CTA's 128 x 256 tile would
+//           move 96 KB through shared memory in the 512 clocks that its products
+//           of one K block take, over the 128 bytes a clock that it has; half of
+//           both operands is 64 KB.
+//   narrow  few rows: bound by the weights' bytes. The weights' rows are the MMA's
+//           128 lanes and up to 128 tokens its columns, so that no tensor time goes
+//           to rows that are not there; K is split over a cluster when there are
+//           too few tiles for the device, and the parts (integers: any order gives
+//           the same sum) are added through distributed shared memory.
+#include <algorithm>
+
+#include "sm100_ptx.cuh"
+
+namespace widek {
+namespace {
+
+using namespace sm100;
+
+constexpr int kBK = 128;              // codes of K in a block: one 128-byte swizzle row
+constexpr int64_t kMaxK = 131071;     // 128 * 128 * K < 2^31
+
+// Instruction descriptor, kind::i8: int32 accumulators, signed operands, K-major.
+constexpr uint32_t idesc_i8(int m, int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                             uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int c0, int c1, int c2) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(smem_addr(src)), "r"(c0), "r"(c1), "r"(c2)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t load_cluster_u32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ float finish(uint32_t acc, float sa, float sw, float bias) {
+    return fmaf((float)(int)acc * sa, sw, bias);
+}
+
+struct Int8Args {
+    const float *sa, *sw;             // [n, m], [n, o]
+    const void* bias;                 // [n, o] or null
+    void* y;                          // [n, m, o]
+    int n, m, k, o, act, vec_store;
+    int* err;
+};
+
+// ---------------------------------------------------------------------------
+// wide: 256 x 256 tiles by pairs of CTAs
+// ---------------------------------------------------------------------------
+constexpr int kWideThreads = 320;     // TMA warp, MMA warp, 2 x 4 epilogue warps
+
+template <typename T>
+struct WideSmem {
+    static constexpr int STAGES = sizeof(T) == 4 ? 4 : 5;     // what 227 KB leave room for
+    static constexpr uint32_t PART = 128 * kBK;                 // one CTA's half of an operand
+    static constexpr uint32_t RING = STAGES * 2 * PART;
+    static constexpr uint32_t OUT_CHUNK = 128 * 32 * sizeof(T);
+    static constexpr uint32_t OUT_BYTES = 4 * OUT_CHUNK;
+    static constexpr uint32_t VEC_BYTES = 2 * 128 * 8;          // (scale, bias) of each warpgroup's columns
+    static constexpr uint32_t TOTAL = 1024 + RING + OUT_BYTES + VEC_BYTES + 8 * (2 * STAGES + 5) + 16;
+    static_assert(TOTAL <= 227 * 1024, "shared memory");
+};
+
+__device__ __forceinline__ void group_sync(int wg) { asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory"); }
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
+    wide_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
+                const __grid_constant__ CUtensorMap tm_y, const Int8Args p) {
+    using S = WideSmem<T>;
+    constexpr int STAGES = S::STAGES;
+    constexpr uint32_t IDESC = idesc_i8(256, 256);
+    constexpr uint32_t TMEM_COLS = 512;      // two accumulators of 256 columns
+
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sA = smem;
+    uint8_t* sB = smem + STAGES * S::PART;
+    uint8_t* sOut = smem + S::RING;
+    float2* sVec = reinterpret_cast<float2*>(sOut + S::OUT_BYTES);
+    uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(sVec) + S::VEC_BYTES);
+    uint64_t* empty = full + STAGES;
+    uint64_t* tfull = empty + STAGES;
+    uint64_t* tempty = tfull + 2;
+    uint64_t* done = tempty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+    const int mt_count = (p.m + 255) / 256, nt_count = (p.o + 255) / 256, kb_count = (p.k + kBK - 1) / kBK;
+    const int tiles = p.n * mt_count * nt_count;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(&tfull[a], 1);
+            mbar_init(&tempty[a], 2 * 8 * 32);   // both CTAs' epilogue threads
+        }
+        mbar_init(done, 1);
+        *abort_flag = 0;
+        mbar_init_fence();
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_desc(&tm_a);
+        tma_prefetch_desc(&tm_w);
+        tma_prefetch_desc(&tm_y);
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(tmem_slot, TMEM_COLS);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    cluster_sync_all();                      // barriers of both CTAs initialised, TMEM allocated
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0) {
+        // TMA producer (both CTAs); bytes land on the leader's full barrier.
+        const uint64_t pol_a = l2_policy_evict_last();
+        const uint64_t pol_w = mt_count == 1 ? l2_policy_evict_first() : l2_policy_evict_normal();
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int tile = pair; tile < tiles && ok; tile += npairs) {
+            const int mt = tile % mt_count, rest = tile / mt_count, nt = rest % nt_count, model = rest / nt_count;
+            for (int kb = 0; kb < kb_count; ++kb) {
+                if (!mbar_wait(&empty[s], ph ^ 1, abort_flag)) { ok = false; break; }
+                if (lane == 0) {
+                    if (rank == 0) mbar_arrive_expect_tx(&full[s], 4 * S::PART);
+                    const uint32_t leader_full = map_to_rank(smem_addr(&full[s]), 0);
+                    tma_load_3d_pair(sA + s * S::PART, &tm_a, leader_full, kb * kBK, mt * 256 + (int)rank * 128, model,
+                                     pol_a);
+                    tma_load_3d_pair(sB + s * S::PART, &tm_w, leader_full, kb * kBK, nt * 256 + (int)rank * 128, model,
+                                     pol_w);
+                }
+                __syncwarp();
+                if (++s == STAGES) { s = 0; ph ^= 1; }
+            }
+        }
+        if (!ok) {
+            *abort_flag = 1;
+            raise_device_error(p.err, DEV_ERR_GEMM_TIMEOUT);
+            // This CTA's copies count on the leader's barrier; give them time
+            // to land (bounded) before the CTA's shared memory is released.
+            const uint64_t t0 = globaltimer_ns();
+            while (globaltimer_ns() - t0 < 1000000ull) { }
+        }
+    } else if (warp == 1) {
+        if (rank == 0 && lane == 0) {
+            int s = 0, local = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            const uint64_t a_desc0 = sdesc_kmajor_sw128(smem_addr(sA)), b_desc0 = sdesc_kmajor_sw128(smem_addr(sB));
+            for (int tile = pair; tile < tiles && ok; tile += npairs, ++local) {
+                const int acc = local & 1;
+                if (!mbar_wait(&tempty[acc], ((local >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t d_tmem = tmem_base + acc * 256;
+                for (int kb = 0; kb < kb_count; ++kb) {
+                    if (!mbar_wait(&full[s], ph, abort_flag)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint64_t ad = a_desc0 + (uint64_t)((s * S::PART) >> 4), bd = b_desc0 + (uint64_t)((s * S::PART) >> 4);
+#pragma unroll
+                    for (int k = 0; k < kBK / 32; ++k) umma_i8_pair(d_tmem, ad + 2 * k, bd + 2 * k, IDESC, (kb | k) != 0);
+                    umma_commit_pair_mc(&empty[s], 0x3);
+                    if (++s == STAGES) { s = 0; ph ^= 1; }
+                }
+                if (!ok) break;
+                umma_commit_pair_mc(&tfull[acc], 0x3);
+            }
+            if (!ok) {
+                *abort_flag = 1;
+                raise_device_error(p.err, DEV_ERR_GEMM_TIMEOUT);
+            }
+            umma_commit_pair_mc(done, 0x1);
+            const volatile int never = 0;
+            mbar_wait(done, 0, &never);
+        }
+        __syncwarp();
+    } else {
+        // Epilogue: warpgroup wg drains columns [128 wg, 128 wg + 128) of this
+        // CTA's 128 rows, 32 at a time through two staging buffers of its own;
+        // warp quarter q is the TMEM lanes (rows) 32 q .. 32 q + 31.
+        const int q = warp & 3, wg = (warp - 2) >> 2, ep_tid = threadIdx.x - 64 - 128 * wg;
+        uint8_t* buf0 = sOut + wg * 2 * S::OUT_CHUNK;
+        float2* vec = sVec + wg * 128;
+        const uint32_t leader_tempty0 = map_to_rank(smem_addr(&tempty[0]), 0);
+        const T* bias = static_cast<const T*>(p.bias);
+        int oc = 0, local = 0;
+        for (int tile = pair; tile < tiles; tile += npairs, ++local) {
+            const int mt = tile % mt_count, rest = tile / mt_count, nt = rest % nt_count, model = rest / nt_count;
+            const int acc = local & 1, rloc = q * 32 + lane, row0 = mt * 256 + (int)rank * 128, row = row0 + rloc;
+            const int c0 = nt * 256 + wg * 128;
+            {
+                const int c = c0 + ep_tid;
+                const int64_t at = (int64_t)model * p.o + c;
+                group_sync(wg);                          // the group has read the last tile's
+                vec[ep_tid] = c < p.o ? make_float2(p.sw[at], bias ? to_f<T>(bias[at]) : 0.f) : make_float2(0.f, 0.f);
+                group_sync(wg);
+            }
+            const float sa = row < p.m ? p.sa[(int64_t)model * p.m + row] : 0.f;
+            if (!mbar_wait(&tfull[acc], (local >> 1) & 1, abort_flag)) {
+                *abort_flag = 1;
+                raise_device_error(p.err, DEV_ERR_GEMM_TIMEOUT);
+                break;
+            }
+            tc_fence_after();
+            T* yrow = static_cast<T*>(p.y) + ((int64_t)model * p.m + row) * p.o;
+#pragma unroll 1
+            for (int c = 0; c < 128; c += 32) {
+                if (c0 + c >= p.o) break;                // warp-uniform
+                uint32_t r[32];
+                tmem_ld_32x32b_x32(tmem_base + (uint32_t)(acc * 256 + wg * 128 + c) + ((uint32_t)(q * 32) << 16), r);
+                tmem_ld_wait();
+                float v[32];
+                const float4* sv = reinterpret_cast<const float4*>(vec + c);
+#pragma unroll
+                for (int j = 0; j < 32; j += 2) {
+                    const float4 f = sv[j / 2];
+                    v[j] = finish<T>(r[j], sa, f.x, f.y);
+                    v[j + 1] = finish<T>(r[j + 1], sa, f.z, f.w);
+                }
+                if (p.act == WIDEK_ACT_RELU) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = v[j] > 0.f ? v[j] : 0.f;
+                } else if (p.act == WIDEK_ACT_GELU) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = gelu_erf(v[j]);
+                }
+                if (p.vec_store) {
+                    // Rows past m of the last tile are clipped by the store; a
+                    // CTA whose 128 rows all lie past m stores nothing.
+                    uint8_t* buf = buf0 + (oc & 1) * S::OUT_CHUNK;
+                    if (ep_tid == 0) bulk_wait_group_read<1>();
+                    group_sync(wg);
+                    constexpr int PIECES = 32 * sizeof(T) / 16, PER = 16 / sizeof(T);
+#pragma unroll
+                    for (int j = 0; j < PIECES; ++j) {
+                        const int phys = PIECES == 4 ? j ^ ((rloc >> 1) & 3) : j ^ (rloc & 7);
+                        store16<T>(reinterpret_cast<T*>(buf + rloc * 32 * sizeof(T) + phys * 16), v + PER * j);
+                    }
+                    fence_async_shared();
+                    group_sync(wg);
+                    if (ep_tid == 0 && row0 < p.m) {
+                        tma_store_3d(&tm_y, buf, c0 + c, row0, model);
+                        bulk_commit_group();
+                    }
+                    ++oc;
+                } else if (row < p.m) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (c0 + c + j < p.o) yrow[c0 + c + j] = from_f<T>(v[j]);
+                }
+            }
+            tc_fence_before();
+            mbar_arrive_remote(leader_tempty0 + acc * 8);
+        }
+        if (ep_tid == 0) bulk_wait_group_all();
+    }
+
+    tc_fence_before();
+    cluster_sync_all();                      // no CTA leaves while its pair may still touch its smem / TMEM
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, TMEM_COLS);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// narrow: 128 output channels x BN tokens, K split over a cluster
+// ---------------------------------------------------------------------------
+constexpr int kNarrowThreads = 128;
+
+template <typename T, int BN>
+__global__ void __launch_bounds__(kNarrowThreads)
+    narrow_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w, const Int8Args p,
+                  int split, int stages) {
+    constexpr uint32_t W_BYTES = 128 * kBK, A_BYTES = BN * kBK;
+    constexpr uint32_t IDESC = idesc_i8(128, BN);
+    constexpr uint32_t TMEM_COLS = BN < 32 ? 32 : BN;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t full[8], empty[8], tfull;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_word;
+    volatile int* abort_flag = &abort_word;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sW = smem;
+    uint8_t* sA = smem + stages * W_BYTES;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    const int ot_count = (p.o + 127) / 128, mt_count = (p.m + BN - 1) / BN, kb_count = (p.k + kBK - 1) / kBK;
+    const int rank = blockIdx.x % split, tile = blockIdx.x / split;
+    const int mt = tile % mt_count, ot = tile / mt_count % ot_count, model = tile / mt_count / ot_count;
+    const int kb0 = kb_count * rank / split, kbs = kb_count * (rank + 1) / split - kb0;
+
+    if (threadIdx.x == 0) {
+        tma_prefetch_desc(&tm_a);
+        tma_prefetch_desc(&tm_w);
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(&tfull, 1);
+        *abort_flag = 0;
+        mbar_init_fence();
+    }
+    if (warp == 1) {
+        tmem_alloc(&tmem_slot, TMEM_COLS);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const uint64_t pol_a = l2_policy_evict_last();
+            const uint64_t pol_w = mt_count == 1 ? l2_policy_evict_first() : l2_policy_evict_normal();
+            int issued = 0;
+            for (; issued < kbs; ++issued) {
+                const int s = issued % stages;
+                if (!mbar_wait(&empty[s], (uint32_t)(issued / stages & 1) ^ 1, abort_flag)) break;
+                mbar_arrive_expect_tx(&full[s], W_BYTES + A_BYTES);
+                tma_load_3d(sW + s * W_BYTES, &tm_w, &full[s], (kb0 + issued) * kBK, ot * 128, model, pol_w);
+                tma_load_3d(sA + s * A_BYTES, &tm_a, &full[s], (kb0 + issued) * kBK, mt * BN, model, pol_a);
+            }
+            if (issued < kbs) {
+                *abort_flag = 1;
+                raise_device_error(p.err, DEV_ERR_GEMM_TIMEOUT);
+                const volatile int never = 0;            // copies in flight land before the CTA's memory is released
+                for (int j = issued - (issued < stages ? issued : stages); j < issued; ++j)
+                    mbar_wait(&full[j % stages], (uint32_t)(j / stages & 1), &never);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint64_t w_desc0 = sdesc_kmajor_sw128(smem_addr(sW)), a_desc0 = sdesc_kmajor_sw128(smem_addr(sA));
+            for (int i = 0; i < kbs; ++i) {
+                const int s = i % stages;
+                if (!mbar_wait(&full[s], (uint32_t)(i / stages & 1), abort_flag)) {
+                    *abort_flag = 1;
+                    raise_device_error(p.err, DEV_ERR_GEMM_TIMEOUT);
+                    break;
+                }
+                tc_fence_after();
+                const uint64_t wd = w_desc0 + (uint64_t)((s * W_BYTES) >> 4), ad = a_desc0 + (uint64_t)((s * A_BYTES) >> 4);
+#pragma unroll
+                for (int k = 0; k < kBK / 32; ++k) umma_i8(tmem_base, wd + 2 * k, ad + 2 * k, IDESC, (i | k) != 0);
+                umma_commit(&empty[s]);
+            }
+            umma_commit(&tfull);             // also after a failure: the MMAs issued so far end before TMEM is freed
+        }
+    }
+    __syncwarp();
+    const volatile int never = 0;
+    const bool ok = mbar_wait(&tfull, 0, &never);
+    tc_fence_after();
+
+    // Thread = output channel, columns = tokens.
+    const int o = ot * 128 + threadIdx.x, tokens = p.m - mt * BN < BN ? p.m - mt * BN : BN;
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    const int64_t wat = (int64_t)model * p.o + o;
+    const float sw = o < p.o ? p.sw[wat] : 0.f;
+    const float bias = p.bias && o < p.o ? to_f<T>(static_cast<const T*>(p.bias)[wat]) : 0.f;
+    const float* sa = p.sa + (int64_t)model * p.m + mt * BN;
+    T* y = static_cast<T*>(p.y) + ((int64_t)model * p.m + mt * BN) * p.o + o;
+    constexpr int CH = BN < 32 ? BN : 32;
+    auto load = [&](int c, uint32_t (&r)[CH]) {
+        if constexpr (CH == 16) tmem_ld_32x32b_x16(tmem_base + lanes + c, r);
+        else tmem_ld_32x32b_x32(tmem_base + lanes + c, r);
+        tmem_ld_wait();
+    };
+    if (split == 1) {
+#pragma unroll 1
+        for (int c = 0; c < tokens; c += CH) {
+            uint32_t r[CH];
+            load(c, r);
+#pragma unroll
+            for (int j = 0; j < CH; ++j)
+                if (c + j < tokens && o < p.o)
+                    y[(int64_t)(c + j) * p.o] = from_f<T>(apply_act(finish<T>(r[j], sa[c + j], sw, bias), p.act));
+        }
+    } else {
+        // The parts as [token][channel] in the ring's memory (its copies have been
+        // used up); CTA r adds and finishes the tokens r, r + split, ..
+        uint32_t* part = reinterpret_cast<uint32_t*>(smem);
+        if (ok) {
+#pragma unroll 1
+            for (int c = 0; c < tokens; c += CH) {
+                uint32_t r[CH];
+                load(c, r);
+#pragma unroll
+                for (int j = 0; j < CH; ++j) part[(c + j) * 128 + threadIdx.x] = r[j];
+            }
+        }
+        cluster_sync_all();
+        const uint32_t mine = smem_addr(part) + threadIdx.x * 4;
+        for (int c = rank; c < tokens; c += split) {
+            uint32_t acc = 0;
+            for (int k = 0; k < split; ++k) acc += load_cluster_u32(map_to_rank(mine + c * 512, k));
+            if (o < p.o) y[(int64_t)c * p.o] = from_f<T>(apply_act(finish<T>(acc, sa[c], sw, bias), p.act));
+        }
+        cluster_sync_all();                  // no CTA leaves while others read its part
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, TMEM_COLS);
+    }
+}
+
+int rows_map(CUtensorMap* map, const void* base, int64_t n, int64_t rows, int64_t k, int64_t ld, int64_t ms, uint32_t box) {
+    const uint64_t dims[3] = {(uint64_t)k, (uint64_t)rows, (uint64_t)n};
+    const uint64_t strides[2] = {(uint64_t)ld, (uint64_t)ms};
+    const uint32_t boxes[3] = {kBK, box, 1};
+    return encode_tmap_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, base, dims, strides, boxes, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <typename T>
+CUtensorMapDataType out_type() {
+    return sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                          : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+
+template <typename K>
+int reserve(K kernel, size_t bytes) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != cudaSuccess)
+        return set_error(WIDEK_ERR_CUDA, "widek_linear_int8_fwd: %zu bytes of shared memory: %s", bytes, cudaGetErrorString(e));
+    return WIDEK_OK;
+}
+
+struct Int8Launch {
+    Int8Args p;
+    const void *a, *w;
+    int64_t a_ld, a_ms, w_ld, w_ms;
+    cudaStream_t st;
+
+    template <typename T>
+    int wide() {
+        using S = WideSmem<T>;
+        CUtensorMap ta, tw, ty{};
+        int rc = rows_map(&ta, a, p.n, p.m, p.k, a_ld, a_ms, 128);
+        if (rc == WIDEK_OK) rc = rows_map(&tw, w, p.n, p.o, p.k, w_ld, w_ms, 128);
+        p.vec_store = (int64_t)p.o * sizeof(T) % 16 == 0 && aligned16(p.y);
+        if (rc == WIDEK_OK && p.vec_store) {
+            const uint64_t dims[3] = {(uint64_t)p.o, (uint64_t)p.m, (uint64_t)p.n};
+            const uint64_t strides[2] = {(uint64_t)p.o * sizeof(T), (uint64_t)p.m * p.o * sizeof(T)};
+            const uint32_t box[3] = {32, 128, 1};
+            rc = encode_tmap_tiled(&ty, out_type<T>(), 3, p.y, dims, strides, box,
+                                   sizeof(T) == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+        } else {
+            ty = ta;
+        }
+        if (rc == WIDEK_OK) rc = reserve(wide_kernel<T>, S::TOTAL);
+        if (rc != WIDEK_OK) return rc;
+        const int64_t tiles = (int64_t)p.n * ((p.m + 255) / 256) * ((p.o + 255) / 256);
+        const int grid = (int)std::min<int64_t>(2 * tiles, sm_count(current_device()) / 2 * 2);
+        wide_kernel<T><<<grid, kWideThreads, S::TOTAL, st>>>(ta, tw, ty, p);
+        return check_launch("widek_linear_int8_fwd (wide)");
+    }
+
+    template <typename T, int BN>
+    int narrow() {
+        CUtensorMap ta, tw;
+        int rc = rows_map(&ta, a, p.n, p.m, p.k, a_ld, a_ms, BN);
+        if (rc == WIDEK_OK) rc = rows_map(&tw, w, p.n, p.o, p.k, w_ld, w_ms, 128);
+        const int sms = sm_count(current_device()), kb = (p.k + kBK - 1) / kBK;
+        const int64_t tiles = (int64_t)p.n * ((p.m + BN - 1) / BN) * ((p.o + 127) / 128);
+        int split = 1;
+        while (split < 8 && tiles * split < 2 * sms && kb >= 4 * split) split *= 2;
+        const int most = (kb + split - 1) / split, stages = most < 6 ? most : 6;
+        size_t bytes = (size_t)stages * (128 + BN) * kBK;
+        if (split > 1) bytes = std::max<size_t>(bytes, (size_t)BN * 512);
+        // A CTA holds at least 456 bytes of an SM's 228 KB for each of its 512 TMEM
+        // columns that it takes, so that CTAs of a cluster, which wait for one
+        // another, never wait for columns that others of their kind hold.
+        bytes = std::max<size_t>(bytes + 1024, (BN < 32 ? 32 : BN) * 456);
+        if (tiles * split > 0x7fffffff) return set_error(WIDEK_ERR_INVALID, "widek_linear_int8_fwd: over 2^31 tiles");
+        if (rc == WIDEK_OK) rc = reserve(narrow_kernel<T, BN>, bytes);
+        if (rc != WIDEK_OK) return rc;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)(tiles * split));
+        cfg.blockDim = dim3(kNarrowThreads);
+        cfg.dynamicSmemBytes = bytes;
+        cfg.stream = st;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim = {(unsigned)split, 1, 1};
+        cfg.attrs = &attr;
+        cfg.numAttrs = split > 1 ? 1 : 0;
+        cudaLaunchKernelEx(&cfg, narrow_kernel<T, BN>, ta, tw, p, split, stages);
+        return check_launch("widek_linear_int8_fwd (narrow)");
+    }
+
+    template <typename T>
+    int run() {
+        const int64_t pairs = (int64_t)p.n * ((p.m + 255) / 256) * ((p.o + 255) / 256);
+        if (p.m > 128 && pairs * 4 >= sm_count(current_device())) return wide<T>();
+        if (p.m <= 16) return narrow<T, 16>();
+        if (p.m <= 32) return narrow<T, 32>();
+        if (p.m <= 64) return narrow<T, 64>();
+        return narrow<T, 128>();
+    }
+};
+
+}  // namespace
+}  // namespace widek
+
+using namespace widek;
+
+extern "C" int widek_linear_int8_fwd(const void* a, const float* a_scale, const void* w, const float* w_scale,
+                                     const void* bias, void* y, int64_t n, int64_t m, int64_t k, int64_t o, int64_t a_ld,
+                                     int64_t a_ms, int64_t w_ld, int64_t w_ms, int act, int dtype, void* stream) {
+    const char* what = "widek_linear_int8_fwd";
+    if (n < 0 || m < 0 || o < 0 || k < 1 || k > kMaxK)
+        return set_error(WIDEK_ERR_INVALID, "%s: bad sizes n=%lld m=%lld k=%lld o=%lld (k from 1 to %lld)", what,
+                         (long long)n, (long long)m, (long long)k, (long long)o, (long long)kMaxK);
+    if (act < WIDEK_ACT_NONE || act > WIDEK_ACT_GELU) return set_error(WIDEK_ERR_INVALID, "%s: unknown activation %d", what, act);
+    if (dtype_size(dtype) == 0) return set_error(WIDEK_ERR_INVALID, "%s: unknown dtype code %d", what, dtype);
+    if (n == 0 || m == 0 || o == 0) return WIDEK_OK;
+    if (!a || !a_scale || !w || !w_scale || !y) return set_error(WIDEK_ERR_INVALID, "%s: null pointer", what);
+    if (a_ld < 0 || w_ld < 0 || a_ld > (int64_t)1 << 32 || w_ld > (int64_t)1 << 32)
+        return set_error(WIDEK_ERR_INVALID, "%s: bad strides", what);
+    if (n > 0x7fffffff || m > 0x7fffff00 || o > 0x7fffff00 || n * ((m + 15) / 16) > 0x7fffffff / ((o + 127) / 128))
+        return set_error(WIDEK_ERR_INVALID, "%s: too many tiles (n=%lld m=%lld o=%lld)", what, (long long)n, (long long)m,
+                         (long long)o);
+    if (n == 1) {                     // no second model to step to
+        a_ms = m * a_ld;
+        w_ms = o * w_ld;
+    }
+    if (!aligned16(a) || !aligned16(w) || a_ld % 16 != 0 || w_ld % 16 != 0 || a_ms % 16 != 0 || w_ms % 16 != 0 || a_ld < k ||
+        w_ld < k || a_ms < (m - 1) * a_ld + k || w_ms < (o - 1) * w_ld + k)
+        return set_error(WIDEK_ERR_INVALID, "%s: rows of codes must lie a multiple of 16 bytes apart, models behind one "
+                         "another", what);
+    if (a_ld >= (int64_t)1 << 40 || w_ld >= (int64_t)1 << 40 || a_ms >= (int64_t)1 << 40 || w_ms >= (int64_t)1 << 40)
+        return set_error(WIDEK_ERR_INVALID, "%s: strides of 2^40 bytes or more", what);
+    Int8Launch l{{a_scale, w_scale, bias, y, (int)n, (int)m, (int)k, (int)o, act, 0, device_error_ptr()},
+                 a, w, a_ld, a_ms, w_ld, w_ms, static_cast<cudaStream_t>(stream)};
+    return dispatch_dtype(dtype, l);
+}

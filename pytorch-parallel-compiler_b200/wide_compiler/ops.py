@@ -1401,6 +1401,76 @@ def quantize_rows(x: Tensor):
     return codes, scales
 
 
+def _rows16(t: Tensor):
+    """Codes [N, ..., K] whose rows lie one step apart in a model, a multiple of
+    16 bytes (copied if they do not): (codes, bytes between rows, between models)."""
+    shape, st = t.shape, t.stride()
+    rows = math.prod(shape[1:-1])
+    step = None
+    if t.data_ptr() % 16 == 0 and (st[-1] == 1 or shape[-1] == 1):
+        step, want = -(-shape[-1] // 16) * 16, None
+        for size, stride in zip(reversed(shape[1:-1]), reversed(st[1:-1])):
+            if size == 1:
+                continue
+            if want is None:
+                step = want = stride
+            if stride != want:
+                step = None
+                break
+            want *= size
+    if step is not None and step % 16 == 0 and step >= shape[-1]:
+        ms = st[0] if shape[0] > 1 else rows * step
+        if ms % 16 == 0 and ms >= (rows - 1) * step + shape[-1]:
+            return t, step, ms
+    held = _code_rows(t)
+    held.copy_(t)
+    step = -(-shape[-1] // 16) * 16
+    return held, step, rows * step
+
+
+def linear_int8(codes: Tensor, scale: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[Tensor] = None,
+                act: int = ACT_NONE, dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """A linear layer of N models on 8-bit codes (widek_linear_int8_fwd):
+
+        y[i] = act((codes[i] @ weight[i]^T) * scale[i][..., None] * weight_scale[i] + bias[i])
+
+    codes int8 [N, ..., K] with scale float32 [N, ...] (``quantize_rows``,
+    ``residual_norm_quantize``), weight int8 [N, O, K] with weight_scale float32
+    [N, O], bias [N, O] of ``dtype``, which y [N, ..., O] has. The products are
+    summed exactly (K <= 131071), the rest is fp32, rounded once. Rows of codes
+    that start multiples of 16 bytes apart, as those operators make them, are read
+    in place, others are copied first. A row whose scale is not finite comes out
+    as NaN. No gradient."""
+    what = "linear_int8"
+    _no_grad(what, scale, weight_scale, bias)
+    if _compiling():
+        return torch.ops.widek.linear_int8(codes, scale, weight, weight_scale, bias, act, dtype)
+    idx = _device(what, codes, scale, weight, weight_scale, bias)
+    cs, ws = codes.shape, weight.shape
+    if codes.dtype != torch.int8 or weight.dtype != torch.int8:
+        raise TypeError(f"{what}: codes and weight must be int8, got {codes.dtype} and {weight.dtype}")
+    if len(cs) < 2 or len(ws) != 3 or cs[0] != ws[0] or cs[-1] != ws[2]:
+        raise ValueError(f"{what}: codes {tuple(cs)} do not match weight {tuple(ws)}")
+    if scale.shape != cs[:-1] or weight_scale.shape != ws[:2]:
+        raise ValueError(f"{what}: scales {tuple(scale.shape)} and {tuple(weight_scale.shape)} do not match codes "
+                         f"{tuple(cs)} and weight {tuple(ws)}")
+    if scale.dtype != torch.float32 or weight_scale.dtype != torch.float32:
+        raise TypeError(f"{what}: scales must be float32, got {scale.dtype} and {weight_scale.dtype}")
+    if bias is not None and (bias.shape != ws[:2] or bias.dtype != dtype):
+        raise ValueError(f"{what}: bias {tuple(bias.shape)} {bias.dtype} is not {tuple(ws[:2])} {dtype}")
+    y = torch.empty((*cs[:-1], ws[1]), device=codes.device, dtype=dtype)
+    code = N.dtype_code(y)
+    if y.numel() == 0:
+        return y
+    a, a_ld, a_ms = _rows16(codes)
+    w, w_ld, w_ms = _rows16(weight)
+    scale, weight_scale = _dense(scale), _dense(weight_scale)
+    bias = bias if bias is None else _dense(bias)
+    _launch(idx, "widek_linear_int8_fwd", a.data_ptr(), scale.data_ptr(), w.data_ptr(), weight_scale.data_ptr(),
+            N.ptr(bias), y.data_ptr(), cs[0], scale.numel() // cs[0], cs[-1], ws[1], a_ld, a_ms, w_ld, w_ms, act, code)
+    return y
+
+
 # ---------------------------------------------------------------------------
 # Convolutions
 # ---------------------------------------------------------------------------

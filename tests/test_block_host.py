@@ -101,3 +101,69 @@ def test_types_are_checked(monkeypatch):
         ops.residual_norm(x, x, w.half())
     with torch.no_grad(), pytest.raises(TypeError, match="support"):
         ops.quantize_rows(torch.zeros(2, 8, dtype=torch.int32))
+
+
+# ---------------------------------------------------------------------------
+# 8-bit linear layers
+# ---------------------------------------------------------------------------
+
+def int8(a=P, sa=P, w=P, sw=P, y=P, n=2, m=3, k=64, o=5, a_ld=64, a_ms=192, w_ld=64, w_ms=320, act=0, dtype=N.BF16):
+    return N.lib().widek_linear_int8_fwd(a, sa, w, sw, None, y, n, m, k, o, a_ld, a_ms, w_ld, w_ms, act, dtype, None)
+
+
+@pytest.mark.parametrize("bad, word", [
+    (dict(n=-1), "sizes"), (dict(m=-1), "sizes"), (dict(k=0), "sizes"), (dict(k=131072, a_ld=131072, w_ld=131072), "131071"),
+    (dict(o=-1), "sizes"), (dict(act=3), "activation"), (dict(dtype=5), "dtype"), (dict(a=None), "null"),
+    (dict(sa=None), "null"), (dict(w=None), "null"), (dict(sw=None), "null"), (dict(y=None), "null"),
+    (dict(a=P + 8), "16 bytes"), (dict(w=P + 1), "16 bytes"), (dict(a_ld=72), "16 bytes"), (dict(w_ld=48), "16 bytes"),
+    (dict(a_ms=8), "16 bytes"), (dict(w_ms=-16), "16 bytes"), (dict(m=1 << 40), "tiles"), (dict(o=1 << 33), "tiles")])
+def test_linear_int8_refuses(bad, word):
+    assert int8(**bad) == N.WIDEK_ERR_INVALID
+    assert word in N.last_error()
+
+
+def test_linear_int8_of_nothing():
+    for size in ("n", "m", "o"):
+        assert int8(**{size: 0}) == 0
+
+
+@pytest.mark.parametrize("change, error", [
+    (dict(codes=(2, 3, 17)), ValueError), (dict(codes=(3, 3, 16)), ValueError), (dict(codes=(16,)), ValueError),
+    (dict(weight=(2, 16)), ValueError), (dict(scale=(2, 4)), ValueError), (dict(weight_scale=(2, 4)), ValueError),
+    (dict(bias=(2, 6)), ValueError)])
+def test_linear_int8_checks_shapes(change, error, monkeypatch):
+    monkeypatch.setattr(ops, "_device", lambda what, ref, *others: 0)
+    shapes = dict(dict(codes=(2, 3, 16), scale=(2, 3), weight=(2, 5, 16), weight_scale=(2, 5), bias=(2, 5)), **change)
+    args = {k: torch.zeros(s, dtype=torch.int8 if k in ("codes", "weight") else torch.float32) for k, s in shapes.items()}
+    with torch.no_grad(), pytest.raises(error, match="linear_int8"):
+        ops.linear_int8(**args, dtype=torch.float32)
+
+
+def test_linear_int8_checks_types(monkeypatch):
+    monkeypatch.setattr(ops, "_device", lambda what, ref, *others: 0)
+    i8 = lambda *s: torch.zeros(s, dtype=torch.int8)
+    f = lambda *s: torch.zeros(s)
+    with pytest.raises(TypeError, match="int8"):
+        ops.linear_int8(f(2, 3, 16), f(2, 3), i8(2, 5, 16), f(2, 5))
+    with pytest.raises(TypeError, match="float32"):
+        ops.linear_int8(i8(2, 3, 16), f(2, 3).half(), i8(2, 5, 16), f(2, 5))
+    with pytest.raises(ValueError, match="bias"):
+        ops.linear_int8(i8(2, 3, 16), f(2, 3), i8(2, 5, 16), f(2, 5), f(2, 5), dtype=torch.bfloat16)
+    with pytest.raises(TypeError, match="support"):
+        ops.linear_int8(i8(2, 3, 16), f(2, 3), i8(2, 5, 16), f(2, 5), dtype=torch.float64)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.linear_int8(i8(2, 3, 16), f(2, 3).requires_grad_(), i8(2, 5, 16), f(2, 5))
+
+
+def test_rows_of_codes_read_in_place_or_copied():
+    i8 = lambda *s: torch.zeros(s, dtype=torch.int8)
+    base = i8(4096)                                   # 64-byte aligned
+    at = lambda t, *shape: base[t:t + torch.Size(shape).numel()].view(shape)
+    for t, ld, ms in ((at(0, 2, 3, 32), 32, 96), (at(0, 2, 3, 4, 48)[..., :40], 48, 576), (at(0, 1, 1, 7), 16, 16),
+                      (at(0, 2, 6, 32)[:, ::2], 64, 192), (at(16, 4, 64)[..., :50], 64, 64)):
+        got = ops._rows16(t)
+        assert got[0] is t and got[1:] == (ld, ms)
+    for t in (at(0, 2, 3, 33), at(0, 2, 3, 4, 32).transpose(1, 2), at(0, 2, 33, 3).transpose(1, 2), at(1, 2, 3, 32),
+              at(0, 1, 5, 16).expand(3, -1, -1), at(0, 2, 1, 32).expand(-1, 5, -1)):
+        got, ld, ms = ops._rows16(t)
+        assert got is not t and got.shape == t.shape and ld % 16 == 0 and ms == ld * t[0].numel() // t.shape[-1]
