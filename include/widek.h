@@ -774,7 +774,7 @@ WIDEK_API int64_t widek_residual_norm_bwd_workspace(int64_t n, int64_t rows, int
 /* Gradients of widek_residual_norm_fwd from its inputs and stats: dh, dz
  * (nullable: zeros) [n, rows, d] dense; dx, dy like x, dw, dwb, dpw, dpb [n, d],
  * dgate like gate, each nullable. With rows = 0 nothing is written. Sums over
- * rows are taken in a fixed order. n <= 65535. */
+ * rows are taken in a fixed order. */
 WIDEK_API int widek_residual_norm_bwd(const void* x, const void* y, const void* w, const void* wb,
                                       const void* pw, const void* pb, const void* gate,
                                       const float* stats, const void* dh, const void* dz, void* dx,

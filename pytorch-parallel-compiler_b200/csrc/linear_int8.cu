@@ -20,6 +20,7 @@
 //           the same sum) are added through distributed shared memory.
 #include <algorithm>
 
+#include "paged_cache.cuh"
 #include "sm100_ptx.cuh"
 
 namespace widek {
@@ -66,9 +67,53 @@ __device__ __forceinline__ uint32_t load_cluster_u32(uint32_t addr) {
     return v;
 }
 
-template <typename T>
 __device__ __forceinline__ float finish(uint32_t acc, float sa, float sw, float bias) {
     return fmaf((float)(int)acc * sa, sw, bias);
+}
+
+// max(x, 0), NaN kept.
+__device__ __forceinline__ float relu_nan(float x) {
+    float y;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// GELU of two values for a 16-bit result: max(x, 0) - a Q(a) with a = |x| and the
+// normal tail Q(a) = 2^(-a^2 log2(e) / 2 + r(a)), r a polynomial (fit_gelu_tail.py:
+// Q is off by 9e-6 of itself up to a = 8, where f16's half step is 2.4e-4; past 8,
+// where a Q(a) < 5e-15, r stays at its end). By way of erff the epilogue of a prompt's
+// tile takes longer than its products.
+__device__ __forceinline__ void gelu2(float& x0, float& x1) {
+    constexpr float r[9] = {-0.9999924f, -1.1513219f, 0.26315188f, -0.05433736f, 0.008762172f, -0.0010219777f,
+                            7.9574354e-05f, -3.6553492e-06f, 7.428467e-08f};
+    const float a0 = fminf(fabsf(x0), 64.f), a1 = fminf(fabsf(x1), 64.f);      // Q(64) is 0 as well
+    const float b0 = fminf(a0, 8.f), b1 = fminf(a1, 8.f);
+    float p0 = r[8], p1 = r[8];
+#pragma unroll
+    for (int i = 7; i >= 0; --i) fma2(p0, p1, p0, p1, b0, b1, r[i], r[i]);
+    float q0, q1;
+    mul2(q0, q1, a0, a1, -0.72134752f, -0.72134752f);
+    fma2(p0, p1, q0, q1, a0, a1, p0, p1);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(q0) : "f"(p0));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(q1) : "f"(p1));
+    fma2(x0, x1, -a0, -a1, q0, q1, relu_nan(x0), relu_nan(x1));
+}
+
+// The activation of N values (an even number), NaN kept.
+template <typename T, int N>
+__device__ __forceinline__ void activate(float (&v)[N], int act) {
+    if (act == WIDEK_ACT_RELU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = relu_nan(v[j]);
+    } else if (act == WIDEK_ACT_GELU) {
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int j = 0; j < N; j += 2) gelu2(v[j], v[j + 1]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = gelu_erf(v[j]);
+        }
+    }
 }
 
 struct Int8Args {
@@ -245,7 +290,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
                 break;
             }
             tc_fence_after();
-            T* yrow = static_cast<T*>(p.y) + ((int64_t)model * p.m + row) * p.o;
 #pragma unroll 1
             for (int c = 0; c < 128; c += 32) {
                 if (c0 + c >= p.o) break;                // warp-uniform
@@ -257,16 +301,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
 #pragma unroll
                 for (int j = 0; j < 32; j += 2) {
                     const float4 f = sv[j / 2];
-                    v[j] = finish<T>(r[j], sa, f.x, f.y);
-                    v[j + 1] = finish<T>(r[j + 1], sa, f.z, f.w);
+                    v[j] = finish(r[j], sa, f.x, f.y);
+                    v[j + 1] = finish(r[j + 1], sa, f.z, f.w);
                 }
-                if (p.act == WIDEK_ACT_RELU) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = v[j] > 0.f ? v[j] : 0.f;
-                } else if (p.act == WIDEK_ACT_GELU) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = gelu_erf(v[j]);
-                }
+                activate<T>(v, p.act);
                 if (p.vec_store) {
                     // Rows past m of the last tile are clipped by the store; a
                     // CTA whose 128 rows all lie past m stores nothing.
@@ -286,10 +324,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
                         bulk_commit_group();
                     }
                     ++oc;
-                } else if (row < p.m) {
+                } else {
+                    // Rows that start off the 16-byte borders: through this warp's part
+                    // of the staging buffer (rows of 33 values: no bank twice), so that a
+                    // store covers 32 neighbours. Each thread storing its own row took
+                    // 7 to 9 times as long.
+                    T* stage = reinterpret_cast<T*>(buf0 + q * (2 * S::OUT_CHUNK / 4));
+                    __syncwarp();
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (c0 + c + j < p.o) yrow[c0 + c + j] = from_f<T>(v[j]);
+                    for (int j = 0; j < 32; ++j) stage[lane * 33 + j] = from_f<T>(v[j]);
+                    __syncwarp();
+                    const int col = c0 + c + lane, rows = min(32, p.m - row0 - q * 32);
+                    T* dst = static_cast<T*>(p.y) + ((int64_t)model * p.m + row0 + q * 32) * p.o + col;
+                    if (col < p.o) {
+#pragma unroll 8
+                        for (int j = 0; j < rows; ++j, dst += p.o) *dst = stage[j * 33 + lane];
+                    }
                 }
             }
             tc_fence_before();
@@ -416,10 +466,13 @@ __global__ void __launch_bounds__(kNarrowThreads)
         for (int c = 0; c < tokens; c += CH) {
             uint32_t r[CH];
             load(c, r);
+            float v[CH];
+#pragma unroll
+            for (int j = 0; j < CH; ++j) v[j] = c + j < tokens ? finish(r[j], sa[c + j], sw, bias) : 0.f;
+            activate<T>(v, p.act);
 #pragma unroll
             for (int j = 0; j < CH; ++j)
-                if (c + j < tokens && o < p.o)
-                    y[(int64_t)(c + j) * p.o] = from_f<T>(apply_act(finish<T>(r[j], sa[c + j], sw, bias), p.act));
+                if (c + j < tokens && o < p.o) y[(int64_t)(c + j) * p.o] = from_f<T>(v[j]);
         }
     } else {
         // The parts as [token][channel] in the ring's memory (its copies have been
@@ -439,7 +492,9 @@ __global__ void __launch_bounds__(kNarrowThreads)
         for (int c = rank; c < tokens; c += split) {
             uint32_t acc = 0;
             for (int k = 0; k < split; ++k) acc += load_cluster_u32(map_to_rank(mine + c * 512, k));
-            if (o < p.o) y[(int64_t)c * p.o] = from_f<T>(apply_act(finish<T>(acc, sa[c], sw, bias), p.act));
+            float v[2] = {finish(acc, sa[c], sw, bias), 0.f};
+            activate<T>(v, p.act);
+            if (o < p.o) y[(int64_t)c * p.o] = from_f<T>(v[0]);
         }
         cluster_sync_all();                  // no CTA leaves while others read its part
     }

@@ -6,14 +6,14 @@ namespace rnorm {
 
 int bwd_mode(const Args& a, int64_t rows) {
     if (!a.gate) return a.pw ? MODEL : PLAIN;
-    return (int64_t)a.gate_rows == rows ? MODEL : a.gate_rows == 1 ? TOKEN : SEQUENCE;
+    return (int64_t)a.gate_rows == rows ? MODEL : GROUPS;
 }
 
-int bwd_teams(int64_t n, int64_t rows, int d, int sms) {
+int bwd_teams(int64_t n, int64_t rows, int d, int sms, int threads) {
     if (n < 1 || rows < 1) return 1;
-    const TeamShape shape = team_shape(d);
-    const int64_t blocks = (int64_t)sms * (512 / shape.threads);      // resident with 128 registers a thread
-    const int64_t wave = shape.team == WARP ? 4 * blocks : shape.team == BLOCK ? blocks : blocks / 2;
+    const TeamShape shape = team_shape(d, kBwdChannels);
+    const int64_t blocks = (int64_t)sms * (threads / shape.threads);
+    const int64_t wave = shape.team == PAIR ? blocks / 2 : blocks * shape.rows();
     int64_t teams = wave / n;
     if (teams > (rows + 1) / 2) teams = (rows + 1) / 2;
     return teams < 1 ? 1 : (int)teams;
@@ -35,7 +35,7 @@ extern "C" int64_t widek_residual_norm_bwd_workspace(int64_t n, int64_t rows, in
     a.gate = gate_rows > 0 ? &a : nullptr;
     a.pw = has_post ? &a : nullptr;
     a.gate_rows = (uint32_t)(gate_rows > 0 ? gate_rows : 0);
-    const int teams = rnorm::bwd_teams(n, rows, (int)d, sm_count(current_device()));
+    const int teams = rnorm::bwd_teams(n, rows, (int)d, sm_count(current_device()), 1024);
     return n * teams * rnorm::slot_count(rnorm::bwd_mode(a, rows), center != 0) * d * (int64_t)sizeof(float);
 }
 
@@ -51,7 +51,6 @@ extern "C" int widek_residual_norm_bwd(const void* x, const void* y, const void*
     if (rc != WIDEK_OK) return rc;
     if ((dy && !y) || ((dpw || dpb) && !pw) || (dgate && !gate) || ((dwb || dpb) && !center))
         return set_error(WIDEK_ERR_INVALID, "%s: a gradient of an input that is not there", what);
-    if (n > 65535) return set_error(WIDEK_ERR_UNSUPPORTED, "%s: over 65535 models", what);
     if (a.f.rows == 0) return WIDEK_OK;
     const int64_t need = widek_residual_norm_bwd_workspace(n, rows, d, gate ? gate_rows : -1, pw != nullptr, center);
     if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 3))
@@ -61,8 +60,5 @@ extern "C" int widek_residual_norm_bwd(const void* x, const void* y, const void*
     a.f.stats = const_cast<float*>(stats);
     a.dh = dh; a.dz = dz; a.dx = dx; a.dy = dy; a.dw = dw; a.dwb = dwb; a.dpw = dpw; a.dpb = dpb; a.dgate = dgate;
     a.part = static_cast<float*>(workspace);
-    a.teams = rnorm::bwd_teams(n, rows, (int)d, sm_count(current_device()));
-    a.n = n;
-    a.model_rows = rows;
     return dispatch_dtype(dtype, rnorm::BwdLaunch{a, rnorm::bwd_mode(a.f, rows), static_cast<cudaStream_t>(stream)});
 }

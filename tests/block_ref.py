@@ -94,9 +94,12 @@ def residual_norm(x, y, weight, bias=None, post_weight=None, post_bias=None, gat
             pw, pb = over(post_weight, x), zero if post_bias is None else over(post_bias, x)
             u = un.vn * pw + pb
             du = un.err * pw.abs() + 2 * U * ((un.vn * pw).abs() + pb.abs())
+    # the weights are folded, h = un (scale g pw) + (x + scale g pb): two roundings
+    # of each product of weights, one each of the sum and of the last step
     k = scale * g
     h = xd + k * u
-    eh = k.abs() * du + 3 * U * ((k * u).abs() + xd.abs())
+    amp = u.abs() if un is None else (un.vn * pw).abs() + pb.abs()
+    eh = k.abs() * du + 4 * U * (k.abs() * amp + xd.abs())
     hn = Norm(h, eh if y is not None else zero, eps, center)
     z = hn.vn * w + b
     ez = hn.err * w.abs() + 2 * U * ((hn.vn * w).abs() + b.abs())
@@ -128,7 +131,6 @@ def residual_norm(x, y, weight, bias=None, post_weight=None, post_bias=None, gat
     ds, es = k * dx, k.abs() * ex + 3 * U * (k * dx).abs()
     if gate is not None:
         dims = tuple(range(gate.dim() - 1, x.dim() - 1))
-        amp = u.abs() if un is None else (un.vn * pw).abs() + pb.abs()
         terms = scale * dx * u
         summed("dgate", terms, abs(scale) * (amp * ex + dx.abs() * du) + 6 * U * abs(scale) * dx.abs() * amp, dims)
         if dims and un is not None:              # pw A + pb B: two sums that may cancel
