@@ -20,8 +20,7 @@
 //           the same sum) are added through distributed shared memory.
 #include <algorithm>
 
-#include "paged_cache.cuh"
-#include "sm100_ptx.cuh"
+#include "residual_norm.cuh"
 
 namespace widek {
 namespace {
@@ -61,15 +60,16 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void*
                  "r"(smem_addr(src)), "r"(c0), "r"(c1), "r"(c2)
                  : "memory");
 }
+// Arrives on another CTA's mbarrier without waiting for this thread's stores.
+__device__ __forceinline__ void mbar_arrive_remote_relaxed(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 __device__ __forceinline__ uint32_t load_cluster_u32(uint32_t addr) {
     uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
     return v;
 }
 
-__device__ __forceinline__ float finish(uint32_t acc, float sa, float sw, float bias) {
-    return fmaf((float)(int)acc * sa, sw, bias);
-}
 
 // max(x, 0), NaN kept.
 __device__ __forceinline__ float relu_nan(float x) {
@@ -78,42 +78,88 @@ __device__ __forceinline__ float relu_nan(float x) {
     return y;
 }
 
+// Two fp32 values in a register pair, and arithmetic on both at once.
+using F2 = uint64_t;
+__device__ __forceinline__ F2 pair_of(float a, float b) {
+    F2 p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+    return p;
+}
+__device__ __forceinline__ void halves(F2 p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) {
+    F2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ F2 mul(F2 a, F2 b) {
+    F2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
 // GELU of two values for a 16-bit result: max(x, 0) - a Q(a) with a = |x| and the
 // normal tail Q(a) = 2^(-a^2 log2(e) / 2 + r(a)), r a polynomial (fit_gelu_tail.py:
 // Q is off by 9e-6 of itself up to a = 8, where f16's half step is 2.4e-4; past 8,
-// where a Q(a) < 5e-15, r stays at its end). By way of erff the epilogue of a prompt's
-// tile takes longer than its products.
-__device__ __forceinline__ void gelu2(float& x0, float& x1) {
-    constexpr float r[9] = {-0.9999924f, -1.1513219f, 0.26315188f, -0.05433736f, 0.008762172f, -0.0010219777f,
-                            7.9574354e-05f, -3.6553492e-06f, 7.428467e-08f};
-    const float a0 = fminf(fabsf(x0), 64.f), a1 = fminf(fabsf(x1), 64.f);      // Q(64) is 0 as well
-    const float b0 = fminf(a0, 8.f), b1 = fminf(a1, 8.f);
-    float p0 = r[8], p1 = r[8];
+// where a Q(a) < 5e-15, r and the factor a stay at 8). It takes 9 instructions a
+// value; by way of erff the epilogue of a tile takes longer than its products. The
+// constants are set up once, in registers.
+struct Gelu2 {
+    F2 r[9], half;
+    __device__ __forceinline__ Gelu2() {
+        constexpr float c[9] = {-0.9999924f, -1.1513219f, 0.26315188f, -0.05433736f, 0.008762172f, -0.0010219777f,
+                                7.9574354e-05f, -3.6553492e-06f, 7.428467e-08f};
 #pragma unroll
-    for (int i = 7; i >= 0; --i) fma2(p0, p1, p0, p1, b0, b1, r[i], r[i]);
-    float q0, q1;
-    mul2(q0, q1, a0, a1, -0.72134752f, -0.72134752f);
-    fma2(p0, p1, q0, q1, a0, a1, p0, p1);
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(q0) : "f"(p0));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(q1) : "f"(p1));
-    fma2(x0, x1, -a0, -a1, q0, q1, relu_nan(x0), relu_nan(x1));
-}
+        for (int i = 0; i < 9; ++i) {             // r in powers of -a
+            const float v = i % 2 ? -c[i] : c[i];
+            asm volatile("mov.b64 %0, {%1, %1};" : "=l"(r[i]) : "f"(v));
+        }
+        asm volatile("mov.b64 %0, {%1, %1};" : "=l"(half) : "f"(-0.72134752f));
+    }
+    __device__ __forceinline__ F2 operator()(F2 x) const {
+        float x0, x1, e0, e1;
+        halves(x, x0, x1);
+        const F2 b = pair_of(fmaxf(-fabsf(x0), -8.f), fmaxf(-fabsf(x1), -8.f));
+        F2 p = r[8];
+#pragma unroll
+        for (int i = 7; i >= 0; --i) p = fma(p, b, r[i]);
+        p = fma(mul(x, half), x, p);
+        halves(p, e0, e1);
+        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e0));
+        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e1));
+        return fma(b, pair_of(e0, e1), pair_of(relu_nan(x0), relu_nan(x1)));
+    }
+};
 
 // The activation of N values (an even number), NaN kept.
 template <typename T, int N>
-__device__ __forceinline__ void activate(float (&v)[N], int act) {
-    if (act == WIDEK_ACT_RELU) {
+__device__ __forceinline__ void activate(F2 (&v)[N / 2], int act, const Gelu2& gelu) {
+    if (act == WIDEK_ACT_NONE) return;
+    if (sizeof(T) == 2 && act == WIDEK_ACT_GELU) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = relu_nan(v[j]);
-    } else if (act == WIDEK_ACT_GELU) {
-        if constexpr (sizeof(T) == 2) {
-#pragma unroll
-            for (int j = 0; j < N; j += 2) gelu2(v[j], v[j + 1]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = gelu_erf(v[j]);
-        }
+        for (int j = 0; j < N / 2; ++j) v[j] = gelu(v[j]);
+        return;
     }
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) {
+        float a, b;
+        halves(v[j], a, b);
+        v[j] = act == WIDEK_ACT_RELU ? pair_of(relu_nan(a), relu_nan(b)) : pair_of(gelu_erf(a), gelu_erf(b));
+    }
+}
+
+// N values as stored (N * sizeof(T) = 16 bytes).
+template <typename T>
+__device__ __forceinline__ uint4 store_form(const F2* v) {
+    float f[16 / sizeof(T)];
+#pragma unroll
+    for (int j = 0; j < (int)(8 / sizeof(T)); ++j) halves(v[j], f[2 * j], f[2 * j + 1]);
+    const rnorm::Pack<T, 16 / sizeof(T)> p = rnorm::pack<T, 16 / sizeof(T)>(f);
+    return *reinterpret_cast<const uint4*>(&p);
+}
+
+// Two sums with their scales and biases.
+__device__ __forceinline__ F2 finish(uint32_t acc0, uint32_t acc1, F2 sa, F2 sw, F2 bias) {
+    return fma(mul(pair_of((float)(int)acc0, (float)(int)acc1), sa), sw, bias);
 }
 
 struct Int8Args {
@@ -127,7 +173,9 @@ struct Int8Args {
 // ---------------------------------------------------------------------------
 // wide: 256 x 256 tiles by pairs of CTAs
 // ---------------------------------------------------------------------------
-constexpr int kWideThreads = 320;     // TMA warp, MMA warp, 2 x 4 epilogue warps
+constexpr int kGroups = 4;            // of 4 epilogue warps, each finishing a quarter of the columns
+constexpr int kWideThreads = 64 + 128 * kGroups;     // and a TMA warp and an MMA warp
+constexpr int kGroupCols = 256 / kGroups;
 
 template <typename T>
 struct WideSmem {
@@ -135,8 +183,8 @@ struct WideSmem {
     static constexpr uint32_t PART = 128 * kBK;                 // one CTA's half of an operand
     static constexpr uint32_t RING = STAGES * 2 * PART;
     static constexpr uint32_t OUT_CHUNK = 128 * 32 * sizeof(T);
-    static constexpr uint32_t OUT_BYTES = 4 * OUT_CHUNK;
-    static constexpr uint32_t VEC_BYTES = 2 * 128 * 8;          // (scale, bias) of each warpgroup's columns
+    static constexpr uint32_t OUT_BYTES = kGroups * OUT_CHUNK;
+    static constexpr uint32_t VEC_BYTES = 256 * 8;              // (scale, bias) of the columns
     static constexpr uint32_t TOTAL = 1024 + RING + OUT_BYTES + VEC_BYTES + 8 * (2 * STAGES + 5) + 16;
     static_assert(TOTAL <= 227 * 1024, "shared memory");
 };
@@ -157,7 +205,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
     uint8_t* sA = smem;
     uint8_t* sB = smem + STAGES * S::PART;
     uint8_t* sOut = smem + S::RING;
-    float2* sVec = reinterpret_cast<float2*>(sOut + S::OUT_BYTES);
+    float* sVec = reinterpret_cast<float*>(sOut + S::OUT_BYTES);
     uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(sVec) + S::VEC_BYTES);
     uint64_t* empty = full + STAGES;
     uint64_t* tfull = empty + STAGES;
@@ -179,7 +227,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(&tfull[a], 1);
-            mbar_init(&tempty[a], 2 * 8 * 32);   // both CTAs' epilogue threads
+            mbar_init(&tempty[a], 2 * 4 * kGroups);   // both CTAs' epilogue warps
         }
         mbar_init(done, 1);
         *abort_flag = 0;
@@ -188,7 +236,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
     if (warp == 0 && lane == 0) {
         tma_prefetch_desc(&tm_a);
         tma_prefetch_desc(&tm_w);
-        tma_prefetch_desc(&tm_y);
     }
     if (warp == 1) {
         tmem_alloc_pair(tmem_slot, TMEM_COLS);
@@ -263,89 +310,115 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
         }
         __syncwarp();
     } else {
-        // Epilogue: warpgroup wg drains columns [128 wg, 128 wg + 128) of this
-        // CTA's 128 rows, 32 at a time through two staging buffers of its own;
-        // warp quarter q is the TMEM lanes (rows) 32 q .. 32 q + 31.
+        // Epilogue: group wg drains columns [64 wg, 64 wg + 64) of this CTA's 128
+        // rows, 32 at a time through a staging buffer a warp; warp quarter q is
+        // the TMEM lanes (rows) 32 q .. 32 q + 31. Four groups, as two left the
+        // issue slots two thirds empty and a tile of K = 1024 with its GELU waiting
+        // for them (5.0 us a tile, 2.2 of products).
         const int q = warp & 3, wg = (warp - 2) >> 2, ep_tid = threadIdx.x - 64 - 128 * wg;
-        uint8_t* buf0 = sOut + wg * 2 * S::OUT_CHUNK;
-        float2* vec = sVec + wg * 128;
+        uint8_t* buf = sOut + (wg * 4 + q) * (S::OUT_CHUNK / 4);
+        float* vec = sVec + wg * 2 * kGroupCols;             // scales, then biases
+        const Gelu2 gelu;
         const uint32_t leader_tempty0 = map_to_rank(smem_addr(&tempty[0]), 0);
         const T* bias = static_cast<const T*>(p.bias);
-        int oc = 0, local = 0;
+        // A tile's scales and biases are asked for while the last one is finished.
+        float next_sa = 0.f, next_sw = 0.f, next_bias = 0.f;
+        auto ask = [&](int tile) {
+            const int mt = tile % mt_count, rest = tile / mt_count, nt = rest % nt_count, model = rest / nt_count;
+            const int row = mt * 256 + (int)rank * 128 + q * 32 + lane, c = nt * 256 + wg * kGroupCols + ep_tid;
+            next_sa = tile < tiles && row < p.m ? p.sa[(int64_t)model * p.m + row] : 0.f;
+            const bool col = tile < tiles && ep_tid < kGroupCols && c < p.o;
+            const int64_t at = (int64_t)model * p.o + c;
+            next_sw = col ? p.sw[at] : 0.f;
+            next_bias = col && bias ? to_f<T>(bias[at]) : 0.f;
+        };
+        ask(pair);
+        int local = 0;
         for (int tile = pair; tile < tiles; tile += npairs, ++local) {
             const int mt = tile % mt_count, rest = tile / mt_count, nt = rest % nt_count, model = rest / nt_count;
-            const int acc = local & 1, rloc = q * 32 + lane, row0 = mt * 256 + (int)rank * 128, row = row0 + rloc;
-            const int c0 = nt * 256 + wg * 128;
-            {
-                const int c = c0 + ep_tid;
-                const int64_t at = (int64_t)model * p.o + c;
-                group_sync(wg);                          // the group has read the last tile's
-                vec[ep_tid] = c < p.o ? make_float2(p.sw[at], bias ? to_f<T>(bias[at]) : 0.f) : make_float2(0.f, 0.f);
-                group_sync(wg);
+            const int acc = local & 1, row0 = mt * 256 + (int)rank * 128, c0 = nt * 256 + wg * kGroupCols;
+            group_sync(wg);                              // the group has read the last tile's
+            if (ep_tid < kGroupCols) {
+                vec[ep_tid] = next_sw;
+                vec[kGroupCols + ep_tid] = next_bias;
             }
-            const float sa = row < p.m ? p.sa[(int64_t)model * p.m + row] : 0.f;
+            const F2 sa = pair_of(next_sa, next_sa);
+            group_sync(wg);
+            ask(tile + npairs);
             if (!mbar_wait(&tfull[acc], (local >> 1) & 1, abort_flag)) {
                 *abort_flag = 1;
                 raise_device_error(p.err, DEV_ERR_GEMM_TIMEOUT);
                 break;
             }
             tc_fence_after();
+            // The accumulator is given back as soon as it is in registers; its stores are
+            // not waited for.
+            const int cols = min(kGroupCols, p.o - c0);
+            auto release = [&]() {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_remote_relaxed(leader_tempty0 + acc * 8);
+            };
+            if (cols <= 0) release();
 #pragma unroll 1
-            for (int c = 0; c < 128; c += 32) {
-                if (c0 + c >= p.o) break;                // warp-uniform
+            for (int c = 0; c < cols; c += 32) {
                 uint32_t r[32];
-                tmem_ld_32x32b_x32(tmem_base + (uint32_t)(acc * 256 + wg * 128 + c) + ((uint32_t)(q * 32) << 16), r);
+                tmem_ld_32x32b_x32(tmem_base + (uint32_t)(acc * 256 + wg * kGroupCols + c) + ((uint32_t)(q * 32) << 16), r);
                 tmem_ld_wait();
-                float v[32];
-                const float4* sv = reinterpret_cast<const float4*>(vec + c);
+                if (c + 32 >= cols) release();
+                F2 v[16];
+                const ulonglong2* sw = reinterpret_cast<const ulonglong2*>(vec + c);
+                const ulonglong2* sb = reinterpret_cast<const ulonglong2*>(vec + kGroupCols + c);
 #pragma unroll
-                for (int j = 0; j < 32; j += 2) {
-                    const float4 f = sv[j / 2];
-                    v[j] = finish(r[j], sa, f.x, f.y);
-                    v[j + 1] = finish(r[j + 1], sa, f.z, f.w);
+                for (int j = 0; j < 8; ++j) {
+                    const ulonglong2 f = sw[j], g = sb[j];
+                    v[2 * j] = finish(r[4 * j], r[4 * j + 1], sa, f.x, g.x);
+                    v[2 * j + 1] = finish(r[4 * j + 2], r[4 * j + 3], sa, f.y, g.y);
                 }
-                activate<T>(v, p.act);
+                activate<T, 32>(v, p.act, gelu);
                 if (p.vec_store) {
-                    // Rows past m of the last tile are clipped by the store; a
-                    // CTA whose 128 rows all lie past m stores nothing.
-                    uint8_t* buf = buf0 + (oc & 1) * S::OUT_CHUNK;
-                    if (ep_tid == 0) bulk_wait_group_read<1>();
-                    group_sync(wg);
+                    // A warp stores its 32 rows by itself, through its staging buffer. Rows
+                    // past m are clipped by the store; a warp whose rows all lie past m
+                    // stores nothing.
+                    if (lane == 0) bulk_wait_group_read<0>();
+                    __syncwarp();
                     constexpr int PIECES = 32 * sizeof(T) / 16, PER = 16 / sizeof(T);
 #pragma unroll
                     for (int j = 0; j < PIECES; ++j) {
-                        const int phys = PIECES == 4 ? j ^ ((rloc >> 1) & 3) : j ^ (rloc & 7);
-                        store16<T>(reinterpret_cast<T*>(buf + rloc * 32 * sizeof(T) + phys * 16), v + PER * j);
+                        const int phys = PIECES == 4 ? j ^ ((lane >> 1) & 3) : j ^ (lane & 7);
+                        *reinterpret_cast<uint4*>(buf + lane * 32 * sizeof(T) + phys * 16) = store_form<T>(v + PER / 2 * j);
                     }
                     fence_async_shared();
-                    group_sync(wg);
-                    if (ep_tid == 0 && row0 < p.m) {
-                        tma_store_3d(&tm_y, buf, c0 + c, row0, model);
+                    __syncwarp();
+                    if (lane == 0 && row0 + q * 32 < p.m) {
+                        tma_store_3d(&tm_y, buf, c0 + c, row0 + q * 32, model);
                         bulk_commit_group();
                     }
-                    ++oc;
                 } else {
                     // Rows that start off the 16-byte borders: through this warp's part
-                    // of the staging buffer (rows of 33 values: no bank twice), so that a
-                    // store covers 32 neighbours. Each thread storing its own row took
-                    // 7 to 9 times as long.
-                    T* stage = reinterpret_cast<T*>(buf0 + q * (2 * S::OUT_CHUNK / 4));
+                    // of the staging buffer (columns turned by the row: no bank twice), so that a
+                    // store covers 32 neighbours (each thread storing its own row took the
+                    // kernel 5 times as long).
+                    T* stage = reinterpret_cast<T*>(buf);
                     __syncwarp();
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) stage[lane * 33 + j] = from_f<T>(v[j]);
+                    for (int j = 0; j < 32; j += 2) {
+                        float a, b;
+                        halves(v[j / 2], a, b);
+                        stage[lane * 32 + ((j + lane) & 31)] = from_f<T>(a);
+                        stage[lane * 32 + ((j + 1 + lane) & 31)] = from_f<T>(b);
+                    }
                     __syncwarp();
                     const int col = c0 + c + lane, rows = min(32, p.m - row0 - q * 32);
                     T* dst = static_cast<T*>(p.y) + ((int64_t)model * p.m + row0 + q * 32) * p.o + col;
                     if (col < p.o) {
 #pragma unroll 8
-                        for (int j = 0; j < rows; ++j, dst += p.o) *dst = stage[j * 33 + lane];
+                        for (int j = 0; j < rows; ++j, dst += p.o) *dst = stage[j * 32 + ((lane + j) & 31)];
                     }
                 }
             }
-            tc_fence_before();
-            mbar_arrive_remote(leader_tempty0 + acc * 8);
         }
-        if (ep_tid == 0) bulk_wait_group_all();
+        if (lane == 0) bulk_wait_group_all();
     }
 
     tc_fence_before();
@@ -361,6 +434,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
 // ---------------------------------------------------------------------------
 constexpr int kNarrowThreads = 128;
 
+// Adds the S parts of this thread's channel for the tokens rank, rank + S, .., four
+// at a time (their loads from the other CTAs in flight together), and finishes them.
+template <typename T, int S>
+__device__ __forceinline__ void add_parts(const uint32_t* part, int rank, int tokens, const float* sa, float sw,
+                                          float bias, int act, bool live, T* y, int64_t ld) {
+    const Gelu2 gelu;
+    uint32_t from[S];
+#pragma unroll
+    for (int k = 0; k < S; ++k) from[k] = map_to_rank(smem_addr(part) + threadIdx.x * 4, k);
+    for (int c = rank; c < tokens; c += 4 * S) {
+        uint32_t acc[4] = {};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (c + i * S < tokens) {
+#pragma unroll
+                for (int k = 0; k < S; ++k) acc[i] += load_cluster_u32(from[k] + (c + i * S) * 512);
+            }
+        F2 v[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int c0 = c + 2 * i * S, c1 = c0 + S;
+            v[i] = finish(acc[2 * i], acc[2 * i + 1], pair_of(c0 < tokens ? sa[c0] : 0.f, c1 < tokens ? sa[c1] : 0.f),
+                          pair_of(sw, sw), pair_of(bias, bias));
+        }
+        activate<T, 4>(v, act, gelu);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int c0 = c + 2 * i * S, c1 = c0 + S;
+            float a, b;
+            halves(v[i], a, b);
+            if (live && c0 < tokens) y[c0 * ld] = from_f<T>(a);
+            if (live && c1 < tokens) y[c1 * ld] = from_f<T>(b);
+        }
+    }
+}
+
 template <typename T, int BN>
 __global__ void __launch_bounds__(kNarrowThreads)
     narrow_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w, const Int8Args p,
@@ -372,6 +481,7 @@ __global__ void __launch_bounds__(kNarrowThreads)
     __shared__ uint64_t full[8], empty[8], tfull;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
+    __shared__ __align__(16) float s_sa[BN];
     volatile int* abort_flag = &abort_word;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sW = smem;
@@ -383,6 +493,13 @@ __global__ void __launch_bounds__(kNarrowThreads)
     const int mt = tile % mt_count, ot = tile / mt_count % ot_count, model = tile / mt_count / ot_count;
     const int kb0 = kb_count * rank / split, kbs = kb_count * (rank + 1) / split - kb0;
 
+    // Thread = output channel in the end, columns = tokens.
+    const int o = ot * 128 + threadIdx.x, tokens = min(BN, p.m - mt * BN);
+    const int64_t wat = (int64_t)model * p.o + o;
+    if (threadIdx.x < BN)
+        s_sa[threadIdx.x] = threadIdx.x < tokens ? p.sa[(int64_t)model * p.m + mt * BN + threadIdx.x] : 0.f;
+    const float sw = o < p.o ? p.sw[wat] : 0.f;
+    const float bias = p.bias && o < p.o ? to_f<T>(static_cast<const T*>(p.bias)[wat]) : 0.f;
     if (threadIdx.x == 0) {
         tma_prefetch_desc(&tm_a);
         tma_prefetch_desc(&tm_w);
@@ -447,13 +564,7 @@ __global__ void __launch_bounds__(kNarrowThreads)
     const bool ok = mbar_wait(&tfull, 0, &never);
     tc_fence_after();
 
-    // Thread = output channel, columns = tokens.
-    const int o = ot * 128 + threadIdx.x, tokens = p.m - mt * BN < BN ? p.m - mt * BN : BN;
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    const int64_t wat = (int64_t)model * p.o + o;
-    const float sw = o < p.o ? p.sw[wat] : 0.f;
-    const float bias = p.bias && o < p.o ? to_f<T>(static_cast<const T*>(p.bias)[wat]) : 0.f;
-    const float* sa = p.sa + (int64_t)model * p.m + mt * BN;
     T* y = static_cast<T*>(p.y) + ((int64_t)model * p.m + mt * BN) * p.o + o;
     constexpr int CH = BN < 32 ? BN : 32;
     auto load = [&](int c, uint32_t (&r)[CH]) {
@@ -462,17 +573,24 @@ __global__ void __launch_bounds__(kNarrowThreads)
         tmem_ld_wait();
     };
     if (split == 1) {
+        const Gelu2 gelu;
 #pragma unroll 1
         for (int c = 0; c < tokens; c += CH) {
             uint32_t r[CH];
             load(c, r);
-            float v[CH];
+            F2 v[CH / 2];
 #pragma unroll
-            for (int j = 0; j < CH; ++j) v[j] = c + j < tokens ? finish(r[j], sa[c + j], sw, bias) : 0.f;
-            activate<T>(v, p.act);
+            for (int j = 0; j < CH; j += 2)
+                v[j / 2] = finish(r[j], r[j + 1], *reinterpret_cast<const F2*>(s_sa + c + j), pair_of(sw, sw),
+                                  pair_of(bias, bias));
+            activate<T, CH>(v, p.act, gelu);
 #pragma unroll
-            for (int j = 0; j < CH; ++j)
-                if (c + j < tokens && o < p.o) y[(int64_t)(c + j) * p.o] = from_f<T>(v[j]);
+            for (int j = 0; j < CH; j += 2) {
+                float a, b;
+                halves(v[j / 2], a, b);
+                if (c + j < tokens && o < p.o) y[(int64_t)(c + j) * p.o] = from_f<T>(a);
+                if (c + j + 1 < tokens && o < p.o) y[(int64_t)(c + j + 1) * p.o] = from_f<T>(b);
+            }
         }
     } else {
         // The parts as [token][channel] in the ring's memory (its copies have been
@@ -488,14 +606,9 @@ __global__ void __launch_bounds__(kNarrowThreads)
             }
         }
         cluster_sync_all();
-        const uint32_t mine = smem_addr(part) + threadIdx.x * 4;
-        for (int c = rank; c < tokens; c += split) {
-            uint32_t acc = 0;
-            for (int k = 0; k < split; ++k) acc += load_cluster_u32(map_to_rank(mine + c * 512, k));
-            float v[2] = {finish(acc, sa[c], sw, bias), 0.f};
-            activate<T>(v, p.act);
-            if (o < p.o) y[(int64_t)c * p.o] = from_f<T>(v[0]);
-        }
+        if (split == 2) add_parts<T, 2>(part, rank, tokens, s_sa, sw, bias, p.act, o < p.o, y, p.o);
+        else if (split == 4) add_parts<T, 4>(part, rank, tokens, s_sa, sw, bias, p.act, o < p.o, y, p.o);
+        else add_parts<T, 8>(part, rank, tokens, s_sa, sw, bias, p.act, o < p.o, y, p.o);
         cluster_sync_all();                  // no CTA leaves while others read its part
     }
     tc_fence_before();
@@ -536,18 +649,17 @@ struct Int8Launch {
     template <typename T>
     int wide() {
         using S = WideSmem<T>;
-        CUtensorMap ta, tw, ty{};
+        CUtensorMap ta, tw;
         int rc = rows_map(&ta, a, p.n, p.m, p.k, a_ld, a_ms, 128);
         if (rc == WIDEK_OK) rc = rows_map(&tw, w, p.n, p.o, p.k, w_ld, w_ms, 128);
         p.vec_store = (int64_t)p.o * sizeof(T) % 16 == 0 && aligned16(p.y);
+        CUtensorMap ty = ta;
         if (rc == WIDEK_OK && p.vec_store) {
             const uint64_t dims[3] = {(uint64_t)p.o, (uint64_t)p.m, (uint64_t)p.n};
             const uint64_t strides[2] = {(uint64_t)p.o * sizeof(T), (uint64_t)p.m * p.o * sizeof(T)};
-            const uint32_t box[3] = {32, 128, 1};
+            const uint32_t box[3] = {32, 32, 1};
             rc = encode_tmap_tiled(&ty, out_type<T>(), 3, p.y, dims, strides, box,
                                    sizeof(T) == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
-        } else {
-            ty = ta;
         }
         if (rc == WIDEK_OK) rc = reserve(wide_kernel<T>, S::TOTAL);
         if (rc != WIDEK_OK) return rc;
@@ -564,9 +676,15 @@ struct Int8Launch {
         if (rc == WIDEK_OK) rc = rows_map(&tw, w, p.n, p.o, p.k, w_ld, w_ms, 128);
         const int sms = sm_count(current_device()), kb = (p.k + kBK - 1) / kBK;
         const int64_t tiles = (int64_t)p.n * ((p.m + BN - 1) / BN) * ((p.o + 127) / 128);
+        // K is split where that fills the device and leaves each CTA four blocks of it:
+        // (us, alone / in parts) 1 x 4096 -> 4096 for one token 18 / 9.4, 2 x 4176 ->
+        // 4096 for 22 tokens 26 / 16; but 8 x 1024 -> 4096 for 4 tokens 11.9 / 12.9.
         int split = 1;
-        while (split < 8 && tiles * split < 2 * sms && kb >= 4 * split) split *= 2;
-        const int most = (kb + split - 1) / split, stages = most < 6 ? most : 6;
+        while (split < 8 && tiles * split <= (BN > 64 ? sms / 2 : sms) && kb >= 8 * split) split *= 2;
+        // The ring is as deep as lets the SM's share of CTAs (up to 5) be there at once.
+        const int most = (kb + split - 1) / split, share = (int)std::min<int64_t>(5, (tiles * split + sms - 1) / sms);
+        const int fit = 222 * 1024 / std::max(2, share) / ((128 + BN) * kBK);
+        const int stages = std::min(most, std::max(2, std::min(8, fit)));
         size_t bytes = (size_t)stages * (128 + BN) * kBK;
         if (split > 1) bytes = std::max<size_t>(bytes, (size_t)BN * 512);
         // A CTA holds at least 456 bytes of an SM's 228 KB for each of its 512 TMEM

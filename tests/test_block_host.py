@@ -174,10 +174,10 @@ def test_rows_of_codes_read_in_place_or_copied():
 
 
 def test_gelu_of_16_bit_results():
-    """fp32 restatement of gelu2 in csrc/linear_int8.cu with the coefficients read
+    """fp32 restatement of Gelu2 in csrc/linear_int8.cu with the coefficients read
     from it: the normal tail within 9e-6 of itself up to 8."""
     src = (pathlib.Path(ops.__file__).resolve().parents[1] / "csrc" / "linear_int8.cu").read_text()
-    body = src[src.index("constexpr float r[9] = {"):]
+    body = src[src.index("constexpr float c[9] = {"):]
     r = np.float32([float(v) for v in re.findall(r"(-?[0-9.]+(?:e-[0-9]+)?)f", body[body.index("{"):body.index("}")])])
     assert len(r) == 9
     a = np.linspace(0, 8, 200001).astype(np.float32)
