@@ -4,8 +4,10 @@ N small decoders (token embedding, layers of LayerNorm -> WideDecoderAttention
 -> LayerNorm -> two Linear layers, a vocabulary projection) run as one wide
 model: each continues its own prompts, greedily, over a paged key-value cache.
 The prompt goes through ``prefill`` once, then every token is one ``step``.
+With ``--stack`` the layers are a WideDecoderStack (norms fused into the residual
+stream), with ``--int8`` its linear layers run on 8-bit weights.
 
-    python examples/wide_decoder.py [--models 8] [--batch 4] [--prompt 64] [--new 32] [--cache int8]
+    python examples/wide_decoder.py [--models 8] [--batch 4] [--prompt 64] [--new 32] [--cache int8] [--stack] [--int8]
 """
 from __future__ import annotations
 
@@ -89,6 +91,27 @@ class WideDecoder(nn.Module):
         return torch.cat(out, -1), torch.cat(kept, 2)
 
 
+class WideStackDecoder(WideDecoder):
+    """The same decoder with a WideDecoderStack for its layers and last norm."""
+
+    def __init__(self, n: int, vocab: int, d_model: int, layers: int, heads: int, kv_heads: int, max_len: int):
+        super().__init__(n, vocab, d_model, 0, heads, kv_heads, max_len)
+        self.stack = wc.WideDecoderStack(n, d_model, layers, heads, kv_heads, post_norm=True, max_positions=max_len)
+        self.norm = nn.Identity()                        # the stack's last norm
+
+    def caches(self, batch: int, page_size: int = 16, dtype=None):
+        return self.stack.new_caches(batch, self.max_len, page_size, dtype)
+
+    def forward(self, tokens: Tensor) -> Tensor:
+        return self.head(self.stack(self._tokens(tokens)))
+
+    def prefill(self, tokens: Tensor, caches, positions: Tensor) -> Tensor:
+        return self.head(self.stack.prefill(self._tokens(tokens), caches, positions))
+
+    def step(self, tokens: Tensor, caches, lengths: Tensor) -> Tensor:
+        return self.head(self.stack.step(self._tokens(tokens), caches, lengths))
+
+
 def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--models", type=int, default=8)
@@ -96,9 +119,14 @@ def main() -> None:
     ap.add_argument("--prompt", type=int, default=64)
     ap.add_argument("--new", type=int, default=32)
     ap.add_argument("--cache", choices=("model", "int8", "fp8"), default="model")
+    ap.add_argument("--stack", action="store_true")
+    ap.add_argument("--int8", action="store_true")
     a = ap.parse_args()
     torch.manual_seed(0)
-    model = WideDecoder(a.models, 1000, 512, 2, 8, 2, a.prompt + a.new).to("cuda", torch.bfloat16).eval()
+    kind = WideStackDecoder if a.stack or a.int8 else WideDecoder
+    model = kind(a.models, 1000, 512, 2, 8, 2, a.prompt + a.new).to("cuda", torch.bfloat16).eval()
+    if a.int8:
+        model.stack.quantize_()
     prompts = torch.randint(0, 1000, (a.models, a.batch, a.prompt), device="cuda")
     lengths = torch.randint(a.prompt // 2, a.prompt + 1, (a.models, a.batch), device="cuda", dtype=torch.int32)
     dtype = {"model": None, "int8": torch.int8, "fp8": torch.float8_e4m3fn}[a.cache]

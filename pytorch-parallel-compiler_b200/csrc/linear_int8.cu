@@ -19,6 +19,7 @@
 //           too few tiles for the device, and the parts (integers: any order gives
 //           the same sum) are added through distributed shared memory.
 #include <algorithm>
+#include <atomic>
 
 #include "residual_norm.cuh"
 
@@ -632,11 +633,15 @@ CUtensorMapDataType out_type() {
                           : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
 }
 
+// Lets the kernel have `bytes` of shared memory; `had` is what it has, by device.
 template <typename K>
-int reserve(K kernel, size_t bytes) {
+int reserve(K kernel, size_t bytes, std::atomic<int> (&had)[64]) {
+    std::atomic<int>& h = had[current_device() & 63];
+    if (h.load(std::memory_order_relaxed) >= (int)bytes) return WIDEK_OK;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (e != cudaSuccess)
         return set_error(WIDEK_ERR_CUDA, "widek_linear_int8_fwd: %zu bytes of shared memory: %s", bytes, cudaGetErrorString(e));
+    h.store((int)bytes, std::memory_order_relaxed);
     return WIDEK_OK;
 }
 
@@ -661,7 +666,8 @@ struct Int8Launch {
             rc = encode_tmap_tiled(&ty, out_type<T>(), 3, p.y, dims, strides, box,
                                    sizeof(T) == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
         }
-        if (rc == WIDEK_OK) rc = reserve(wide_kernel<T>, S::TOTAL);
+        static std::atomic<int> had[64];
+        if (rc == WIDEK_OK) rc = reserve(wide_kernel<T>, S::TOTAL, had);
         if (rc != WIDEK_OK) return rc;
         const int64_t tiles = (int64_t)p.n * ((p.m + 255) / 256) * ((p.o + 255) / 256);
         const int grid = (int)std::min<int64_t>(2 * tiles, sm_count(current_device()) / 2 * 2);
@@ -692,7 +698,9 @@ struct Int8Launch {
         // another, never wait for columns that others of their kind hold.
         bytes = std::max<size_t>(bytes + 1024, (BN < 32 ? 32 : BN) * 456);
         if (tiles * split > 0x7fffffff) return set_error(WIDEK_ERR_INVALID, "widek_linear_int8_fwd: over 2^31 tiles");
-        if (rc == WIDEK_OK) rc = reserve(narrow_kernel<T, BN>, bytes);
+        static std::atomic<int> had[64];
+        // (the most that any call asks for, so that calls on two threads cannot take it back)
+        if (rc == WIDEK_OK) rc = reserve(narrow_kernel<T, BN>, 224 * 1024, had);
         if (rc != WIDEK_OK) return rc;
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3((unsigned)(tiles * split));

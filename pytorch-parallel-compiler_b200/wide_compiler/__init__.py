@@ -21,7 +21,8 @@ from .core.ensemble_util import pack_inputs, unpack_outputs
 from .core.paged_cache import WidePagedCache
 from .core.primitives import (WideLinear, WideConv1d, WideConv2d, WideConv3d, WideBatchNorm1d, WideBatchNorm2d,
                               WideLayerNorm, WideGroupNorm, WideInstanceNorm1d, WideInstanceNorm2d, WideEmbedding,
-                              WideAttention, WideDecoderAttention, WideGRU, WideLSTM)
+                              WideAttention, WideDecoderAttention, WideDecoderStack, WideLinearInt8, WideGRU,
+                              WideLSTM)
 
 _HAS_BENCHMARK = False
 benchmark_primitive = None
@@ -42,7 +43,7 @@ __all__ = [
     'WideLinear', 'WideConv1d', 'WideConv2d', 'WideConv3d', 'WideBatchNorm1d', 'WideBatchNorm2d',
     'WideLayerNorm', 'WideGroupNorm', 'WideInstanceNorm1d', 'WideInstanceNorm2d', 'WideEmbedding',
     'WideAttention', 'WideGRU', 'WideLSTM',
-    'WideDecoderAttention', 'WidePagedCache',
+    'WideDecoderAttention', 'WideDecoderStack', 'WideLinearInt8', 'WidePagedCache',
     'benchmark_primitive', 'benchmark_multi', 'benchmark_all', 'benchmark_custom', 'list_benchmark_primitives',
     'BenchmarkResult', 'SweepParams',
 ]

@@ -348,8 +348,96 @@ def _(q, k_pages, v_pages, table, k_scale, v_scale, lengths, scale, window):
     return q.new_empty(q.shape)
 
 
+@torch.library.custom_op("widek::residual_norm", mutates_args=())
+def residual_norm(x: Tensor, y: Tensor, weight: Tensor, bias: Optional[Tensor], post_weight: Optional[Tensor],
+                  post_bias: Optional[Tensor], gate: Optional[Tensor], scale: float, eps: float,
+                  center: bool) -> Tuple[Tensor, Tensor]:
+    """Residual sum, gate and norms of a block boundary (ops.residual_norm)."""
+    with torch.no_grad():
+        return ops.residual_norm(x, y, weight, bias, post_weight, post_bias, gate, scale, eps, center)
+
+
+@residual_norm.register_fake
+def _(x, y, weight, bias, post_weight, post_bias, gate, scale, eps, center):
+    return x.new_empty(x.shape), x.new_empty(x.shape)
+
+
+_register_autograd(residual_norm, _AG.residual_norm_t)
+
+
+@torch.library.custom_op("widek::row_norm", mutates_args=())
+def row_norm(x: Tensor, weight: Tensor, bias: Optional[Tensor], eps: float, center: bool) -> Tensor:
+    """The norm of ops.residual_norm alone (without y)."""
+    with torch.no_grad():
+        return ops.residual_norm(x, None, weight, bias, eps=eps, center=center)[1]
+
+
+@row_norm.register_fake
+def _(x, weight, bias, eps, center):
+    return x.new_empty(x.shape)
+
+
+_register_autograd(row_norm, lambda x, weight, bias, eps, center: _AG._norm_t(x.float(), weight, bias, eps,
+                                                                              center).to(x.dtype))
+
+
+def _fake_codes(x):
+    k = x.shape[-1]
+    held = x.new_empty((*x.shape[:-1], (k + 15) // 16 * 16), dtype=torch.int8)
+    return held[..., :k], x.new_empty(x.shape[:-1], dtype=torch.float32)
+
+
+@torch.library.custom_op("widek::residual_norm_quantize", mutates_args=())
+def residual_norm_quantize(x: Tensor, y: Tensor, weight: Tensor, bias: Optional[Tensor], post_weight: Optional[Tensor],
+                           post_bias: Optional[Tensor], gate: Optional[Tensor], scale: float, eps: float,
+                           center: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    """The same with the norm as 8-bit codes (ops.residual_norm_quantize)."""
+    return ops.residual_norm_quantize(x, y, weight, bias, post_weight, post_bias, gate, scale, eps, center)
+
+
+@residual_norm_quantize.register_fake
+def _(x, y, weight, bias, post_weight, post_bias, gate, scale, eps, center):
+    return (x.new_empty(x.shape), *_fake_codes(x))
+
+
+@torch.library.custom_op("widek::row_norm_quantize", mutates_args=())
+def row_norm_quantize(x: Tensor, weight: Tensor, bias: Optional[Tensor], eps: float,
+                      center: bool) -> Tuple[Tensor, Tensor]:
+    """Norm of rows as 8-bit codes (ops.residual_norm_quantize without y)."""
+    return ops.residual_norm_quantize(x, None, weight, bias, eps=eps, center=center)[1:]
+
+
+@row_norm_quantize.register_fake
+def _(x, weight, bias, eps, center):
+    return _fake_codes(x)
+
+
+@torch.library.custom_op("widek::quantize_rows", mutates_args=())
+def quantize_rows(x: Tensor) -> Tuple[Tensor, Tensor]:
+    """Rows as 8-bit codes and scales (ops.quantize_rows)."""
+    return ops.quantize_rows(x)
+
+
+@quantize_rows.register_fake
+def _(x):
+    return _fake_codes(x)
+
+
+@torch.library.custom_op("widek::linear_int8", mutates_args=())
+def linear_int8(codes: Tensor, scale: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[Tensor], act: int,
+                dtype: torch.dtype) -> Tensor:
+    """A linear layer on 8-bit codes (ops.linear_int8)."""
+    return ops.linear_int8(codes, scale, weight, weight_scale, bias, act, dtype)
+
+
+@linear_int8.register_fake
+def _(codes, scale, weight, weight_scale, bias, act, dtype):
+    return codes.new_empty((*codes.shape[:-1], weight.shape[1]), dtype=dtype)
+
+
 OPERATORS = ('linear', 'layernorm', 'batchnorm', 'groupnorm', 'embedding', 'conv', 'gru', 'lstm', 'attention',
              'swap01', 'unary', 'binary', 'qk_norm_rope', 'qk_norm_rope_write', 'cache_write', 'cache_read',
-             'causal_attention', 'decode_attention')
+             'causal_attention', 'decode_attention', 'residual_norm', 'row_norm', 'residual_norm_quantize',
+             'row_norm_quantize', 'quantize_rows', 'linear_int8')
 
 __all__ = ['OPERATORS']

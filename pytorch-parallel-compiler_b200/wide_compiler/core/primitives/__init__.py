@@ -12,7 +12,9 @@ from .wide_groupnorm import WideGroupNorm, GroupNormStrategy
 from .wide_instancenorm import WideInstanceNorm1d, WideInstanceNorm2d, InstanceNormStrategy
 from .wide_embedding import WideEmbedding, EmbeddingStrategy
 from .wide_attention import WideAttention, AttentionStrategy
+from .wide_linear_int8 import WideLinearInt8
 from .wide_decoder_attention import WideDecoderAttention
+from .wide_decoder_stack import WideDecoderStack, WideDecoderLayer
 from .wide_gru import WideGRU, GRUStrategy
 from .wide_lstm import WideLSTM, LSTMStrategy
 
@@ -44,7 +46,7 @@ __all__ = [
     'WideInstanceNorm1d', 'WideInstanceNorm2d', 'InstanceNormStrategy',
     'WideEmbedding', 'EmbeddingStrategy',
     'WideAttention', 'AttentionStrategy',
-    'WideDecoderAttention',
+    'WideDecoderAttention', 'WideDecoderStack', 'WideDecoderLayer', 'WideLinearInt8',
     'WideGRU', 'GRUStrategy',
     'WideLSTM', 'LSTMStrategy',
     'BUILTIN_PRIMITIVES',

@@ -12,6 +12,10 @@ Parameters are N-first: ``qkv_weight`` [N, (Hq + 2 Hk) D, d_model] (queries,
 then keys, then values), ``q_norm`` / ``k_norm`` [N, D], ``out_weight``
 [N, d_model, Hq D], optional ``qkv_bias`` / ``out_bias``.
 
+``quantize_()`` turns the projections into 8-bit ones for serving
+(WideLinearInt8); the input may then be the (codes, scales) of its rows as
+``ops.residual_norm_quantize`` makes them.
+
 Kernels: the projections are grouped GEMMs; norm and rotation run in one pass
 over the projection's output in place (``ops.qk_norm_rope``), in a step
 together with the cache write (``ops.qk_norm_rope_write``); whole sequences use
@@ -19,13 +23,16 @@ the flash-style core, steps ``ops.decode_attention``.
 """
 from __future__ import annotations
 
-from typing import List, Optional
+from typing import List, Optional, Tuple, Union
 
 import torch
 from torch import Tensor, nn
 
 from ... import ops
 from ..paged_cache import WidePagedCache
+from .wide_linear_int8 import WideLinearInt8
+
+Rows = Union[Tensor, Tuple[Tensor, Tensor]]      # x, or the codes and scales of its rows
 
 
 class WideDecoderAttention(nn.Module):
@@ -52,6 +59,8 @@ class WideDecoderAttention(nn.Module):
         for i in range(n):
             nn.init.xavier_uniform_(self.qkv_weight[i])
             nn.init.xavier_uniform_(self.out_weight[i])
+        self.qkv_int8: Optional[WideLinearInt8] = None           # the projections after quantize_()
+        self.out_int8: Optional[WideLinearInt8] = None
         self._tables = {}                # fp32 whatever the module's type, so not buffers
 
     def rotation(self, device: torch.device, rows: Optional[int] = None):
@@ -88,20 +97,46 @@ class WideDecoderAttention(nn.Module):
             raise ValueError(f"WideDecoderAttention: {x.shape[2]} tokens where there are positions for {most}")
         return torch.arange(x.shape[2], device=x.device)
 
+    @torch.no_grad()
+    def quantize_(self) -> 'WideDecoderAttention':
+        """Turns the projections (on the GPU) into 8-bit ones, in place; their
+        weights are given up. For serving: there is no gradient from then on."""
+        if self.qkv_int8 is None:
+            self.qkv_int8 = WideLinearInt8.from_weight(self.qkv_weight, self.qkv_bias)
+            self.out_int8 = WideLinearInt8.from_weight(self.out_weight, self.out_bias)
+            for name in ('qkv_weight', 'out_weight', 'qkv_bias', 'out_bias'):
+                setattr(self, name, None)
+            self.q_norm.requires_grad_(False)
+            self.k_norm.requires_grad_(False)
+        return self
+
+    def _first(self, x: Rows) -> Tensor:
+        """x, or its codes: what has its shape and device."""
+        if isinstance(x, tuple):
+            if self.qkv_int8 is None:
+                raise TypeError("WideDecoderAttention: codes are for a layer whose projections are quantised "
+                                "(quantize_)")
+            return x[0]
+        return x
+
     def _check(self, x: Tensor) -> None:
         if x.dim() != 4 or x.shape[0] != self.n or x.shape[3] != self.d_model:
             raise ValueError(f"WideDecoderAttention: input must be [N={self.n}, B, T, D={self.d_model}], got "
                              f"{tuple(x.shape)}")
 
-    def _project(self, x: Tensor):
-        self._check(x)
-        qkv = ops.linear(x, self.qkv_weight, self.qkv_bias)
+    def _project(self, x: Rows):
+        self._check(self._first(x))
+        if self.qkv_int8 is not None:
+            qkv = self.qkv_int8(x)
+        else:
+            qkv = ops.linear(x, self.qkv_weight, self.qkv_bias)
         d, hq, hk = self.head_dim, self.n_heads, self.n_kv_heads
         cut = lambda a, h: qkv[..., a * d:(a + h) * d].unflatten(-1, (h, d))
         return cut(0, hq), cut(hq, hk), cut(hq + hk, hk)
 
     def _output(self, o: Tensor) -> Tensor:
-        return ops.linear(o.flatten(-2), self.out_weight, self.out_bias)
+        o = o.flatten(-2)
+        return ops.linear(o, self.out_weight, self.out_bias) if self.out_int8 is None else self.out_int8(o)
 
     def new_cache(self, batch: int, max_len: int, page_size: int = 64, dtype: Optional[torch.dtype] = None
                   ) -> WidePagedCache:
@@ -110,38 +145,40 @@ class WideDecoderAttention(nn.Module):
             raise ValueError(f"WideDecoderAttention: a cache of {max_len} tokens goes past max_positions = "
                              f"{self.max_positions}")
         return WidePagedCache.allocate(self.n, batch, self.n_kv_heads, self.head_dim, max_len, page_size,
-                                       self.qkv_weight.dtype if dtype is None else dtype, self.qkv_weight.device)
+                                       self.q_norm.dtype if dtype is None else dtype, self.q_norm.device)
 
-    def forward(self, x: Tensor, positions: Optional[Tensor] = None) -> Tensor:
+    def forward(self, x: Rows, positions: Optional[Tensor] = None) -> Tensor:
         """x [N, B, T, d_model] -> the same shape, causal over the T tokens
         (padding, whose ``positions`` are negative, at their end)."""
-        self._check(x)
-        positions = self._positions(x, positions, self.max_positions)
+        first = self._first(x)
+        self._check(first)
+        positions = self._positions(first, positions, self.max_positions)
         q, k, v = self._project(x)
-        q, k = ops.qk_norm_rope(q, k, self.q_norm, self.k_norm, *self.rotation(x.device), positions, self.eps,
+        q, k = ops.qk_norm_rope(q, k, self.q_norm, self.k_norm, *self.rotation(first.device), positions, self.eps,
                                 self.interleaved)
         return self._output(ops.causal_attention(q, k, v))
 
     @torch.no_grad()
-    def prefill(self, x: Tensor, cache: WidePagedCache, positions: Optional[Tensor] = None) -> Tensor:
+    def prefill(self, x: Rows, cache: WidePagedCache, positions: Optional[Tensor] = None) -> Tensor:
         """``forward`` on prompts from position 0, padded at the end where
         ``positions`` ([B, T] or [N, B, T]) is negative, with the keys and
         values written to the cache."""
-        self._check(x)
-        positions = self._positions(x, positions, min(self.max_positions, cache.max_len))
+        first = self._first(x)
+        self._check(first)
+        positions = self._positions(first, positions, min(self.max_positions, cache.max_len))
         q, k, v = self._project(x)
-        q, k = ops.qk_norm_rope(q, k, self.q_norm, self.k_norm, *self._cache_rotation(x, cache), positions, self.eps,
+        q, k = ops.qk_norm_rope(q, k, self.q_norm, self.k_norm, *self._cache_rotation(first, cache), positions, self.eps,
                                 self.interleaved)
         ops.cache_write(cache, k, v, positions)
         return self._output(ops.causal_attention(q, k, v))
 
     @torch.no_grad()
-    def step(self, x: Tensor, cache: WidePagedCache, lengths: Tensor, window: int = 0) -> Tensor:
+    def step(self, x: Rows, cache: WidePagedCache, lengths: Tensor, window: int = 0) -> Tensor:
         """One new token: x [N, B, 1, d_model]; ``lengths`` [B] or [N, B] are
         the tokens of each sequence with the new one, whose position is
         length - 1 (a length of 0 leaves the sequence out: zeros attend)."""
         q, k, v = self._project(x)
-        q = ops.qk_norm_rope_write(q, k, v, self.q_norm, self.k_norm, *self._cache_rotation(x, cache),
+        q = ops.qk_norm_rope_write(q, k, v, self.q_norm, self.k_norm, *self._cache_rotation(q, cache),
                                    (lengths - 1).unsqueeze(-1), cache, self.eps, self.interleaved)
         o = ops.decode_attention(q.squeeze(2), cache, lengths, window=window)
         return self._output(o.unsqueeze(2))
@@ -150,6 +187,8 @@ class WideDecoderAttention(nn.Module):
     def from_modules(cls, modules: List['WideDecoderAttention']) -> 'WideDecoderAttention':
         """Fuses layers of the same configuration (each of any n) into one."""
         t = modules[0]
+        if any(m.qkv_int8 is not None for m in modules):
+            raise ValueError("WideDecoderAttention: layers are fused before they are quantised")
         wide = cls(sum(m.n for m in modules), t.d_model, t.n_heads, t.n_kv_heads, t.head_dim, t.rotary_dim,
                    t.max_positions, t.theta, t.interleaved, t.eps, t.qkv_bias is not None)
         wide = wide.to(device=t.qkv_weight.device, dtype=t.qkv_weight.dtype)

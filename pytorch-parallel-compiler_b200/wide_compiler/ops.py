@@ -1258,30 +1258,44 @@ def decode_attention(q: Tensor, cache, lengths: Tensor, scale: Optional[float] =
 # Block boundaries: the residual stream and its norms, rows as 8-bit codes
 # ---------------------------------------------------------------------------
 
-def _block_args(what: str, x: Tensor, y: Optional[Tensor], weight: Tensor, bias: Optional[Tensor],
-                post_weight: Optional[Tensor], post_bias: Optional[Tensor], gate: Optional[Tensor]):
-    """Checks the tensors of a residual norm; returns the device's index, the
-    dense tensors and (n, rows, d, gate_rows)."""
-    idx = _device(what, x, y, weight, bias, post_weight, post_bias, gate)
-    _same_dtype(what, x, y, weight, bias, post_weight, post_bias, gate)
-    shape = x.shape
+def _block_args(what: str, x: Tensor, y: Optional[Tensor], *params: Optional[Tensor]):
+    """Checks the tensors of a residual norm (params: weight, bias, post_weight,
+    post_bias, gate); returns the device's index, the dense tensors and
+    (n, rows, d, gate_rows)."""
+    idx, dtype, shape = x.get_device(), x.dtype, x.shape
     if len(shape) < 2:
         raise ValueError(f"{what}: x must be [N, ..., D], got {tuple(shape)}")
-    if y is not None and y.shape != shape:
-        raise ValueError(f"{what}: y {tuple(y.shape)} does not match x {tuple(shape)}")
+    gate = params[4]
     n, d = shape[0], shape[-1]
-    for name, p in (("weight", weight), ("bias", bias), ("post_weight", post_weight), ("post_bias", post_bias)):
-        if p is not None and p.shape != (n, d):
-            raise ValueError(f"{what}: {name} must be [N, D] = [{n}, {d}], got {tuple(p.shape)}")
-    rows, gate_rows = math.prod(shape[1:-1]), -1
-    if gate is not None:
-        lead = gate.dim() - 1
-        if lead < 1 or lead >= len(shape) or gate.shape[:-1] != shape[:lead] or gate.shape[-1] != d:
-            raise ValueError(f"{what}: gate {tuple(gate.shape)} is not [N, D], or leading dims of x {tuple(shape)} and D")
-        gate_rows = math.prod(shape[lead:-1])
-    dense = [t if t is None or t.is_contiguous() else t.contiguous()
-             for t in (x, y, weight, bias, post_weight, post_bias, gate)]
-    return idx, dense, (n, rows, d, gate_rows)
+    nd, fine = (n, d), idx >= 0
+    dense = [x if x.is_contiguous() else x.contiguous(), None]
+    if y is not None:
+        fine = fine and y.shape == shape and y.dtype == dtype and y.get_device() == idx
+        dense[1] = y if y.is_contiguous() else y.contiguous()
+    for p in params:
+        if p is not None:
+            fine = fine and p.dtype == dtype and p.get_device() == idx and (p is gate or p.shape == nd)
+            p = p if p.is_contiguous() else p.contiguous()
+        dense.append(p)
+    if not fine:                     # say what is wrong
+        _device(what, x, y, *params)
+        _same_dtype(what, x, y, *params)
+        if y is not None and y.shape != shape:
+            raise ValueError(f"{what}: y {tuple(y.shape)} does not match x {tuple(shape)}")
+        for name, p in zip(("weight", "bias", "post_weight", "post_bias"), params):
+            if p is not None and p.shape != nd:
+                raise ValueError(f"{what}: {name} must be [N, D] = [{n}, {d}], got {tuple(p.shape)}")
+    rows = math.prod(shape[1:-1])
+    if gate is None:
+        return idx, dense, (n, rows, d, -1)
+    lead = gate.dim() - 1
+    if lead < 1 or lead >= len(shape) or gate.shape[:-1] != shape[:lead] or gate.shape[-1] != d:
+        raise ValueError(f"{what}: gate {tuple(gate.shape)} is not [N, D], or leading dims of x {tuple(shape)} and D")
+    return idx, dense, (n, rows, d, math.prod(shape[lead:-1]))
+
+
+def _ptrs(tensors):
+    return [None if t is None else t.data_ptr() for t in tensors]
 
 
 def residual_norm(x: Tensor, y: Optional[Tensor], weight: Tensor, bias: Optional[Tensor] = None,
@@ -1311,10 +1325,10 @@ def residual_norm(x: Tensor, y: Optional[Tensor], weight: Tensor, bias: Optional
 
 def _residual_norm(x, y, weight, bias, post_weight, post_bias, gate, scale, eps, center, need_stats: bool):
     idx, dense, sizes = _block_args("residual_norm", x, y, weight, bias, post_weight, post_bias, gate)
-    h = x if y is None else x.new_empty(x.shape)
-    z = x.new_empty(x.shape)
+    h = x if y is None else torch.empty_like(dense[0])
+    z = torch.empty_like(dense[0])
     stats = torch.empty((sizes[0], sizes[1], 4), device=x.device, dtype=torch.float32) if need_stats else None
-    _launch(idx, "widek_residual_norm_fwd", *map(N.ptr, dense), N.ptr(h), z.data_ptr(), N.ptr(stats), *sizes, scale, eps,
+    _launch(idx, "widek_residual_norm_fwd", *_ptrs(dense), h.data_ptr(), z.data_ptr(), N.ptr(stats), *sizes, scale, eps,
             center, N.dtype_code(x))
     return h, z, stats
 
@@ -1343,16 +1357,16 @@ def residual_norm_bwd(x: Tensor, y: Optional[Tensor], weight: Tensor, bias: Opti
                           *sizes, has_post, center)
     ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8)
     dh, dz = (g if g is None or g.is_contiguous() else g.contiguous() for g in (dh, dz))
-    _launch(idx, "widek_residual_norm_bwd", *map(N.ptr, dense), stats.data_ptr(), N.ptr(dh), N.ptr(dz),
-            *map(N.ptr, grads), *sizes, scale, eps, center, N.dtype_code(x), ws.data_ptr(), ws_bytes)
+    _launch(idx, "widek_residual_norm_bwd", *_ptrs(dense), stats.data_ptr(), N.ptr(dh), N.ptr(dz),
+            *_ptrs(grads), *sizes, scale, eps, center, N.dtype_code(x), ws.data_ptr(), ws_bytes)
     return grads
 
 
 def _code_rows(x: Tensor) -> Tensor:
-    """Room for the codes of x's rows, which start 16 bytes (or a multiple) apart."""
+    """Room for the codes of x's rows (x dense), which start 16 bytes (or a multiple) apart."""
     d = x.shape[-1]
     if d % 16 == 0:
-        return torch.empty(x.shape, device=x.device, dtype=torch.int8)
+        return torch.empty_like(x, dtype=torch.int8)
     return torch.empty((*x.shape[:-1], -(-d // 16) * 16), device=x.device, dtype=torch.int8)[..., :d]
 
 
@@ -1371,10 +1385,10 @@ def residual_norm_quantize(x: Tensor, y: Optional[Tensor], weight: Tensor, bias:
         return torch.ops.widek.residual_norm_quantize(x, y, weight, bias, post_weight, post_bias, gate, scale, eps,
                                                       center)
     idx, dense, sizes = _block_args(what, x, y, weight, bias, post_weight, post_bias, gate)
-    h = x if y is None else x.new_empty(x.shape)
-    codes = _code_rows(x)
+    h = x if y is None else torch.empty_like(dense[0])
+    codes = _code_rows(dense[0])
     scales = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
-    _launch(idx, "widek_residual_norm_quantize_fwd", *map(N.ptr, dense), N.ptr(h), codes.data_ptr(), scales.data_ptr(),
+    _launch(idx, "widek_residual_norm_quantize_fwd", *_ptrs(dense), h.data_ptr(), codes.data_ptr(), scales.data_ptr(),
             -(-sizes[2] // 16) * 16, *sizes, scale, eps, center, N.dtype_code(x))
     return h, codes, scales
 
@@ -1394,7 +1408,7 @@ def quantize_rows(x: Tensor):
         raise ValueError(f"{what}: x must be [..., K], got a number")
     k = x.shape[-1]
     xd = x if x.is_contiguous() else x.contiguous()
-    codes = _code_rows(x)
+    codes = _code_rows(xd)
     scales = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
     _launch(idx, "widek_quantize_rows_fwd", xd.data_ptr(), codes.data_ptr(), scales.data_ptr(), scales.numel(), k, k,
             -(-k // 16) * 16, N.dtype_code(x))
@@ -1406,6 +1420,9 @@ def _rows16(t: Tensor):
     16 bytes (copied if they do not): (codes, bytes between rows, between models)."""
     shape, st = t.shape, t.stride()
     rows = math.prod(shape[1:-1])
+    step = shape[-1]
+    if step % 16 == 0 and t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t, step, rows * step
     step = None
     if t.data_ptr() % 16 == 0 and (st[-1] == 1 or shape[-1] == 1):
         step, want = -(-shape[-1] // 16) * 16, None
@@ -1422,9 +1439,9 @@ def _rows16(t: Tensor):
         ms = st[0] if shape[0] > 1 else rows * step
         if ms % 16 == 0 and ms >= (rows - 1) * step + shape[-1]:
             return t, step, ms
-    held = _code_rows(t)
-    held.copy_(t)
     step = -(-shape[-1] // 16) * 16
+    held = torch.empty((*shape[:-1], step), device=t.device, dtype=torch.int8)[..., :shape[-1]]
+    held.copy_(t)
     return held, step, rows * step
 
 

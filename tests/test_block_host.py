@@ -189,3 +189,64 @@ def test_gelu_of_16_bit_results():
     tail = np.array([math.erfc(float(v) / math.sqrt(2)) / 2 for v in a])
     # the exponent's own roundings: 2 of at most 46 * 2^-24
     assert np.abs(np.exp2(e.astype(np.float64)) / tail - 1).max() < 9e-6 + 2 * 46 * 2.0 ** -24 * math.log(2)
+
+
+# ---------------------------------------------------------------------------
+# Modules and torch.library operators
+# ---------------------------------------------------------------------------
+
+def test_fake_implementations():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from wide_compiler import _autograd as AG
+    w = torch.ops.widek
+    with FakeTensorMode():
+        t = lambda *s, dt=torch.bfloat16: torch.empty(*s, device='cuda', dtype=dt)
+        x, nd, gate = t(2, 3, 5, 40), t(2, 40), t(2, 3, 40)
+        same = lambda a, b: all(p.shape == q.shape and p.dtype == q.dtype and p.device == q.device for p, q in zip(a, b))
+        assert same(w.residual_norm(x, x, nd, None, nd, None, gate, 1.0, 1e-6, False),
+                    AG.residual_norm_t(x, x, nd, None, nd, None, gate, 1.0, 1e-6, False))
+        assert w.row_norm(x, nd, nd, 1e-6, True).shape == x.shape
+        for codes, scale in (w.quantize_rows(x), w.row_norm_quantize(x, nd, None, 1e-6, False),
+                             w.residual_norm_quantize(x, x, nd, None, None, None, None, 1.0, 1e-6, False)[1:]):
+            assert codes.shape == x.shape and codes.dtype == torch.int8 and codes.stride(-2) == 48
+            assert scale.shape == x.shape[:-1] and scale.dtype == torch.float32
+        y = w.linear_int8(codes, scale, t(2, 7, 40, dt=torch.int8), t(2, 7, dt=torch.float32), None, 0, torch.float16)
+        assert y.shape == (2, 3, 5, 7) and y.dtype == torch.float16
+
+
+def test_stack_is_built_and_refuses():
+    import wide_compiler as wc
+    s = wc.WideDecoderStack(2, 32, 3, 4, 2, norm='layer', post_norm=True, gate_init=0.1, max_positions=9)
+    names = {k for k, _ in s.named_parameters()}
+    assert {'layers.2.attn_gate', 'layers.0.mlp_post.bias', 'norm.bias', 'layers.1.up.weight'} <= names
+    assert s.layers[0].attn.max_positions == 9 and 'layers=3' in repr(s)
+    plain = wc.WideDecoderStack(2, 32, 1, 4)
+    assert not any('bias' in k or 'gate' in k or 'post' in k for k in plain.state_dict())
+    with pytest.raises(ValueError, match="norm must be"):
+        wc.WideDecoderStack(2, 32, 1, 4, norm='batch')
+    with pytest.raises(ValueError, match="input must be"):
+        s(torch.zeros(2, 3, 32))
+    with pytest.raises(ValueError, match="gates for 3 layers"):
+        s(torch.zeros(2, 1, 3, 32), gates=[torch.zeros(2, 32)])
+
+
+def test_codes_need_a_quantised_layer():
+    import wide_compiler as wc
+    attn = wc.WideDecoderAttention(2, 32, 4)
+    with pytest.raises(TypeError, match="quantise"):
+        attn((torch.zeros(2, 1, 3, 32, dtype=torch.int8), torch.ones(2, 1, 3)))
+
+
+def test_int8_layer_keeps_its_scales_when_cast():
+    import wide_compiler as wc
+    layer = wc.WideLinearInt8(2, 17, 5)
+    layer.weight_scale.fill_(1 / 3)
+    for bias in (True, False):
+        layer = wc.WideLinearInt8(2, 17, 5, bias)
+        layer.weight_scale.fill_(1 / 3)
+        want = layer.weight_scale.clone()
+        layer.to(torch.float16)
+        assert layer.dtype == torch.float16 and torch.equal(layer.weight_scale, want)
+        assert layer.codes.shape == (2, 5, 17) and layer.codes.stride(1) == 32
+        layer.to(torch.float32)
+        assert layer.dtype == torch.float32 and layer.weight_scale.dtype == torch.float32
