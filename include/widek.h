@@ -762,9 +762,9 @@ WIDEK_API int widek_residual_norm_quantize_fwd(const void* x, const void* y, con
                                                int64_t gate_rows, double scale, double eps, int center,
                                                int dtype, void* stream);
 
-/* Such codes of the rows of x [rows, d], x_ld elements apart (any d). */
+/* Such codes of the rows of x [rows, d] (any d). */
 WIDEK_API int widek_quantize_rows_fwd(const void* x, void* codes, float* scales, int64_t rows,
-                                      int64_t d, int64_t x_ld, int64_t ld, int dtype, void* stream);
+                                      int64_t d, int64_t ld, int dtype, void* stream);
 
 /* Workspace bytes widek_residual_norm_bwd needs (-1 for bad arguments);
  * gate_rows as there, has_post: with pw. */

@@ -244,54 +244,97 @@ struct ForwardLaunch {
     }
 };
 
-// Codes of rows of any length: 8 values a thread stay in registers; what is past
-// them in longer rows is read twice (the second time from L2).
-template <typename T, int VE, int V, int TEAM>
-__global__ void __launch_bounds__(TEAM == WARP ? 128 : 1024)
+// The largest magnitude of a pack joined to `top`, NaN kept: magnitudes of 16-bit
+// types as their bits, two at a time, of fp32 as numbers.
+template <typename T, int VE>
+struct Top {
+    uint32_t bits = 0;
+    float number = 0.f;
+    __device__ __forceinline__ void take(const Pack<T, VE>& p) {
+        if constexpr (sizeof(T) == 2 && VE >= 2) {
+#pragma unroll
+            for (int j = 0; j < VE / 2; ++j) bits = __vmaxu2(bits, reinterpret_cast<const uint32_t*>(p.v)[j] & 0x7fff7fffu);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VE; ++j) number = amax2(number, to_f<T>(p.v[j]));
+        }
+    }
+    __device__ __forceinline__ float value() const {
+        if constexpr (sizeof(T) == 2 && VE >= 2) {
+            const uint16_t m = (uint16_t)max(bits & 0xffffu, bits >> 16);
+            return to_f<T>(*reinterpret_cast<const T*>(&m));
+        } else {
+            return number;
+        }
+    }
+};
+
+template <typename T, int VE>
+__device__ __forceinline__ void put_codes(uint8_t* row, int c, const Pack<T, VE>& p, float scale) {
+    float v[VE];
+    Pack<uint8_t, VE> o;
+#pragma unroll
+    for (int j = 0; j < VE; ++j) v[j] = to_f<T>(p.v[j]);
+    codes_i8<VE>(v, scale, o.v);
+    reinterpret_cast<Pack<uint8_t, VE>*>(row)[c] = o;
+}
+
+// Codes of rows: the walk of the norms, K values a thread.
+template <typename T, int VE, int K, int TEAM>
+__global__ void __launch_bounds__(TEAM == WARP ? 128 : kBlockThreads, TEAM == WARP ? 8 : 2)
     quantize_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, float* __restrict__ scales, int64_t rows, int d,
-                    int64_t ld, int64_t x_ld, int lanes) {
+                    int64_t ld, int teams, int lanes) {
+    constexpr int V = K / VE;
     __shared__ __align__(16) float slots[2][32];
+    extern __shared__ __align__(16) uint8_t ring_bytes[];
     const Seat<TEAM> at(lanes);
     Reduce<TEAM, 1> red(slots, at);
-    const int64_t row = at.team;
-    if (row >= rows) return;
+    if (at.team >= teams) return;
+    const Walk walk(at.team, teams, rows);
     const int nvec = d / VE;
-    const T* xr = x + row * x_ld;
-    uint8_t* out = codes + row * ld;
-    using P = Pack<T, VE>;
-    P p[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int c = at.t + at.threads * i;
-        if (c < nvec) p[i] = *reinterpret_cast<const P*>(xr + (int64_t)c * VE);
-    }
-    float top = 0.f;
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-        if (at.t + at.threads * i < nvec) {
-#pragma unroll
-            for (int j = 0; j < VE; ++j) top = amax2(top, to_f<T>(p[i].v[j]));
-        }
-    for (int c = at.t + at.threads * V; c < nvec; c += at.threads) {
-        const P q = *reinterpret_cast<const P*>(xr + (int64_t)c * VE);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) top = amax2(top, to_f<T>(q.v[j]));
-    }
-    const float scale = code_scale(red.amax(top), true);
-    if (at.t == 0) scales[row] = scale;
-    auto put = [&](const P& q, int c) {
-        float v[VE];
-        Pack<uint8_t, VE> o;
-#pragma unroll
-        for (int j = 0; j < VE; ++j) v[j] = to_f<T>(q.v[j]);
-        codes_i8<VE>(v, scale, o.v);
-        *reinterpret_cast<Pack<uint8_t, VE>*>(out + (int64_t)c * VE) = o;
+    Ring<T, VE, K, 1> ring(ring_bytes, at.t, at.threads, nvec);
+    auto fetch = [&](int stage, int row) {
+        if (row < walk.end) ring.fetch(stage, 0, x, row, d);
+        ring.commit();
     };
+    for (int k = 0; k < ring.AHEAD; ++k) fetch(k, walk.first + k);
+    int stage = 0;
+    for (int row = walk.first; row < walk.end; ++row) {
+        if constexpr (!ring.REGS) {
+            fetch(stage == 0 ? ring.STAGES - 1 : stage - 1, row + ring.STAGES - 1);
+            ring.wait();
+        }
+        Pack<T, VE> p[V];
+        ring.packs(stage, 0, p);
+        if constexpr (ring.REGS) fetch(0, row + 1);
+        Top<T, VE> top;
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-        if (at.t + at.threads * i < nvec) put(p[i], at.t + at.threads * i);
-    for (int c = at.t + at.threads * V; c < nvec; c += at.threads)
-        put(*reinterpret_cast<const P*>(xr + (int64_t)c * VE), c);
+        for (int i = 0; i < V; ++i) top.take(p[i]);          // zeros past the end
+        const float scale = code_scale(red.amax(top.value()), true);
+        if (at.t == 0) scales[row] = scale;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (at.t + at.threads * i < nvec) put_codes<T, VE>(codes + row * ld, at.t + at.threads * i, p[i], scale);
+        stage = stage == ring.STAGES - 1 ? 0 : stage + 1;
+    }
+    ring.finish();
+}
+
+// Rows that a block's registers do not hold: read twice, the second time from L2.
+template <typename T, int VE>
+__global__ void __launch_bounds__(1024)
+    quantize_long_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, float* __restrict__ scales, int d, int64_t ld) {
+    __shared__ __align__(16) float slots[2][32];
+    const Seat<BLOCK> at(32);
+    Reduce<BLOCK, 1> red(slots, at);
+    const int64_t row = blockIdx.x;
+    const Pack<T, VE>* xr = reinterpret_cast<const Pack<T, VE>*>(x + row * d);
+    const int nvec = d / VE;
+    Top<T, VE> top;
+    for (int c = at.t; c < nvec; c += at.threads) top.take(xr[c]);
+    const float scale = code_scale(red.amax(top.value()), true);
+    if (at.t == 0) scales[row] = scale;
+    for (int c = at.t; c < nvec; c += at.threads) put_codes<T, VE>(codes + row * ld, c, xr[c], scale);
 }
 
 struct QuantizeLaunch {
@@ -300,32 +343,53 @@ struct QuantizeLaunch {
     float* scales;
     int64_t rows;
     int d;
-    int64_t ld, x_ld;
+    int64_t ld;
     cudaStream_t st;
 
-    template <typename T, int VE, int V, int TEAM>
-    int go(int threads, int lanes) {
-        const int64_t per = TEAM == WARP ? threads / lanes : 1;
-        quantize_kernel<T, VE, V, TEAM><<<(unsigned)((rows + per - 1) / per), threads, 0, st>>>(
-            static_cast<const T*>(x), static_cast<uint8_t*>(codes), scales, rows, d, ld, x_ld, lanes);
+    template <typename T, int VE, int K, int TEAM>
+    int go(const TeamShape& shape) {
+        auto kernel = quantize_kernel<T, VE, K, TEAM>;
+        const int smem = Ring<T, VE, K, 1>::bytes(shape.threads);
+        static std::atomic<int> resident[64][kBlockThreads / 32 + 1];      // asked for once a kernel, block and device
+        const int dev = current_device() & 63;
+        int per = resident[dev][shape.threads / 32].load(std::memory_order_relaxed);
+        if (per == 0) {
+            if (smem > 40 * 1024) {
+                cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
+                if (e != cudaSuccess)
+                    return set_error(WIDEK_ERR_CUDA, "widek_quantize_rows_fwd: shared memory: %s", cudaGetErrorString(e));
+            }
+            if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, shape.threads, smem) != cudaSuccess || per < 1)
+                per = 1;
+            resident[dev][shape.threads / 32].store(per, std::memory_order_relaxed);
+        }
+        const int64_t teams = std::min<int64_t>((int64_t)sm_count(dev) * per * shape.rows(), rows);
+        kernel<<<(unsigned)((teams + shape.rows() - 1) / shape.rows()), shape.threads, smem, st>>>(
+            static_cast<const T*>(x), static_cast<uint8_t*>(codes), scales, rows, d, ld, (int)teams, shape.lanes);
         return check_launch("widek_quantize_rows_fwd");
     }
+    template <typename T, int VE, int K>
+    int team() {
+        const TeamShape s = team_shape(d < 1 ? 1 : d, K);
+        return s.team == WARP ? go<T, VE, K, WARP>(s) : go<T, VE, K, BLOCK>(s);
+    }
+    // Few rows, 8 values a thread on many threads; many, 32 a thread and few
+    // reductions: 32768 rows of 4096 bf16 values 141 / 82 us before the walk.
     template <typename T, int VE>
     int pick() {
-        if (d <= 256) {
-            const TeamShape s = team_shape(d < 1 ? 1 : d, 8);
-            return go<T, VE, 8 / VE, WARP>(s.threads, s.lanes);
+        constexpr int MOST = VE == 1 ? 16 : 32;
+        if (d > MOST * kBlockThreads) {
+            quantize_long_kernel<T, VE><<<(unsigned)rows, 1024, 0, st>>>(static_cast<const T*>(x), static_cast<uint8_t*>(codes),
+                                                                     scales, d, ld);
+            return check_launch("widek_quantize_rows_fwd");
         }
-        // Few rows: 8 values a thread, many threads. Many: 32 a thread, few reductions.
-        if (d <= 8192 && rows * d < (int64_t)sm_count(current_device()) * 16384)
-            return go<T, VE, 8 / VE, BLOCK>((d + 255) / 256 * 32, 32);
-        if (d <= 1024) return go<T, VE, 32 / VE, WARP>(128, 32);
-        return go<T, VE, 32 / VE, BLOCK>(std::min(1024, (d + 1023) / 1024 * 32), 32);
+        if (d <= 8 * kBlockThreads && (d <= 256 || rows * d < (int64_t)sm_count(current_device()) * 16384))
+            return team<T, VE, 8>();
+        return team<T, VE, MOST>();
     }
     template <typename T>
     int run() {
-        int ve = vec_elems<T>(d, {x});
-        while (ve > 1 && x_ld % ve != 0) ve /= 2;
+        const int ve = vec_elems<T>(d, {x});
         if constexpr (sizeof(T) == 2) {
             if (ve == 8) return pick<T, 8>();
             if (ve == 2) return pick<T, 2>();
@@ -386,16 +450,16 @@ extern "C" int widek_residual_norm_quantize_fwd(const void* x, const void* y, co
     return rnorm::forward(what, a, true, dtype, stream);
 }
 
-extern "C" int widek_quantize_rows_fwd(const void* x, void* codes, float* scales, int64_t rows, int64_t d, int64_t x_ld,
-                                       int64_t ld, int dtype, void* stream) {
+extern "C" int widek_quantize_rows_fwd(const void* x, void* codes, float* scales, int64_t rows, int64_t d, int64_t ld,
+                                       int dtype, void* stream) {
     const char* what = "widek_quantize_rows_fwd";
-    if (rows < 0 || d < 0 || rows > 0x7fffffff || d > 0x7fffffff || x_ld < 0)
+    if (rows < 0 || d < 0 || rows > 0x7fffffff || d > 0x7fffff00)
         return set_error(WIDEK_ERR_INVALID, "%s: bad sizes rows=%lld d=%lld", what, (long long)rows, (long long)d);
     if (dtype_size(dtype) == 0) return set_error(WIDEK_ERR_INVALID, "%s: unknown dtype code %d", what, dtype);
     int rc = rnorm::check_codes(what, codes, ld, d);
     if (rc != WIDEK_OK) return rc;
     if (rows == 0) return WIDEK_OK;
     if (!scales || (d > 0 && (!x || !codes))) return set_error(WIDEK_ERR_INVALID, "%s: null pointer", what);
-    return dispatch_dtype(dtype, rnorm::QuantizeLaunch{x, codes, scales, rows, (int)d, ld, x_ld,
+    return dispatch_dtype(dtype, rnorm::QuantizeLaunch{x, codes, scales, rows, (int)d, ld,
                                                        static_cast<cudaStream_t>(stream)});
 }

@@ -285,6 +285,13 @@ struct Ring {
     __device__ __forceinline__ void finish() {
         if constexpr (!REGS) asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
+    __device__ __forceinline__ void packs(int stage, int tensor, P (&out)[V]) const {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if constexpr (REGS) out[i] = held[tensor][i];
+            else out[i] = own[((stage * TENSORS + tensor) * V + i) * blockDim.x];
+        }
+    }
     __device__ __forceinline__ void get(int stage, int tensor, float (&out)[K]) const {
 #pragma unroll
         for (int i = 0; i < V; ++i) {

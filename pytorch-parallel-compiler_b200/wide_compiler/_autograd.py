@@ -473,10 +473,13 @@ class ResidualNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, weight, bias, post_weight, post_bias, gate, scale, eps, center):
         from . import ops
-        h, z, stats = ops._residual_norm(x, y, weight, bias, post_weight, post_bias, gate, scale, eps, center, True)
-        ctx.scale, ctx.eps, ctx.center, ctx.has_y = scale, eps, center, y is not None
+        h, z, stats, checked = ops._residual_norm(x, y, weight, bias, post_weight, post_bias, gate, scale, eps, center,
+                                                  True)
+        ctx.args, ctx.has_y = (scale, eps, center), y is not None
+        ctx.idx, dense, ctx.sizes = checked
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, y, weight, bias, post_weight, post_bias, gate, stats)
+        ctx.dense = all(a is b for a, b in zip(dense, (x, y, weight, bias, post_weight, post_bias, gate)))
         return (h, z) if ctx.has_y else z
 
     @staticmethod
@@ -488,9 +491,12 @@ class ResidualNormFn(torch.autograd.Function):
         if dh is None and dz is None:
             return (None,) * 10
         if torch.is_grad_enabled():          # a gradient of these gradients is asked for: the kernel's have no graph
-            return torch_grads(residual_norm_t if ctx.has_y else row_norm_t,
-                               (*tensors, ctx.scale, ctx.eps, ctx.center), (*need, False, False, False), grads)
-        return (*ops.residual_norm_bwd(*tensors, stats, dh, dz, ctx.scale, ctx.eps, ctx.center, need), None, None, None)
+            return torch_grads(residual_norm_t if ctx.has_y else row_norm_t, (*tensors, *ctx.args),
+                               (*need, False, False, False), grads)
+        if not ctx.dense:
+            tensors = [t if t is None else t.contiguous() for t in tensors]
+        got = ops._residual_norm_bwd(ctx.idx, tensors, ctx.sizes, stats, dh, dz, *ctx.args, need)
+        return (*got, None, None, None)
 
 
 class Swap01Fn(torch.autograd.Function):

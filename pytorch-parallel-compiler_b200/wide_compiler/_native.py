@@ -117,7 +117,7 @@ SIGNATURES = {
                                                      _c_void_p],
     "widek_residual_norm_fwd": [_c_void_p] * 10 + [_i64] * 4 + [_dbl, _dbl, _int, _int, _c_void_p],
     "widek_residual_norm_quantize_fwd": [_c_void_p] * 10 + [_i64] * 5 + [_dbl, _dbl, _int, _int, _c_void_p],
-    "widek_quantize_rows_fwd": [_c_void_p] * 3 + [_i64] * 4 + [_int, _c_void_p],
+    "widek_quantize_rows_fwd": [_c_void_p] * 3 + [_i64] * 3 + [_int, _c_void_p],
     "widek_linear_int8_fwd": [_c_void_p] * 6 + [_i64] * 8 + [_int, _int, _c_void_p],
     "widek_residual_norm_bwd_workspace": [_i64] * 4 + [_int, _int],
     "widek_residual_norm_bwd": [_c_void_p] * 17 + [_i64] * 4 + [_dbl, _dbl, _int, _int, _c_void_p, _i64, _c_void_p],

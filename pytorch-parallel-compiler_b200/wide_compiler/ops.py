@@ -1324,13 +1324,14 @@ def residual_norm(x: Tensor, y: Optional[Tensor], weight: Tensor, bias: Optional
 
 
 def _residual_norm(x, y, weight, bias, post_weight, post_bias, gate, scale, eps, center, need_stats: bool):
-    idx, dense, sizes = _block_args("residual_norm", x, y, weight, bias, post_weight, post_bias, gate)
+    """(h, z, statistics), and what was checked: (device, dense tensors, sizes)."""
+    checked = idx, dense, sizes = _block_args("residual_norm", x, y, weight, bias, post_weight, post_bias, gate)
     h = x if y is None else torch.empty_like(dense[0])
     z = torch.empty_like(dense[0])
     stats = torch.empty((sizes[0], sizes[1], 4), device=x.device, dtype=torch.float32) if need_stats else None
-    _launch(idx, "widek_residual_norm_fwd", *_ptrs(dense), h.data_ptr(), z.data_ptr(), N.ptr(stats), *sizes, scale, eps,
-            center, N.dtype_code(x))
-    return h, z, stats
+    _launch(idx, "widek_residual_norm_fwd", *_ptrs(dense), h.data_ptr(), z.data_ptr(),
+            None if stats is None else stats.data_ptr(), *sizes, scale, eps, center, N.dtype_code(x))
+    return h, z, stats, checked
 
 
 def residual_norm_bwd(x: Tensor, y: Optional[Tensor], weight: Tensor, bias: Optional[Tensor],
@@ -1343,22 +1344,31 @@ def residual_norm_bwd(x: Tensor, y: Optional[Tensor], weight: Tensor, bias: Opti
     what = "residual_norm backward"
     idx, dense, sizes = _block_args(what, x, y, weight, bias, post_weight, post_bias, gate)
     _device(what, x, stats, dh, dz)
+    _same_dtype(what, x, dh, dz)
     for g in (dh, dz):
         if g is not None and g.shape != x.shape:
             raise ValueError(f"{what}: a gradient {tuple(g.shape)} for {tuple(x.shape)}")
-    _same_dtype(what, x, dh, dz)
     if stats.shape != (sizes[0], sizes[1], 4) or stats.dtype != torch.float32 or not stats.is_contiguous():
         raise ValueError(f"{what}: stats must be dense float32 [N, rows, 4]")
+    return _residual_norm_bwd(idx, dense, sizes, stats, dh, dz, scale, eps, center, need)
+
+
+def _residual_norm_bwd(idx: int, dense, sizes, stats: Tensor, dh: Optional[Tensor], dz: Optional[Tensor], scale: float,
+                       eps: float, center: bool, need):
+    """residual_norm_bwd on checked, dense tensors."""
+    x, has_post = dense[0], dense[4] is not None
     if x.numel() == 0:
         return [torch.zeros_like(t) if t is not None and k else None for t, k in zip(dense, need)]
     grads = [torch.empty_like(t) if t is not None and k else None for t, k in zip(dense, need)]
-    has_post = post_weight is not None
-    ws_bytes = _workspace("widek_residual_norm_bwd_workspace", idx, ("residual_norm_bwd", *sizes, has_post, center, idx),
-                          *sizes, has_post, center)
+    ws_bytes = _workspace("widek_residual_norm_bwd_workspace", idx, (sizes, has_post, center, idx), *sizes, has_post, center)
     ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8)
-    dh, dz = (g if g is None or g.is_contiguous() else g.contiguous() for g in (dh, dz))
-    _launch(idx, "widek_residual_norm_bwd", *_ptrs(dense), stats.data_ptr(), N.ptr(dh), N.ptr(dz),
-            *_ptrs(grads), *sizes, scale, eps, center, N.dtype_code(x), ws.data_ptr(), ws_bytes)
+    if dh is not None and not dh.is_contiguous():
+        dh = dh.contiguous()
+    if dz is not None and not dz.is_contiguous():
+        dz = dz.contiguous()
+    _launch(idx, "widek_residual_norm_bwd", *_ptrs(dense), stats.data_ptr(), None if dh is None else dh.data_ptr(),
+            None if dz is None else dz.data_ptr(), *_ptrs(grads), *sizes, scale, eps, center, N.dtype_code(x),
+            ws.data_ptr(), ws_bytes)
     return grads
 
 
@@ -1410,7 +1420,7 @@ def quantize_rows(x: Tensor):
     xd = x if x.is_contiguous() else x.contiguous()
     codes = _code_rows(xd)
     scales = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
-    _launch(idx, "widek_quantize_rows_fwd", xd.data_ptr(), codes.data_ptr(), scales.data_ptr(), scales.numel(), k, k,
+    _launch(idx, "widek_quantize_rows_fwd", xd.data_ptr(), codes.data_ptr(), scales.data_ptr(), scales.numel(), k,
             -(-k // 16) * 16, N.dtype_code(x))
     return codes, scales
 

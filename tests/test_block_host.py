@@ -35,7 +35,7 @@ def test_forward_refuses(bad, word):
 def test_no_rows_is_no_call():
     assert rnorm(x=None, y=None, w=None, h=None, z=None, n=0) == 0
     assert rnorm(x=None, y=None, w=None, h=None, z=None, rows=0) == 0
-    assert N.lib().widek_quantize_rows_fwd(None, None, None, 0, 7, 7, 16, N.F32, None) == 0
+    assert N.lib().widek_quantize_rows_fwd(None, None, None, 0, 7, 16, N.F32, None) == 0
 
 
 def test_codes_refuse():
@@ -45,8 +45,8 @@ def test_codes_refuse():
     for args in ((60,), (72,), (64, P + 8)):
         assert call(*args) == N.WIDEK_ERR_INVALID
         assert "16 bytes" in N.last_error()
-    quant = lambda rows=3, d=64, x_ld=64, ld=64, x=P, scales=P, dtype=N.F32: lib.widek_quantize_rows_fwd(
-        x, P, scales, rows, d, x_ld, ld, dtype, None)
+    quant = lambda rows=3, d=64, ld=64, x=P, scales=P, dtype=N.F32: lib.widek_quantize_rows_fwd(
+        x, P, scales, rows, d, ld, dtype, None)
     for bad in (dict(rows=-1), dict(d=-1), dict(ld=63), dict(ld=72), dict(x=None), dict(scales=None), dict(dtype=7)):
         assert quant(**bad) == N.WIDEK_ERR_INVALID
 
