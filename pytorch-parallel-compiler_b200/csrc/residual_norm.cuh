@@ -58,7 +58,6 @@ __device__ __forceinline__ Pack<T, VE> pack(const float* v) {
 template <typename T>
 inline int vec_elems(int64_t d, std::initializer_list<const void*> ptrs) {
     for (int ve = 16 / (int)sizeof(T); ve > 1; ve /= 2) {
-        if (sizeof(T) == 4 && ve == 2) continue;       // one fp32 a vector is copied without waiting as well
         bool ok = d % ve == 0;
         for (const void* p : ptrs) ok = ok && reinterpret_cast<uintptr_t>(p) % (ve * sizeof(T)) == 0;
         if (ok) return ve;
@@ -95,7 +94,7 @@ struct TeamShape {
 constexpr int kBlockThreads = 512; // at most: 128 registers a thread
 // Lanes for d channels, k a thread, else a block, else a pair of them.
 inline TeamShape team_shape(int d, int k) {
-    if (d <= 32 * k) return {WARP, 128, d <= 8 * k ? 8 : d <= 16 * k ? 16 : 32};
+    if (d <= 32 * k) return {WARP, 128, d <= 4 * k ? 4 : d <= 8 * k ? 8 : d <= 16 * k ? 16 : 32};
     const int threads = (d + 32 * k - 1) / (32 * k) * 32;
     if (threads <= kBlockThreads) return {BLOCK, threads, 32};
     return {PAIR, (threads + 63) / 64 * 32, 32};

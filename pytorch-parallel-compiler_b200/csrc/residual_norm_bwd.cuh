@@ -261,64 +261,114 @@ __device__ __forceinline__ void put(void* p, int64_t i, float v) {
     if (p) static_cast<T*>(p)[i] = from_f<T>(v);
 }
 
-// Sums of the teams' parts, 32 (or 8) channels a block: row k of the block takes the
-// teams k, k + blockDim.y, .., then the rows' sums are added in order. Blocks past
-// the models' (GROUPS) finish the gates whose rows were split between teams.
+// How the blocks of finish_kernel go over the gates that were split between teams
+// (GROUPS): by gates, a block for blockDim.x channels as for a model, where a gate has
+// many teams; else a block for as many channels as threads, by gates or, where those
+// are more, by the places between two teams of a model, of which a gate's first counts.
+struct GateBlocks {
+    int64_t items;
+    int channels;                  // of a block
+    bool by_gate, side_by_side;    // teams over blockDim.y
+    __host__ __device__ GateBlocks(const BwdArgs& a, int tx, int ty) {
+        const int64_t gates = (uint32_t)a.f.rows / a.f.gate_rows, places = a.f.n * (a.f.teams - 1);
+        side_by_side = gates * 8 < places;
+        by_gate = gates <= places;
+        items = by_gate ? gates : places;
+        channels = side_by_side ? tx : tx * ty;
+    }
+};
+
+// Sums of the teams' parts: a block adds up blockDim.x channels of a model (or gate),
+// its row k every blockDim.y-th team from k on, then the rows' sums in order.
 template <typename T, int MODE, bool CENTER>
 __global__ void __launch_bounds__(1024) finish_kernel(const BwdArgs a) {
     constexpr int N = CENTER ? 2 : 1;
     constexpr int SLOTS = slot_count(MODE, CENTER);
     constexpr int SUMS = MODE == PLAIN ? N : 2 * N;
     __shared__ float sums[SUMS][1024];
-    const int d = a.f.d, c = blockIdx.y * blockDim.x + threadIdx.x;
+    const int d = a.f.d, per = (d + blockDim.x - 1) / blockDim.x;
     const int64_t slot = (int64_t)SLOTS * d;
+    const bool of_gate = MODE == GROUPS && blockIdx.x >= (uint32_t)(a.f.n * per);
     float v[SUMS] = {};
-    int64_t model = blockIdx.x;
-    const bool of_gate = MODE == GROUPS && model >= a.f.n;
-    const int64_t gate = model - a.f.n;
+    int64_t model = blockIdx.x / per, gate = 0;
+    int c = (int)(blockIdx.x % per) * blockDim.x + threadIdx.x;
+    bool side_by_side = true;
     if (!of_gate) {
         if (c < d) {
             const float* p = a.part + model * a.f.teams * slot + c;
-#pragma unroll 4
+#pragma unroll 8
             for (int k = threadIdx.y; k < a.f.teams; k += blockDim.y) {
 #pragma unroll
                 for (int q = 0; q < SUMS; ++q) v[q] += p[k * slot + (MODE == GROUPS && q >= N ? q + 2 * N : q) * d];
             }
         }
-    } else {
-        const int64_t first = gate * a.f.gate_rows;
-        model = first / a.f.model_rows;
-        const int64_t r0 = first - model * a.f.model_rows, r1 = r0 + a.f.gate_rows;
-        // the last team whose first row is not past r
-        auto team_of = [&](int64_t r) { return ((r + 1) * a.f.teams - 1) / a.f.model_rows; };
-        const int64_t k0 = team_of(r0), k1 = team_of(r1 - 1);
+    } else if constexpr (MODE == GROUPS) {
+        const GateBlocks g(a, blockDim.x, blockDim.y);
+        const uint32_t block = blockIdx.x - (uint32_t)(a.f.n * per), gper = (d + g.channels - 1) / g.channels;
+        side_by_side = g.side_by_side;
+        c = (int)(block % gper) * g.channels + (side_by_side ? threadIdx.x : threadIdx.y * blockDim.x + threadIdx.x);
+        // One thread finds the gate, its model and teams: the divisions of 64-bit
+        // numbers by all of them took most of the kernel's time.
+        __shared__ int64_t found[4];
+        __shared__ int first_of_team;
+        if (threadIdx.x == 0 && threadIdx.y == 0) {
+            const int64_t item = block / gper, rows = a.f.model_rows, teams = a.f.teams;
+            int64_t m, gt, place = 0;
+            if (g.by_gate) {
+                gt = item;
+                m = gt * a.f.gate_rows / rows;
+            } else {
+                m = item / (teams - 1);
+                place = item - m * (teams - 1) + 1;
+                gt = (m * rows + rows * place / teams) / a.f.gate_rows;
+            }
+            const int64_t r0 = gt * a.f.gate_rows - m * rows;
+            // the last team whose first row is not past r: ((r + 1) teams - 1) / rows
+            const int64_t k0 = ((r0 + 1) * teams - 1) / rows, k1 = ((r0 + a.f.gate_rows) * teams - 1) / rows;
+            found[0] = gt;
+            found[1] = m;
+            found[2] = k0;
+            found[3] = place > 0 && place != k0 + 1 ? k0 : k1;      // k0: nothing to do here
+            first_of_team = r0 <= rows * k0 / teams;
+        }
+        __syncthreads();
+        gate = found[0];
+        model = found[1];
+        const int k0 = (int)found[2], k1 = (int)found[3];
         if (k0 == k1) return;
         if (c < d) {
+            // it is its teams' first gate but, unless it starts where that team does, of
+            // the one that it starts in
+            const float* p = a.part + (model * a.f.teams + k0) * slot + (int64_t)N * d + c;
+            const int step = side_by_side ? blockDim.y : 1;
 #pragma unroll 4
-            for (int64_t k = k0 + threadIdx.y; k <= k1; k += blockDim.y) {
-                const bool leading = r0 <= a.f.model_rows * k / a.f.teams;
-                const float* p = a.part + (model * a.f.teams + k) * slot + (leading ? N : 2 * N) * d + c;
+            for (int k = side_by_side ? threadIdx.y : 0; k <= k1 - k0; k += step) {
+                const float* pk = p + k * slot + (k > 0 || first_of_team ? 0 : N * d);
 #pragma unroll
-                for (int q = 0; q < N; ++q) v[N + q] += p[q * d];
+                for (int q = 0; q < N; ++q) v[N + q] += pk[q * d];
             }
         }
     }
+    if (side_by_side) {
 #pragma unroll
-    for (int q = 0; q < SUMS; ++q) sums[q][threadIdx.y * blockDim.x + threadIdx.x] = v[q];
-    __syncthreads();
-    if (threadIdx.y != 0 || c >= d) return;
+        for (int q = 0; q < SUMS; ++q) sums[q][threadIdx.y * blockDim.x + threadIdx.x] = v[q];
+        __syncthreads();
+        if (threadIdx.y != 0) return;
 #pragma unroll
-    for (int q = 0; q < SUMS; ++q) {
-        v[q] = 0.f;
-        for (int k = 0; k < blockDim.y; ++k) v[q] += sums[q][k * blockDim.x + threadIdx.x];
+        for (int q = 0; q < SUMS; ++q) {
+            v[q] = 0.f;
+#pragma unroll 4
+            for (int k = 0; k < blockDim.y; ++k) v[q] += sums[q][k * blockDim.x + threadIdx.x];
+        }
     }
+    if (c >= d) return;
     const int64_t at = model * d + c;
     if constexpr (MODE != PLAIN) {
         float va = v[N] * a.f.scale, vb = CENTER ? v[SUMS - 1] * a.f.scale : 0.f;
-        if (of_gate || MODE == MODEL) {
-            const float dg = fmaf(va, at_or<T>(a.f.pw, at, 1.f), vb * at_or<T>(a.f.pb, at, 0.f));
-            put<T>(a.dgate, of_gate ? gate * d + c : at, dg);
-            if (of_gate) return;
+        if (of_gate || MODE == MODEL)
+            put<T>(a.dgate, of_gate ? gate * d + c : at, fmaf(va, at_or<T>(a.f.pw, at, 1.f), vb * at_or<T>(a.f.pb, at, 0.f)));
+        if (of_gate) return;
+        if constexpr (MODE == MODEL) {
             const float g = at_or<T>(a.f.gate, at, 1.f);
             va *= g;
             vb *= g;
@@ -366,14 +416,19 @@ int bwd_go(BwdArgs a, cudaStream_t st) {
     cudaLaunchKernelEx(&cfg, kernel, a, shape.lanes);
     int rc = check_launch("widek_residual_norm_bwd");
     if (rc != WIDEK_OK) return rc;
-    // short rows: fewer channels a block, to add more teams at a time
-    const int tx = a.f.d <= 64 ? 8 : 32;
+    // Many teams (short rows, few models): fewer channels a block, more teams at a
+    // time. Blocks of 256 threads where they finish gates, of which there may be many
+    // (144 gates of 263 teams a model: 11 us, with blocks of 1024 threads 106).
+    const bool gates = MODE == GROUPS && a.dgate && a.f.gate_rows > 1;       // else a gate is one team's
+    const int tx = !gates && a.f.teams >= 128 ? 16 : 32, most = gates ? (a.f.teams >= 512 ? 32 : 8) : tx == 16 ? 64 : 16;
     int ty = 1;
-    while (ty < 1024 / tx && ty < a.f.teams) ty *= 2;
-    // gates of more rows than one may be split between teams
-    const int64_t gates = MODE == GROUPS && a.dgate && a.f.gate_rows > 1 && a.f.teams > 1 ? a.f.rows / a.f.gate_rows : 0;
-    finish_kernel<T, MODE, CENTER>
-        <<<dim3((unsigned)(a.f.n + gates), (a.f.d + tx - 1) / tx), dim3(tx, ty), 0, st>>>(a);
+    while (ty < most && ty < a.f.teams) ty *= 2;
+    int64_t blocks = a.f.n * ((a.f.d + tx - 1) / tx);
+    if (gates) {
+        const GateBlocks g(a, tx, ty);
+        blocks += g.items * ((a.f.d + g.channels - 1) / g.channels);
+    }
+    finish_kernel<T, MODE, CENTER><<<(unsigned)blocks, dim3(tx, ty), 0, st>>>(a);
     return check_launch("widek_residual_norm_bwd (sums)");
 }
 
@@ -394,10 +449,9 @@ template <typename T>
 int BwdLaunch::run() {
     const Args& f = a.f;
     const int ve = vec_elems<T>(f.d, {f.x, f.y, f.w, f.wb, f.pw, f.pb, f.gate, a.dh, a.dz, a.dx, a.dy, a.dgate});
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (sizeof(T) == 2)
         if (ve == 8) return bwd_center_of<T, 8>(a, mode, st);
-        if (ve == 2) return bwd_center_of<T, 2>(a, mode, st);
-    }
+    if (ve == 2) return bwd_center_of<T, 2>(a, mode, st);
     return ve == 4 ? bwd_center_of<T, 4>(a, mode, st) : bwd_center_of<T, 1>(a, mode, st);
 }
 #endif
