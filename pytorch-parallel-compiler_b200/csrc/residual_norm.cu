@@ -189,21 +189,10 @@ struct ForwardLaunch {
     int go(const TeamShape& shape) {
         void (*kernel)(Args, int) = forward_kernel<T, VE, K, TEAM, CENTER, CODES>;
         const int smem = Ring<T, VE, K, 3>::bytes(shape.threads);
-        if (smem > 40 * 1024) {
-            cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-            if (e != cudaSuccess)
-                return set_error(WIDEK_ERR_CUDA, "widek_residual_norm_fwd: %d bytes of shared memory: %s", smem,
-                                 cudaGetErrorString(e));
-        }
-        // One wave of teams (asked for once a kernel, block and device), a row each at least.
         static std::atomic<int> resident[64][kBlockThreads / 32 + 1];
         const int dev = current_device() & 63;
-        int per = resident[dev][shape.threads / 32].load(std::memory_order_relaxed);
-        if (per == 0) {
-            if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, shape.threads, smem) != cudaSuccess || per < 1)
-                per = 1;
-            resident[dev][shape.threads / 32].store(per, std::memory_order_relaxed);
-        }
+        const int per = resident_blocks(resident[dev][shape.threads / 32], kernel, shape.threads, smem);
+        // one wave of teams, a row each at least
         const int64_t wave = (int64_t)sm_count(dev) * per * shape.rows() / (TEAM == PAIR ? 2 : 1);
         a.teams = (int)std::max<int64_t>(1, std::min<int64_t>(wave / a.n, a.model_rows));
         cudaLaunchConfig_t cfg{};
@@ -354,19 +343,9 @@ struct QuantizeLaunch {
     int go(const TeamShape& shape) {
         auto kernel = quantize_kernel<T, VE, K, TEAM>;
         const int smem = Ring<T, VE, K, 1>::bytes(shape.threads);
-        static std::atomic<int> resident[64][kBlockThreads / 32 + 1];      // asked for once a kernel, block and device
+        static std::atomic<int> resident[64][kBlockThreads / 32 + 1];
         const int dev = current_device() & 63;
-        int per = resident[dev][shape.threads / 32].load(std::memory_order_relaxed);
-        if (per == 0) {
-            if (smem > 40 * 1024) {
-                cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
-                if (e != cudaSuccess)
-                    return set_error(WIDEK_ERR_CUDA, "widek_quantize_rows_fwd: shared memory: %s", cudaGetErrorString(e));
-            }
-            if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, shape.threads, smem) != cudaSuccess || per < 1)
-                per = 1;
-            resident[dev][shape.threads / 32].store(per, std::memory_order_relaxed);
-        }
+        const int per = resident_blocks(resident[dev][shape.threads / 32], kernel, shape.threads, smem);
         const int64_t teams = std::min<int64_t>((int64_t)sm_count(dev) * per * shape.rows(), rows);
         kernel<<<(unsigned)((teams + shape.rows() - 1) / shape.rows()), shape.threads, smem, st>>>(
             static_cast<const T*>(x), static_cast<uint8_t*>(codes), scales, rows, d, ld, (int)teams, shape.lanes);

@@ -5,6 +5,7 @@
 #include "paged_cache.cuh"
 #include "sm100_ptx.cuh"
 
+#include <atomic>
 #include <initializer_list>
 #include <type_traits>
 
@@ -338,6 +339,18 @@ struct Walk {
         end = (int)(model * model_rows + model_rows * (k + 1) / teams);
     }
 };
+
+// Blocks of `kernel` that an SM holds at once, asked for once; the kernel may have as
+// much shared memory as any launch of it takes from then on.
+template <typename K>
+inline int resident_blocks(std::atomic<int>& known, K kernel, int threads, int smem) {
+    int per = known.load(std::memory_order_relaxed);
+    if (per > 0) return per;
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, threads, smem) != cudaSuccess || per < 1) per = 1;
+    known.store(per, std::memory_order_relaxed);
+    return per;
+}
 
 // Checks the sizes and pointers that the entry points share and fills `a`.
 // gate_rows: rows that share a row of the gate, -1 without one.

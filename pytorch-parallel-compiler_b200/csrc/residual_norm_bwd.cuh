@@ -387,20 +387,10 @@ int bwd_go(BwdArgs a, cudaStream_t st) {
                                    : shape.team == BLOCK ? backward_kernel<T, VE, MODE, CENTER, BLOCK>
                                                          : backward_kernel<T, VE, MODE, CENTER, PAIR>;
     const int smem = Ring<T, VE, kBwdChannels, MODE == GROUPS ? 5 : 4>::bytes(shape.threads);
-    if (smem > 40 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess)
-            return set_error(WIDEK_ERR_CUDA, "widek_residual_norm_bwd: %d bytes of shared memory: %s", smem,
-                             cudaGetErrorString(e));
-    }
-    static std::atomic<int> resident[64][kBlockThreads / 32 + 1][2];       // asked for once a kernel, block and device
+    // (by the kind of team too: how the sums are split may not depend on earlier calls)
+    static std::atomic<int> resident[64][3][kBlockThreads / 32 + 1];
     const int dev = current_device() & 63;
-    std::atomic<int>& known = resident[dev][shape.threads / 32][shape.team == PAIR];
-    int per = known.load(std::memory_order_relaxed);
-    if (per == 0) {
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, shape.threads, smem) != cudaSuccess || per < 1) per = 1;
-        known.store(per, std::memory_order_relaxed);
-    }
+    const int per = resident_blocks(resident[dev][shape.team][shape.threads / 32], kernel, shape.threads, smem);
     a.f.teams = bwd_teams(a.f.n, a.f.model_rows, a.f.d, sm_count(dev), std::min(1024, per * shape.threads));
     const int64_t teams = a.f.n * a.f.teams;
     cudaLaunchConfig_t cfg{};

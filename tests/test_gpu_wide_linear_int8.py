@@ -203,3 +203,26 @@ def test_a_served_feed_forward(rows):
     R.assert_within(a, *expect(codes.cpu(), scale.cpu(), up.cpu(), us.cpu(), None, ops.ACT_GELU, BF16))
     R.assert_within(c2, a.cpu().double() / s2.cpu().double()[..., None], torch.full(c2.shape, 0.5 + 128 * R.U))
     R.assert_within(out, *expect(c2.cpu(), s2.cpu(), down.cpu(), ds.cpu(), None, ops.ACT_NONE, BF16))
+
+
+def test_offsets_past_32_bits():
+    """Rows of results past 2^31 values, and codes past 2^31."""
+    m, k, o = 270000, 64, 8192
+    codes, scale, w, ws, _ = case(1, (1,), k, o, BF16, False)
+    many = codes.to(DEV).expand(1, m, k).contiguous()
+    s = scale.to(DEV).expand(1, m).contiguous()
+    s[0, -1] *= 2
+    y = ops.linear_int8(many, s, w.to(DEV), ws.to(DEV))
+    want, bound = expect(codes, scale, w, ws, None, ops.ACT_NONE, BF16)
+    for row, f in ((0, 1), (m // 2, 1), (m - 2, 1), (m - 1, 2)):
+        R.assert_within(y[:, row:row + 1], want * f, bound * f)
+    del y
+    k = 131056
+    big = torch.ones(1, 17000, k, dtype=torch.int8, device=DEV)
+    big[0, -1] = -3
+    one = torch.ones(1, 17000, device=DEV)
+    wide = torch.ones(1, 20, k, dtype=torch.int8, device=DEV)
+    for y in (ops.linear_int8(big, one, wide, one[:, :20].contiguous(), dtype=F32),
+              ops.linear_int8(wide, one[:, :20].contiguous(), big, one, dtype=F32).transpose(1, 2)):
+        assert (y[0, :-1] == k).all() and (y[0, -1] == -3 * k).all()
+    no_device_error()

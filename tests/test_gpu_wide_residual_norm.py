@@ -349,3 +349,74 @@ def test_another_stream():
     s.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert torch.equal(codes, ops.quantize_rows(want[1])[0])
+
+
+# ---------------------------------------------------------------------------
+# Far offsets, threads, call history
+# ---------------------------------------------------------------------------
+
+def test_offsets_past_32_bits():
+    """The last rows of tensors of over 2^31 values are what a call on them alone
+    gives."""
+    n, rows, d = 1, 270000, 8192
+    t = {k: torch.randn(n, rows, d, device=DEV, dtype=BF16) for k in ("x", "y")}
+    w = 1 + 0.2 * torch.randn(n, d, device=DEV, dtype=BF16)
+    h, z = ops.residual_norm(t["x"], t["y"], w, post_weight=w)
+    last = {k: v[:, -5:].contiguous() for k, v in t.items()}
+    h2, z2 = ops.residual_norm(last["x"], last["y"], w, post_weight=w)
+    ref = R.residual_norm(last["x"].cpu(), last["y"].cpu(), w.cpu(), post_weight=w.cpu())
+    for got, alone, name in ((h[:, -5:], h2, "h"), (z[:, -5:], z2, "z")):
+        R.assert_within(got, *ref[name], name)
+        R.assert_within(alone, *ref[name], name)
+    del h
+    codes, scales = ops.quantize_rows(z)
+    c2, s2 = ops.quantize_rows(z[:, -5:].contiguous())
+    assert torch.equal(codes[:, -5:], c2) and torch.equal(scales[:, -5:], s2)
+    _, codes, scales = ops.residual_norm_quantize(t["x"], t["y"], w, post_weight=w)
+    s, es, q, eq = R.codes(*ref["z32"])
+    R.assert_within(scales[:, -5:], s, es, "scales")
+    R.assert_within(codes[:, -5:], q, 0.5 + eq, "codes")
+
+
+@pytest.mark.grad
+def test_gradients_do_not_depend_on_earlier_calls():
+    """The split of the sums is the sizes' alone: rows of 240 (lanes of a warp) and of
+    1000 channels (a block of as many threads) in both orders."""
+    def grads(d):
+        t = tensors((3, 4, 500, d), BF16, False, True, 0, d)
+        leaves = [v.requires_grad_(True) for v in t.values() if v is not None]
+        out = ops.residual_norm(**t)
+        return torch.autograd.grad(out, leaves, (t["x"].detach(), t["y"].detach()))
+
+    a = grads(240), grads(1000)
+    b = grads(1000), grads(240)
+    assert all(torch.equal(x, y) for x, y in zip((*a[0], *a[1]), (*b[1], *b[0])))
+
+
+def test_calls_from_several_threads():
+    import threading
+    sizes = [(2, 300, 1024), (2, 40, 8192), (2, 300, 200), (2, 90, 3000)]
+    args = [tensors(s, F32, True, True, 0, i) for i, s in enumerate(sizes)]
+    want = [ops.residual_norm(**t, center=True) for t in args]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        s = torch.cuda.Stream()
+        try:
+            with torch.cuda.stream(s):
+                for _ in range(50):
+                    got = ops.residual_norm(**args[i], center=True)
+                    codes, _ = ops.quantize_rows(got[1])
+            s.synchronize()
+            if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                failed.append(i)
+        except Exception as e:           # reported by the main thread
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(sizes))]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not failed
