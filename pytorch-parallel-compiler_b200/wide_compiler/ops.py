@@ -1298,6 +1298,11 @@ def _ptrs(tensors):
     return [None if t is None else t.data_ptr() for t in tensors]
 
 
+def _empty(shape, device, dtype) -> Tensor:
+    # sizes one by one: a tuple of them takes twice as long to parse
+    return torch.empty(*shape, device=device, dtype=dtype) if shape else torch.empty((), device=device, dtype=dtype)
+
+
 def residual_norm(x: Tensor, y: Optional[Tensor], weight: Tensor, bias: Optional[Tensor] = None,
                   post_weight: Optional[Tensor] = None, post_bias: Optional[Tensor] = None,
                   gate: Optional[Tensor] = None, scale: float = 1.0, eps: float = 1e-6, center: bool = False):
@@ -1328,7 +1333,7 @@ def _residual_norm(x, y, weight, bias, post_weight, post_bias, gate, scale, eps,
     checked = idx, dense, sizes = _block_args("residual_norm", x, y, weight, bias, post_weight, post_bias, gate)
     h = x if y is None else torch.empty_like(dense[0])
     z = torch.empty_like(dense[0])
-    stats = torch.empty((sizes[0], sizes[1], 4), device=x.device, dtype=torch.float32) if need_stats else None
+    stats = torch.empty(sizes[0], sizes[1], 4, device=x.device, dtype=torch.float32) if need_stats else None
     _launch(idx, "widek_residual_norm_fwd", *_ptrs(dense), h.data_ptr(), z.data_ptr(),
             None if stats is None else stats.data_ptr(), *sizes, scale, eps, center, N.dtype_code(x))
     return h, z, stats, checked
@@ -1377,7 +1382,7 @@ def _code_rows(x: Tensor) -> Tensor:
     d = x.shape[-1]
     if d % 16 == 0:
         return torch.empty_like(x, dtype=torch.int8)
-    return torch.empty((*x.shape[:-1], -(-d // 16) * 16), device=x.device, dtype=torch.int8)[..., :d]
+    return _empty((*x.shape[:-1], -(-d // 16) * 16), x.device, torch.int8)[..., :d]
 
 
 def residual_norm_quantize(x: Tensor, y: Optional[Tensor], weight: Tensor, bias: Optional[Tensor] = None,
@@ -1397,7 +1402,7 @@ def residual_norm_quantize(x: Tensor, y: Optional[Tensor], weight: Tensor, bias:
     idx, dense, sizes = _block_args(what, x, y, weight, bias, post_weight, post_bias, gate)
     h = x if y is None else torch.empty_like(dense[0])
     codes = _code_rows(dense[0])
-    scales = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    scales = _empty(x.shape[:-1], x.device, torch.float32)
     _launch(idx, "widek_residual_norm_quantize_fwd", *_ptrs(dense), h.data_ptr(), codes.data_ptr(), scales.data_ptr(),
             -(-sizes[2] // 16) * 16, *sizes, scale, eps, center, N.dtype_code(x))
     return h, codes, scales
@@ -1419,7 +1424,7 @@ def quantize_rows(x: Tensor):
     k = x.shape[-1]
     xd = x if x.is_contiguous() else x.contiguous()
     codes = _code_rows(xd)
-    scales = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    scales = _empty(x.shape[:-1], x.device, torch.float32)
     _launch(idx, "widek_quantize_rows_fwd", xd.data_ptr(), codes.data_ptr(), scales.data_ptr(), scales.numel(), k,
             -(-k // 16) * 16, N.dtype_code(x))
     return codes, scales
@@ -1455,6 +1460,23 @@ def _rows16(t: Tensor):
     return held, step, rows * step
 
 
+def _linear_int8_refuse(what, codes, scale, weight, weight_scale, bias, dtype):
+    """Says what is wrong with the arguments."""
+    _device(what, codes, scale, weight, weight_scale, bias)
+    cs, ws = codes.shape, weight.shape
+    if codes.dtype != torch.int8 or weight.dtype != torch.int8:
+        raise TypeError(f"{what}: codes and weight must be int8, got {codes.dtype} and {weight.dtype}")
+    if len(cs) < 2 or len(ws) != 3 or cs[0] != ws[0] or cs[-1] != ws[2]:
+        raise ValueError(f"{what}: codes {tuple(cs)} do not match weight {tuple(ws)}")
+    if scale.shape != cs[:-1] or weight_scale.shape != ws[:2]:
+        raise ValueError(f"{what}: scales {tuple(scale.shape)} and {tuple(weight_scale.shape)} do not match codes "
+                         f"{tuple(cs)} and weight {tuple(ws)}")
+    if scale.dtype != torch.float32 or weight_scale.dtype != torch.float32:
+        raise TypeError(f"{what}: scales must be float32, got {scale.dtype} and {weight_scale.dtype}")
+    if bias is not None and (bias.shape != ws[:2] or bias.dtype != dtype):
+        raise ValueError(f"{what}: bias {tuple(bias.shape)} {bias.dtype} is not {tuple(ws[:2])} {dtype}")
+
+
 def linear_int8(codes: Tensor, scale: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[Tensor] = None,
                 act: int = ACT_NONE, dtype: torch.dtype = torch.bfloat16) -> Tensor:
     """A linear layer of N models on 8-bit codes (widek_linear_int8_fwd):
@@ -1472,27 +1494,24 @@ def linear_int8(codes: Tensor, scale: Tensor, weight: Tensor, weight_scale: Tens
     _no_grad(what, scale, weight_scale, bias)
     if _compiling():
         return torch.ops.widek.linear_int8(codes, scale, weight, weight_scale, bias, act, dtype)
-    idx = _device(what, codes, scale, weight, weight_scale, bias)
-    cs, ws = codes.shape, weight.shape
-    if codes.dtype != torch.int8 or weight.dtype != torch.int8:
-        raise TypeError(f"{what}: codes and weight must be int8, got {codes.dtype} and {weight.dtype}")
-    if len(cs) < 2 or len(ws) != 3 or cs[0] != ws[0] or cs[-1] != ws[2]:
-        raise ValueError(f"{what}: codes {tuple(cs)} do not match weight {tuple(ws)}")
-    if scale.shape != cs[:-1] or weight_scale.shape != ws[:2]:
-        raise ValueError(f"{what}: scales {tuple(scale.shape)} and {tuple(weight_scale.shape)} do not match codes "
-                         f"{tuple(cs)} and weight {tuple(ws)}")
-    if scale.dtype != torch.float32 or weight_scale.dtype != torch.float32:
-        raise TypeError(f"{what}: scales must be float32, got {scale.dtype} and {weight_scale.dtype}")
-    if bias is not None and (bias.shape != ws[:2] or bias.dtype != dtype):
-        raise ValueError(f"{what}: bias {tuple(bias.shape)} {bias.dtype} is not {tuple(ws[:2])} {dtype}")
-    y = torch.empty((*cs[:-1], ws[1]), device=codes.device, dtype=dtype)
+    idx, cs, ws = codes.get_device(), codes.shape, weight.shape
+    outer = ws[:2]
+    fine = (idx >= 0 and weight.get_device() == idx and scale.get_device() == idx and weight_scale.get_device() == idx
+            and codes.dtype == weight.dtype == torch.int8 and scale.dtype == weight_scale.dtype == torch.float32
+            and len(cs) > 1 and len(ws) == 3 and cs[0] == ws[0] and cs[-1] == ws[2] and scale.shape == cs[:-1]
+            and weight_scale.shape == outer
+            and (bias is None or (bias.shape == outer and bias.dtype == dtype and bias.get_device() == idx)))
+    if not fine:
+        _linear_int8_refuse(what, codes, scale, weight, weight_scale, bias, dtype)
+    y = torch.empty(*cs[:-1], ws[1], device=codes.device, dtype=dtype)
     code = N.dtype_code(y)
     if y.numel() == 0:
         return y
     a, a_ld, a_ms = _rows16(codes)
     w, w_ld, w_ms = _rows16(weight)
     scale, weight_scale = _dense(scale), _dense(weight_scale)
-    bias = bias if bias is None else _dense(bias)
+    if bias is not None:
+        bias = _dense(bias)
     _launch(idx, "widek_linear_int8_fwd", a.data_ptr(), scale.data_ptr(), w.data_ptr(), weight_scale.data_ptr(),
             N.ptr(bias), y.data_ptr(), cs[0], scale.numel() // cs[0], cs[-1], ws[1], a_ld, a_ms, w_ld, w_ms, act, code)
     return y
