@@ -12,12 +12,19 @@
 //           under the products of the next. A single CTA's 128 x 256 tile would
 //           move 96 KB through shared memory in the 512 clocks that its products
 //           of one K block take, over the 128 bytes a clock that it has; half of
-//           both operands is 64 KB.
+//           both operands is 64 KB. Bound by the tensor cores from K = 2048 on, under
+//           the power cap (8 x 4096 rows of 4096 -> 4096: 377 us, 2919 TOP/s; 75 % of
+//           the tensor cycles of an SM's time in ncu), by the results' bytes at K = 256
+//           (77.6 us for 268 MB, a fill takes 70), between them by both; by the
+//           epilogue's instructions where a GELU meets a short K (1024 -> 4096: 126 us
+//           without, 150 with).
 //   narrow  few rows: bound by the weights' bytes. The weights' rows are the MMA's
 //           128 lanes and up to 128 tokens its columns, so that no tensor time goes
 //           to rows that are not there; K is split over a cluster when there are
 //           too few tiles for the device, and the parts (integers: any order gives
-//           the same sum) are added through distributed shared memory.
+//           the same sum) are added through distributed shared memory. 8 models of
+//           4096 -> 16384 for one token: 92 us, 5.9 TB/s; small ones are latency (33 MB
+//           of weights 11.6 to 13.5 us, the least 5.4).
 #include <algorithm>
 #include <atomic>
 
@@ -314,8 +321,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
         // Epilogue: group wg drains columns [64 wg, 64 wg + 64) of this CTA's 128
         // rows, 32 at a time through a staging buffer a warp; warp quarter q is
         // the TMEM lanes (rows) 32 q .. 32 q + 31. Four groups, as two left the
-        // issue slots two thirds empty and a tile of K = 1024 with its GELU waiting
-        // for them (5.0 us a tile, 2.2 of products).
+        // issue slots two thirds empty; a warp stores by itself (TMA), and an arrival
+        // that waited for its stores held a tile without products at 4.9 us, where it
+        // takes 2.8.
         const int q = warp & 3, wg = (warp - 2) >> 2, ep_tid = threadIdx.x - 64 - 128 * wg;
         uint8_t* buf = sOut + (wg * 4 + q) * (S::OUT_CHUNK / 4);
         float* vec = sVec + wg * 2 * kGroupCols;             // scales, then biases
@@ -398,8 +406,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
                 } else {
                     // Rows that start off the 16-byte borders: through this warp's part
                     // of the staging buffer (columns turned by the row: no bank twice), so that a
-                    // store covers 32 neighbours (each thread storing its own row took the
-                    // kernel 5 times as long).
+                    // store covers 32 neighbours (119544 rows of 404 results 88 us; each
+                    // thread storing its own row 486).
                     T* stage = reinterpret_cast<T*>(buf);
                     __syncwarp();
 #pragma unroll

@@ -12,6 +12,14 @@
 // rows are on their way to shared memory meanwhile, and a row is read and written
 // once. Statistics are sums over the values in registers (the variance around the
 // mean that was taken first), in fp32; z is taken from the unrounded h.
+//
+// Bound by memory, not far from the instructions' bound: norm + residual of 134 M
+// bf16 values (65536 rows of 2048) takes 187 us (floor at the measured copy rate 166);
+// one row a block without a walk took 270, 8 channels a thread 244. Into codes 16.8 M
+// f16 values 26 us (18), rows of 4096 bf16 values into codes 71 (62). Short rows cost
+// their reductions: LayerNorms of 143208 rows of 152 f16 channels 70 us (27). Rows of an
+// odd number of 16-bit channels go one channel at a time, through registers: 165188 rows
+// of 105 bf16 channels 98 us (21).
 #include "residual_norm.cuh"
 
 #include <algorithm>

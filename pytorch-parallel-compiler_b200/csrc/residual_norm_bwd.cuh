@@ -15,6 +15,12 @@
 // scale gate A, dpb = scale gate B. Where gates change (GROUPS) that is finished
 // whenever the walk leaves a gate's rows: at once when all of them were this
 // team's, else through the first or last partial sums of the teams that share it.
+//
+// Bound by memory latency: 33.6 M bf16 values (two RMS norms, a gate a model) take 71
+// us (62 at the measured copy rate) and 6 for the sums, LayerNorms before blocks of 16.8
+// M f16 values 47 (31). Weights folded together and two values an instruction took the
+// first from 106 to 74 us, as many blocks as its 94 registers allow to 71. Without the
+// ring in shared memory the loads ahead spill.
 #include "residual_norm.cuh"
 
 #include <algorithm>
@@ -406,11 +412,12 @@ int bwd_go(BwdArgs a, cudaStream_t st) {
     cudaLaunchKernelEx(&cfg, kernel, a, shape.lanes);
     int rc = check_launch("widek_residual_norm_bwd");
     if (rc != WIDEK_OK) return rc;
-    // Many teams (short rows, few models): fewer channels a block, more teams at a
-    // time. Blocks of 256 threads where they finish gates, of which there may be many
+    // Many teams and few blocks (short rows, few models): fewer channels a block, more
+    // teams at a time. Blocks of 256 threads where they finish gates, of which there may be many
     // (144 gates of 263 teams a model: 11 us, with blocks of 1024 threads 106).
     const bool gates = MODE == GROUPS && a.dgate && a.f.gate_rows > 1;       // else a gate is one team's
-    const int tx = !gates && a.f.teams >= 128 ? 16 : 32, most = gates ? (a.f.teams >= 512 ? 32 : 8) : tx == 16 ? 64 : 16;
+    const bool few = a.f.n * ((a.f.d + 31) / 32) < sm_count(dev);
+    const int tx = !gates && few && a.f.teams >= 128 ? 16 : 32, most = gates ? (a.f.teams >= 512 ? 32 : 8) : tx == 16 ? 64 : 16;
     int ty = 1;
     while (ty < most && ty < a.f.teams) ty *= 2;
     int64_t blocks = a.f.n * ((a.f.d + tx - 1) / tx);
