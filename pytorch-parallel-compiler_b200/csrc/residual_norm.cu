@@ -79,8 +79,15 @@ __device__ __forceinline__ float factor_of(float (&v)[K], Reduce<TEAM, 1>& red, 
     return rsqrtf(fmaf(s[0], inv_d, eps));
 }
 
+// Blocks an SM that the registers are cut to: 64 a thread for RMS norms with 8
+// channels, else 128 (the odd 16-bit rows, which wait in registers, as many as they want).
+constexpr int forward_blocks(int team, int k, bool center, bool regs) {
+    const bool wide = k > 8 || center;
+    return regs ? 1 : team == WARP ? (wide ? 4 : 8) : wide ? 1 : 2;
+}
+
 template <typename T, int VE, int K, int TEAM, bool CENTER, bool CODES>
-__global__ void __launch_bounds__(TEAM == WARP ? 128 : kBlockThreads, sizeof(T) * VE < 4 ? 1 : TEAM == WARP ? (K > 8 || CENTER ? 4 : 8) : K > 8 || CENTER ? 1 : 2)
+__global__ void __launch_bounds__(TEAM == WARP ? 128 : kBlockThreads, forward_blocks(TEAM, K, CENTER, sizeof(T) * VE < 4))
     forward_kernel(const Args a, int lanes) {
     __shared__ __align__(16) float slots[2][32];
     extern __shared__ __align__(16) uint8_t ring_bytes[];

@@ -69,6 +69,36 @@ def test_forward_few_and_many_rows(rows, d):
     R.assert_within(z, *want["z"], "z")
 
 
+# rows enough for 16 channels (norms) and 32 (codes) a thread, in every vector and team
+MANY = [(1, 60000, 60), (2, 15000, 104), (1, 20000, 250), (3, 4000, 501), (1, 9000, 1000), (2, 800, 4092), (1, 700, 8190)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("center", [False, True])
+@pytest.mark.parametrize("shape", MANY)
+def test_many_rows_of_every_kind(shape, center, dtype):
+    t = tensors(shape, dtype, center, True, 1 if shape[2] < 300 else 0, sum(shape))
+    want = R.residual_norm(**cpu(t), center=center)
+    h, z = ops.residual_norm(**t, center=center)
+    R.assert_within(h, *want["h"], "h")
+    R.assert_within(z, *want["z"], "z")
+    h, codes, scales = ops.residual_norm_quantize(**t, center=center)
+    R.assert_within(h, *want["h"], "h")
+    check_codes(*want["z32"], codes, scales, shape[-1])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("shape", MANY + [(1, 300, 16384), (1, 400, 16380), (2, 300, 16383)])
+def test_codes_of_many_rows(shape, dtype):
+    x = torch.randn(*shape, device=DEV).to(dtype)
+    x[0, 5, shape[-1] // 2] = -50
+    codes, scales = ops.quantize_rows(x)
+    top = x.float().abs().amax(-1).clamp(min=2.0 ** -40)
+    want = top / torch.full_like(top, 127.0)
+    assert torch.equal(scales, want)
+    assert torch.equal(codes.float(), torch.round(x.float() / want.unsqueeze(-1)))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("center", [False, True])
 def test_without_y_h_is_x(center, dtype):
