@@ -371,8 +371,10 @@ struct QuantizeLaunch {
         const TeamShape s = team_shape(d < 1 ? 1 : d, K);
         return s.team == WARP ? go<T, VE, K, WARP>(s) : go<T, VE, K, BLOCK>(s);
     }
-    // Few rows, 8 values a thread on many threads; many, 32 a thread and few
-    // reductions: 32768 rows of 4096 bf16 values 141 / 82 us before the walk.
+    // Few rows, 8 values a thread on many threads; many, more and fewer reductions, as
+    // far as a row still has four warps (bf16, 8 / 16 / 32 a thread: 30000 rows of 512
+    // 14.2 / 12.9 / 13.5 us, 68000 of 1024 51 / 42.5 / 44, 8192 of 2048 15.5 / 12.7 /
+    // 13.8, 32768 of 4096 108 / 76 / 76; 16384 of 4096 with a cold cache - / 43 / 38).
     template <typename T, int VE>
     int pick() {
         constexpr int MOST = VE == 1 ? 16 : 32;
@@ -383,6 +385,7 @@ struct QuantizeLaunch {
         }
         if (d <= 8 * kBlockThreads && (d <= 256 || rows * d < (int64_t)sm_count(current_device()) * 16384))
             return team<T, VE, 8>();
+        if (d <= 16 * 128) return team<T, VE, 16>();
         return team<T, VE, MOST>();
     }
     template <typename T>

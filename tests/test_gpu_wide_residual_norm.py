@@ -192,6 +192,23 @@ def test_quantize_rows(shape, dtype):
     assert len(shape) < 2 or codes.stride(-2) % 16 == 0
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("shape", [(20001, 130), (10007, 258), (9001, 333), (5003, 500), (2503, 1000), (1201, 2050),
+                                   (701, 4096), (401, 8192), (301, 8200), (201, 9001), (205, 12290), (151, 16384)])
+def test_quantize_many_rows(shape, dtype):
+    """Every count of values a thread, with several rows a team: the quotients of the
+    largest value and of the values, rounded once each."""
+    gen = torch.Generator(device=DEV).manual_seed(sum(shape))
+    x = torch.randn(*shape, generator=gen, device=DEV)
+    x = (x * torch.exp(2 * torch.randn(shape[0], 1, generator=gen, device=DEV))).to(dtype)
+    codes, scales = ops.quantize_rows(x)
+    x = x.cpu().float()
+    top = x.abs().amax(-1).clamp(min=2.0 ** -40)
+    want = top / torch.full_like(top, 127.0)
+    assert torch.equal(scales.cpu(), want)
+    assert torch.equal(codes.cpu().float(), torch.round(x / want.unsqueeze(-1)))
+
+
 def test_rows_that_are_not_finite():
     x = torch.randn(4, 50, device=DEV)
     x[1, 7], x[2, 3] = math.inf, math.nan
