@@ -627,6 +627,13 @@ __global__ void __launch_bounds__(kNarrowThreads)
     }
 }
 
+// A pair's kernel (wide_kernel; linear_tc_pair_kernel, 194 KB and the system's 1)
+// leaves less of an SM's 228 KB than this and the 2 KB for alignment and the system.
+constexpr int kBesidePair = 36 * 1024;
+static_assert(WideSmem<float>::TOTAL + kBesidePair + 3 * 1024 > 228 * 1024, "a part of K beside a pair");
+static_assert(WideSmem<__half>::TOTAL + kBesidePair + 3 * 1024 > 228 * 1024, "a part of K beside a pair");
+static_assert(WideSmem<__nv_bfloat16>::TOTAL + kBesidePair + 3 * 1024 > 228 * 1024, "a part of K beside a pair");
+
 int rows_map(CUtensorMap* map, const void* base, int64_t n, int64_t rows, int64_t k, int64_t ld, int64_t ms, uint32_t box) {
     const uint64_t dims[3] = {(uint64_t)k, (uint64_t)rows, (uint64_t)n};
     const uint64_t strides[2] = {(uint64_t)ld, (uint64_t)ms};
@@ -699,10 +706,11 @@ struct Int8Launch {
         const int fit = 222 * 1024 / std::max(2, share) / ((128 + BN) * kBK);
         const int stages = std::min(most, std::max(2, std::min(8, fit)));
         size_t bytes = (size_t)stages * (128 + BN) * kBK;
-        if (split > 1) bytes = std::max<size_t>(bytes, (size_t)BN * 512);
+        if (split > 1) bytes = std::max<size_t>({bytes, (size_t)BN * 512, (size_t)kBesidePair});
         // A CTA holds at least 456 bytes of an SM's 228 KB for each of its 512 TMEM
         // columns that it takes, so that CTAs of a cluster, which wait for one
-        // another, never wait for columns that others of their kind hold.
+        // another, never wait for columns that others of their kind hold; and kBesidePair
+        // keeps them off an SM where a pair of CTAs, which wait too, holds all columns.
         bytes = std::max<size_t>(bytes + 1024, (BN < 32 ? 32 : BN) * 456);
         if (tiles * split > 0x7fffffff) return set_error(WIDEK_ERR_INVALID, "widek_linear_int8_fwd: over 2^31 tiles");
         static std::atomic<int> had[64];
