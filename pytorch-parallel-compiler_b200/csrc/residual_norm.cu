@@ -107,8 +107,9 @@ __global__ void __launch_bounds__(TEAM == WARP ? 128 : kBlockThreads, forward_bl
         g = a.gate_div.divmod((uint32_t)row, in_gate);
         return row - (int)in_gate + (int)a.gate_rows;
     };
-    auto fetch = [&](int stage, int row) {
-        if (row < walk.end) {
+    auto fetch = [&](int stage, int from, int ahead) {
+        if (walk.has(from, ahead)) {
+            const int row = from + ahead;
             ring.fetch(stage, 1, a.y, row, d);
             ring.fetch(stage, 0, a.x, row, d);
             if (row == fetch_gate) {
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(TEAM == WARP ? 128 : kBlockThreads, forward_bl
         }
         ring.commit();
     };
-    for (int k = 0; k < ring.AHEAD; ++k) fetch(k, walk.first + k);
+    for (int k = 0; k < ring.AHEAD; ++k) fetch(k, walk.first, k);
     // k = scale gate pw, kb = scale gate pb
     float w[K], wb[K], k[K], kb[K];
     load_weights<T, VE>(a.w, walk.model, d, at.t, at.threads, 1.f, w);
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(TEAM == WARP ? 128 : kBlockThreads, forward_bl
     for (int row = walk.first; row < walk.end; ++row) {
         float v[K], x[K], mu = 0.f, ru = 1.f, mh;
         if constexpr (!ring.REGS) {
-            fetch(stage == 0 ? ring.STAGES - 1 : stage - 1, row + ring.STAGES - 1);
+            fetch(stage == 0 ? ring.STAGES - 1 : stage - 1, row, ring.STAGES - 1);
             ring.wait();
         }
         if (row == use_gate) {
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(TEAM == WARP ? 128 : kBlockThreads, forward_bl
         ring.get(stage, 0, x);
         if (a.y) {
             ring.get(stage, 1, v);
-            if constexpr (ring.REGS) fetch(0, row + 1);
+            if constexpr (ring.REGS) fetch(0, row, 1);
             if (a.pw) {
                 ru = factor_of<VE, K, TEAM, CENTER>(v, red, at, nvec, inv_d, a.eps, mu);
                 scale_vec<K>(v, v, ru);
@@ -164,7 +165,7 @@ __global__ void __launch_bounds__(TEAM == WARP ? 128 : kBlockThreads, forward_bl
             fma_vec<K>(v, v, k, x);
             store_row<T, VE>(a.h, row, d, at.t, at.threads, v);
         } else {
-            if constexpr (ring.REGS) fetch(0, row + 1);
+            if constexpr (ring.REGS) fetch(0, row, 1);
 #pragma unroll
             for (int j = 0; j < K; ++j) v[j] = x[j];
         }
@@ -301,20 +302,20 @@ __global__ void __launch_bounds__(TEAM == WARP ? 128 : kBlockThreads, TEAM == WA
     const Walk walk(at.team, teams, rows);
     const int nvec = d / VE;
     Ring<T, VE, K, 1> ring(ring_bytes, at.t, at.threads, nvec);
-    auto fetch = [&](int stage, int row) {
-        if (row < walk.end) ring.fetch(stage, 0, x, row, d);
+    auto fetch = [&](int stage, int row, int ahead) {
+        if (walk.has(row, ahead)) ring.fetch(stage, 0, x, row + ahead, d);
         ring.commit();
     };
-    for (int k = 0; k < ring.AHEAD; ++k) fetch(k, walk.first + k);
+    for (int k = 0; k < ring.AHEAD; ++k) fetch(k, walk.first, k);
     int stage = 0;
     for (int row = walk.first; row < walk.end; ++row) {
         if constexpr (!ring.REGS) {
-            fetch(stage == 0 ? ring.STAGES - 1 : stage - 1, row + ring.STAGES - 1);
+            fetch(stage == 0 ? ring.STAGES - 1 : stage - 1, row, ring.STAGES - 1);
             ring.wait();
         }
         Pack<T, VE> p[V];
         ring.packs(stage, 0, p);
-        if constexpr (ring.REGS) fetch(0, row + 1);
+        if constexpr (ring.REGS) fetch(0, row, 1);
         Top<T, VE> top;
 #pragma unroll
         for (int i = 0; i < V; ++i) top.take(p[i]);          // zeros past the end

@@ -338,6 +338,8 @@ struct Walk {
         first = (int)(model * model_rows + model_rows * k / teams);
         end = (int)(model * model_rows + model_rows * (k + 1) / teams);
     }
+    // Whether the row `ahead` rows on is the walk's too; their sum may not fit in 32 bits.
+    __device__ __forceinline__ bool has(int row, int ahead) const { return ahead < end - row; }
 };
 
 // Blocks of `kernel` that an SM holds at once, asked for once; the kernel may have as

@@ -101,8 +101,9 @@ __global__ void __launch_bounds__(TEAM == WARP ? 128 : kBlockThreads) backward_k
     if (!a.f.y) ring.clear(1);
     if (!a.dh) ring.clear(2);
     if (!a.dz) ring.clear(3);
-    auto fetch = [&](int stage, int row) {
-        if (row < walk.end) {
+    auto fetch = [&](int stage, int from, int ahead) {
+        if (walk.has(from, ahead)) {
+            const int row = from + ahead;
             ring.fetch(stage, 0, a.f.x, row, d);
             ring.fetch(stage, 1, a.f.y, row, d);
             ring.fetch(stage, 3, a.dz, row, d);
@@ -115,7 +116,7 @@ __global__ void __launch_bounds__(TEAM == WARP ? 128 : kBlockThreads) backward_k
         }
         ring.commit();
     };
-    for (int k = 0; k < ring.AHEAD; ++k) fetch(k, walk.first + k);
+    for (int k = 0; k < ring.AHEAD; ++k) fetch(k, walk.first, k);
     const float4* stats = reinterpret_cast<const float4*>(a.f.stats);
     float4 st = stats[walk.first];
 
@@ -146,7 +147,7 @@ __global__ void __launch_bounds__(TEAM == WARP ? 128 : kBlockThreads) backward_k
     for (int row = walk.first; row < walk.end; ++row) {
         float x[K], y[K], dz[K], dh[K], hn[K], s[N];
         if constexpr (!ring.REGS) {
-            fetch(stage == 0 ? ring.STAGES - 1 : stage - 1, row + ring.STAGES - 1);
+            fetch(stage == 0 ? ring.STAGES - 1 : stage - 1, row, ring.STAGES - 1);
             ring.wait();
         }
         const float mu = st.x, ru = st.y, mh = st.z, rh = st.w;
@@ -166,7 +167,7 @@ __global__ void __launch_bounds__(TEAM == WARP ? 128 : kBlockThreads) backward_k
         }
         if constexpr (ring.REGS) {
             ring.get(stage, 2, dh);
-            fetch(0, row + 1);
+            fetch(0, row, 1);
         }
         // un in place of y, then hn
         if constexpr (YSIDE) {
