@@ -338,12 +338,12 @@ __global__ void __launch_bounds__(1024)
     Reduce<BLOCK, 1> red(slots, at);
     const int64_t row = blockIdx.x;
     const Pack<T, VE>* xr = reinterpret_cast<const Pack<T, VE>*>(x + row * d);
-    const int nvec = d / VE;
+    const uint32_t nvec = d / VE;          // unsigned: a place past the end of a long row may pass 2^31
     Top<T, VE> top;
-    for (int c = at.t; c < nvec; c += at.threads) top.take(xr[c]);
+    for (uint32_t c = at.t; c < nvec; c += at.threads) top.take(xr[c]);
     const float scale = code_scale(red.amax(top.value()), true);
     if (at.t == 0) scales[row] = scale;
-    for (int c = at.t; c < nvec; c += at.threads) put_codes<T, VE>(codes + row * ld, c, xr[c], scale);
+    for (uint32_t c = at.t; c < nvec; c += at.threads) put_codes<T, VE>(codes + row * ld, c, xr[c], scale);
 }
 
 struct QuantizeLaunch {

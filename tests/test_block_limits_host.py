@@ -61,3 +61,29 @@ int main() {{
     return 0;
 }}
 """)
+
+
+def test_places_of_the_longest_row(tmp_path):
+    """Rows that a block takes at 1024 values a turn: no turn past the end, up to the longest row of
+    single values."""
+    text = source("residual_norm.cu")
+    longest = int(re.search(r"d > (0x[0-9a-f]+)\)", text[text.index("int widek_quantize_rows_fwd("):]).group(1), 16)
+    kernel = text[text.index("quantize_long_kernel("):]
+    loops = re.findall(r"for \((.* c = .*?)\) (?:top|put)", kernel[:kernel.index("\n}\n")])
+    assert len(loops) == 2
+    turns = "".join(f"""
+        {{
+            int64_t n = 0;
+            for ({loop}) if (c < 0 || c >= {longest} || ++n > {-(-longest // 1024)}) return 3;
+            if (n < {longest // 1024}) return 4;
+        }}""" for loop in loops)
+    run_on_host(tmp_path, f"""
+#include <cstdint>
+int main() {{
+    const int nvec = {longest};
+    for (int t = 0; t < 1024; t += 1023) {{
+        struct {{ int t, threads; }} at{{t, 1024}};{turns}
+    }}
+    return 0;
+}}
+""")
