@@ -569,7 +569,11 @@ __global__ void __launch_bounds__(kNarrowThreads)
     }
     __syncwarp();
     const volatile int never = 0;
-    const bool ok = mbar_wait(&tfull, 0, &never);
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(&tfull, 0, &never));     // a warp reads TMEM as one
+    if (!ok) {                               // stores nothing, and says so
+        *abort_flag = 1;
+        raise_device_error(p.err, DEV_ERR_GEMM_TIMEOUT);
+    }
     tc_fence_after();
 
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
@@ -583,7 +587,7 @@ __global__ void __launch_bounds__(kNarrowThreads)
     if (split == 1) {
         const Gelu2 gelu;
 #pragma unroll 1
-        for (int c = 0; c < tokens; c += CH) {
+        for (int c = 0; ok && c < tokens; c += CH) {
             uint32_t r[CH];
             load(c, r);
             F2 v[CH / 2];
@@ -614,9 +618,9 @@ __global__ void __launch_bounds__(kNarrowThreads)
             }
         }
         cluster_sync_all();
-        if (split == 2) add_parts<T, 2>(part, rank, tokens, s_sa, sw, bias, p.act, o < p.o, y, p.o);
-        else if (split == 4) add_parts<T, 4>(part, rank, tokens, s_sa, sw, bias, p.act, o < p.o, y, p.o);
-        else add_parts<T, 8>(part, rank, tokens, s_sa, sw, bias, p.act, o < p.o, y, p.o);
+        if (ok && split == 2) add_parts<T, 2>(part, rank, tokens, s_sa, sw, bias, p.act, o < p.o, y, p.o);
+        else if (ok && split == 4) add_parts<T, 4>(part, rank, tokens, s_sa, sw, bias, p.act, o < p.o, y, p.o);
+        else if (ok) add_parts<T, 8>(part, rank, tokens, s_sa, sw, bias, p.act, o < p.o, y, p.o);
         cluster_sync_all();                  // no CTA leaves while others read its part
     }
     tc_fence_before();
