@@ -584,6 +584,14 @@ __global__ void __launch_bounds__(kNarrowThreads)
         else tmem_ld_32x32b_x32(tmem_base + lanes + c, r);
         tmem_ld_wait();
     };
+    auto free_columns = [&]() {
+        tc_fence_before();
+        __syncthreads();
+        if (warp == 1) {
+            tc_fence_after();
+            tmem_dealloc(tmem_base, TMEM_COLS);
+        }
+    };
     if (split == 1) {
         const Gelu2 gelu;
 #pragma unroll 1
@@ -604,6 +612,7 @@ __global__ void __launch_bounds__(kNarrowThreads)
                 if (c + j + 1 < tokens && o < p.o) y[(int64_t)(c + j + 1) * p.o] = from_f<T>(b);
             }
         }
+        free_columns();
     } else {
         // The parts as [token][channel] in the ring's memory (its copies have been
         // used up); CTA r adds and finishes the tokens r, r + split, ..
@@ -617,17 +626,14 @@ __global__ void __launch_bounds__(kNarrowThreads)
                 for (int j = 0; j < CH; ++j) part[(c + j) * 128 + threadIdx.x] = r[j];
             }
         }
+        // A CTA that waits for others holds no columns: a pair of CTAs (of any kernel) may
+        // hold one SM's while it waits for its partner's, and the two would wait for ever.
+        free_columns();
         cluster_sync_all();
         if (ok && split == 2) add_parts<T, 2>(part, rank, tokens, s_sa, sw, bias, p.act, o < p.o, y, p.o);
         else if (ok && split == 4) add_parts<T, 4>(part, rank, tokens, s_sa, sw, bias, p.act, o < p.o, y, p.o);
         else if (ok) add_parts<T, 8>(part, rank, tokens, s_sa, sw, bias, p.act, o < p.o, y, p.o);
         cluster_sync_all();                  // no CTA leaves while others read its part
-    }
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 1) {
-        tc_fence_after();
-        tmem_dealloc(tmem_base, TMEM_COLS);
     }
 }
 
@@ -712,9 +718,9 @@ struct Int8Launch {
         size_t bytes = (size_t)stages * (128 + BN) * kBK;
         if (split > 1) bytes = std::max<size_t>({bytes, (size_t)BN * 512, (size_t)kBesidePair});
         // A CTA holds at least 456 bytes of an SM's 228 KB for each of its 512 TMEM
-        // columns that it takes, so that CTAs of a cluster, which wait for one
-        // another, never wait for columns that others of their kind hold; and kBesidePair
-        // keeps them off an SM where a pair of CTAs, which wait too, holds all columns.
+        // columns that it takes, so that an SM starts no CTA of this kernel that would wait
+        // for the columns of others; and kBesidePair keeps parts of K, whose cluster
+        // would wait along, off an SM where a pair of CTAs holds all columns to its end.
         bytes = std::max<size_t>(bytes + 1024, (BN < 32 ? 32 : BN) * 456);
         if (tiles * split > 0x7fffffff) return set_error(WIDEK_ERR_INVALID, "widek_linear_int8_fwd: over 2^31 tiles");
         static std::atomic<int> had[64];

@@ -26,3 +26,15 @@ def test_the_last_wait_of_narrow_tiles_is_reported():
     calls = re.findall(r"if \((.*)\) add_parts<", adding)
     assert len(calls) == adding.count("add_parts<") == 3
     assert all(c.startswith("ok") for c in calls), "parts are added without a look at the wait"
+
+
+def test_no_columns_are_held_in_a_wait_for_other_blocks():
+    """A part of K gives its tensor memory back before it waits for the other parts: a
+    pair of blocks that waits for those columns may hold what the other parts wait for."""
+    body = kernel("narrow_kernel")
+    frees = re.search(r"auto (\w+) = \[&\]\(\) \{[^}]*__syncthreads\(\);[^}]*tmem_dealloc\(", body, re.S)
+    parts = body[body.index("if (split == 1)"):].split("} else {", 1)[1]
+    first = parts.index("cluster_sync_all();")
+    assert frees and f"{frees.group(1)}();" in parts[:first]
+    assert "tmem_ld" not in parts[first:] and "load(" not in parts[first:]
+    assert body.count("tmem_dealloc(") == 1 and body.count(f"{frees.group(1)}();") == 2
