@@ -280,10 +280,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
         if (!ok) {
             *abort_flag = 1;
             raise_device_error(p.err, DEV_ERR_GEMM_TIMEOUT);
-            // This CTA's copies count on the leader's barrier; give them time
-            // to land (bounded) before the CTA's shared memory is released.
-            const uint64_t t0 = globaltimer_ns();
-            while (globaltimer_ns() - t0 < 1000000ull) { }
         }
     } else if (warp == 1) {
         if (rank == 0 && lane == 0) {
@@ -430,6 +426,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
     }
 
     tc_fence_before();
+    __syncthreads();
+    if (warp == 0 && *abort_flag) {
+        // A role failed. This CTA's copies count on the leader's barrier; give them time to
+        // land (bounded) before the pair's shared memory is released.
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 1000000ull) { }
+    }
+    __syncwarp();
     cluster_sync_all();                      // no CTA leaves while its pair may still touch its smem / TMEM
     if (warp == 1) {
         tc_fence_after();
@@ -528,11 +532,11 @@ __global__ void __launch_bounds__(kNarrowThreads)
     tc_fence_after();
     const uint32_t tmem_base = tmem_slot;
 
+    int issued = 0;                          // blocks asked for, by thread 0
     if (warp == 0) {
         if (lane == 0) {
             const uint64_t pol_a = l2_policy_evict_last();
             const uint64_t pol_w = mt_count == 1 ? l2_policy_evict_first() : l2_policy_evict_normal();
-            int issued = 0;
             for (; issued < kbs; ++issued) {
                 const int s = issued % stages;
                 if (!mbar_wait(&empty[s], (uint32_t)(issued / stages & 1) ^ 1, abort_flag)) break;
@@ -543,9 +547,6 @@ __global__ void __launch_bounds__(kNarrowThreads)
             if (issued < kbs) {
                 *abort_flag = 1;
                 raise_device_error(p.err, DEV_ERR_GEMM_TIMEOUT);
-                const volatile int never = 0;            // copies in flight land before the CTA's memory is released
-                for (int j = issued - (issued < stages ? issued : stages); j < issued; ++j)
-                    mbar_wait(&full[j % stages], (uint32_t)(j / stages & 1), &never);
             }
         }
     } else if (warp == 1) {
@@ -591,6 +592,10 @@ __global__ void __launch_bounds__(kNarrowThreads)
             tc_fence_after();
             tmem_dealloc(tmem_base, TMEM_COLS);
         }
+        // After a failure of any role: copies in flight land before the CTA's memory is released.
+        if (threadIdx.x == 0 && *abort_flag)
+            for (int j = max(issued - stages, 0); j < issued; ++j)
+                mbar_wait_ns(&full[j % stages], (uint32_t)(j / stages & 1), &never, kWaitLimitNs / 8);
     };
     if (split == 1) {
         const Gelu2 gelu;

@@ -38,3 +38,15 @@ def test_no_columns_are_held_in_a_wait_for_other_blocks():
     assert frees and f"{frees.group(1)}();" in parts[:first]
     assert "tmem_ld" not in parts[first:] and "load(" not in parts[first:]
     assert body.count("tmem_dealloc(") == 1 and body.count(f"{frees.group(1)}();") == 2
+
+
+def test_copies_in_flight_land_after_any_failure():
+    """Whichever role gives up, a block's memory is not released before its copies
+    have landed or a limit has passed: the wait stands behind all roles."""
+    body = kernel("narrow_kernel")
+    end = body[body.index("auto free_columns"):body.index("if (split == 1)")]
+    assert re.search(r"__syncthreads\(\);.*if \(threadIdx.x == 0 && \*abort_flag\)\s*for \(int j = [^;]*; j < issued; \+\+j\)"
+                     r"\s*mbar_wait_ns\(&full\[j % stages\]", end, re.S)
+    body = kernel("wide_kernel")
+    end = body[body.rindex("__syncthreads();"):]
+    assert re.search(r"if \(warp == 0 && \*abort_flag\) \{.*globaltimer_ns\(\) - t0 < 1000000ull.*cluster_sync_all\(\);", end, re.S)
