@@ -1294,6 +1294,11 @@ def _block_args(what: str, x: Tensor, y: Optional[Tensor], *params: Optional[Ten
     return idx, dense, (n, rows, d, math.prod(shape[lead:-1]))
 
 
+def _no_parts_of_y(what: str, post_weight: Optional[Tensor], post_bias: Optional[Tensor], gate: Optional[Tensor]) -> None:
+    if post_weight is not None or post_bias is not None or gate is not None:
+        raise ValueError(f"{what}: a norm or gate of y, but no y")
+
+
 def _ptrs(tensors):
     return [None if t is None else t.data_ptr() for t in tensors]
 
@@ -1318,6 +1323,8 @@ def residual_norm(x: Tensor, y: Optional[Tensor], weight: Tensor, bias: Optional
     each model) or x's leading dims and D ([N, B, D] for each sequence,
     [N, B, T, D] for each token). z is taken from the unrounded h. y None: h is
     x itself. Returns (h, z)."""
+    if y is None:
+        _no_parts_of_y("residual_norm", post_weight, post_bias, gate)
     if _compiling():
         if y is None:
             return x, torch.ops.widek.row_norm(x, weight, bias, eps, center)
@@ -1394,6 +1401,8 @@ def residual_norm_quantize(x: Tensor, y: Optional[Tensor], weight: Tensor, bias:
     fp32 z (see ``quantize_rows``). No gradient."""
     what = "residual_norm_quantize"
     _no_grad(what, x, y, weight, bias, post_weight, post_bias, gate)
+    if y is None:
+        _no_parts_of_y(what, post_weight, post_bias, gate)
     if _compiling():
         if y is None:
             return x, *torch.ops.widek.row_norm_quantize(x, weight, bias, eps, center)
