@@ -100,10 +100,12 @@ class WideDecoderAttention(nn.Module):
     @torch.no_grad()
     def quantize_(self) -> 'WideDecoderAttention':
         """Turns the projections (on the GPU) into 8-bit ones, in place; their
-        weights are given up. For serving: there is no gradient from then on."""
+        weights are given up, both or (when one fails) neither. For serving: there
+        is no gradient from then on."""
         if self.qkv_int8 is None:
-            self.qkv_int8 = WideLinearInt8.from_weight(self.qkv_weight, self.qkv_bias)
-            self.out_int8 = WideLinearInt8.from_weight(self.out_weight, self.out_bias)
+            qkv = WideLinearInt8.from_weight(self.qkv_weight, self.qkv_bias)
+            out = WideLinearInt8.from_weight(self.out_weight, self.out_bias)
+            self.qkv_int8, self.out_int8 = qkv, out
             for name in ('qkv_weight', 'out_weight', 'qkv_bias', 'out_bias'):
                 setattr(self, name, None)
             self.q_norm.requires_grad_(False)

@@ -1,0 +1,42 @@
+"""Layers that are turned into 8-bit ones in place, when that fails on the way
+(device memory that runs out): a stand-in for the quantiser, no GPU."""
+import pytest
+import torch
+
+import wide_compiler as wc
+from wide_compiler import ops
+
+
+@pytest.fixture
+def quantiser(monkeypatch):
+    """ops.quantize_rows in torch, which fails at the calls listed in `fails`."""
+    calls = []
+
+    def quantize_rows(x):
+        calls.append(x)
+        if not x.is_floating_point():
+            raise TypeError(f"quantize_rows: {x.dtype}")
+        if len(calls) in quantize_rows.fails:
+            raise torch.cuda.OutOfMemoryError("no room")
+        scale = x.abs().amax(-1).clamp(min=2.0 ** -40) / 127
+        return torch.round(x / scale[..., None]).to(torch.int8), scale
+
+    quantize_rows.fails, quantize_rows.calls = (), calls
+    monkeypatch.setattr(ops, "quantize_rows", quantize_rows)
+    return quantize_rows
+
+
+@pytest.mark.parametrize("fails", [1, 2])
+def test_attention_is_quantised_whole_or_not_at_all(quantiser, fails):
+    attn = wc.WideDecoderAttention(2, 32, 4, bias=True)
+    before = {k: v.clone() for k, v in attn.state_dict().items()}
+    quantiser.fails = (fails,)
+    with pytest.raises(torch.cuda.OutOfMemoryError):
+        attn.quantize_()
+    after = attn.state_dict()
+    assert attn.qkv_int8 is None and attn.out_int8 is None
+    assert before.keys() == after.keys() and all(torch.equal(before[k], after[k]) for k in before)
+    assert attn.qkv_weight.requires_grad
+    attn.quantize_()
+    assert isinstance(attn.qkv_int8, wc.WideLinearInt8) and isinstance(attn.out_int8, wc.WideLinearInt8)
+    assert attn.qkv_weight is None and attn.out_bias is None and not attn.q_norm.requires_grad
