@@ -84,11 +84,14 @@ class WideDecoderStack(nn.Module):
     @torch.no_grad()
     def quantize_(self) -> 'WideDecoderStack':
         """Turns all linear layers (on the GPU) into 8-bit ones, in place, for
-        serving: there is no gradient from then on."""
+        serving: there is no gradient from then on. Goes layer by layer; after a
+        failure (no memory) the rest is as it was, and a next call goes on there."""
         if not self.quantized:
             for layer in self.layers:
+                up, down = (m if isinstance(m, WideLinearInt8) else WideLinearInt8.from_wide(m)
+                            for m in (layer.up, layer.down))
                 layer.attn.quantize_()
-                layer.up, layer.down = WideLinearInt8.from_wide(layer.up), WideLinearInt8.from_wide(layer.down)
+                layer.up, layer.down = up, down
             self.quantized = True
             self.requires_grad_(False)
         return self

@@ -40,3 +40,31 @@ def test_attention_is_quantised_whole_or_not_at_all(quantiser, fails):
     attn.quantize_()
     assert isinstance(attn.qkv_int8, wc.WideLinearInt8) and isinstance(attn.out_int8, wc.WideLinearInt8)
     assert attn.qkv_weight is None and attn.out_bias is None and not attn.q_norm.requires_grad
+
+
+@pytest.mark.parametrize("fails", [2, 4, 5, 8])
+def test_a_stack_goes_on_where_it_stopped(quantiser, fails):
+    """Layers of four products: the layer in which it failed is as it was, and so are the later ones."""
+    stack = wc.WideDecoderStack(2, 32, 2, 4, hidden=48, bias=True)
+    quantiser.fails = (fails,)
+    with pytest.raises(torch.cuda.OutOfMemoryError):
+        stack.quantize_()
+    done = (fails - 1) // 4
+    assert not stack.quantized
+    for i, layer in enumerate(stack.layers):
+        kinds = {type(layer.up), type(layer.down)}
+        assert kinds == {wc.WideLinearInt8 if i < done else wc.WideLinear}
+        assert (layer.attn.qkv_int8 is not None) == (layer.attn.out_int8 is not None) == (i < done)
+    stack.quantize_()
+    assert stack.quantized and not any(p.requires_grad for p in stack.parameters())
+    for layer in stack.layers:
+        assert {type(m) for m in (layer.up, layer.down, layer.attn.qkv_int8, layer.attn.out_int8)} == {wc.WideLinearInt8}
+
+
+def test_a_layer_that_was_quantised_before():
+    """The layers of a stack may have been quantised one by one."""
+    stack = wc.WideDecoderStack(1, 32, 1, 4)
+    up = wc.WideLinearInt8(1, 32, 128, bias=False)
+    stack.layers[0].up, stack.layers[0].down = up, wc.WideLinearInt8(1, 128, 32, bias=False)
+    stack.layers[0].attn.qkv_int8, stack.layers[0].attn.out_int8 = wc.WideLinearInt8(1, 32, 96), wc.WideLinearInt8(1, 32, 32)
+    assert stack.quantize_().layers[0].up is up and stack.quantized
