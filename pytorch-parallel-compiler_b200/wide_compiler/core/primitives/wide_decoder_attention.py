@@ -63,6 +63,12 @@ class WideDecoderAttention(nn.Module):
         self.out_int8: Optional[WideLinearInt8] = None
         self._tables = {}                # fp32 whatever the module's type, so not buffers
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for name in ('qkv_int8', 'out_int8'):            # layers pickled before there were 8-bit projections
+            if name not in self._modules:
+                self.__dict__.setdefault(name, None)
+
     def rotation(self, device: torch.device, rows: Optional[int] = None):
         """cos / sin [rows, rotary_dim / 2] in fp32 (rows: max_positions unless
         given), angles in 64 bits; made once for each use they serve."""

@@ -1,5 +1,8 @@
 """Layers that are turned into 8-bit ones in place, when that fails on the way
 (device memory that runs out): a stand-in for the quantiser, no GPU."""
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -68,3 +71,22 @@ def test_a_layer_that_was_quantised_before():
     stack.layers[0].up, stack.layers[0].down = up, wc.WideLinearInt8(1, 128, 32, bias=False)
     stack.layers[0].attn.qkv_int8, stack.layers[0].attn.out_int8 = wc.WideLinearInt8(1, 32, 96), wc.WideLinearInt8(1, 32, 32)
     assert stack.quantize_().layers[0].up is up and stack.quantized
+
+
+def test_layers_pickled_before_there_were_8_bit_projections():
+    """They lack the attributes that came with quantize_()."""
+    attn = wc.WideDecoderAttention(2, 32, 4)
+    state = {k: v for k, v in attn.__dict__.items() if k not in ('qkv_int8', 'out_int8')}
+    old = wc.WideDecoderAttention.__new__(wc.WideDecoderAttention)
+    old.__setstate__(state)
+    assert old.qkv_int8 is None and old.out_int8 is None
+    with pytest.raises(TypeError, match="quantise"):
+        old((torch.zeros(2, 1, 3, 32, dtype=torch.int8), torch.ones(2, 1, 3)))
+    assert wc.WideDecoderAttention.from_modules([old, attn]).n == 4
+
+
+def test_quantised_layers_are_copied_and_pickled(quantiser):
+    attn = wc.WideDecoderAttention(2, 32, 4).quantize_()
+    for other in (copy.deepcopy(attn), pickle.loads(pickle.dumps(attn))):
+        assert torch.equal(other.qkv_int8.weight, attn.qkv_int8.weight) and other.qkv_weight is None
+        assert other.qkv_int8 is not attn.qkv_int8 and other.quantize_() is other
