@@ -34,3 +34,29 @@ def test_parts_of_k_beside_wide_tiles():
     for side, out in enumerate(outs):
         assert all(torch.equal(y, want[side][i % len(want[side])]) for i, y in enumerate(out))
     no_device_error()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows", [1, 3, 4000])
+@pytest.mark.parametrize("post", [False, True])
+def test_codes_of_one_channel_under_a_layer_norm(rows, post, dtype):
+    """A single channel is its own mean: v - mean is exactly 0, and 0 * factor * weight + bias is exactly the
+    bias. So z == bias, scale = max(|bias|, 2^-40) / 127 in fp32, code = +-127 or, for no bias, 0."""
+    gen = torch.Generator().manual_seed(rows)
+    n = 5
+    x, y = ((3 * torch.randn(n, rows, 1, generator=gen)).to(dtype).to(DEV) for _ in range(2))
+    weight = (1 + 0.3 * torch.randn(n, 1, generator=gen)).to(dtype).to(DEV)
+    bias = torch.tensor([[0.3], [-1.7], [0.0], [5.0], [-2.0 ** -14]]).to(dtype).to(DEV)
+    pw, pb = (weight, bias.flip(0).contiguous()) if post else (None, None)
+    want = bias.float()[:, None].expand(n, rows, 1)
+    top = want.abs().amax(-1).clamp(min=2.0 ** -40)
+    scale = top / torch.full_like(top, 127.0)
+    h, z = ops.residual_norm(x, y, weight, bias, pw, pb, center=True)
+    h8, codes, scales = ops.residual_norm_quantize(x, y, weight, bias, pw, pb, center=True)
+    assert torch.equal(z.float(), want) and torch.equal(h, h8)
+    assert torch.equal(scales, scale)
+    assert torch.equal(codes.float(), torch.round(want / scale.unsqueeze(-1)))
+    assert codes.float().abs().amax() == 127 and not codes[2].any()
+    u = pb.float()[:, None] if post else y.float()
+    assert torch.equal(h, (x.float() + u).to(dtype))
+    no_device_error()
