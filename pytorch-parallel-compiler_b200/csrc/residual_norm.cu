@@ -228,8 +228,9 @@ struct ForwardLaunch {
     int team() {
         const TeamShape s = team_shape(a.d, K);
         if (s.team == WARP) return a.center ? go<T, VE, K, WARP, true, CODES>(s) : go<T, VE, K, WARP, false, CODES>(s);
-        if (s.team == BLOCK) return a.center ? go<T, VE, K, BLOCK, true, CODES>(s) : go<T, VE, K, BLOCK, false, CODES>(s);
-        return a.center ? go<T, VE, K, PAIR, true, CODES>(s) : go<T, VE, K, PAIR, false, CODES>(s);
+        if constexpr (VE < 4)            // wider vectors hold rows past 4096 in one block, 16 channels a thread
+            if (s.team == PAIR) return a.center ? go<T, VE, K, PAIR, true, CODES>(s) : go<T, VE, K, PAIR, false, CODES>(s);
+        return a.center ? go<T, VE, K, BLOCK, true, CODES>(s) : go<T, VE, K, BLOCK, false, CODES>(s);
     }
     template <typename T, int VE>
     int pick() {
@@ -370,7 +371,9 @@ struct QuantizeLaunch {
     template <typename T, int VE, int K>
     int team() {
         const TeamShape s = team_shape(d < 1 ? 1 : d, K);
-        return s.team == WARP ? go<T, VE, K, WARP>(s) : go<T, VE, K, BLOCK>(s);
+        if constexpr (K <= 16)           // 32 values a thread are for rows past 2048
+            if (s.team == WARP) return go<T, VE, K, WARP>(s);
+        return go<T, VE, K, BLOCK>(s);
     }
     // Few rows, 8 values a thread on many threads; many, more and fewer reductions, as
     // far as a row still has four warps (bf16, 8 / 16 / 32 a thread: 30000 rows of 512
