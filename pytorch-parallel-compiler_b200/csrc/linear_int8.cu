@@ -704,18 +704,26 @@ struct Int8Launch {
         return check_launch("widek_linear_int8_fwd (wide)");
     }
 
+    int64_t narrow_tiles(int bn) const { return (int64_t)p.n * ((p.m + bn - 1) / bn) * ((p.o + 127) / 128); }
+    // K is split where that fills the device and leaves each CTA four blocks of it:
+    // (us, alone / in parts) 1 x 4096 -> 4096 for one token 18 / 9.4, 2 x 4176 ->
+    // 4096 for 22 tokens 26 / 16; but 8 x 1024 -> 4096 for 4 tokens 11.9 / 12.9.
+    int parts_of_k(int bn) const {
+        const int sms = sm_count(current_device()), kb = (p.k + kBK - 1) / kBK;
+        const int64_t tiles = narrow_tiles(bn);
+        int split = 1;
+        while (split < 8 && tiles * split <= (bn > 64 ? sms / 2 : sms) && kb >= 8 * split) split *= 2;
+        return split;
+    }
+
     template <typename T, int BN>
     int narrow() {
         CUtensorMap ta, tw;
         int rc = rows_map(&ta, a, p.n, p.m, p.k, a_ld, a_ms, BN);
         if (rc == WIDEK_OK) rc = rows_map(&tw, w, p.n, p.o, p.k, w_ld, w_ms, 128);
         const int sms = sm_count(current_device()), kb = (p.k + kBK - 1) / kBK;
-        const int64_t tiles = (int64_t)p.n * ((p.m + BN - 1) / BN) * ((p.o + 127) / 128);
-        // K is split where that fills the device and leaves each CTA four blocks of it:
-        // (us, alone / in parts) 1 x 4096 -> 4096 for one token 18 / 9.4, 2 x 4176 ->
-        // 4096 for 22 tokens 26 / 16; but 8 x 1024 -> 4096 for 4 tokens 11.9 / 12.9.
-        int split = 1;
-        while (split < 8 && tiles * split <= (BN > 64 ? sms / 2 : sms) && kb >= 8 * split) split *= 2;
+        const int64_t tiles = narrow_tiles(BN);
+        const int split = parts_of_k(BN);
         // The ring is as deep as lets the SM's share of CTAs (up to 5) be there at once.
         const int most = (kb + split - 1) / split, share = (int)std::min<int64_t>(5, (tiles * split + sms - 1) / sms);
         const int fit = 222 * 1024 / std::max(2, share) / ((128 + BN) * kBK);
@@ -748,8 +756,16 @@ struct Int8Launch {
 
     template <typename T>
     int run() {
-        const int64_t pairs = (int64_t)p.n * ((p.m + 255) / 256) * ((p.o + 255) / 256);
-        if (p.m > 128 && pairs * 4 >= sm_count(current_device())) return wide<T>();
+        // Past 128 rows wide tiles, even a single one, unless few tiles meet a long K, which
+        // narrow ones share out: in four or more parts, or in two of 64 blocks. Device times
+        // in us, wide / narrow: 129 rows of 256 -> 128 6.8 / 8.4, 512 of 1024 -> 512 9.2 /
+        // 11.6, 20 x 256 of 4096 -> 256 18.5 / 23.8, 8 x 129 of 1024 -> 4096 15.7 / 23.4; in
+        // parts: 256 of 2048 -> 256 11.6 / 9.9, 1024 of 4096 -> 512 16.4 / 12.3, 129 of 65536
+        // -> 128 150 / 35; in two: 16 x 130 of 4096 -> 256 17.5 / 18.9, of 16384 48.3 / 47.7.
+        if (p.m > 128) {
+            const int parts = parts_of_k(128);
+            return parts >= 4 || (parts == 2 && p.k >= 128 * kBK) ? narrow<T, 128>() : wide<T>();
+        }
         if (p.m <= 16) return narrow<T, 16>();
         if (p.m <= 32) return narrow<T, 32>();
         if (p.m <= 64) return narrow<T, 64>();

@@ -60,3 +60,23 @@ def test_codes_of_one_channel_under_a_layer_norm(rows, post, dtype):
     u = pb.float()[:, None] if post else y.float()
     assert torch.equal(h, (x.float() + u).to(dtype))
     no_device_error()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n, m, k, o", [(1, 129, 16, 16), (1, 129, 64, 8), (1, 130, 333, 517), (2, 257, 1040, 130), (1, 300, 1920, 96),
+                                        (1, 256, 2048, 256), (1, 511, 4096, 300), (3, 140, 2000, 1000), (2, 129, 16384, 1500)])
+def test_more_rows_than_narrow_tiles_and_few_tiles(n, m, k, o, dtype):
+    """Single 256 x 256 tiles and K in parts on both sides of the rule between them: the exact sum with its
+    scales, and the same rows 100 at a time (narrow tiles of one block of rows) to the bit."""
+    codes, scale, w, ws = int8_case(n, m, k, o, m + k)
+    y = ops.linear_int8(codes, scale, w, ws, act=ops.ACT_RELU, dtype=dtype)
+    acc = torch.matmul(codes.double().cpu(), w.double().cpu().transpose(1, 2))
+    want = (acc * scale.double().cpu().unsqueeze(-1) * ws.double().cpu()[:, None]).clamp(min=0)
+    # rounded to fp32, times two scales (each half a step of 2^-24), and to the type (subnormals: half a step of those)
+    bound = want * (3 * 2.0 ** -24 * (1 + 2.0 ** -20) + torch.finfo(dtype).eps / 2) + torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+    y64 = y.double().cpu()
+    most = torch.finfo(dtype).max
+    assert ((y64 - want).abs() <= bound)[want < most].all() and (y64[want > most * 1.001] == float("inf")).all()
+    parts = [ops.linear_int8(codes[:, i:i + 100], scale[:, i:i + 100], w, ws, act=ops.ACT_RELU, dtype=dtype) for i in range(0, m, 100)]
+    assert torch.equal(torch.cat(parts, 1), y)
+    no_device_error()
