@@ -756,15 +756,21 @@ struct Int8Launch {
 
     template <typename T>
     int run() {
-        // Past 128 rows wide tiles, even a single one, unless few tiles meet a long K, which
-        // narrow ones share out: in four or more parts, or in two of 64 blocks. Device times
-        // in us, wide / narrow: 129 rows of 256 -> 128 6.8 / 8.4, 512 of 1024 -> 512 9.2 /
-        // 11.6, 20 x 256 of 4096 -> 256 18.5 / 23.8, 8 x 129 of 1024 -> 4096 15.7 / 23.4; in
-        // parts: 256 of 2048 -> 256 11.6 / 9.9, 1024 of 4096 -> 512 16.4 / 12.3, 129 of 65536
-        // -> 128 150 / 35; in two: 16 x 130 of 4096 -> 256 17.5 / 18.9, of 16384 48.3 / 47.7.
+        // Past 128 rows wide tiles where they fill a quarter of the device's pairs. Fewer of
+        // them finish later than four times as many narrow ones when results are fp32 or rows
+        // off the 16-byte borders (device times in us, wide / narrow: f32, 12 pairs, K = 64
+        // 8.2 / 6.0, K = 1024 10.7 / 10.9; odd bf16 9.8 / 9.0 and 12.2 / 12.4), and else only
+        // when those share out a long K, in four or more parts, or in two of 64 blocks: 129 rows
+        // of 256 -> 128 6.8 / 8.4, 20 x 256 of 4096 -> 256 18.5 / 23.8; in parts 256 of 2048 ->
+        // 256 11.6 / 9.9, 129 of 65536 -> 128 150 / 35; in two 16 x 130 of 4096 -> 256 17.5 / 18.9,
+        // of 16384 48.3 / 47.7. From a quarter on: 4 x 129 of 1024 -> 2560 10.8 / 12.7, 8 x 256 of
+        // 4096 -> 4096 35 / 64; but f32 of K = 64 8.7 / 8.4, odd bf16 of 80 pairs 15.3 / 11.2.
         if (p.m > 128) {
+            const int64_t pairs = (int64_t)p.n * ((p.m + 255) / 256) * ((p.o + 255) / 256);
+            const bool vectors = sizeof(T) == 2 && p.o % 8 == 0 && aligned16(p.y);
             const int parts = parts_of_k(128);
-            return parts >= 4 || (parts == 2 && p.k >= 128 * kBK) ? narrow<T, 128>() : wide<T>();
+            const bool share = !vectors || parts >= 4 || (parts == 2 && p.k >= 128 * kBK);
+            return pairs * 4 < sm_count(current_device()) && share ? narrow<T, 128>() : wide<T>();
         }
         if (p.m <= 16) return narrow<T, 16>();
         if (p.m <= 32) return narrow<T, 32>();
