@@ -80,7 +80,9 @@ __device__ __forceinline__ float factor_of(float (&v)[K], Reduce<TEAM, 1>& red, 
 }
 
 // Blocks an SM that the registers are cut to: 64 a thread for RMS norms with 8
-// channels, else 128 (the odd 16-bit rows, which wait in registers, as many as they want).
+// channels, else 128 (the odd 16-bit rows, which wait in registers, as many as the block
+// leaves them: 128 in blocks of 512, where RMS norms into codes by pairs of blocks spill
+// 148 bytes). LayerNorms of 16 channels a thread spill 16 to 64 bytes in their cut.
 constexpr int forward_blocks(int team, int k, bool center, bool regs) {
     const bool wide = k > 8 || center;
     return regs ? 1 : team == WARP ? (wide ? 4 : 8) : wide ? 1 : 2;

@@ -20,7 +20,9 @@
 // us (62 at the measured copy rate) and 6 for the sums, LayerNorms before blocks of 16.8
 // M f16 values 47 (31). Weights folded together and two values an instruction took the
 // first from 106 to 74 us, as many blocks as its 94 registers allow to 71. Without the
-// ring in shared memory the loads ahead spill.
+// ring in shared memory the loads ahead spill, and do so for 16-bit rows of an odd number
+// of channels, which it cannot hold: past 256 channels with gates that change 0.3 to 1.8
+// KB a thread. LayerNorms with such gates spill 30 to 110 bytes in vectors too.
 #include "residual_norm.cuh"
 
 #include <algorithm>
@@ -413,9 +415,18 @@ int bwd_go(BwdArgs a, cudaStream_t st) {
     cudaLaunchKernelEx(&cfg, kernel, a, shape.lanes);
     int rc = check_launch("widek_residual_norm_bwd");
     if (rc != WIDEK_OK) return rc;
-    // Many teams and few blocks (short rows, few models): fewer channels a block, more
-    // teams at a time. Blocks of 256 threads where they finish gates, of which there may be many
-    // (144 gates of 263 teams a model: 11 us, with blocks of 1024 threads 106).
+    // Blocks of tx channels and up to `most` teams at a time. Device times in us:
+    //  - many blocks, or few teams: 32 x 16 (8 models of 1024 channels, 92 teams: 5.7, with
+    //    16 x 64 8.8; 2 of 4096, 74 teams: 5.4 and 17);
+    //  - few blocks of many teams (short rows, few models): 16 x 64, from where both are
+    //    equal (1 x 1024, 100 teams: 5.0, with 32 x 16 5.3; 150: 5.4 and 6.5; 740: 8.4 and 20;
+    //    3 x 64, 3157 teams: 21 and 55);
+    //  - where they finish gates, of which there may be many, 32 x 8 (144 gates of 131 teams a
+    //    model: 11, with 16 teams at a time 18, with 32 51; 32 gates of 74 teams 8.8, 12, 29;
+    //    but 24 gates of 276 teams 18, 11, 12), and 32 x 32 from 512 teams on, where each
+    //    gate's sum is long (144 gates of 789 teams 17, with 16 25, with 8 47; 6 of 600 7.7,
+    //    12, 22). Between 130 and 511 teams few gates would have 32 as well: 9 gates of 450
+    //    teams take 17, with 32 6.5.
     const bool gates = MODE == GROUPS && a.dgate && a.f.gate_rows > 1;       // else a gate is one team's
     const bool few = a.f.n * ((a.f.d + 31) / 32) < sm_count(dev);
     const int tx = !gates && few && a.f.teams >= 128 ? 16 : 32, most = gates ? (a.f.teams >= 512 ? 32 : 8) : tx == 16 ? 64 : 16;
