@@ -80,3 +80,38 @@ def test_more_rows_than_narrow_tiles_and_few_tiles(n, m, k, o, dtype):
     parts = [ops.linear_int8(codes[:, i:i + 100], scale[:, i:i + 100], w, ws, act=ops.ACT_RELU, dtype=dtype) for i in range(0, m, 100)]
     assert torch.equal(torch.cat(parts, 1), y)
     no_device_error()
+
+
+@pytest.mark.parametrize("n, m, k, o", [(1, 540000, 48, 4096), (1, 540000, 48, 4097), (300000, 8, 16, 1024)])
+def test_products_past_32_bits(n, m, k, o):
+    """Over 2^31 results (wide tiles by whole vectors and value by value, narrow ones of many models): the last
+    rows are what a call on them alone gives."""
+    gen = torch.Generator(device=DEV).manual_seed(n + o)
+    ints = lambda *s: torch.randint(-127, 128, s, generator=gen, dtype=torch.int8, device=DEV)
+    codes, w = ints(n, m, k), ints(n, o, k)
+    scale, ws = torch.rand(n, m, generator=gen, device=DEV), torch.rand(n, o, generator=gen, device=DEV)
+    y = ops.linear_int8(codes, scale, w, ws, dtype=BF16)
+    alone = ops.linear_int8(codes[-1:, -5:], scale[-1:, -5:], w[-1:], ws[-1:], dtype=BF16)
+    assert torch.equal(y[-1:, -5:], alone)
+    no_device_error()
+
+
+@pytest.mark.grad
+def test_gradients_past_32_bits():
+    """Rows of over 2^31 values: the last rows' gradients are those of a call on them alone."""
+    n, rows, d = 1, 270000, 8192
+    x, y, dh, dz = (torch.randn(n, rows, d, device=DEV, dtype=BF16) for _ in range(4))
+    w = 1 + 0.2 * torch.randn(n, d, device=DEV, dtype=BF16)
+    need = (True, True) + (False,) * 5
+
+    def grads(x, y, dh, dz):
+        _, _, stats, _ = ops._residual_norm(x, y, w, None, w, None, None, 1.0, 1e-6, False, True)
+        return ops.residual_norm_bwd(x, y, w, None, w, None, None, stats, dh, dz, need=need)[:2]
+
+    got = grads(x, y, dh, dz)
+    want = grads(*(t[:, -5:].contiguous() for t in (x, y, dh, dz)))
+    for a, b in zip(got, want):
+        # the forward's statistics are summed in another order for few rows: the factors are off by 90 * 2^-24 of
+        # themselves, terms of up to 6 by 4e-5; each side is rounded to bf16 once, by up to 2^-8 of its value
+        torch.testing.assert_close(a[:, -5:].float(), b.float(), rtol=2.0 ** -7, atol=1e-4)
+    no_device_error()
