@@ -596,6 +596,7 @@ __global__ void __launch_bounds__(kNarrowThreads)
         if (threadIdx.x == 0 && *abort_flag)
             for (int j = max(issued - stages, 0); j < issued; ++j)
                 mbar_wait_ns(&full[j % stages], (uint32_t)(j / stages & 1), &never, kWaitLimitNs / 8);
+        __syncwarp();                        // the cluster's barriers take whole warps
     };
     if (split == 1) {
         const Gelu2 gelu;
